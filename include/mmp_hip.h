@@ -485,6 +485,65 @@ int mmp_matmul_t(int dtype, int trans_a, int trans_b, int64_t batch, int64_t M,
                  int64_t sC);
 
 /* ======================================================================== */
+/* Operators of sequence models.  No counterpart in the reference, whose    */
+/* users write them with take, cumsum, max / sum and one reduction per      */
+/* array.  dtype: MMP_F16, MMP_F32 or MMP_F64; "wide" is double for MMP_F64 */
+/* and float otherwise, the type of sums, states and statistics.  Index     */
+/* dtypes: MMP_I32 or MMP_I64.  Outputs are contiguous; row strides, and    */
+/* sb / st, the strides of sequences and steps, are in elements, and the    */
+/* elements of a row or step are adjacent.                                  */
+/* ======================================================================== */
+
+/* out[i] = scale * table[tokens[i]], i < n, rows of dim elements; zeros for a
+ * token outside [0, rows). */
+int mmp_embedding(int dtype, int index_dtype, int64_t n, const void *tokens,
+                  int64_t rows, int64_t dim, const void *table, int64_t row_stride,
+                  double scale, void *out);
+
+/* out[v] = scale * the sum of grad[i] over the tokens i equal to v, in order
+ * of i, v < rows; a token outside [0, rows) adds nothing.  n, rows and dim are
+ * below 2^31.  Takes memory from the allocator for the call. */
+int mmp_embedding_grad(int dtype, int index_dtype, int64_t n, const void *tokens,
+                       const void *grad, int64_t row_stride, int64_t rows,
+                       int64_t dim, double scale, void *out);
+
+/* h_t = f_t h_{t-1} + u_t along the steps of (batch, steps, dim) arrays, where
+ * logits != 0 means f = 1 / (1 + exp(-gate)), u = (1 - f) x, and 0 f = gate,
+ * u = x.  initial (h_{-1}; NULL for zeros) and final (the last state, or
+ * initial where there are no steps) are (batch, dim) of the wide type. */
+int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t steps, int64_t dim,
+                   const void *gate, int64_t gate_sb, int64_t gate_st,
+                   const void *x, int64_t x_sb, int64_t x_st,
+                   const void *initial, void *h, void *final_state);
+
+/* Its gradient, from grad (of h), grad_final (of final; NULL for zeros), the
+ * inputs and h. */
+int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t steps, int64_t dim,
+                        const void *grad, int64_t grad_sb, int64_t grad_st,
+                        const void *gate, int64_t gate_sb, int64_t gate_st,
+                        const void *x, int64_t x_sb, int64_t x_st,
+                        const void *h, int64_t h_sb, int64_t h_st,
+                        const void *initial, const void *grad_final, void *grad_gate,
+                        void *grad_x, void *grad_initial);
+
+/* loss[r] = log(sum exp(x)) - x[targets[r]] (wide) of each row x of logits, and
+ * where grad is not NULL grad[r] = w (softmax(x) - onehot(targets[r])) with
+ * w = scale * weight[r] (wide; NULL for ones).  A target outside [0, classes)
+ * gives a loss and a gradient of 0.  classes >= 1. */
+int mmp_cross_entropy(int dtype, int index_dtype, int64_t rows, int64_t classes,
+                      const void *logits, int64_t row_stride, const void *targets,
+                      const void *weight, double scale, void *loss, void *grad);
+
+/* norm = sqrt(sum of the squares of all `count` arrays of sizes[i] contiguous
+ * elements of dtypes[i]), stored as norm_dtype (MMP_F32 or MMP_F64), summed in
+ * double; where outs is not NULL, outs[i] = arrays[i] * min(1, limit / norm)
+ * (outs[i] may be arrays[i]; NaN where the norm is NaN).  limit >= 0.  Takes
+ * memory from the allocator for the call. */
+int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *sizes,
+                  const void *const *arrays, void *const *outs, double limit,
+                  int norm_dtype, void *norm);
+
+/* ======================================================================== */
 /* Runtime compilation: replaces createLibraryFromString + setFunction +    */
 /* runFunction (_metal_backend.py:237-257, 313-357) for the fusion engine  */
 /* (_fusion.py:443-486) and RawKernel (raw_kernel.py:32-62)                 */

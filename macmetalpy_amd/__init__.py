@@ -106,6 +106,7 @@ _gate_mod.setup()  # the native dispatch gate takes over the hot elementwise pat
 from . import linalg
 from . import random
 from . import fft
+from . import nn
 
 # NumPy 2 aliases (reference __init__.py:262-272)
 acos = arccos

@@ -213,6 +213,8 @@ EXPORTS = (
     "mmp_mask_tile_counts", "mmp_mask_positions", "mmp_mask_compact",
     "mmp_bincount", "mmp_histogram",
     "mmp_lu", "mmp_lu_solve", "mmp_cholesky", "mmp_qr", "mmp_qr_q", "mmp_eigh", "mmp_svd",
+    "mmp_embedding", "mmp_embedding_grad", "mmp_recurrence", "mmp_recurrence_grad",
+    "mmp_cross_entropy", "mmp_clip_norm",
     "mmp_rtc_compile", "mmp_rtc_build", "mmp_rtc_launch", "mmp_rtc_launch_threads",
     "mmp_wait_status",
     "mmp_debug_fail_next",

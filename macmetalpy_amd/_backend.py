@@ -125,6 +125,18 @@ _SIGNATURES = {
                    _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64],
     "mmp_matmul_t": [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64,
                      _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64],
+    "mmp_embedding": [_c_int, _c_int, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64,
+                      ctypes.c_double, _c_vp],
+    "mmp_embedding_grad": [_c_int, _c_int, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
+                           ctypes.c_double, _c_vp],
+    "mmp_recurrence": [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64,
+                       _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp],
+    "mmp_recurrence_grad": [_c_int, _c_int, _c_i64, _c_i64, _c_i64] + [_c_vp, _c_i64, _c_i64] * 4
+                           + [_c_vp] * 5,
+    "mmp_cross_entropy": [_c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
+                          ctypes.c_double, _c_vp, _c_vp],
+    "mmp_clip_norm": [_c_i64, ctypes.POINTER(_c_int), _c_i64p, ctypes.POINTER(_c_vp),
+                      ctypes.POINTER(_c_vp), ctypes.c_double, _c_int, _c_vp],
     "mmp_rtc_compile": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_c_vp)],
     "mmp_rtc_build": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _c_vp, _c_sz,
                       ctypes.POINTER(_c_sz)],
@@ -533,6 +545,40 @@ class HipBackend:
                  C: int, ldc: int, sC: int) -> None:
         _check(self._lib.mmp_matmul_t(dcode, ta, tb, batch, M, N, K, A, lda, sA, B, ldb, sB,
                                       C, ldc, sC), "mmp_matmul_t")
+
+    def embedding(self, dcode, icode, n, tokens, rows, dim, table, row_stride, scale, out) -> None:
+        _check(self._lib.mmp_embedding(dcode, icode, n, tokens, rows, dim, table, row_stride,
+                                       scale, out), "mmp_embedding")
+
+    def embedding_grad(self, dcode, icode, n, tokens, grad, row_stride, rows, dim, scale,
+                       out) -> None:
+        _check(self._lib.mmp_embedding_grad(dcode, icode, n, tokens, grad, row_stride, rows, dim,
+                                            scale, out), "mmp_embedding_grad")
+
+    def recurrence(self, dcode, logits, batch, steps, dim, gate, x, initial, h, final) -> None:
+        """``gate`` and ``x`` as (pointer, sequence stride, step stride)."""
+        _check(self._lib.mmp_recurrence(dcode, logits, batch, steps, dim, *gate, *x, initial, h,
+                                        final), "mmp_recurrence")
+
+    def recurrence_grad(self, dcode, logits, batch, steps, dim, grad, gate, x, h, initial,
+                        grad_final, grad_gate, grad_x, grad_initial) -> None:
+        """``grad`` to ``h`` as (pointer, sequence stride, step stride)."""
+        _check(self._lib.mmp_recurrence_grad(dcode, logits, batch, steps, dim, *grad, *gate, *x,
+                                             *h, initial, grad_final, grad_gate, grad_x,
+                                             grad_initial), "mmp_recurrence_grad")
+
+    def cross_entropy(self, dcode, icode, rows, classes, logits, row_stride, targets, weight,
+                      scale, loss, grad) -> None:
+        _check(self._lib.mmp_cross_entropy(dcode, icode, rows, classes, logits, row_stride,
+                                           targets, weight, scale, loss, grad),
+               "mmp_cross_entropy")
+
+    def clip_norm(self, dcodes, sizes, arrays, outs, limit, norm_code, norm) -> None:
+        n = len(sizes)
+        ptrs = _c_vp * max(1, n)
+        _check(self._lib.mmp_clip_norm(n, (_c_int * max(1, n))(*dcodes), _i64_array(sizes),
+                                       ptrs(*arrays), None if outs is None else ptrs(*outs),
+                                       limit, norm_code, norm), "mmp_clip_norm")
 
     # ------------------------------------------ reference kernel interface
     def execute_kernel(self, shader_src: str, func_name, grid_size, buffers) -> None:

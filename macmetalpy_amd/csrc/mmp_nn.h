@@ -1,0 +1,107 @@
+// mmp_nn.h -- what the operators of sequence models share: vectors of a few
+// elements at any address, and the exponentials that they need.
+#pragma once
+#include "mmp_ops.h"
+#include "mmp_internal.h"
+
+namespace mmpn {
+
+// The type that sums and states are held in: 32 bits for float16 and float32,
+// 64 for float64.
+template <typename T> struct Wide { typedef float type; };
+template <> struct Wide<double> { typedef double type; };
+
+// N adjacent elements, moved by one instruction (or by two or four of 16
+// bytes).  The address need only be a multiple of the element's size: rows of
+// odd lengths start anywhere, and the device's vector loads and stores take any
+// address.
+template <typename T, int N> struct Vec {
+  typedef unsigned int Words __attribute__((ext_vector_type(sizeof(T) * N >= 4 ? sizeof(T) * N / 4 : 1)));
+  T e[N];
+};
+
+template <typename T, int N, bool STREAM = false>
+__device__ __forceinline__ Vec<T, N> load_vec(const T *p) {
+  Vec<T, N> r;
+  if constexpr (sizeof(T) * N >= 4) {
+    typedef typename Vec<T, N>::Words W;
+    typedef W U __attribute__((aligned(sizeof(T))));
+    W w;
+    if constexpr (STREAM) w = __builtin_nontemporal_load(reinterpret_cast<const U *>(p));
+    else w = *reinterpret_cast<const U *>(p);
+    __builtin_memcpy(&r, &w, sizeof(r));
+  } else {
+    for (int i = 0; i < N; ++i) r.e[i] = p[i];
+  }
+  return r;
+}
+
+template <typename T, int N, bool STREAM = false>
+__device__ __forceinline__ void store_vec(T *p, const Vec<T, N> &v) {
+  if constexpr (sizeof(T) * N >= 4) {
+    typedef typename Vec<T, N>::Words W;
+    typedef W U __attribute__((aligned(sizeof(T))));
+    W w;
+    __builtin_memcpy(&w, &v, sizeof(v));
+    if constexpr (STREAM) __builtin_nontemporal_store(w, reinterpret_cast<U *>(p));
+    else *reinterpret_cast<U *>(p) = w;
+  } else {
+    for (int i = 0; i < N; ++i) p[i] = v.e[i];
+  }
+}
+
+// exp(x) in 32 bits: 2^(x log2 e) by the hardware's exponential.  The product's
+// rounding error, which |x| would scale, is carried over to the result, so
+// the relative error stays at a few units of the last place.  Below the normal
+// range the hardware gives 0.
+__device__ __forceinline__ float exp_of(float x) {
+  const float l2e = 1.44269502f, l2e_lo = 1.92596303e-8f;  // log2 e in two parts
+  const float t = x * l2e;
+  const float r = __builtin_fmaf(x, l2e_lo, __builtin_fmaf(x, l2e, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  // infinite x: r is NaN and e is exact already
+  const float c = __builtin_fmaf(e, r * 0.693147182f, e);
+  return __builtin_isfinite(t) ? c : e;
+}
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+
+__device__ __forceinline__ float recip(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ double recip(double x) { return 1.0 / x; }
+
+__device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
+// f = 1 / (1 + exp(-g)) and u = 1 - f = 1 / (1 + exp(g)), each to its own
+// last place: the exponential's argument is never positive, so neither
+// overflows, and u keeps its digits where f is near 1.
+template <typename A> __device__ __forceinline__ void sigmoid_pair(A g, A &f, A &u) {
+  const A e = exp_of(g < 0 ? g : -g);
+  const A r = recip(1 + e);
+  const A s = e * r;
+  f = g < 0 ? s : r;
+  u = g < 0 ? r : s;
+}
+
+// float16 -> float32 and back, one rounding.
+template <typename A, typename T> __device__ __forceinline__ A widen(T v) { return (A)v; }
+
+}  // namespace mmpn
+
+// Dispatch a floating dtype code onto a C++ type `T`.
+#define MMP_DISPATCH_FLOAT(dtype, what, ...)                                  \
+  switch (dtype) {                                                            \
+    case MMP_F16: { typedef mmp_half T; __VA_ARGS__ }                         \
+    case MMP_F32: { typedef float T; __VA_ARGS__ }                            \
+    case MMP_F64: { typedef double T; __VA_ARGS__ }                           \
+    default:                                                                  \
+      return mmpi::fail(MMP_E_UNSUPPORTED, what ": dtype code %d is not floating", \
+                        (int)(dtype));                                        \
+  }
+// Dispatch an index dtype code (MMP_I32, MMP_I64) onto a C++ type `I`.
+#define MMP_DISPATCH_INDEX(dtype, what, ...)                                  \
+  switch (dtype) {                                                            \
+    case MMP_I32: { typedef mmp_i32 I; __VA_ARGS__ }                          \
+    case MMP_I64: { typedef mmp_i64 I; __VA_ARGS__ }                          \
+    default:                                                                  \
+      return mmpi::fail(MMP_E_UNSUPPORTED, what ": index dtype code %d", (int)(dtype)); \
+  }
