@@ -50,18 +50,18 @@ __device__ __forceinline__ void store_vec(T *p, const Vec<T, N> &v) {
   }
 }
 
-// exp(x) in 32 bits: 2^(x log2 e) by the hardware's exponential.  The product's
-// rounding error, which |x| would scale, is carried over to the result, so
-// the relative error stays at a few units of the last place.  Below the normal
-// range the hardware gives 0.
+// exp(x) of x <= 0 or NaN in 32 bits: 2^(x log2 e) by the hardware's
+// exponential.  The product's rounding error, which grows with |x|, is carried
+// over to the result, so the relative error stays at a few units of the last
+// place.  Below the normal range the result is 0; so it is for x < -126, where
+// x is cut off because -inf has no product to correct.
 __device__ __forceinline__ float exp_of(float x) {
   const float l2e = 1.44269502f, l2e_lo = 1.92596303e-8f;  // log2 e in two parts
+  x = x < -126.0f ? -126.0f : x;
   const float t = x * l2e;
   const float r = __builtin_fmaf(x, l2e_lo, __builtin_fmaf(x, l2e, -t));
   const float e = __builtin_amdgcn_exp2f(t);
-  // infinite x: r is NaN and e is exact already
-  const float c = __builtin_fmaf(e, r * 0.693147182f, e);
-  return __builtin_isfinite(t) ? c : e;
+  return __builtin_fmaf(e, r * 0.693147182f, e);
 }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 

@@ -11,7 +11,8 @@ namespace mmpi {
 // SCRATCH_REDUCE_PLAIN.
 enum { SCRATCH_REDUCE_PARTIALS = 0, SCRATCH_REDUCE_TICKETS = 1,
        SCRATCH_SCAN_FLAGS = 2, SCRATCH_SCAN_VALUES = 3,
-       SCRATCH_SCAN_COUNTER = 4, SCRATCH_REDUCE_PLAIN = 5, SCRATCH_NSLOTS = 6 };
+       SCRATCH_SCAN_COUNTER = 4, SCRATCH_REDUCE_PLAIN = 5, SCRATCH_RECUR_TILES = 6,
+       SCRATCH_NSLOTS = 7 };
 
 // HIP counts at most 2^32 - 1 work-items per grid dimension.
 inline bool grid_fits(long long blocks, int threads) { return blocks <= 0xffffffffLL / threads; }

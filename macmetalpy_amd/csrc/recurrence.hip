@@ -9,13 +9,40 @@
 //   logits:   grad_g = d_t (h_{t-1} - x_t) f (1 - f),  grad_x = d_t (1 - f)
 //   factors:  grad_a = d_t h_{t-1},                    grad_x = d_t
 // and c_0 is the initial state's gradient.
+//
+// Bound by memory: 3 arrays forwards, 6 (5 with factors) backwards.  Each is
+// read or written once.  n steps together are one step h -> A h + B, with A
+// the product of their factors and B what they make of h = 0, so time is cut
+// into tiles: a workgroup loads kTile steps of 64 channels (float16) into
+// registers, each thread joins kSteps steps of its own, the workgroup
+// joins its threads' (A, B) in LDS, and the tile's state before its first step
+// comes from the tiles before it by look-back; then each thread runs its steps
+// from its state and writes.
+//
+// Look-back: a tile publishes (A, B) and, as soon as it knows it, the state
+// after its last step.  It reads the kLook tiles before it until one of them
+// has that state and all after it have (A, B), and goes through those in
+// order, state = A state + B: the same operations whichever tile had its state
+// first, so the results' bits do not depend on timing.  Nothing promises that
+// an earlier tile's workgroup has started, so the wait is bounded: after
+// kPolls reads a tile goes back as far as it must and joins the steps of the
+// tiles that are missing itself.
 #include "mmp_nn.h"
 
 namespace {
 
+using mmpn::Vec;
 using mmpn::Wide;
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 512;
+constexpr int kLanes = 16;               // threads side by side on a step: 128 bytes
+constexpr int kSlices = kBlock / kLanes; // threads one after another in time
+constexpr int kSteps = 8;                // steps of a thread
+constexpr int kTile = kSlices * kSteps;  // steps of a workgroup
+constexpr int kPolls = 256;
+constexpr int kWaves = 4;                // per SIMD: two workgroups a CU, so 128 registers
+template <typename T> constexpr int vec_of() { return 8 / sizeof(T); }
+template <typename T> constexpr int channels_of() { return kLanes * vec_of<T>(); }
 
 // Steps of a (batch, steps, dim) array: adjacent channels, any other strides.
 template <typename T> struct Steps {
@@ -23,62 +50,560 @@ template <typename T> struct Steps {
   long long sb, st;
 };
 
-template <typename T, bool LOGITS>
-__global__ __launch_bounds__(kBlock) void k_recur(long long batch, long long steps, long long dim,
-                                                  Steps<T> gate, Steps<T> x,
-                                                  const typename Wide<T>::type *__restrict__ initial,
-                                                  T *__restrict__ h,
-                                                  typename Wide<T>::type *__restrict__ final_) {
-  typedef typename Wide<T>::type A;
-  const long long i = (long long)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= batch * dim) return;
-  const long long b = i / dim, c = i - b * dim;
-  A s = initial ? initial[i] : 0;
-  for (long long t = 0; t < steps; ++t) {
-    const A g = (A)gate.p[b * gate.sb + t * gate.st + c], v = (A)x.p[b * x.sb + t * x.st + c];
-    A f = g, u = v;
-    if constexpr (LOGITS) {
-      A r;
-      mmpn::sigmoid_pair(g, f, r);
-      u = r * v;
-    }
-    s = mmpn::fma_of(f, s, u);
-    h[(b * steps + t) * dim + c] = (T)s;
-  }
-  final_[i] = s;
+// A tile's descriptor holds 2 wide values per channel, each 32 bits of them in
+// a word with a tag above: generation << 2 | state, 1 for (A, B), 2 for the
+// state after the tile.  Words are written and read with relaxed atomics
+// and taken only where all tags of a channel agree and are this call's, so
+// they are never cleared and need no fence.
+struct Look {
+  unsigned long long *desc;
+  unsigned gen;       // this call's
+  unsigned read_gen;  // the one that readers take (another one to force the slow way)
+  long long polls;
+};
+template <typename A> constexpr int words_of() { return (int)sizeof(A) / 2; }
+
+template <typename A, int CH>
+__device__ __forceinline__ void publish(const Look &lk, long long tile, int ch, unsigned state, A a,
+                                        A b) {
+  constexpr int NW = words_of<A>();
+  unsigned w[NW];
+  const A v[2] = {a, b};
+  __builtin_memcpy(w, v, sizeof(v));
+  const unsigned long long tag = (unsigned long long)(lk.gen << 2 | state) << 32;
+#pragma unroll
+  for (int k = 0; k < NW; ++k)
+    __hip_atomic_store(lk.desc + (tile * NW + k) * CH + ch, tag | w[k], __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <typename T, bool LOGITS>
-__global__ __launch_bounds__(kBlock) void k_recur_grad(
-    long long batch, long long steps, long long dim, Steps<T> grad, Steps<T> gate, Steps<T> x,
+// The state of tile's descriptor for a channel: 0 (not there), 1 or 2.
+template <typename A> struct Desc {
+  unsigned long long w[words_of<A>()];
+};
+template <typename A, int CH>
+__device__ __forceinline__ Desc<A> read_desc(const Look &lk, long long tile, int ch) {
+  Desc<A> d;
+#pragma unroll
+  for (int k = 0; k < words_of<A>(); ++k)
+    d.w[k] = __hip_atomic_load(lk.desc + (tile * words_of<A>() + k) * CH + ch, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+  return d;
+}
+template <typename A>
+__device__ __forceinline__ unsigned parse(const Look &lk, const Desc<A> &d, A &a, A &b) {
+  const unsigned tag = (unsigned)(d.w[0] >> 32);
+  bool same = (tag >> 2) == lk.read_gen;
+  unsigned w[words_of<A>()];
+#pragma unroll
+  for (int k = 0; k < words_of<A>(); ++k) {
+    same = same && (unsigned)(d.w[k] >> 32) == tag;
+    w[k] = (unsigned)d.w[k];
+  }
+  A v[2];
+  __builtin_memcpy(v, w, sizeof(v));
+  a = v[0];
+  b = v[1];
+  return same ? tag & 3u : 0u;
+}
+
+// The state before tile t of a sequence whose tiles' descriptors begin at
+// `base`; a wave, a channel a lane (`on`: the lane has one).  own(j, a, b)
+// joins the steps of tile j.
+template <typename A, int CH, int W, typename Own>
+__device__ A look_back(const Look &lk, long long base, long long t, int ch, bool on, A initial,
+                       Own own) {
+  for (long long poll = 0; poll < lk.polls; ++poll) {
+    Desc<A> d[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const long long j = t - 1 - k < 0 ? 0 : t - 1 - k;
+      d[k] = read_desc<A, CH>(lk, base + j, ch);
+    }
+    A h = 0;
+    bool ok = !on;
+#pragma unroll
+    for (int k = W - 1; k >= 0; --k) {
+      A a, b;
+      const unsigned st = parse(lk, d[k], a, b);
+      if (t - 1 - k < 0) {
+        h = initial;
+        ok = true;
+      } else if (st == 2) {
+        h = a;
+        ok = true;
+      } else if (st == 1) {
+        h = mmpn::fma_of(a, h, b);
+      } else {
+        ok = !on;
+      }
+    }
+    if (__ballot(!ok) == 0) return h;
+    __builtin_amdgcn_s_sleep(1);
+  }
+  // Back to a tile that every channel knows the state after, or to the first.
+  A h = initial, a, b;
+  long long j = t - 1;
+  for (; j >= 0; --j) {
+    const unsigned st = parse(lk, read_desc<A, CH>(lk, base + j, ch), a, b);
+    if (__ballot(on && st != 2) == 0) {
+      h = a;
+      break;
+    }
+  }
+  for (++j; j < t; ++j) {
+    const unsigned st = parse(lk, read_desc<A, CH>(lk, base + j, ch), a, b);
+    if (__ballot(on && st == 0) != 0) {
+      A a2, b2;
+      own(j, a2, b2);
+      if (st == 0) {
+        a = a2;
+        b = b2;
+      }
+    }
+    h = st == 2 ? a : mmpn::fma_of(a, h, b);
+  }
+  return h;
+}
+
+// One step's factor and addend.
+template <bool LOGITS, typename A> __device__ __forceinline__ void factor(A g, A x, A &f, A &u) {
+  if constexpr (LOGITS) {
+    A r;
+    mmpn::sigmoid_pair(g, f, r);
+    u = r * x;
+  } else {
+    f = g;
+    u = x;
+  }
+}
+
+// `count` of V adjacent elements (all of them, but at a row's end), zeros else.
+template <typename T, int V> __device__ __forceinline__ Vec<T, V> load_some(const T *p, int count) {
+  if (count >= V) return mmpn::load_vec<T, V>(p);
+  Vec<T, V> v;
+#pragma unroll
+  for (int k = 0; k < V; ++k) v.e[k] = k < count ? p[k] : (T)0;
+  return v;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) {
+  if (count >= V) {
+    mmpn::store_vec<T, V>(p, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < count) p[k] = v.e[k];
+  }
+}
+
+// A value that the compiler takes for another one from here on, so that it
+// works out the gates again where they are used again instead of keeping
+// them (and what they were widened to) in registers over the wait.
+template <typename T, int V> __device__ __forceinline__ void forget(Vec<T, V> &v) {
+  unsigned w[sizeof(v) / 4];
+  __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+  for (unsigned k = 0; k < sizeof(v) / 4; ++k) asm volatile("" : "+v"(w[k]));
+  __builtin_memcpy(&v, w, sizeof(v));
+}
+
+// Where a workgroup is: `groups` sequences times channel groups, and in each
+// `tiles` tiles.  Early tiles have the low workgroup ids, which start first.
+struct Place {
+  long long seq, base;
+  int group;     // of channels
+  long long t;   // tile of the sequence
+};
+__device__ __forceinline__ Place place(long long tiles, long long groups, int cgroups) {
+  Place p;
+  p.t = blockIdx.x / groups;
+  const long long g = blockIdx.x - p.t * groups;
+  p.seq = g / cgroups;
+  p.group = (int)(g - p.seq * cgroups);
+  p.base = g * tiles;
+  return p;
+}
+
+// Joins the slices' (A, B), which sa and sb hold: each becomes that of all
+// slices before it, and the tile's is returned.  A channel a lane.
+template <typename A, int CH>
+__device__ __forceinline__ void join_slices(A *sa, A *sb, int ch, A &ta, A &tb) {
+  A pa = 1, pb = 0;
+#pragma unroll 8
+  for (int s = 0; s < kSlices; ++s) {
+    const A a = sa[s * CH + ch], b = sb[s * CH + ch];
+    sa[s * CH + ch] = pa;
+    sb[s * CH + ch] = pb;
+    pb = mmpn::fma_of(a, pb, b);
+    pa = a * pa;
+  }
+  ta = pa;
+  tb = pb;
+}
+
+template <typename T, bool LOGITS, int W>
+__global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
+    long long steps, int dim, long long tiles, long long groups, int cgroups, Steps<T> gate,
+    Steps<T> x, const typename Wide<T>::type *__restrict__ initial, T *__restrict__ h,
+    typename Wide<T>::type *__restrict__ final_, Look lk) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), CH = channels_of<T>();
+  __shared__ A sa[kSlices * CH], sb[kSlices * CH], sh[CH];
+  const Place pl = place(tiles, groups, cgroups);
+  const int tid = threadIdx.x, c = (tid & (kLanes - 1)) * V, s = tid / kLanes;
+  const int ch = pl.group * CH + c;  // the thread's first channel
+  const int count = dim - ch;
+  const long long t0 = pl.t * kTile + s * kSteps;
+  const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
+  const T *px = x.p + pl.seq * x.sb + t0 * x.st + ch;
+  A f[kSteps][V], u[kSteps][V];
+  {
+    Vec<T, V> g[kSteps], v[kSteps];
+    if (count >= V && t0 + kSteps <= steps) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        g[i] = mmpn::load_vec<T, V>(pg + i * gate.st);
+        v[i] = mmpn::load_vec<T, V>(px + i * x.st);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int n = t0 + i < steps ? count : 0;
+        g[i] = load_some<T, V>(pg + i * gate.st, n);
+        v[i] = load_some<T, V>(px + i * x.st, n);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) factor<LOGITS>((A)g[i].e[k], (A)v[i].e[k], f[i][k], u[i][k]);
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    A a = 1, b = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      a = f[i][k] * a;
+      b = mmpn::fma_of(f[i][k], b, u[i][k]);
+    }
+    sa[s * CH + c + k] = a;
+    sb[s * CH + c + k] = b;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    const int my = tid < CH ? tid : CH - 1;
+    const bool on = tid < CH && pl.group * CH + tid < dim;
+    const long long at = pl.seq * dim + pl.group * CH + tid;
+    A a, b;
+    if (tid < CH) join_slices<A, CH>(sa, sb, tid, a, b);
+    A state = on && initial ? initial[at] : (A)0;
+    if (tiles > 1) {
+      if (on && pl.t > 0 && pl.t + 1 < tiles) publish<A, CH>(lk, pl.base + pl.t, my, 1, a, b);
+      if (pl.t > 0)
+        state = look_back<A, CH, W>(
+            lk, pl.base, pl.t, my, on, state, [&](long long j, A &ja, A &jb) {
+              ja = 1;
+              jb = 0;
+              if (!on) return;
+              const T *qg = gate.p + pl.seq * gate.sb + j * kTile * gate.st + pl.group * CH + tid;
+              const T *qx = x.p + pl.seq * x.sb + j * kTile * x.st + pl.group * CH + tid;
+              for (int w = 0; w < kSlices; ++w) {
+                A wa = 1, wb = 0;
+                for (int i = 0; i < kSteps; ++i) {
+                  const long long r = w * kSteps + i;
+                  A ff, uu;
+                  factor<LOGITS>((A)qg[r * gate.st], (A)qx[r * x.st], ff, uu);
+                  wa = ff * wa;
+                  wb = mmpn::fma_of(ff, wb, uu);
+                }
+                jb = mmpn::fma_of(wa, jb, wb);
+                ja = wa * ja;
+              }
+            });
+      if (on && pl.t + 1 < tiles)
+        publish<A, CH>(lk, pl.base + pl.t, my, 2, mmpn::fma_of(a, state, b), (A)0);
+    }
+    if (tid < CH) sh[tid] = state;
+  }
+  __syncthreads();
+  A st[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    st[k] = mmpn::fma_of(sa[s * CH + c + k], sh[c + k], sb[s * CH + c + k]);
+  T *ph = h + (pl.seq * steps + t0) * dim + ch;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    if (t0 + i >= steps) break;
+    Vec<T, V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      st[k] = mmpn::fma_of(f[i][k], st[k], u[i][k]);
+      o.e[k] = (T)st[k];
+    }
+    store_some<T, V>(ph + (long long)i * dim, o, count);
+  }
+  if (t0 < steps && t0 + kSteps >= steps)
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < count) final_[pl.seq * dim + ch + k] = st[k];
+}
+
+// Backwards: tile 0 holds the last steps, a thread's first step is its latest.
+template <typename T, bool LOGITS, int W>
+__global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
+    long long steps, int dim, long long tiles, long long groups, int cgroups, Steps<T> grad,
+    Steps<T> gate, Steps<T> x, Steps<T> h, const typename Wide<T>::type *__restrict__ initial,
+    const typename Wide<T>::type *__restrict__ grad_final, T *__restrict__ grad_gate,
+    T *__restrict__ grad_x, typename Wide<T>::type *__restrict__ grad_initial, Look lk) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), CH = channels_of<T>();
+  __shared__ A sa[kSlices * CH], sb[kSlices * CH], sh[CH];
+  const Place pl = place(tiles, groups, cgroups);
+  const int tid = threadIdx.x, c = (tid & (kLanes - 1)) * V, s = tid / kLanes;
+  const int ch = pl.group * CH + c;
+  const int count = dim - ch;
+  const long long t0 = steps - 1 - (pl.t * kTile + s * kSteps);  // the thread's latest step
+  const T *pd = grad.p + pl.seq * grad.sb + t0 * grad.st + ch;
+  const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
+  const T *px = x.p + pl.seq * x.sb + t0 * x.st + ch;
+  const T *ph = h.p + pl.seq * h.sb + (t0 - 1) * h.st + ch;
+  Vec<T, V> g[kSteps], d[kSteps], v[kSteps], before[kSteps];
+  if (count >= V && t0 >= kSteps) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      g[i] = mmpn::load_vec<T, V>(pg - i * gate.st);
+      d[i] = mmpn::load_vec<T, V>(pd - i * grad.st);
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if constexpr (LOGITS) v[i] = mmpn::load_vec<T, V>(px - i * x.st);
+      before[i] = mmpn::load_vec<T, V>(ph - i * h.st);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int n = t0 >= i ? count : 0;
+      g[i] = load_some<T, V>(pg - i * gate.st, n);
+      d[i] = load_some<T, V>(pd - i * grad.st, n);
+      if constexpr (LOGITS) v[i] = load_some<T, V>(px - i * x.st, n);
+      before[i] = load_some<T, V>(ph - i * h.st, t0 > i ? count : 0);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    A a = 1, b = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      A f, u;
+      factor<LOGITS>((A)g[i].e[k], (A)0, f, u);
+      a = f * a;
+      b = f * ((A)d[i].e[k] + b);
+    }
+    sa[s * CH + c + k] = a;
+    sb[s * CH + c + k] = b;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    const int my = tid < CH ? tid : CH - 1;
+    const bool on = tid < CH && pl.group * CH + tid < dim;
+    const long long at = pl.seq * dim + pl.group * CH + tid;
+    A a, b;
+    if (tid < CH) join_slices<A, CH>(sa, sb, tid, a, b);
+    A state = on && grad_final ? grad_final[at] : (A)0;
+    if (tiles > 1) {
+      if (on && pl.t > 0 && pl.t + 1 < tiles) publish<A, CH>(lk, pl.base + pl.t, my, 1, a, b);
+      if (pl.t > 0)
+        state = look_back<A, CH, W>(
+            lk, pl.base, pl.t, my, on, state, [&](long long j, A &ja, A &jb) {
+              ja = 1;
+              jb = 0;
+              if (!on) return;
+              const long long q = steps - 1 - j * kTile;
+              const T *qd = grad.p + pl.seq * grad.sb + q * grad.st + pl.group * CH + tid;
+              const T *qg = gate.p + pl.seq * gate.sb + q * gate.st + pl.group * CH + tid;
+              for (int w = 0; w < kSlices; ++w) {
+                A wa = 1, wb = 0;
+                for (int i = 0; i < kSteps; ++i) {
+                  const long long r = w * kSteps + i;
+                  A ff, uu;
+                  factor<LOGITS>((A)qg[-r * gate.st], (A)0, ff, uu);
+                  wa = ff * wa;
+                  wb = ff * ((A)qd[-r * grad.st] + wb);
+                }
+                jb = mmpn::fma_of(wa, jb, wb);
+                ja = wa * ja;
+              }
+            });
+      if (on && pl.t + 1 < tiles)
+        publish<A, CH>(lk, pl.base + pl.t, my, 2, mmpn::fma_of(a, state, b), (A)0);
+    }
+    if (tid < CH) sh[tid] = state;
+  }
+  __syncthreads();
+  A carry[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    carry[k] = mmpn::fma_of(sa[s * CH + c + k], sh[c + k], sb[s * CH + c + k]);
+  const long long o0 = (pl.seq * steps + t0) * dim + ch;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    forget(g[i]);
+    forget(d[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    if (t0 < i) break;
+    Vec<T, V> og, ox;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      A hb = (A)before[i].e[k];
+      if (t0 == i) hb = initial && k < count ? initial[pl.seq * dim + ch + k] : (A)0;
+      const A dd = (A)d[i].e[k] + carry[k];
+      if constexpr (LOGITS) {
+        A f, u;
+        mmpn::sigmoid_pair((A)g[i].e[k], f, u);
+        const A du = dd * u;
+        og.e[k] = (T)(du * f * (hb - (A)v[i].e[k]));
+        ox.e[k] = (T)du;
+        carry[k] = f * dd;
+      } else {
+        og.e[k] = (T)(dd * hb);
+        ox.e[k] = (T)dd;
+        carry[k] = (A)g[i].e[k] * dd;
+      }
+    }
+    store_some<T, V>(grad_gate + o0 - (long long)i * dim, og, count);
+    store_some<T, V>(grad_x + o0 - (long long)i * dim, ox, count);
+  }
+  if (t0 >= 0 && t0 < kSteps)
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < count) grad_initial[pl.seq * dim + ch + k] = carry[k];
+}
+
+// Few steps: a thread per V channels goes through them.
+constexpr int kShortBlock = 256;
+template <typename T, bool LOGITS, int V>
+__global__ __launch_bounds__(kShortBlock) void k_recur_short(
+    long long n, long long steps, int dim, int vecs, Steps<T> gate, Steps<T> x,
+    const typename Wide<T>::type *__restrict__ initial, T *__restrict__ h,
+    typename Wide<T>::type *__restrict__ final_) {
+  typedef typename Wide<T>::type A;
+  const long long i = (long long)blockIdx.x * kShortBlock + threadIdx.x;
+  if (i >= n) return;
+  const long long b = i / vecs;
+  const int c = (int)(i - b * vecs) * V, count = dim - c;
+  Vec<A, V> s;
+  if (initial) {
+    s = load_some<A, V>(initial + b * dim + c, count);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) s.e[k] = 0;
+  }
+  const T *pg = gate.p + b * gate.sb + c, *px = x.p + b * x.sb + c;
+  T *ph = h + b * steps * dim + c;
+  for (long long t = 0; t < steps; ++t) {
+    const Vec<T, V> g = load_some<T, V>(pg + t * gate.st, count);
+    const Vec<T, V> v = load_some<T, V>(px + t * x.st, count);
+    Vec<T, V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      A f, u;
+      factor<LOGITS>((A)g.e[k], (A)v.e[k], f, u);
+      s.e[k] = mmpn::fma_of(f, s.e[k], u);
+      o.e[k] = (T)s.e[k];
+    }
+    store_some<T, V>(ph + t * dim, o, count);
+  }
+  store_some<A, V>(final_ + b * dim + c, s, count);
+}
+
+template <typename T, bool LOGITS, int V>
+__global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
+    long long n, long long steps, int dim, int vecs, Steps<T> grad, Steps<T> gate, Steps<T> x,
     Steps<T> h, const typename Wide<T>::type *__restrict__ initial,
     const typename Wide<T>::type *__restrict__ grad_final, T *__restrict__ grad_gate,
     T *__restrict__ grad_x, typename Wide<T>::type *__restrict__ grad_initial) {
   typedef typename Wide<T>::type A;
-  const long long i = (long long)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= batch * dim) return;
-  const long long b = i / dim, c = i - b * dim;
-  A carry = grad_final ? grad_final[i] : 0;
-  for (long long t = steps - 1; t >= 0; --t) {
-    const A g = (A)gate.p[b * gate.sb + t * gate.st + c];
-    const A before = t > 0 ? (A)h.p[b * h.sb + (t - 1) * h.st + c] : initial ? initial[i] : 0;
-    const A d = (A)grad.p[b * grad.sb + t * grad.st + c] + carry;
-    const long long o = (b * steps + t) * dim + c;
-    if constexpr (LOGITS) {
-      A f, u;
-      mmpn::sigmoid_pair(g, f, u);
-      const A v = (A)x.p[b * x.sb + t * x.st + c], du = d * u;
-      grad_gate[o] = (T)(du * f * (before - v));
-      grad_x[o] = (T)du;
-      carry = f * d;
-    } else {
-      grad_gate[o] = (T)(d * before);
-      grad_x[o] = (T)d;
-      carry = g * d;
-    }
+  const long long i = (long long)blockIdx.x * kShortBlock + threadIdx.x;
+  if (i >= n) return;
+  const long long b = i / vecs;
+  const int c = (int)(i - b * vecs) * V, count = dim - c;
+  Vec<A, V> carry;
+  if (grad_final) {
+    carry = load_some<A, V>(grad_final + b * dim + c, count);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) carry.e[k] = 0;
   }
-  grad_initial[i] = carry;
+  const T *pd = grad.p + b * grad.sb + c, *pg = gate.p + b * gate.sb + c;
+  const T *px = x.p + b * x.sb + c, *ph = h.p + b * h.sb + c;
+  for (long long t = steps - 1; t >= 0; --t) {
+    const Vec<T, V> d = load_some<T, V>(pd + t * grad.st, count);
+    const Vec<T, V> g = load_some<T, V>(pg + t * gate.st, count);
+    Vec<T, V> v, before;
+    if constexpr (LOGITS) v = load_some<T, V>(px + t * x.st, count);
+    before = load_some<T, V>(ph + (t - 1) * h.st, t > 0 ? count : 0);
+    Vec<T, V> og, ox;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      A hb = (A)before.e[k];
+      if (t == 0 && initial && k < count) hb = initial[b * dim + c + k];
+      const A dd = (A)d.e[k] + carry.e[k];
+      if constexpr (LOGITS) {
+        A f, u;
+        mmpn::sigmoid_pair((A)g.e[k], f, u);
+        const A du = dd * u;
+        og.e[k] = (T)(du * f * (hb - (A)v.e[k]));
+        ox.e[k] = (T)du;
+        carry.e[k] = f * dd;
+      } else {
+        og.e[k] = (T)(dd * hb);
+        ox.e[k] = (T)dd;
+        carry.e[k] = (A)g.e[k] * dd;
+      }
+    }
+    const long long o = (b * steps + t) * dim + c;
+    store_some<T, V>(grad_gate + o, og, count);
+    store_some<T, V>(grad_x + o, ox, count);
+  }
+  store_some<A, V>(grad_initial + b * dim + c, carry, count);
 }
+
+// Up to this many steps a thread goes through them; a tile's threads would
+// mostly have none.
+constexpr int64_t kShort = 16;
+constexpr int kLook = 8;
+
+// The tiles of a call, and their descriptors.
+struct Plan {
+  int64_t tiles, groups;
+  int cgroups;
+};
+template <typename T> Plan plan(int64_t batch, int64_t steps, int64_t dim) {
+  Plan p;
+  p.tiles = mmpi::ceil_div(steps, kTile);
+  p.cgroups = (int)mmpi::ceil_div(dim, channels_of<T>());
+  p.groups = batch * p.cgroups;
+  return p;
+}
+template <typename T> int look_of(const Plan &p, Look *lk) {
+  typedef typename Wide<T>::type A;
+  *lk = Look{nullptr, 0, 0, 0};
+  if (p.tiles == 1) return MMP_OK;
+  int st = MMP_OK;
+  lk->desc = (unsigned long long *)mmpi::scratch(
+      mmpi::SCRATCH_RECUR_TILES, 8ull * words_of<A>() * channels_of<T>() * p.tiles * p.groups, &st);
+  if (st) return st;
+  const mmpi::WaitParams w = mmpi::wait_params();
+  lk->gen = mmpi::next_generation();
+  lk->read_gen = (lk->gen + w.tag_offset) & 0x3fffffffu;
+  lk->polls = w.tag_offset ? 1 : kPolls;
+  return MMP_OK;
+}
+
+constexpr int64_t kMost = 0x7fffffffLL;
 
 }  // namespace
 
@@ -92,16 +617,33 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
   if (batch == 0 || dim == 0) return MMP_OK;
   if (!final_ || (steps > 0 && (!gate || !x || !h)))
     return mmpi::fail(MMP_E_ARG, "mmp_recurrence: null pointer");
-  const int64_t blocks = mmpi::ceil_div(batch * dim, kBlock);
-  if (!mmpi::grid_fits(blocks, kBlock))
-    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many channels");
+  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: 2^31 channels or more");
   MMP_DISPATCH_FLOAT(dtype, "mmp_recurrence", {
     typedef typename Wide<T>::type A;
-    auto kernel = logits ? k_recur<T, true> : k_recur<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(),
-                       (long long)batch, (long long)steps, (long long)dim,
-                       Steps<T>{(const T *)gate, gate_sb, gate_st},
-                       Steps<T>{(const T *)x, x_sb, x_st}, (const A *)initial, (T *)h, (A *)final_);
+    const Steps<T> sg{(const T *)gate, gate_sb, gate_st}, sx{(const T *)x, x_sb, x_st};
+    if (steps <= kShort) {
+      constexpr int V = vec_of<T>();
+      const int64_t vecs = mmpi::ceil_div(dim, V), n = batch * vecs;
+      const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
+      if (!mmpi::grid_fits(blocks, kShortBlock))
+        return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many channels");
+      auto kernel = logits ? k_recur_short<T, true, V> : k_recur_short<T, false, V>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kShortBlock), 0, mmpi::stream(),
+                         (long long)n, (long long)steps, (int)dim, (int)vecs, sg, sx,
+                         (const A *)initial, (T *)h, (A *)final_);
+      return mmpi::check_launch("mmp_recurrence(short)");
+    }
+    const Plan p = plan<T>(batch, steps, dim);
+    if (!mmpi::grid_fits(p.groups * p.tiles, kBlock))
+      return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many tiles");
+    std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
+    Look lk;
+    if (int st = look_of<T>(p, &lk)) return st;
+    auto kernel = logits ? k_recur_tiles<T, true, kLook> : k_recur_tiles<T, false, kLook>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
+                       mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
+                       (long long)p.groups, p.cgroups, sg, sx, (const A *)initial, (T *)h,
+                       (A *)final_, lk);
     return mmpi::check_launch("mmp_recurrence");
   })
 }
@@ -119,19 +661,35 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
   if (batch == 0 || dim == 0) return MMP_OK;
   if (!grad_initial || (steps > 0 && (!grad || !gate || !x || !h || !grad_gate || !grad_x)))
     return mmpi::fail(MMP_E_ARG, "mmp_recurrence_grad: null pointer");
-  const int64_t blocks = mmpi::ceil_div(batch * dim, kBlock);
-  if (!mmpi::grid_fits(blocks, kBlock))
-    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many channels");
+  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: 2^31 channels or more");
   MMP_DISPATCH_FLOAT(dtype, "mmp_recurrence_grad", {
     typedef typename Wide<T>::type A;
-    auto kernel = logits ? k_recur_grad<T, true> : k_recur_grad<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(),
-                       (long long)batch, (long long)steps, (long long)dim,
-                       Steps<T>{(const T *)grad, grad_sb, grad_st},
-                       Steps<T>{(const T *)gate, gate_sb, gate_st},
-                       Steps<T>{(const T *)x, x_sb, x_st}, Steps<T>{(const T *)h, h_sb, h_st},
-                       (const A *)initial, (const A *)grad_final, (T *)grad_gate, (T *)grad_x,
-                       (A *)grad_initial);
+    const Steps<T> sd{(const T *)grad, grad_sb, grad_st}, sg{(const T *)gate, gate_sb, gate_st};
+    const Steps<T> sx{(const T *)x, x_sb, x_st}, sh{(const T *)h, h_sb, h_st};
+    if (steps <= kShort) {
+      constexpr int V = vec_of<T>();
+      const int64_t vecs = mmpi::ceil_div(dim, V), n = batch * vecs;
+      const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
+      if (!mmpi::grid_fits(blocks, kShortBlock))
+        return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many channels");
+      auto kernel = logits ? k_recur_grad_short<T, true, V> : k_recur_grad_short<T, false, V>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kShortBlock), 0, mmpi::stream(),
+                         (long long)n, (long long)steps, (int)dim, (int)vecs, sd, sg, sx, sh,
+                         (const A *)initial, (const A *)grad_final, (T *)grad_gate, (T *)grad_x,
+                         (A *)grad_initial);
+      return mmpi::check_launch("mmp_recurrence_grad(short)");
+    }
+    const Plan p = plan<T>(batch, steps, dim);
+    if (!mmpi::grid_fits(p.groups * p.tiles, kBlock))
+      return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many tiles");
+    std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
+    Look lk;
+    if (int st = look_of<T>(p, &lk)) return st;
+    auto kernel = logits ? k_recur_grad_tiles<T, true, kLook> : k_recur_grad_tiles<T, false, kLook>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
+                       mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
+                       (long long)p.groups, p.cgroups, sd, sg, sx, sh, (const A *)initial,
+                       (const A *)grad_final, (T *)grad_gate, (T *)grad_x, (A *)grad_initial, lk);
     return mmpi::check_launch("mmp_recurrence_grad");
   })
 }
