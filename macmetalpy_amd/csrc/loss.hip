@@ -8,78 +8,411 @@
 // are classes that cannot be: they add nothing and get no gradient.  A row
 // that holds nothing else, or a logit of +inf, has no distribution and gives
 // NaN.
+//
+// Bound by memory: the logits are read once and the gradient is written once,
+// so a row whose gradient is wanted stays in registers between the two, from
+// 8 threads of a wave with 4 vectors of 16 bytes each (256 float16 classes) to a
+// workgroup of 1024 threads with 16 (131,072).  Longer rows are read again for
+// their gradient, out of the last cache mostly.  The loss alone is one pass with a running
+// maximum and sum.  Few long rows are cut into parts that their own workgroups
+// sum, and joined by a second launch.
 #include "mmp_nn.h"
 
 namespace {
 
+using mmpn::Vec;
 using mmpn::Wide;
 
-constexpr int kBlock = 256;
+template <typename T> constexpr int vec_of() { return 16 / sizeof(T); }
+
+// exp(x - m) of an element.  The exponent's rounding grows with |x - m|; a
+// float16 gradient has 11 bits of its own, so only wider ones correct it.
+template <typename T, typename A> __device__ __forceinline__ A exp_diff(A x, A m) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f((x - m) * 1.44269502f);
+  else return mmpn::exp_of(x - m);
+}
+
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double max_of(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ float log_of(float x) { return logf(x); }
+__device__ __forceinline__ double log_of(double x) { return log(x); }
 
 // A maximum and the sum of exponentials relative to it.
 template <typename A> struct Stat {
   A m, s;
 };
+// Of equal maxima (also -inf, where the difference would be NaN) both sums as
+// they are.  A NaN is in the sum, so the maxima may leave it out.
 template <typename A> __device__ __forceinline__ Stat<A> join(Stat<A> a, Stat<A> b) {
-  // the larger maximum, NaN if either is; of equal ones (also -inf, where the
-  // difference would be NaN) both sums as they are
-  const A m = a.m != a.m ? a.m : b.m != b.m ? b.m : a.m > b.m ? a.m : b.m;
+  const A m = max_of(a.m, b.m);
   const A ea = a.m == m ? (A)1 : mmpn::exp_of(a.m - m);
   const A eb = b.m == m ? (A)1 : mmpn::exp_of(b.m - m);
   return {m, a.s * ea + b.s * eb};
 }
 
-template <typename T, typename I>
-__global__ __launch_bounds__(kBlock) void k_loss(const T *__restrict__ logits, long long classes,
-                                                 long long stride, const I *__restrict__ targets,
-                                                 const typename Wide<T>::type *__restrict__ weight,
-                                                 double scale,
-                                                 typename Wide<T>::type *__restrict__ loss,
-                                                 T *__restrict__ grad) {
+// A row as vectors of 16 bytes at addresses that are multiples of 16: the first
+// may begin before the row and the last end after it (inside the same 16
+// bytes, so inside the allocation); what is not the row's counts as -inf.
+template <typename T> struct Row {
+  static constexpr int V = vec_of<T>();
+  const T *base;
+  int head, classes, vecs;
+  __device__ __forceinline__ Row(const T *x, int n)
+      : head((int)(((uintptr_t)x & 15) / sizeof(T))), classes(n) {
+    base = x - head;
+    vecs = (int)(((long long)head + n + V - 1) / V);
+  }
+  typedef typename Vec<T, V>::Words Words;
+  // vector v with what is outside of the row replaced; v < vecs
+  template <bool STREAM> __device__ __forceinline__ Words load(int v) const {
+    Words w = mmpn::words_of<T, V>(mmpn::load_vec<T, V, STREAM>(base + (long long)v * V));
+    if (v == 0 || v == vecs - 1) {
+      const Words fill = nothing();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unsigned keep = 0;
+#pragma unroll
+        for (int q = 0; q < (sizeof(T) == 2 ? 2 : 1); ++q) {
+          const long long c = (long long)v * V + (j * 4 + q * 2) / (int)sizeof(T) - head;
+          if (c >= 0 && c < classes) keep |= sizeof(T) == 2 ? 0xffffu << (16 * q) : 0xffffffffu;
+        }
+        w[j] = (w[j] & keep) | (fill[j] & ~keep);
+      }
+    }
+    return w;
+  }
+  static __device__ __forceinline__ Words nothing() {
+    Vec<T, V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.e[k] = (T)-__builtin_inff();
+    return mmpn::words_of<T, V>(r);
+  }
+  // vector v of the row g of the gradient
+  __device__ __forceinline__ void store(T *g, int v, const Vec<T, V> &r) const {
+    T *p = g + ((long long)v * V - head);
+    if (v == 0 || v == vecs - 1) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const long long c = (long long)v * V + k - head;
+        if (c >= 0 && c < classes) p[k] = r.e[k];
+      }
+    } else {
+      mmpn::store_vec<T, V, true>(p, r);
+    }
+  }
+};
+
+// The gradient of a vector; `at` is the target's place in it, if it is there.
+template <typename T, typename A>
+__device__ __forceinline__ Vec<T, vec_of<T>()> grad_of(
+    typename Vec<T, vec_of<T>()>::Words words, A m, A by, A w, long long at) {
+  const Vec<T, vec_of<T>()> x = mmpn::elements_of<T, vec_of<T>()>(words);
+  Vec<T, vec_of<T>()> g;
+#pragma unroll
+  for (int k = 0; k < vec_of<T>(); ++k) g.e[k] = (T)(exp_diff<T, A>((A)x.e[k], m) * by);
+  if (at >= 0 && at < vec_of<T>()) {
+#pragma unroll
+    for (int k = 0; k < vec_of<T>(); ++k)
+      if (k == at) g.e[k] = (T)(exp_diff<T, A>((A)x.e[k], m) * by - w);
+  }
+  return g;
+}
+
+// What a call works on.
+template <typename T> struct Loss {
   typedef typename Wide<T>::type A;
-  __shared__ A sm[kBlock / 64], ss[kBlock / 64];
-  const long long row = blockIdx.x;
-  const long long t = (long long)targets[row];
-  const T *x = logits + row * stride;
-  T *g = grad ? grad + row * classes : nullptr;
-  if (t < 0 || t >= classes) {
-    if (threadIdx.x == 0) loss[row] = 0;
-    if (g)
-      for (long long c = threadIdx.x; c < classes; c += kBlock) g[c] = (T)0;
+  const T *logits;
+  long long rows, stride;
+  int classes, wide;  // wide: targets of 64 bits
+  const void *targets;
+  const A *weight;
+  double scale;
+  A *loss;
+  T *grad;
+  __device__ __forceinline__ long long target(long long r) const {
+    return wide ? ((const long long *)targets)[r] : (long long)((const int *)targets)[r];
+  }
+  __device__ __forceinline__ bool counts(long long t) const { return t >= 0 && t < classes; }
+  __device__ __forceinline__ A factor(long long r) const {
+    return (A)scale * (weight ? weight[r] : (A)1);
+  }
+  // log(sum exp(x)) - x_t
+  __device__ __forceinline__ A value(long long r, long long t, A m, A s) const {
+    return log_of(s) + (m - (A)logits[r * stride + t]);
+  }
+};
+
+// Over the L threads of a row: lanes of a wave, or all of the workgroup.
+template <int L, typename A, typename F> __device__ __forceinline__ A over_row(A v, A *lds, F f) {
+#pragma unroll
+  for (int d = (L < 64 ? L : 64) / 2; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d, 64));
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < L / 64; ++w) v = f(v, lds[w]);
+  }
+  return v;
+}
+
+template <int L> constexpr int block_of() { return L < 256 ? 256 : L; }
+
+template <typename T>
+__device__ __forceinline__ void zero_row(T *g, int classes, int lane, int lanes) {
+  for (int c = lane; c < classes; c += lanes) g[c] = (T)0;
+}
+
+// Loss and gradient of rows of up to L * K - 1 vectors, held in registers.
+template <typename T, int L, int K>
+__global__ __launch_bounds__(block_of<L>(), L >= 512 ? 4 : 1) void k_loss_held(Loss<T> p) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), kRows = block_of<L>() / L;
+  __shared__ A lm[L > 64 ? L / 64 : 1], ls[L > 64 ? L / 64 : 1];
+  const int lane = threadIdx.x % L;
+  const long long r = (long long)blockIdx.x * kRows + threadIdx.x / L;
+  if (r >= p.rows) return;
+  const long long t = p.target(r);
+  T *g = p.grad + r * p.classes;
+  if (!p.counts(t)) {
+    if (lane == 0) p.loss[r] = 0;
+    zero_row(g, p.classes, lane, L);
     return;
   }
+  const Row<T> row(p.logits + r * p.stride, p.classes);
+  typename Row<T>::Words x[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int v = i * L + lane;
+    x[i] = row.nothing();
+    if (v < row.vecs) x[i] = row.template load<true>(v);
+  }
   A m = -__builtin_inf();
-  for (long long c = threadIdx.x; c < classes; c += kBlock) {
-    const A v = (A)x[c];
-    m = v > m || v != v ? v : m;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const Vec<T, V> e = mmpn::elements_of<T, V>(x[i]);
+#pragma unroll
+    for (int k = 0; k < V; ++k) m = max_of(m, (A)e.e[k]);
   }
+  m = over_row<L>(m, lm, [](A a, A b) { return max_of(a, b); });
   A s = 0;
-  for (long long c = threadIdx.x; c < classes; c += kBlock) {
-    const A v = (A)x[c];
-    s += mmpn::exp_of(v - m);
-  }
-  Stat<A> st{m, m == -__builtin_inf() ? (A)0 : s};  // nothing but -inf: their differences are NaN
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) st = join(st, Stat<A>{__shfl_xor(st.m, d, 64), __shfl_xor(st.s, d, 64)});
-  if ((threadIdx.x & 63) == 0) {
-    sm[threadIdx.x >> 6] = st.m;
-    ss[threadIdx.x >> 6] = st.s;
-  }
-  __syncthreads();
-  st = {sm[0], ss[0]};
+  for (int i = 0; i < K; ++i) {
+    mmpn::forget(x[i]);
+    const Vec<T, V> e = mmpn::elements_of<T, V>(x[i]);
+    A part = 0;
 #pragma unroll
-  for (int w = 1; w < kBlock / 64; ++w) st = join(st, Stat<A>{sm[w], ss[w]});
-  if (threadIdx.x == 0) {
-    if constexpr (sizeof(A) == 8) loss[row] = (st.m - (A)x[t]) + log(st.s);
-    else loss[row] = (st.m - (A)x[t]) + logf(st.s);
+    for (int k = 0; k < V; ++k) part += exp_diff<T, A>((A)e.e[k], m);
+    s += part;
   }
-  if (!g) return;
-  const A w = (A)scale * (weight ? weight[row] : (A)1), inv = (A)1 / st.s;
-  for (long long c = threadIdx.x; c < classes; c += kBlock) {
-    const A p = mmpn::exp_of((A)x[c] - st.m) * inv;
-    g[c] = (T)((c == t ? p - 1 : p) * w);
+  s = over_row<L>(s, ls, [](A a, A b) { return a + b; });
+  if (lane == 0) p.loss[r] = p.value(r, t, m, s);
+  const A w = p.factor(r), by = w / s;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int v = i * L + lane;
+    mmpn::forget(x[i]);
+    if (v < row.vecs)
+      row.store(g, v, grad_of<T, A>(x[i], m, by, w, t + row.head - (long long)v * V));
   }
 }
+
+// A thread's part of a row: vectors `from` to `to` in steps of `step`, a
+// running maximum and sum over kTogether of them at a time.
+constexpr int kTogether = 4;
+template <bool STREAM, typename T, typename A>
+__device__ __forceinline__ Stat<A> pass(const Row<T> &row, int from, int to, int step) {
+  constexpr int V = vec_of<T>();
+  Stat<A> st{-__builtin_inf(), 0};
+  for (int v0 = from; v0 < to; v0 += kTogether * step) {
+    typename Row<T>::Words x[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int v = v0 + i * step;
+      x[i] = row.nothing();
+      if (v < to) x[i] = row.template load<STREAM>(v);
+    }
+    A m = st.m;
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const Vec<T, V> e = mmpn::elements_of<T, V>(x[i]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) m = max_of(m, (A)e.e[k]);
+    }
+    // nothing but -inf so far: differences to 0 instead, which add nothing
+    const A ref = m == -__builtin_inf() ? (A)0 : m;
+    A s = st.s * mmpn::exp_of(st.m - ref);
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const Vec<T, V> e = mmpn::elements_of<T, V>(x[i]);
+      A part = 0;
+#pragma unroll
+      for (int k = 0; k < V; ++k) part += exp_diff<T, A>((A)e.e[k], ref);
+      s += part;
+    }
+    st = {m, s};
+  }
+  return st;
+}
+
+template <int L, typename A> __device__ __forceinline__ Stat<A> join_row(Stat<A> st, Stat<A> *lds) {
+#pragma unroll
+  for (int d = (L < 64 ? L : 64) / 2; d > 0; d >>= 1)
+    st = join(st, Stat<A>{__shfl_xor(st.m, d, 64), __shfl_xor(st.s, d, 64)});
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = st;
+    __syncthreads();
+    st = lds[0];
+#pragma unroll
+    for (int w = 1; w < L / 64; ++w) st = join(st, lds[w]);
+  }
+  return st;
+}
+
+// Rows of any length: the loss, and the gradient by reading the row again.
+template <typename T, int L, bool GRAD>
+__global__ __launch_bounds__(block_of<L>()) void k_loss_pass(Loss<T> p) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), kRows = block_of<L>() / L;
+  __shared__ Stat<A> lds[L > 64 ? L / 64 : 1];
+  const int lane = threadIdx.x % L;
+  const long long r = (long long)blockIdx.x * kRows + threadIdx.x / L;
+  if (r >= p.rows) return;
+  const long long t = p.target(r);
+  T *g = GRAD ? p.grad + r * p.classes : nullptr;
+  if (!p.counts(t)) {
+    if (lane == 0) p.loss[r] = 0;
+    if constexpr (GRAD) zero_row(g, p.classes, lane, L);
+    return;
+  }
+  const Row<T> row(p.logits + r * p.stride, p.classes);
+  Stat<A> st = pass<!GRAD, T, A>(row, lane, row.vecs, L);
+  st = join_row<L>(st, lds);
+  if (lane == 0) p.loss[r] = p.value(r, t, st.m, st.s);
+  if constexpr (GRAD) {
+    const A w = p.factor(r), by = w / st.s;
+    // the end of the row was read last, so it is the likeliest to be near
+    for (int v = lane + (row.vecs - 1 - lane) / L * L; v >= 0; v -= L)
+      row.store(g, v, grad_of<T, A>(row.template load<true>(v), st.m, by, w,
+                                    t + row.head - (long long)v * V));
+  }
+}
+
+// Few long rows: `parts` workgroups a row, each with its statistics in `part`,
+// then as many again that join them.
+constexpr int kPartBlock = 256;
+template <typename T>
+__global__ __launch_bounds__(kPartBlock) void k_loss_part(Loss<T> p, int parts,
+                                                          Stat<typename Wide<T>::type> *part) {
+  typedef typename Wide<T>::type A;
+  __shared__ Stat<A> lds[kPartBlock / 64];
+  const long long r = blockIdx.x / parts;
+  const int q = (int)(blockIdx.x - r * parts);
+  if (!p.counts(p.target(r))) return;
+  const Row<T> row(p.logits + r * p.stride, p.classes);
+  const int per = (row.vecs + parts - 1) / parts;
+  const int from = q * per, to = from + per < row.vecs ? from + per : row.vecs;
+  Stat<A> st = pass<false, T, A>(row, from + threadIdx.x, to, kPartBlock);
+  st = join_row<kPartBlock>(st, lds);
+  if (threadIdx.x == 0) part[blockIdx.x] = st;
+}
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(kPartBlock) void k_loss_join(Loss<T> p, int parts,
+                                                          const Stat<typename Wide<T>::type> *part) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>();
+  const long long r = GRAD ? blockIdx.x / parts : blockIdx.x;
+  const int q = GRAD ? (int)(blockIdx.x - r * parts) : 0;
+  const long long t = p.target(r);
+  const bool counts = p.counts(t);
+  // every wave joins the row's parts for itself
+  Stat<A> st{-__builtin_inf(), 0};
+  if (counts)
+    for (int i = threadIdx.x & 63; i < parts; i += 64) st = join(st, part[r * parts + i]);
+  st = join_row<64>(st, (Stat<A> *)nullptr);
+  if (q == 0 && threadIdx.x == 0) p.loss[r] = counts ? p.value(r, t, st.m, st.s) : (A)0;
+  if constexpr (GRAD) {
+    const Row<T> row(p.logits + r * p.stride, p.classes);
+    const int per = (row.vecs + parts - 1) / parts;
+    const int from = q * per, to = from + per < row.vecs ? from + per : row.vecs;
+    T *g = p.grad + r * p.classes;
+    const A w = p.factor(r), by = w / st.s;
+    for (int v = from + threadIdx.x; v < to; v += kPartBlock) {
+      Vec<T, V> o;
+      if (counts) {
+        o = grad_of<T, A>(row.template load<false>(v), st.m, by, w,
+                          t + row.head - (long long)v * V);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.e[k] = (T)0;
+      }
+      row.store(g, v, o);
+    }
+  }
+}
+
+template <typename T, int L, int K> int launch_held(const Loss<T> &p) {
+  const unsigned blocks = (unsigned)mmpi::ceil_div(p.rows, block_of<L>() / L);
+  hipLaunchKernelGGL((k_loss_held<T, L, K>), dim3(blocks), dim3(block_of<L>()), 0, mmpi::stream(), p);
+  return mmpi::check_launch("mmp_cross_entropy(held)");
+}
+template <typename T, int L, bool GRAD> int launch_pass(const Loss<T> &p) {
+  const unsigned blocks = (unsigned)mmpi::ceil_div(p.rows, block_of<L>() / L);
+  hipLaunchKernelGGL((k_loss_pass<T, L, GRAD>), dim3(blocks), dim3(block_of<L>()), 0,
+                     mmpi::stream(), p);
+  return mmpi::check_launch("mmp_cross_entropy(pass)");
+}
+
+// Temporaries from the library's stream-ordered pool, released on scope exit.
+struct Temp {
+  void *p = nullptr;
+  ~Temp() {
+    if (p) (void)mmp_free(p);
+  }
+  int get(size_t bytes) { return mmp_alloc(bytes ? bytes : 1, &p); }
+};
+
+template <typename T> int loss_impl(const Loss<T> &p) {
+  typedef typename Wide<T>::type A;
+  // Vectors of a row wherever it begins: one more than fit its length.
+  const int64_t vecs = p.classes / vec_of<T>() + 2;
+  const int64_t cus = mmpi::cu_count();
+  // Parts of at least 16 KiB, for about two workgroups a CU.
+  int64_t parts = 2 * cus / p.rows;
+  if (parts > vecs / 1024) parts = vecs / 1024;
+  if (parts >= 2) {
+    Temp part;
+    if (int st = part.get((size_t)(p.rows * parts) * sizeof(Stat<A>))) return st;
+    hipLaunchKernelGGL((k_loss_part<T>), dim3((unsigned)(p.rows * parts)), dim3(kPartBlock), 0,
+                       mmpi::stream(), p, (int)parts, (Stat<A> *)part.p);
+    if (int st = mmpi::check_launch("mmp_cross_entropy(part)")) return st;
+    if (p.grad)
+      hipLaunchKernelGGL((k_loss_join<T, true>), dim3((unsigned)(p.rows * parts)),
+                         dim3(kPartBlock), 0, mmpi::stream(), p, (int)parts,
+                         (const Stat<A> *)part.p);
+    else
+      hipLaunchKernelGGL((k_loss_join<T, false>), dim3((unsigned)p.rows), dim3(kPartBlock), 0,
+                         mmpi::stream(), p, (int)parts, (const Stat<A> *)part.p);
+    return mmpi::check_launch("mmp_cross_entropy(join)");
+  }
+  if (p.grad) {
+    if (vecs <= 8 * 4) return launch_held<T, 8, 4>(p);
+    if (vecs <= 64 * 4) return launch_held<T, 64, 4>(p);
+    if (vecs <= 256 * 4) return launch_held<T, 256, 4>(p);
+    if (vecs <= 512 * 4) return launch_held<T, 512, 4>(p);
+    if (vecs <= 512 * 8) return launch_held<T, 512, 8>(p);
+    if (vecs <= 512 * 12) return launch_held<T, 512, 12>(p);
+    if (vecs <= 512 * 16) return launch_held<T, 512, 16>(p);
+    if (vecs <= 1024 * 12) return launch_held<T, 1024, 12>(p);
+    if (vecs <= 1024 * 16) return launch_held<T, 1024, 16>(p);
+    return launch_pass<T, 1024, true>(p);
+  }
+  if (vecs <= 8 * 4) return launch_pass<T, 8, false>(p);
+  if (vecs <= 64 * 16) return launch_pass<T, 64, false>(p);
+  return launch_pass<T, 256, false>(p);
+}
+
+constexpr int64_t kMost = 0x7fffffffLL;
 
 }  // namespace
 
@@ -91,15 +424,14 @@ extern "C" int mmp_cross_entropy(int dtype, int index_dtype, int64_t rows, int64
   if (rows == 0) return MMP_OK;
   if (classes == 0) return mmpi::fail(MMP_E_ARG, "mmp_cross_entropy: no classes");
   if (!logits || !targets || !loss) return mmpi::fail(MMP_E_ARG, "mmp_cross_entropy: null pointer");
-  if (!mmpi::grid_fits(rows, kBlock))
-    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: too many rows");
+  if (index_dtype != MMP_I32 && index_dtype != MMP_I64)
+    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: index dtype code %d", index_dtype);
+  if (!mmpi::grid_fits(rows, 1024) || classes > kMost - 64)
+    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: too many rows or classes");
   MMP_DISPATCH_FLOAT(dtype, "mmp_cross_entropy", {
-    MMP_DISPATCH_INDEX(index_dtype, "mmp_cross_entropy", {
-      typedef typename Wide<T>::type A;
-      hipLaunchKernelGGL((k_loss<T, I>), dim3((unsigned)rows), dim3(kBlock), 0, mmpi::stream(),
-                         (const T *)logits, (long long)classes, (long long)row_stride,
-                         (const I *)targets, (const A *)weight, scale, (A *)loss, (T *)grad);
-      return mmpi::check_launch("mmp_cross_entropy");
-    })
+    typedef typename Wide<T>::type A;
+    return loss_impl<T>(Loss<T>{(const T *)logits, (long long)rows, (long long)row_stride,
+                                (int)classes, index_dtype == MMP_I64, targets, (const A *)weight,
+                                scale, (A *)loss, (T *)grad});
   })
 }

@@ -50,6 +50,28 @@ __device__ __forceinline__ void store_vec(T *p, const Vec<T, N> &v) {
   }
 }
 
+// Vectors that are kept for a while are kept as words: as elements, a float16
+// vector that passes a branch takes a register for each of its halves.
+template <typename T, int N> __device__ __forceinline__ typename Vec<T, N>::Words words_of(const Vec<T, N> &v) {
+  static_assert(sizeof(T) * N % 4 == 0, "whole words");
+  return __builtin_bit_cast(typename Vec<T, N>::Words, v);
+}
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> elements_of(typename Vec<T, N>::Words w) {
+  return __builtin_bit_cast(Vec<T, N>, w);
+}
+
+// Words that the compiler takes for others from here on, so that it works out
+// again what it made of them before, where that is used again, instead of
+// keeping all of it (widened values first of all) in registers in between.
+template <typename W> __device__ __forceinline__ void forget(W &w) {
+#pragma unroll
+  for (unsigned k = 0; k < sizeof(W) / 4; ++k) {
+    unsigned u = w[k];
+    asm volatile("" : "+v"(u));
+    w[k] = u;
+  }
+}
+
 // exp(x) of x <= 0 or NaN in 32 bits: 2^(x log2 e) by the hardware's
 // exponential.  The product's rounding error, which grows with |x|, is carried
 // over to the result, so the relative error stays at a few units of the last

@@ -197,17 +197,6 @@ __device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) 
   }
 }
 
-// A value that the compiler takes for another one from here on, so that it
-// works out the gates again where they are used again instead of keeping
-// them (and what they were widened to) in registers over the wait.
-template <typename T, int V> __device__ __forceinline__ void forget(Vec<T, V> &v) {
-  unsigned w[sizeof(v) / 4];
-  __builtin_memcpy(w, &v, sizeof(v));
-#pragma unroll
-  for (unsigned k = 0; k < sizeof(v) / 4; ++k) asm volatile("" : "+v"(w[k]));
-  __builtin_memcpy(&v, w, sizeof(v));
-}
-
 // Where a workgroup is: `groups` sequences times channel groups, and in each
 // `tiles` tiles.  Early tiles have the low workgroup ids, which start first.
 struct Place {
@@ -368,40 +357,50 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
   const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
   const T *px = x.p + pl.seq * x.sb + t0 * x.st + ch;
   const T *ph = h.p + pl.seq * h.sb + (t0 - 1) * h.st + ch;
-  Vec<T, V> g[kSteps], d[kSteps], v[kSteps], before[kSteps];
+  typedef typename Vec<T, V>::Words Words;
+  Words wg[kSteps], wd[kSteps], wx[kSteps], wh[kSteps];
   if (count >= V && t0 >= kSteps) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      g[i] = mmpn::load_vec<T, V>(pg - i * gate.st);
-      d[i] = mmpn::load_vec<T, V>(pd - i * grad.st);
+      wg[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(pg - i * gate.st));
+      wd[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(pd - i * grad.st));
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      if constexpr (LOGITS) v[i] = mmpn::load_vec<T, V>(px - i * x.st);
-      before[i] = mmpn::load_vec<T, V>(ph - i * h.st);
+      if constexpr (LOGITS) wx[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(px - i * x.st));
+      wh[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(ph - i * h.st));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int n = t0 >= i ? count : 0;
-      g[i] = load_some<T, V>(pg - i * gate.st, n);
-      d[i] = load_some<T, V>(pd - i * grad.st, n);
-      if constexpr (LOGITS) v[i] = load_some<T, V>(px - i * x.st, n);
-      before[i] = load_some<T, V>(ph - i * h.st, t0 > i ? count : 0);
+      wg[i] = mmpn::words_of<T, V>(load_some<T, V>(pg - i * gate.st, n));
+      wd[i] = mmpn::words_of<T, V>(load_some<T, V>(pd - i * grad.st, n));
+      if constexpr (LOGITS) wx[i] = mmpn::words_of<T, V>(load_some<T, V>(px - i * x.st, n));
+      wh[i] = mmpn::words_of<T, V>(load_some<T, V>(ph - i * h.st, t0 > i ? count : 0));
+    }
+  }
+  A pa[V], pb[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    pa[k] = 1;
+    pb[k] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const Vec<T, V> g = mmpn::elements_of<T, V>(wg[i]), d = mmpn::elements_of<T, V>(wd[i]);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      A f, u;
+      factor<LOGITS>((A)g.e[k], (A)0, f, u);
+      pa[k] = f * pa[k];
+      pb[k] = f * ((A)d.e[k] + pb[k]);
     }
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    A a = 1, b = 0;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      A f, u;
-      factor<LOGITS>((A)g[i].e[k], (A)0, f, u);
-      a = f * a;
-      b = f * ((A)d[i].e[k] + b);
-    }
-    sa[s * CH + c + k] = a;
-    sb[s * CH + c + k] = b;
+    sa[s * CH + c + k] = pa[k];
+    sb[s * CH + c + k] = pb[k];
   }
   __syncthreads();
   if (tid < 64) {
@@ -448,29 +447,29 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
   const long long o0 = (pl.seq * steps + t0) * dim + ch;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    forget(g[i]);
-    forget(d[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
     if (t0 < i) break;
-    Vec<T, V> og, ox;
+    mmpn::forget(wg[i]);
+    mmpn::forget(wd[i]);
+    const Vec<T, V> g = mmpn::elements_of<T, V>(wg[i]), d = mmpn::elements_of<T, V>(wd[i]);
+    const Vec<T, V> before = mmpn::elements_of<T, V>(wh[i]);
+    Vec<T, V> v, og, ox;
+    if constexpr (LOGITS) v = mmpn::elements_of<T, V>(wx[i]);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      A hb = (A)before[i].e[k];
+      A hb = (A)before.e[k];
       if (t0 == i) hb = initial && k < count ? initial[pl.seq * dim + ch + k] : (A)0;
-      const A dd = (A)d[i].e[k] + carry[k];
+      const A dd = (A)d.e[k] + carry[k];
       if constexpr (LOGITS) {
         A f, u;
-        mmpn::sigmoid_pair((A)g[i].e[k], f, u);
+        mmpn::sigmoid_pair((A)g.e[k], f, u);
         const A du = dd * u;
-        og.e[k] = (T)(du * f * (hb - (A)v[i].e[k]));
+        og.e[k] = (T)(du * f * (hb - (A)v.e[k]));
         ox.e[k] = (T)du;
         carry[k] = f * dd;
       } else {
         og.e[k] = (T)(dd * hb);
         ox.e[k] = (T)dd;
-        carry[k] = (A)g[i].e[k] * dd;
+        carry[k] = (A)g.e[k] * dd;
       }
     }
     store_some<T, V>(grad_gate + o0 - (long long)i * dim, og, count);
