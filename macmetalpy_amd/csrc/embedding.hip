@@ -7,12 +7,13 @@
 // gradient, so ragged batches can be filled up with -1.  Sums are held in 32
 // bits (64 for float64) and rounded once.
 //
-// Both are bound by memory.  The gradient first orders the tokens' positions by
-// row, equal ones ascending, so that the sums keep their bits.  One pass of a
-// radix sort splits them into at most 256 groups of neighbouring rows (tiles of the
-// tokens count and then place their own, in order), and a workgroup orders a
-// group's by row with counters in LDS.  More than 2^20 rows are too many for those:
-// then every 8 bits of the row have a pass, from the lowest on.
+// Both are bound by memory.  The gradient first brings the tokens' positions of
+// each row together, ascending, so that the sums keep their bits.  One pass of a
+// radix sort splits them by the low 8 bits of the row (tiles of the tokens
+// count and then place their own, in order): low ones, because the frequent
+// words of a vocabulary are neighbours, and one group of half the tokens would
+// be one workgroup's.  That orders a group's by row with counters in LDS.  More than 2^20
+// rows are too many for those: then every 8 bits of the row have a pass.
 //
 // Then a few lanes sum a row's positions.  Words' frequencies are skewed: a row
 // of more than kWindow positions is summed in windows of kWindow places of the
@@ -61,8 +62,9 @@ __global__ __launch_bounds__(kBlock) void k_embed(const I *__restrict__ tokens, 
 }
 
 // ---------------------------------------------------------------- grouping
+constexpr int kWindow = 64;  // places of the order that are summed together
 constexpr int kDigits = 256, kMaxTiles = 256;
-constexpr int kSplitWaves = kBlock / 64;
+constexpr int kSplitBlock = 1024, kSplitWaves = kSplitBlock / 64;
 
 // A token's position and row.
 struct Entry {
@@ -94,87 +96,117 @@ __device__ __forceinline__ unsigned lanes_below(unsigned long long mask) {
   return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
                                    __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
 }
-// The lanes of `among` whose low `bits` bits of d are this lane's.
+// The lanes of `among` whose d, a number of `bits` bits, is this lane's: with a
+// ballot on each bit, unless it is the same for all.
 __device__ __forceinline__ unsigned long long lanes_alike(unsigned long long among, unsigned d,
                                                           int bits) {
-  for (int b = 0; b < bits; ++b) {
-    const bool one = (d >> b) & 1;
-    const unsigned long long m = __ballot(one);
-    among &= one ? m : ~m;
-  }
+  if (among == 0) return 0;
+  const int lead = __ffsll((long long)among) - 1;
+  if ((__ballot(d == (unsigned)__builtin_amdgcn_readlane((int)d, lead)) & among) == among)
+    return among;
+  for (int b0 = 0; b0 < bits; b0 += 4)  // bits above the number's are 0 for all
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int set = (int)(d << (31 - b0 - b)) >> 31;  // all ones or 0
+      among &= ~(__ballot(set) ^ (unsigned long long)(long long)set);
+    }
   return among;
+}
+
+// counters[d] += 1 for every lane of `among`, in a wave's own counters.  Lanes with
+// one d are counted together: as atomics they would queue (131,072 equal tokens
+// 186 us in k_group).
+__device__ __forceinline__ void tally(unsigned *counters, bool there, unsigned d, int bits) {
+  const unsigned long long same = lanes_alike(__ballot(there), d, bits);
+  if (there && lanes_below(same) == 0) counters[d] += (unsigned)__popcll(same);
 }
 
 // count[t][d]: entries of tile t with digit d = row >> shift & 255.
 template <typename S>
-__global__ __launch_bounds__(kBlock) void k_split_count(S src, unsigned tile_len, int shift,
-                                                        unsigned *__restrict__ count) {
-  __shared__ unsigned h[kDigits];
-  h[threadIdx.x] = 0;
+__global__ __launch_bounds__(kSplitBlock) void k_split_count(S src, unsigned tile_len, int shift,
+                                                             unsigned *__restrict__ count) {
+  __shared__ unsigned h[kSplitWaves][kDigits];
+  const int tid = threadIdx.x, wave = tid >> 6;
+  for (int k = tid; k < kSplitWaves * kDigits; k += kSplitBlock) h[0][k] = 0;
   __syncthreads();
   const unsigned n = src.count();
   const unsigned from = blockIdx.x * tile_len < n ? blockIdx.x * tile_len : n;
   const unsigned to = n - from < tile_len ? n : from + tile_len;
-#pragma unroll 4
-  for (unsigned i = from + threadIdx.x; i < to; i += kBlock) {
-    Entry e;
-    if (src.get(i, e)) atomicAdd(&h[e.row >> shift & (kDigits - 1)], 1u);
+  for (unsigned i0 = from; i0 < to; i0 += kSplitBlock) {
+    Entry e{0, 0};
+    const bool there = i0 + tid < to && src.get(i0 + tid, e);
+    tally(h[wave], there, e.row >> shift & (kDigits - 1), 8);
   }
   __syncthreads();
-  count[blockIdx.x * kDigits + threadIdx.x] = h[threadIdx.x];
+  if (tid < kDigits) {
+    unsigned c = 0;
+    for (int w = 0; w < kSplitWaves; ++w) c += h[w][tid];
+    count[blockIdx.x * kDigits + tid] = c;
+  }
 }
 
 // Places the entries by digit, otherwise in order; first[d] is where digit d
 // begins, and first[256] the number of all.  Every workgroup adds up the
-// counts of the tiles before its own.
+// counts of the tiles before its own, four threads a digit.
 template <typename S>
-__global__ __launch_bounds__(kBlock) void k_split(S src, unsigned tile_len, int shift,
-                                                  const unsigned *__restrict__ count,
-                                                  unsigned *__restrict__ first,
-                                                  Entry *__restrict__ out) {
+__global__ __launch_bounds__(kSplitBlock) void k_split(S src, unsigned tile_len, int shift,
+                                                       const unsigned *__restrict__ count,
+                                                       unsigned *__restrict__ first,
+                                                       Entry *__restrict__ out) {
+  constexpr int kEach = kSplitBlock / kDigits;
   __shared__ unsigned next[kSplitWaves][kDigits];
-  __shared__ unsigned part[kSplitWaves];
+  __shared__ unsigned sums[2][kEach][kDigits], part[kDigits / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int w = 0; w < kSplitWaves; ++w) next[w][tid] = 0;
+  for (int k = tid; k < kSplitWaves * kDigits; k += kSplitBlock) next[0][k] = 0;
   const unsigned n = src.count();
-  const unsigned quarter = tile_len / kSplitWaves, tile = blockIdx.x * tile_len;
-  unsigned from = tile + wave * quarter;
+  const unsigned piece = tile_len / kSplitWaves;
+  unsigned from = blockIdx.x * tile_len + wave * piece;
   from = from < n ? from : n;
-  const unsigned to = n - from < quarter ? n : from + quarter;
-  unsigned before = 0, total = 0;
-#pragma unroll 8
-  for (unsigned t = 0; t < gridDim.x; ++t) {
-    const unsigned c = count[t * kDigits + tid];
-    before += t < blockIdx.x ? c : 0;
-    total += c;
+  const unsigned to = n - from < piece ? n : from + piece;
+  {
+    const int d = tid & (kDigits - 1);
+    unsigned before = 0, total = 0;
+#pragma unroll 16
+    for (unsigned t = tid / kDigits; t < gridDim.x; t += kEach) {
+      const unsigned c = count[t * kDigits + d];
+      before += t < blockIdx.x ? c : 0;
+      total += c;
+    }
+    sums[0][tid / kDigits][d] = before;
+    sums[1][tid / kDigits][d] = total;
   }
   __syncthreads();
-#pragma unroll 4
-  for (unsigned i = from + lane; i < to; i += 64) {
-    Entry e;
-    if (src.get(i, e)) atomicAdd(&next[wave][e.row >> shift & (kDigits - 1)], 1u);
+  for (unsigned i0 = from; i0 < to; i0 += 64) {
+    Entry e{0, 0};
+    const bool there = i0 + lane < to && src.get(i0 + lane, e);
+    tally(next[wave], there, e.row >> shift & (kDigits - 1), 8);
   }
-  unsigned incl = total;
+  unsigned total = 0, incl = 0;
+  if (tid < kDigits) {
+    for (int k = 0; k < kEach; ++k) total += sums[1][k][tid];
+    incl = total;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const unsigned o = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += o;
+    for (int d = 1; d < 64; d <<= 1) {
+      const unsigned o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += o;
+    }
+    if (lane == 63) part[wave] = incl;
   }
-  if (lane == 63) part[wave] = incl;
   __syncthreads();
-  unsigned at = incl - total;
-  for (int w = 0; w < wave; ++w) at += part[w];
-  if (blockIdx.x == 0) {
-    first[tid] = at;
-    if (tid == kDigits - 1) first[kDigits] = at + total;
-  }
-  at += before;
+  if (tid < kDigits) {
+    unsigned at = incl - total;
+    for (int w = 0; w < wave; ++w) at += part[w];
+    if (blockIdx.x == 0) {
+      first[tid] = at;
+      if (tid == kDigits - 1) first[kDigits] = at + total;
+    }
+    for (int k = 0; k < kEach; ++k) at += sums[0][k][tid];
 #pragma unroll
-  for (int w = 0; w < kSplitWaves; ++w) {
-    const unsigned c = next[w][tid];
-    next[w][tid] = at;
-    at += c;
+    for (int w = 0; w < kSplitWaves; ++w) {
+      const unsigned c = next[w][tid];
+      next[w][tid] = at;
+      at += c;
+    }
   }
   __syncthreads();
   for (unsigned i0 = from; i0 < to; i0 += 64) {
@@ -191,18 +223,22 @@ __global__ __launch_bounds__(kBlock) void k_split(S src, unsigned tile_len, int 
   }
 }
 
-// Workgroup g orders group g, rows [g << bits, (g + 1) << bits), by row.
-// order: the positions; start[v]: where row v's begin, start[rows] their number.
-constexpr int kGroupBlock = 512, kGroupRows = 4096;
+// A row's positions in the order.
+struct Span {
+  unsigned from, to;
+};
+
+// Workgroup g orders group g, the rows v with v % 256 = g, by v / 256: order has
+// the positions, span the rows' places in it.
+constexpr int kGroupBlock = 1024, kGroupRows = 4096;
 __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__ entries,
                                                        const unsigned *__restrict__ first,
-                                                       unsigned rows, int bits, int waves,
-                                                       unsigned *__restrict__ start,
+                                                       unsigned rows, unsigned bins, int bits,
+                                                       int waves, Span *__restrict__ span,
                                                        unsigned *__restrict__ order) {
-  extern __shared__ unsigned next[];  // [waves][1 << bits]
+  extern __shared__ unsigned next[];  // [waves][bins]
   __shared__ unsigned part[kGroupBlock / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const unsigned bins = 1u << bits, row0 = blockIdx.x << bits;
   for (unsigned k = tid; k < waves * bins; k += kGroupBlock) next[k] = 0;
   const unsigned base = first[blockIdx.x], n = first[blockIdx.x + 1] - base;
   const unsigned per = (n + waves * 64 - 1) / (waves * 64) * 64;
@@ -211,9 +247,17 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__
   const unsigned to = n - from < per ? n : from + per;
   unsigned *mine = next + wave * bins;
   __syncthreads();
-#pragma unroll 4
-  for (unsigned i = from + lane; i < to; i += 64)
-    atomicAdd(&mine[entries[base + i].row - row0], 1u);
+  constexpr int kLoads = 4;
+  for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
+    unsigned row[kLoads];
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      const unsigned i = i0 + l * 64 + lane;
+      row[l] = entries[base + (i < to ? i : from)].row;
+    }
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) tally(mine, i0 + l * 64 + lane < to, row[l] / kDigits, bits);
+  }
   __syncthreads();
   // exclusive sums over the rows, neighbouring ones a thread's, and within a
   // row over the waves
@@ -232,48 +276,59 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__
   unsigned at = base + incl - total;
   for (int w = 0; w < wave; ++w) at += part[w];
   for (unsigned k = tid * mult; k < (tid + 1) * mult && k < bins; ++k) {
-    if (row0 + k < rows) start[row0 + k] = at;
+    const unsigned begin = at, v = k * kDigits + blockIdx.x;
     for (int w = 0; w < waves; ++w) {
       const unsigned c = next[w * bins + k];
       next[w * bins + k] = at;
       at += c;
     }
-    if (row0 + k == rows - 1) start[rows] = at;
+    if (v < rows) span[v] = {begin, at};
   }
   __syncthreads();
-  for (unsigned i0 = from; i0 < to; i0 += 64) {
-    const bool there = i0 + lane < to;
-    const Entry e = entries[base + (there ? i0 + lane : from)];
-    const unsigned k = e.row - row0;
-    const unsigned long long same = lanes_alike(__ballot(there), k, bits);
-    const unsigned rank = lanes_below(same);
-    if (there) {
-      const unsigned o = mine[k];
-      order[o + rank] = e.at;
-      if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
+  for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
+    Entry e[kLoads];
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      const unsigned i = i0 + l * 64 + lane;
+      e[l] = entries[base + (i < to ? i : from)];
+    }
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      const bool there = i0 + l * 64 + lane < to;
+      const unsigned k = e[l].row / kDigits;
+      const unsigned long long same = lanes_alike(__ballot(there), k, bits);
+      const unsigned rank = lanes_below(same);
+      if (there) {
+        const unsigned o = mine[k];
+        order[o + rank] = e[l].at;
+        if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
+      }
     }
   }
 }
 
-// From entries in the order of their rows: start and order as above.
+// From entries in the order of their rows: the same.
 __global__ __launch_bounds__(kBlock) void k_starts(const Entry *__restrict__ entries,
                                                    const unsigned *__restrict__ count,
-                                                   unsigned rows, unsigned *__restrict__ start,
+                                                   unsigned rows, Span *__restrict__ span,
                                                    unsigned *__restrict__ order) {
   const unsigned i = blockIdx.x * kBlock + threadIdx.x, n = *count;
   if (i < n) order[i] = entries[i].at;
-  if (i > rows) return;
-  unsigned lo = 0, hi = n;  // the first entry of row i or a later one
-  while (lo < hi) {
-    const unsigned mid = lo + (hi - lo) / 2;
-    if (entries[mid].row < i) lo = mid + 1;
-    else hi = mid;
-  }
-  start[i] = lo;
+  if (i >= rows) return;
+  auto begin_of = [&](unsigned row) {  // the first entry of a row or a later one
+    unsigned lo = 0, hi = n;
+    while (lo < hi) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (entries[mid].row < row) lo = mid + 1;
+      else hi = mid;
+    }
+    return lo;
+  };
+  span[i] = {begin_of(i), begin_of(i + 1)};
 }
 
 // ---------------------------------------------------------------- row sums
-constexpr int kWindow = 64;
+constexpr int kInFlight = 4;  // vectors of a thread that are added, and as many on their way
 
 // sum += the vectors at column `at` of the rows that `from` to `to` of the order
 // name, one after another.  The next kLoads vectors are on their way while as
@@ -316,66 +371,74 @@ __device__ __forceinline__ void add_rows(A (&sum)[V], const T *__restrict__ grad
 
 // Window w of the order: the sums of its pieces of rows of more than kWindow
 // positions, part[2 w] of one that began before it and part[2 w + 1] of one
-// that begins in it.
+// that begins in it; begins[w] is that row, or -1.
 template <typename T, typename I, int V>
-__global__ __launch_bounds__(kBlock) void k_window_sums(const I *__restrict__ tokens,
-                                                        const T *__restrict__ grad, long long stride,
-                                                        long long rows, int dim, int lanes,
-                                                        unsigned windows,
-                                                        const unsigned *__restrict__ start,
-                                                        const unsigned *__restrict__ order,
-                                                        typename Wide<T>::type *__restrict__ part) {
+__device__ __forceinline__ void window_sums(const I *__restrict__ tokens, const T *__restrict__ grad,
+                                            long long stride, unsigned total, int dim, int lanes,
+                                            unsigned w, const Span *__restrict__ span,
+                                            const unsigned *__restrict__ order,
+                                            typename Wide<T>::type *__restrict__ part,
+                                            int *__restrict__ begins) {
   typedef typename Wide<T>::type A;
-  const unsigned w = blockIdx.x * (kBlock / lanes) + threadIdx.x / lanes;
-  const unsigned total = start[rows];
-  if (w >= windows || w * (unsigned)kWindow >= total) return;
   const unsigned p0 = w * kWindow, p1 = total - p0 < kWindow ? total : p0 + kWindow;
-#pragma unroll
+#pragma unroll 1
   for (int piece = 0; piece < 2; ++piece) {
     const long long r = (long long)tokens[order[piece ? p1 - 1 : p0]];
-    const unsigned from = start[r], to = start[r + 1];
-    if (to - from <= kWindow || (from >= p0) != (piece == 1)) continue;
+    const unsigned from = span[r].from, to = span[r].to;
+    const bool mine = to - from > kWindow && (from >= p0) == (piece == 1);
+    if (piece == 1 && (threadIdx.x & (lanes - 1)) == 0) begins[w] = mine ? (int)r : -1;
+    if (!mine) continue;
     for (int c = (threadIdx.x & (lanes - 1)) * V; c < dim; c += lanes * V) {
       const int at = c + V > dim ? dim - V : c;
       A sum[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) sum[k] = 0;
-      add_rows<T, V, 8, A>(sum, grad, stride, order, from > p0 ? from : p0, to < p1 ? to : p1, at);
-      A *dst = part + (2ll * w + piece) * dim + at;
+      add_rows<T, V, kInFlight, A>(sum, grad, stride, order, from > p0 ? from : p0,
+                                   to < p1 ? to : p1, at);
+      Vec<A, V> o;
 #pragma unroll
-      for (int k = 0; k < V; ++k) dst[k] = sum[k];
+      for (int k = 0; k < V; ++k) o.e[k] = sum[k];
+      mmpn::store_vec<A, V>(part + (2ll * w + piece) * dim + at, o);
     }
   }
 }
 
-// Rows of the gradient: kRows for `lanes` threads.  Those of up to kFirst
-// positions, most of them, are read all at once (one after another they would
-// wait for their order, then for their vectors), then the longer ones; one in
-// windows is the whole workgroup's.
+// The first `window_blocks` workgroups sum windows (the longest work starts
+// first).  The others have kRows rows of the gradient for `lanes` threads: those
+// of up to kFirst positions, most of them, are read all at once (one
+// after another they would wait for their order, then for their vectors), then
+// those of up to a window.
 constexpr int kRows = 4, kFirst = 2;
-template <typename T, int V>
+template <typename T, typename I, int V>
 __global__ __launch_bounds__(kBlock) void k_row_sums(
-    const T *__restrict__ grad, long long stride, long long rows, int dim, int lanes,
-    typename Wide<T>::type scale, const unsigned *__restrict__ start,
-    const unsigned *__restrict__ order, const typename Wide<T>::type *__restrict__ part,
-    T *__restrict__ out) {
+    const I *__restrict__ tokens, const T *__restrict__ grad, long long stride, long long rows,
+    int dim, int lanes, typename Wide<T>::type scale, unsigned window_blocks,
+    const Span *__restrict__ span, const unsigned *__restrict__ count,
+    const unsigned *__restrict__ order, typename Wide<T>::type *__restrict__ part,
+    int *__restrict__ begins, T *__restrict__ out) {
   typedef typename Wide<T>::type A;
-  __shared__ A lds[kBlock * V];
-  __shared__ int long_rows[kBlock * kRows], count;
   const int per = kBlock / lanes, g = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
-  const long long v0 = (long long)blockIdx.x * per * kRows;
-  if (threadIdx.x == 0) count = 0;
-  __syncthreads();
-  const long long v = v0 + g * kRows;
+  if (blockIdx.x < window_blocks) {
+    const unsigned w = blockIdx.x * per + g, total = *count;
+    if ((unsigned long long)w * kWindow < total)
+      window_sums<T, I, V>(tokens, grad, stride, total, dim, lanes, w, span, order, part,
+                              begins);
+    return;
+  }
+  const long long v = ((long long)(blockIdx.x - window_blocks) * per + g) * kRows;
   {
-    unsigned edge[kRows + 1], id[kRows][kFirst];
+    Span p[kRows];
+    unsigned id[kRows][kFirst];
 #pragma unroll
-    for (int r = 0; r <= kRows; ++r) edge[r] = start[v + r < rows ? v + r : rows];
+    for (int r = 0; r < kRows; ++r) {
+      p[r] = {0, kWindow + 1};  // not one of these rows
+      if (v + r < rows) p[r] = span[v + r];
+    }
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
       for (int i = 0; i < kFirst; ++i)
-        if (edge[r] + i < edge[r + 1]) id[r][i] = order[edge[r] + i];
+        if (p[r].from + i < p[r].to && p[r].to - p[r].from <= kFirst) id[r][i] = order[p[r].from + i];
     for (int c = lane * V; c < dim; c += lanes * V) {
       const int at = c + V > dim ? dim - V : c;
       Vec<T, V> x[kRows][kFirst];
@@ -383,7 +446,7 @@ __global__ __launch_bounds__(kBlock) void k_row_sums(
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int i = 0; i < kFirst; ++i)
-          if (edge[r] + i < edge[r + 1] && edge[r + 1] - edge[r] <= kFirst)
+          if (p[r].from + i < p[r].to && p[r].to - p[r].from <= kFirst)
             x[r][i] = mmpn::load_vec<T, V, true>(grad + (long long)id[r][i] * stride + at);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
@@ -392,71 +455,93 @@ __global__ __launch_bounds__(kBlock) void k_row_sums(
         for (int k = 0; k < V; ++k) sum[k] = 0;
 #pragma unroll
         for (int i = 0; i < kFirst; ++i)
-          if (edge[r] + i < edge[r + 1]) {
+          if (p[r].from + i < p[r].to) {
 #pragma unroll
             for (int k = 0; k < V; ++k) sum[k] += (A)x[r][i].e[k];
           }
         Vec<T, V> o;
 #pragma unroll
         for (int k = 0; k < V; ++k) o.e[k] = (T)(sum[k] * scale);
-        if (v + r < rows && edge[r + 1] - edge[r] <= kFirst)
+        if (p[r].to - p[r].from <= kFirst)
           mmpn::store_vec<T, V, true>(out + (v + r) * dim + at, o);
       }
     }
   }
 #pragma unroll 1
   for (int r = 0; r < kRows && v + r < rows; ++r) {
-    const unsigned from = start[v + r], to = start[v + r + 1];
-    if (to - from <= kFirst) continue;
-    if (to - from > kWindow) {
-      if (lane == 0) long_rows[atomicAdd(&count, 1)] = g * kRows + r;
-      continue;
-    }
+    const unsigned from = span[v + r].from, to = span[v + r].to;
+    if (to - from <= kFirst || to - from > kWindow) continue;
     for (int c = lane * V; c < dim; c += lanes * V) {
       const int at = c + V > dim ? dim - V : c;
       A sum[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) sum[k] = 0;
-      add_rows<T, V, 4, A>(sum, grad, stride, order, from, to, at);
+      add_rows<T, V, kInFlight, A>(sum, grad, stride, order, from, to, at);
       Vec<T, V> o;
 #pragma unroll
       for (int k = 0; k < V; ++k) o.e[k] = (T)(sum[k] * scale);
       mmpn::store_vec<T, V, true>(out + (v + r) * dim + at, o);
     }
   }
+}
+
+// The rows in windows, of those that begin in kLongWindows windows kLongCols
+// columns a workgroup, whose threads add up windows in kLongParts parts.
+constexpr int kLongWindows = 32, kLongCols = 64, kLongParts = 16;
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_long_rows(
+    int dim, typename Wide<T>::type scale, const Span *__restrict__ span,
+    const unsigned *__restrict__ count, const typename Wide<T>::type *__restrict__ part,
+    const int *__restrict__ begins, T *__restrict__ out) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = kLongCols * kLongParts / kBlock;  // columns of a thread
+  __shared__ A lds[kLongParts][kLongCols];
+  __shared__ unsigned long long there;
+  __shared__ int row_of[kLongWindows];
+  const int c = (threadIdx.x % (kLongCols / V)) * V, g = threadIdx.x / (kLongCols / V);
+  const unsigned chunks = (dim + kLongCols - 1) / kLongCols;
+  const unsigned first = blockIdx.x / chunks * kLongWindows;
+  const int c0 = (int)(blockIdx.x % chunks) * kLongCols;
+  if (threadIdx.x < 64) {
+    const unsigned w = first + threadIdx.x;
+    int v = -1;
+    if (threadIdx.x < kLongWindows && (unsigned long long)w * kWindow < *count) v = begins[w];
+    const unsigned long long m = __ballot(v >= 0);
+    if (v >= 0) row_of[threadIdx.x] = v;
+    if (threadIdx.x == 0) there = m;
+  }
   __syncthreads();
-  const int n = count;
-  for (int q = 0; q < n; ++q) {
-    const long long v = v0 + long_rows[q];
-    const unsigned w0 = start[v] / kWindow, w1 = (start[v + 1] - 1) / kWindow;
-    for (int c0 = 0; c0 < dim; c0 += lanes * V) {
-      const int c = c0 + lane * V, at = c + V > dim ? dim - V : c;
-      A sum[V];
+  for (unsigned long long left = there; left; left &= left - 1) {
+    const long long v = row_of[__ffsll((long long)left) - 1];
+    const unsigned w0 = span[v].from / kWindow, w1 = (span[v].to - 1) / kWindow;
+    const unsigned each = (w1 - w0 + kLongParts) / kLongParts;
+    const unsigned from = w0 + g * each, to = from + each < w1 + 1 ? from + each : w1 + 1;
+    A sum[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) sum[k] = 0;
-      if (c < dim) {
-#pragma unroll 4
-        for (unsigned w = w0 + g; w <= w1; w += per) {
-          const A *src = part + (2ll * w + (w == w0)) * dim + at;
+    for (int k = 0; k < V; ++k) sum[k] = 0;
+    if (c0 + c + V <= dim) {
+#pragma unroll 8
+      for (unsigned w = from; w < to; ++w) {
+        const Vec<A, V> x = mmpn::load_vec<A, V>(part + (2ll * w + (w == w0)) * dim + c0 + c);
 #pragma unroll
-          for (int k = 0; k < V; ++k) sum[k] += src[k];
-        }
+        for (int k = 0; k < V; ++k) sum[k] += x.e[k];
       }
+    } else {
+      for (unsigned w = from; w < to; ++w)
 #pragma unroll
-      for (int k = 0; k < V; ++k) lds[(g * lanes + lane) * V + k] = sum[k];
-      __syncthreads();
-      if (g == 0 && c < dim) {
-        Vec<T, V> r;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          A s = 0;
-          for (int o = 0; o < per; ++o) s += lds[(o * lanes + lane) * V + k];
-          r.e[k] = (T)(s * scale);
-        }
-        mmpn::store_vec<T, V, true>(out + v * dim + at, r);
-      }
-      __syncthreads();
+        for (int k = 0; k < V; ++k)
+          if (c0 + c + k < dim) sum[k] += part[(2ll * w + (w == w0)) * dim + c0 + c + k];
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k) lds[g][c + k] = sum[k];
+    __syncthreads();
+    if (threadIdx.x < kLongCols && c0 + (int)threadIdx.x < dim) {
+      A s = 0;
+#pragma unroll
+      for (int o = 0; o < kLongParts; ++o) s += lds[o][threadIdx.x];
+      out[v * dim + c0 + threadIdx.x] = (T)(s * scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -481,44 +566,42 @@ constexpr int64_t kMost = 0x7fffffffLL;
 // Orders the tokens' positions by row; ea, eb: room for n entries each.
 template <typename I>
 int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *eb, unsigned *count,
-                 unsigned *first, unsigned *start, unsigned *order) {
+                 unsigned *first, Span *span, unsigned *order) {
   // up to 256 tiles of at least 1024 tokens, which every workgroup of k_split
   // adds up
-  unsigned tile = (unsigned)(mmpi::ceil_div(mmpi::ceil_div(n, kMaxTiles), 256) * 256);
-  if (tile < 1024) tile = 1024;
+  const unsigned tile = n == 0 ? 1024 : (unsigned)(mmpi::ceil_div(mmpi::ceil_div(n, kMaxTiles), 1024) * 1024);
   const unsigned tiles = n ? (unsigned)mmpi::ceil_div(n, tile) : 1;
   auto pass = [&](auto src, int shift, Entry *out) -> int {
     typedef decltype(src) S;
-    hipLaunchKernelGGL((k_split_count<S>), dim3(tiles), dim3(kBlock), 0, mmpi::stream(), src, tile,
-                       shift, count);
+    hipLaunchKernelGGL((k_split_count<S>), dim3(tiles), dim3(kSplitBlock), 0, mmpi::stream(),
+                       src, tile, shift, count);
     if (int st = mmpi::check_launch("mmp_embedding_grad(count)")) return st;
-    hipLaunchKernelGGL((k_split<S>), dim3(tiles), dim3(kBlock), 0, mmpi::stream(), src, tile,
-                       shift, (const unsigned *)count, first, out);
+    hipLaunchKernelGGL((k_split<S>), dim3(tiles), dim3(kSplitBlock), 0, mmpi::stream(), src,
+                       tile, shift, (const unsigned *)count, first, out);
     return mmpi::check_launch("mmp_embedding_grad(split)");
   };
-  int bits = 0;
-  while ((rows - 1) >> bits) ++bits;  // of a row
   if (rows <= (unsigned)kDigits * kGroupRows) {
-    const int low = bits > 8 ? bits - 8 : 0;
-    if (int st = pass(Tokens<I>{tokens, n, rows}, low, ea)) return st;
-    const unsigned groups = ((rows - 1) >> low) + 1;
-    const int waves = low > 11 ? 4 : 8;  // 64 KiB of counters at most
-    hipLaunchKernelGGL(k_group, dim3(groups), dim3(kGroupBlock), (unsigned)(waves * 4) << low,
-                       mmpi::stream(), (const Entry *)ea, (const unsigned *)first, rows, low, waves,
-                       start, order);
+    if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
+    const unsigned bins = (unsigned)mmpi::ceil_div(rows, kDigits);
+    int bits = 0;
+    while ((bins - 1) >> bits) ++bits;
+    const int waves = bins > 2048 ? 4 : bins > 1024 ? 8 : 16;  // 64 KiB of counters at most
+    hipLaunchKernelGGL(k_group, dim3(rows < kDigits ? rows : kDigits), dim3(kGroupBlock),
+                       (unsigned)waves * bins * 4, mmpi::stream(), (const Entry *)ea,
+                       (const unsigned *)first, rows, bins, bits, waves, span, order);
     return mmpi::check_launch("mmp_embedding_grad(group)");
   }
   if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
-  for (int shift = 8; shift < bits; shift += 8) {
+  for (int shift = 8; (rows - 1) >> shift; shift += 8) {
     if (int st = pass(Entries{ea, first + kDigits}, shift, eb)) return st;
     Entry *t = ea;
     ea = eb;
     eb = t;
   }
-  const unsigned most = n > rows + 1 ? n : rows + 1;
+  const unsigned most = n > rows ? n : rows;
   hipLaunchKernelGGL(k_starts, dim3((unsigned)mmpi::ceil_div(most, kBlock)), dim3(kBlock), 0,
                      mmpi::stream(), (const Entry *)ea, (const unsigned *)(first + kDigits), rows,
-                     start, order);
+                     span, order);
   return mmpi::check_launch("mmp_embedding_grad(starts)");
 }
 
@@ -527,37 +610,42 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
               double scale, T *out) {
   typedef typename Wide<T>::type A;
   constexpr int V = 16 / sizeof(T);
-  Temp order, start, part, entries, counts;
+  Temp order, spans, part, entries, counts;
   const bool twice = rows > (int64_t)kDigits * kGroupRows;
   if (int st = order.get((size_t)n * 4)) return st;
-  if (int st = start.get((size_t)(rows + 1) * 4)) return st;
+  if (int st = spans.get((size_t)rows * sizeof(Span))) return st;
   if (int st = entries.get((size_t)n * sizeof(Entry) * (twice ? 2 : 1))) return st;
-  if (int st = counts.get((size_t)(kMaxTiles * kDigits + kDigits + 1) * 4)) return st;
-  unsigned *count = (unsigned *)counts.p;
+  const int64_t windows = n > kWindow ? mmpi::ceil_div(n, kWindow) : 0;
+  // counts of tiles, beginnings of groups, rows that begin in windows
+  if (int st = counts.get((size_t)(kMaxTiles * kDigits + kDigits + 1 + windows) * 4)) return st;
+  unsigned *count = (unsigned *)counts.p, *first = count + kMaxTiles * kDigits;
+  int *begins = (int *)(first + kDigits + 1);
+  Span *span = (Span *)spans.p;
   if (int st = order_tokens<I>((unsigned)n, tokens, (unsigned)rows, (Entry *)entries.p,
-                               (Entry *)entries.p + n, count, count + kMaxTiles * kDigits,
-                               (unsigned *)start.p, (unsigned *)order.p))
+                               (Entry *)entries.p + n, count, first, span, (unsigned *)order.p))
     return st;
   const int vec = dim >= V ? V : 1;
   const int lanes = row_lanes(dim, vec);
-  const int64_t windows = mmpi::ceil_div(n, kWindow);
-  const int64_t blocks = mmpi::ceil_div(rows, kBlock / lanes * kRows);
   const int64_t wblocks = mmpi::ceil_div(windows, kBlock / lanes);
-  if (!mmpi::grid_fits(blocks, kBlock) || !mmpi::grid_fits(wblocks, kBlock))
+  const int64_t blocks = mmpi::ceil_div(rows, kBlock / lanes * kRows) + wblocks;
+  if (!mmpi::grid_fits(blocks, kBlock))
     return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many rows or tokens");
-  if (n > kWindow) {
+  if (windows)
     if (int st = part.get((size_t)windows * 2 * dim * sizeof(A))) return st;
-    auto kernel = vec == V ? k_window_sums<T, I, V> : k_window_sums<T, I, 1>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)wblocks), dim3(kBlock), 0, mmpi::stream(), tokens,
-                       grad, (long long)stride, (long long)rows, dim, lanes, (unsigned)windows,
-                       (const unsigned *)start.p, (const unsigned *)order.p, (A *)part.p);
-    if (int st = mmpi::check_launch("mmp_embedding_grad(windows)")) return st;
-  }
-  auto kernel = vec == V ? k_row_sums<T, V> : k_row_sums<T, 1>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), grad,
-                     (long long)stride, (long long)rows, dim, lanes, (A)scale,
-                     (const unsigned *)start.p, (const unsigned *)order.p, (const A *)part.p, out);
-  return mmpi::check_launch("mmp_embedding_grad");
+  auto kernel = vec == V ? k_row_sums<T, I, V> : k_row_sums<T, I, 1>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), tokens, grad,
+                     (long long)stride, (long long)rows, dim, lanes, (A)scale, (unsigned)wblocks,
+                     (const Span *)span, (const unsigned *)first + kDigits,
+                     (const unsigned *)order.p, (A *)part.p, begins, out);
+  if (int st = mmpi::check_launch("mmp_embedding_grad")) return st;
+  if (!windows) return MMP_OK;
+  const int64_t lblocks = mmpi::ceil_div(windows, kLongWindows) * mmpi::ceil_div(dim, kLongCols);
+  if (!mmpi::grid_fits(lblocks, kBlock))
+    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many tokens and columns");
+  hipLaunchKernelGGL((k_long_rows<T>), dim3((unsigned)lblocks), dim3(kBlock), 0, mmpi::stream(),
+                     dim, (A)scale, (const Span *)span, (const unsigned *)first + kDigits,
+                     (const A *)part.p, (const int *)begins, out);
+  return mmpi::check_launch("mmp_embedding_grad(long)");
 }
 
 }  // namespace
