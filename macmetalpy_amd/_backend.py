@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+from array import array
 from typing import Optional, Sequence
 
 import numpy as np
@@ -135,8 +136,7 @@ _SIGNATURES = {
                            + [_c_vp] * 5,
     "mmp_cross_entropy": [_c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
                           ctypes.c_double, _c_vp, _c_vp],
-    "mmp_clip_norm": [_c_i64, ctypes.POINTER(_c_int), _c_i64p, ctypes.POINTER(_c_vp),
-                      ctypes.POINTER(_c_vp), ctypes.c_double, _c_int, _c_vp],
+    "mmp_clip_norm": [_c_i64, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_double, _c_int, _c_vp],
     "mmp_rtc_compile": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_c_vp)],
     "mmp_rtc_build": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _c_vp, _c_sz,
                       ctypes.POINTER(_c_sz)],
@@ -574,11 +574,11 @@ class HipBackend:
                "mmp_cross_entropy")
 
     def clip_norm(self, dcodes, sizes, arrays, outs, limit, norm_code, norm) -> None:
-        n = len(sizes)
-        ptrs = _c_vp * max(1, n)
-        _check(self._lib.mmp_clip_norm(n, (_c_int * max(1, n))(*dcodes), _i64_array(sizes),
-                                       ptrs(*arrays), None if outs is None else ptrs(*outs),
-                                       limit, norm_code, norm), "mmp_clip_norm")
+        lists = [array(kind, v) for kind, v in zip("iqQQ", (dcodes, sizes, arrays, outs or ()))]
+        at = [v.buffer_info()[0] for v in lists]
+        if outs is None:
+            at[3] = None
+        _check(self._lib.mmp_clip_norm(len(sizes), *at, limit, norm_code, norm), "mmp_clip_norm")
 
     # ------------------------------------------ reference kernel interface
     def execute_kernel(self, shader_src: str, func_name, grid_size, buffers) -> None:

@@ -23,6 +23,7 @@
 //    mmp_binary_scalar), else the generated fused kernel, looked up by the
 //    program's structure in a C++ table, with its parameter block packed
 //    here and launched through mmp_rtc_launch;
+//  * empty(shape, dtype): a device array to write results into;
 //  * DeviceBuffer: the owning handle of one device allocation, freed with
 //    mmp_free when the last reference goes.
 //
@@ -1620,6 +1621,55 @@ PyObject *gate_reduce(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return arr;
 }
 
+// ------------------------------------------------------------ empty
+// empty(shape, dtype): an uninitialised device array (ndarray._empty_device)
+// of a tuple of Python ints and one of the library's dtypes.
+PyObject *gate_empty(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  long long n = 0;
+  int dt = nargs == 2 ? dtype_index(args[1]) : -1;
+  for (int i = 0; nargs == 2 && dt < 0 && i < kNDT; ++i) {  // an equal dtype object
+    const int same = PyObject_RichCompareBool(dtypes[i], args[1], Py_EQ);
+    if (same < 0) return nullptr;
+    if (same) dt = i;
+  }
+  if (dt < 0 || !shape_size(args[0], &n)) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "empty(shape tuple, dtype)");
+    return nullptr;
+  }
+  if (!p_alloc) {
+    PyObject *r = PyObject_CallNoArgs(py_ensure_device);
+    if (!r) return nullptr;
+    Py_DECREF(r);
+    if (!p_alloc) {
+      PyErr_SetString(PyExc_RuntimeError, "the library is not bound");
+      return nullptr;
+    }
+  }
+  PyObject *buf = new_devbuf(n * itemsize[dt]);
+  PyObject *arr = buf ? T_ndarray->tp_alloc(T_ndarray, 0) : nullptr;
+  PyObject *d = arr ? PyDict_New() : nullptr;
+  PyObject *strides = d ? contig_strides(args[0]) : nullptr;
+  PyObject *zero = strides ? PyLong_FromLong(0) : nullptr;
+  bool bad = !zero;
+  if (!bad) {
+    *_PyObject_GetDictPtr(arr) = d;
+    bad = PyDict_SetItem(d, s_buffer, buf) || PyDict_SetItem(d, s_np_data, Py_None) ||
+          PyDict_SetItem(d, s_shape, args[0]) || PyDict_SetItem(d, s_dtype, dtypes[dt]) ||
+          PyDict_SetItem(d, s_strides, strides) || PyDict_SetItem(d, s_offset, zero) ||
+          PyDict_SetItem(d, s_base, Py_None) || PyDict_SetItem(d, s_fnode, Py_None);
+    d = nullptr;
+  }
+  Py_XDECREF(d);
+  Py_XDECREF(strides);
+  Py_XDECREF(zero);
+  Py_XDECREF(buf);
+  if (bad) {
+    Py_XDECREF(arr);
+    return nullptr;
+  }
+  return arr;
+}
+
 // ------------------------------------------------------------ setup
 PyObject *descr(PyObject *cls, const char *name) {
   PyObject *d = PyObject_GetAttrString(cls, name);
@@ -1823,6 +1873,8 @@ PyMethodDef methods[] = {
      "run_sum(root, axis_last, out_dtype, out_ptr, mean): fused sum epilogue."},
     {"reduce", (PyCFunction)(void (*)(void))gate_reduce, METH_FASTCALL,
      "reduce(code, x, axis): whole-array or last-axis reduction, or None."},
+    {"empty", (PyCFunction)(void (*)(void))gate_empty, METH_FASTCALL,
+     "empty(shape, dtype): an uninitialised device array."},
     {"stats", (PyCFunction)gate_stats, METH_NOARGS, "Counters of the native and fallback paths."},
     {"forget_dtypes", (PyCFunction)gate_forget_dtypes, METH_NOARGS,
      "Empty the result-dtype tables (after a float64 policy change)."},

@@ -14,7 +14,7 @@ namespace {
 using mmpn::Vec;
 using mmpn::Wide;
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256, kNormBlock = 1024;
 constexpr int kArrays = 64;  // of one launch: they go in the kernel's arguments
 
 struct Table {
@@ -36,41 +36,86 @@ __device__ __forceinline__ int array_of(const Table &t, unsigned chunk) {
   return lo;
 }
 
-__device__ __forceinline__ double block_sum(double s, double *lds) {
+template <int BLOCK> __device__ __forceinline__ double block_sum(double s, double *lds) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) s += __shfl_xor(s, m, 64);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
   double r = 0;
 #pragma unroll
-  for (int w = 0; w < kBlock / 64; ++w) r += lds[w];
+  for (int w = 0; w < BLOCK / 64; ++w) r += lds[w];
   return r;
 }
+
+// The elements of a chunk that are before the first address that is a multiple
+// of 16, then vectors of 16 bytes, then the rest.
+template <typename T> struct Chunk {
+  static constexpr int V = 16 / sizeof(T);
+  const T *x;
+  long long from, to;  // of the array
+  long long head, vecs;
+  int array;
+  __device__ __forceinline__ Chunk(const Table &t, unsigned chunk, long long chunk_len) {
+    array = array_of(t, chunk);
+    from = (long long)(chunk - t.first[array]) * chunk_len;
+    to = t.n[array] - from < chunk_len ? t.n[array] : from + chunk_len;
+    x = (const T *)t.in[array] + from;
+    const long long n = to - from;
+    head = (long long)((16 - ((uintptr_t)x & 15)) & 15) / (long long)sizeof(T);
+    head = head < n ? head : n;
+    vecs = (n - head) / V;
+  }
+};
+
+// A vector's squares.  float16's fit 32 bits without rounding; wider ones are
+// widened first.
+template <typename T> __device__ __forceinline__ double squares(const Vec<T, 16 / sizeof(T)> &v) {
+  double s = 0;
+#pragma unroll
+  for (int k = 0; k < (int)(16 / sizeof(T)); ++k) {
+    if constexpr (sizeof(T) == 2) s += (double)((float)v.e[k] * (float)v.e[k]);
+    else s = __builtin_fma((double)v.e[k], (double)v.e[k], s);
+  }
+  return s;
+}
+
+constexpr int kLoads = 8;  // vectors of a thread in flight
 
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_squares(Table t, long long chunk_len,
                                                     double *__restrict__ part) {
   __shared__ double lds[kBlock / 64];
-  const int a = array_of(t, blockIdx.x);
-  const long long from = (long long)(blockIdx.x - t.first[a]) * chunk_len;
-  const long long to = t.n[a] - from < chunk_len ? t.n[a] : from + chunk_len;
-  const T *x = (const T *)t.in[a];
+  const Chunk<T> c(t, blockIdx.x, chunk_len);
+  const T *x = c.x + c.head;
   double s = 0;
-  for (long long i = from + threadIdx.x; i < to; i += kBlock) {
-    const double v = (double)x[i];
+  long long i0 = threadIdx.x;
+  for (; i0 + (kLoads - 1) * kBlock < c.vecs; i0 += kLoads * kBlock) {
+    Vec<T, Chunk<T>::V> v[kLoads];
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) v[l] = mmpn::load_vec<T, Chunk<T>::V>(x + (i0 + l * kBlock) * Chunk<T>::V);
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) s += squares<T>(v[l]);
+  }
+  for (; i0 < c.vecs; i0 += kBlock) s += squares<T>(mmpn::load_vec<T, Chunk<T>::V>(x + i0 * Chunk<T>::V));
+  // at most 7 elements before the vectors and 7 after them
+  const long long rest = c.to - c.from - c.vecs * Chunk<T>::V;
+  if (threadIdx.x < rest) {
+    const double v = (double)c.x[threadIdx.x < c.head ? threadIdx.x : threadIdx.x + c.vecs * Chunk<T>::V];
     s = __builtin_fma(v, v, s);
   }
-  s = block_sum(s, lds);
+  s = block_sum<kBlock>(s, lds);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
 template <typename N>
-__global__ __launch_bounds__(kBlock) void k_norm(const double *__restrict__ part, long long n,
-                                                 N *__restrict__ norm, double *__restrict__ full) {
-  __shared__ double lds[kBlock / 64];
+__global__ __launch_bounds__(kNormBlock) void k_norm(const double *__restrict__ part, long long n,
+                                                     N *__restrict__ norm,
+                                                     double *__restrict__ full) {
+  __shared__ double lds[kNormBlock / 64];
   double s = 0;
-  for (long long i = threadIdx.x; i < n; i += kBlock) s += part[i];
-  s = sqrt(block_sum(s, lds));
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < n; i += kNormBlock) s += part[i];
+  s = sqrt(block_sum<kNormBlock>(s, lds));
   if (threadIdx.x == 0) {
     *norm = (N)s;
     *full = s;
@@ -81,15 +126,36 @@ template <typename T>
 __global__ __launch_bounds__(kBlock) void k_clip(Table t, long long chunk_len, double limit,
                                                  const double *__restrict__ norm) {
   typedef typename Wide<T>::type A;
-  const int a = array_of(t, blockIdx.x);
-  const long long from = (long long)(blockIdx.x - t.first[a]) * chunk_len;
-  const long long to = t.n[a] - from < chunk_len ? t.n[a] : from + chunk_len;
-  const T *x = (const T *)t.in[a];
-  T *y = (T *)t.out[a];
+  constexpr int V = Chunk<T>::V;
+  // backwards: what was summed last is the likeliest to be in a cache
+  const Chunk<T> c(t, gridDim.x - 1 - blockIdx.x, chunk_len);
+  const T *x = c.x + c.head;
+  T *y0 = (T *)t.out[c.array] + c.from, *y = y0 + c.head;
   const double n = *norm;
   // a norm that is NaN scales by NaN: a broken step shows
   const A by = (A)(n <= limit ? 1.0 : limit / n);
-  for (long long i = from + threadIdx.x; i < to; i += kBlock) y[i] = (T)((A)x[i] * by);
+  if (by == 1 && y0 == c.x) return;  // in place, and nothing to change
+  auto scaled = [&](const Vec<T, V> &v) {
+    Vec<T, V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.e[k] = (T)((A)v.e[k] * by);
+    return r;
+  };
+  long long i0 = threadIdx.x;
+  for (; i0 + (kLoads - 1) * kBlock < c.vecs; i0 += kLoads * kBlock) {
+    Vec<T, V> v[kLoads];
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) v[l] = mmpn::load_vec<T, V, true>(x + (i0 + l * kBlock) * V);
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) mmpn::store_vec<T, V, true>(y + (i0 + l * kBlock) * V, scaled(v[l]));
+  }
+  for (; i0 < c.vecs; i0 += kBlock)
+    mmpn::store_vec<T, V, true>(y + i0 * V, scaled(mmpn::load_vec<T, V, true>(x + i0 * V)));
+  const long long rest = c.to - c.from - c.vecs * V;
+  if (threadIdx.x < rest) {
+    const long long i = threadIdx.x < c.head ? threadIdx.x : threadIdx.x + c.vecs * V;
+    y0[i] = (T)((A)c.x[i] * by);
+  }
 }
 
 struct Temp {
@@ -121,8 +187,9 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
       return mmpi::fail(MMP_E_ARG, "mmp_clip_norm: null pointer");
     total += sizes[i];
   }
-  int64_t chunk = mmpi::ceil_div(total, 4096);
-  chunk = chunk < 4096 ? 4096 : mmpi::ceil_div(chunk, 1024) * 1024;
+  // About 4096 chunks, of 16,384 elements at least and whole rounds of a workgroup's vectors.
+  int64_t chunk = mmpi::ceil_div(mmpi::ceil_div(total, 4096), 16384) * 16384;
+  if (chunk == 0) chunk = 16384;
   int64_t chunks = 0;
   for (int64_t i = 0; i < count; ++i) chunks += mmpi::ceil_div(sizes[i], chunk);
   Temp part;
@@ -166,10 +233,10 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
     }
     if (pass == 1) break;
     if (norm_dtype == MMP_F32)
-      hipLaunchKernelGGL((k_norm<float>), dim3(1), dim3(kBlock), 0, mmpi::stream(),
+      hipLaunchKernelGGL((k_norm<float>), dim3(1), dim3(kNormBlock), 0, mmpi::stream(),
                          (const double *)sums, (long long)chunks, (float *)norm, full);
     else
-      hipLaunchKernelGGL((k_norm<double>), dim3(1), dim3(kBlock), 0, mmpi::stream(),
+      hipLaunchKernelGGL((k_norm<double>), dim3(1), dim3(kNormBlock), 0, mmpi::stream(),
                          (const double *)sums, (long long)chunks, (double *)norm, full);
     if (int st = mmpi::check_launch("mmp_clip_norm(norm)")) return st;
     if (!outs) break;

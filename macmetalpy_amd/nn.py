@@ -22,19 +22,25 @@ import math
 import numpy as np
 
 from . import _elementwise as ew
+from ._abi import DTYPE_CODES as _CODE
 from ._backend import HipBackend
-from ._dtypes import dtype_code
-from .ndarray import ndarray, _prod
+from ._native import empty as _empty
+from .ndarray import ndarray, _c_contiguous_strides, _prod
 
 __all__ = ["embedding", "embedding_grad", "gated_recurrence", "gated_recurrence_grad",
            "cross_entropy", "cross_entropy_grad", "global_norm", "clip_by_global_norm"]
 
 _F32, _F64, _I32, _I64 = (np.dtype(t) for t in (np.float32, np.float64, np.int32, np.int64))
 _FLOATS = frozenset((np.dtype(np.float16), _F32, _F64))
+# The type that sums and states are held in.
+_WIDE = {dt: _F64 if dt == _F64 else _F32 for dt in _FLOATS}
 
 
 def _device(a) -> ndarray:
-    if not isinstance(a, ndarray):
+    if type(a) is ndarray:
+        if a._fusion_node is None and a._np_data is None:
+            return a
+    elif not isinstance(a, ndarray):
         from .creation import asarray
         a = asarray(a)
     return a._ensure_gpu()
@@ -47,25 +53,19 @@ def _floating(a, what) -> ndarray:
     return a
 
 
-def _wide(dtype):
-    """The type that sums and states of ``dtype`` are held in."""
-    return _F64 if dtype == _F64 else _F32
+def _contiguous(a, dtype) -> ndarray:
+    if a._dtype != dtype:
+        return a._contiguous_copy(dtype)
+    return a if a._strides == _c_contiguous_strides(a._shape) else a._contiguous_copy()
 
 
 def _integers(a, what) -> ndarray:
     """Contiguous int32 or int64 indices."""
     a = _device(a)
-    if a._dtype.kind not in "iu":
-        raise TypeError(f"{what} must be integers, not {a._dtype}")
-    if a._dtype != _I32 and a._dtype != _I64:
-        return a._contiguous_copy(_I64)
-    return a if a._is_c_contiguous() else a._contiguous_copy()
-
-
-def _contiguous(a, dtype) -> ndarray:
-    if a._dtype != dtype:
-        return a._contiguous_copy(dtype)
-    return a if a._is_c_contiguous() else a._contiguous_copy()
+    dtype = a._dtype
+    if dtype.kind not in "iu":
+        raise TypeError(f"{what} must be integers, not {dtype}")
+    return _contiguous(a, dtype if dtype == _I32 or dtype == _I64 else _I64)
 
 
 def _collapsed(a, axes):
@@ -86,22 +86,27 @@ def _collapsed(a, axes):
 def _rows(a):
     """(array, row stride) of ``a`` as rows of adjacent elements: ``a`` itself
     where its strides allow it, else a contiguous copy."""
-    if a._shape[-1] <= 1 or a._strides[-1] == 1:
-        stride = _collapsed(a, a.ndim - 1)
-        if stride is not None:
-            return a, stride
-    return a._contiguous_copy(), a._shape[-1]
+    shape, strides = a._shape, a._strides
+    if strides != _c_contiguous_strides(shape):
+        if shape[-1] <= 1 or strides[-1] == 1:
+            stride = _collapsed(a, len(shape) - 1)
+            if stride is not None:
+                return a, stride
+        a = a._contiguous_copy()
+    return a, shape[-1]
 
 
 def _steps(a):
     """(array, (pointer, sequence stride, step stride)) of a (..., steps,
     channels) array with adjacent channels, ``a`` itself where possible."""
-    if a._shape[-1] <= 1 or a._strides[-1] == 1:
-        stride = _collapsed(a, a.ndim - 2)
-        if stride is not None:
-            return a, (a._ptr, stride, a._strides[-2])
-    a = a._contiguous_copy()
-    return a, (a._ptr, a._shape[-2] * a._shape[-1], a._shape[-1])
+    shape, strides = a._shape, a._strides
+    if strides != _c_contiguous_strides(shape):
+        if shape[-1] <= 1 or strides[-1] == 1:
+            stride = _collapsed(a, len(shape) - 2)
+            if stride is not None:
+                return a, (a._ptr, stride, strides[-2])
+        a = a._contiguous_copy()
+    return a, (a._ptr, shape[-2] * shape[-1], shape[-1])
 
 
 def _scalar(v, what) -> float:
@@ -122,10 +127,10 @@ def embedding(table, tokens, scale=1.0) -> ndarray:
     scale = _scalar(scale, "scale")
     rows, dim = table._shape
     table, stride = _rows(table)
-    out = ndarray._empty_device(tokens._shape + (dim,), table._dtype)
+    out = _empty(tokens._shape + (dim,), table._dtype)
     n = tokens.size
     if n and dim:
-        HipBackend().embedding(dtype_code(table._dtype), dtype_code(tokens._dtype), n, tokens._ptr,
+        HipBackend().embedding(_CODE[table._dtype], _CODE[tokens._dtype], n, tokens._ptr,
                                rows, dim, table._ptr, stride, scale, out._ptr)
     return out
 
@@ -147,9 +152,9 @@ def embedding_grad(grad, tokens, rows, scale=1.0) -> ndarray:
     scale = _scalar(scale, "scale")
     dim = grad._shape[-1]
     grad, stride = _rows(grad)
-    out = ndarray._empty_device((rows, dim), grad._dtype)
+    out = _empty((rows, dim), grad._dtype)
     if rows and dim:
-        HipBackend().embedding_grad(dtype_code(grad._dtype), dtype_code(tokens._dtype),
+        HipBackend().embedding_grad(_CODE[grad._dtype], _CODE[tokens._dtype],
                                     tokens.size, tokens._ptr, grad._ptr, stride, rows, dim, scale,
                                     out._ptr)
     return out
@@ -203,15 +208,15 @@ def gated_recurrence(gate, x, initial=None, *, logits=True):
     most 1 in size."""
     (gate, x), dtype = _sequences((("gate", gate), ("x", x)))
     steps, dim = x._shape[-2:]
-    wide = _wide(dtype)
+    wide = _WIDE[dtype]
     state_shape = x._shape[:-2] + (dim,)
     initial = _state(initial, state_shape, wide, "initial")
-    h = ndarray._empty_device(x._shape, dtype)
-    final = ndarray._empty_device(state_shape, wide)
+    h = _empty(x._shape, dtype)
+    final = _empty(state_shape, wide)
     if final.size:
         gate, at_gate = _steps(gate)
         x, at_x = _steps(x)
-        HipBackend().recurrence(dtype_code(dtype), 1 if logits else 0, _prod(x._shape[:-2]), steps,
+        HipBackend().recurrence(_CODE[dtype], 1 if logits else 0, _prod(x._shape[:-2]), steps,
                                 dim, at_gate, at_x, _ptr(initial), h._ptr, final._ptr)
     return h, final
 
@@ -223,19 +228,19 @@ def gated_recurrence_grad(grad, gate, x, h, initial=None, grad_final=None, *, lo
     have the sequences' type, ``grad_initial`` the states'."""
     (grad, gate, x, h), dtype = _sequences((("grad", grad), ("gate", gate), ("x", x), ("h", h)))
     steps, dim = x._shape[-2:]
-    wide = _wide(dtype)
+    wide = _WIDE[dtype]
     state_shape = x._shape[:-2] + (dim,)
     initial = _state(initial, state_shape, wide, "initial")
     grad_final = _state(grad_final, state_shape, wide, "grad_final")
-    grad_gate = ndarray._empty_device(x._shape, dtype)
-    grad_x = ndarray._empty_device(x._shape, dtype)
-    grad_initial = ndarray._empty_device(state_shape, wide)
+    grad_gate = _empty(x._shape, dtype)
+    grad_x = _empty(x._shape, dtype)
+    grad_initial = _empty(state_shape, wide)
     if grad_initial.size:
         grad, at_grad = _steps(grad)
         gate, at_gate = _steps(gate)
         x, at_x = _steps(x)
         h, at_h = _steps(h)
-        HipBackend().recurrence_grad(dtype_code(dtype), 1 if logits else 0, _prod(x._shape[:-2]),
+        HipBackend().recurrence_grad(_CODE[dtype], 1 if logits else 0, _prod(x._shape[:-2]),
                                      steps, dim, at_grad, at_gate, at_x, at_h, _ptr(initial),
                                      _ptr(grad_final), grad_gate._ptr, grad_x._ptr,
                                      grad_initial._ptr)
@@ -251,7 +256,7 @@ def _loss(logits, targets, weight, want_grad):
     classes, dtype = logits._shape[-1], logits._dtype
     if classes == 0:
         raise ValueError("logits have no classes")
-    wide, scale, each = _wide(dtype), 1.0, None
+    wide, scale, each = _WIDE[dtype], 1.0, None
     if isinstance(weight, (ndarray, np.ndarray)) and weight.ndim:
         each = _floating(weight, "weight")
         if each._shape != targets._shape:
@@ -260,12 +265,12 @@ def _loss(logits, targets, weight, want_grad):
         each = _contiguous(each, wide)
     else:
         scale = _scalar(weight, "weight")
-    loss = ndarray._empty_device(targets._shape, wide)
-    grad = ndarray._empty_device(logits._shape, dtype) if want_grad else None
+    loss = _empty(targets._shape, wide)
+    grad = _empty(logits._shape, dtype) if want_grad else None
     n = targets.size
     if n:
         logits, stride = _rows(logits)
-        HipBackend().cross_entropy(dtype_code(dtype), dtype_code(targets._dtype), n, classes,
+        HipBackend().cross_entropy(_CODE[dtype], _CODE[targets._dtype], n, classes,
                                    logits._ptr, stride, targets._ptr, _ptr(each), scale, loss._ptr,
                                    _ptr(grad))
     return loss, grad
@@ -291,12 +296,12 @@ def cross_entropy_grad(logits, targets, weight=1.0):
 def _clip(arrays, limit, out):
     arrays = [_floating(a, "every array") for a in arrays]
     wide = _F64 if any(a._dtype == _F64 for a in arrays) else _F32
-    norm = ndarray._empty_device((), wide)
-    given = [a if a._is_c_contiguous() else a._contiguous_copy() for a in arrays]
+    norm = _empty((), wide)
+    given = [_contiguous(a, a._dtype) for a in arrays]
     if limit is None:
         outs = None
     elif out is None:
-        outs = [ndarray._empty_device(a._shape, a._dtype) for a in arrays]
+        outs = [_empty(a._shape, a._dtype) for a in arrays]
     else:
         outs = list(out)
         if len(outs) != len(arrays):
@@ -311,10 +316,10 @@ def _clip(arrays, limit, out):
             if not o._is_c_contiguous():
                 raise ValueError("out must be contiguous")
             ew.flush_lazy(o._buffer)
-    HipBackend().clip_norm([dtype_code(a._dtype) for a in given], [a.size for a in given],
+    HipBackend().clip_norm([_CODE[a._dtype] for a in given], [a.size for a in given],
                            [a._ptr for a in given],
                            None if outs is None else [o._ptr for o in outs],
-                           0.0 if limit is None else limit, dtype_code(wide), norm._ptr)
+                           0.0 if limit is None else limit, _CODE[wide], norm._ptr)
     return outs, norm
 
 
