@@ -94,18 +94,18 @@ __device__ __forceinline__ float fma_of(float a, float b, float c) { return __bu
 __device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 // f = 1 / (1 + exp(-g)) and u = 1 - f = 1 / (1 + exp(g)), each to its own
-// last place: the exponential's argument is never positive, so neither
-// overflows, and u keeps its digits where f is near 1.
-template <typename A> __device__ __forceinline__ void sigmoid_pair(A g, A &f, A &u) {
-  const A e = exp_of(g < 0 ? g : -g);
+// last places: the exponential's argument is never positive, so neither
+// overflows, and u keeps its digits where f is near 1.  g was rounded to a T: of
+// a float16, whose 11 bits move exp(g) by more, the exponential is not corrected.
+template <typename T, typename A> __device__ __forceinline__ void sigmoid_pair(A g, A &f, A &u) {
+  A e;
+  if constexpr (sizeof(T) == 2) e = __builtin_amdgcn_exp2f((g < 0 ? g : -g) * 1.44269502f);
+  else e = exp_of(g < 0 ? g : -g);
   const A r = recip(1 + e);
   const A s = e * r;
   f = g < 0 ? s : r;
   u = g < 0 ? r : s;
 }
-
-// float16 -> float32 and back, one rounding.
-template <typename A, typename T> __device__ __forceinline__ A widen(T v) { return (A)v; }
 
 }  // namespace mmpn
 

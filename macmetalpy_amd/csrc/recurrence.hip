@@ -35,14 +35,24 @@ using mmpn::Vec;
 using mmpn::Wide;
 
 constexpr int kBlock = 512;
-constexpr int kLanes = 16;               // threads side by side on a step: 128 bytes
-constexpr int kSlices = kBlock / kLanes; // threads one after another in time
-constexpr int kSteps = 8;                // steps of a thread
-constexpr int kTile = kSlices * kSteps;  // steps of a workgroup
+constexpr int kLook = 4;                 // tiles that look-back reads at once
 constexpr int kPolls = 256;
 constexpr int kWaves = 4;                // per SIMD: two workgroups a CU, so 128 registers
-template <typename T> constexpr int vec_of() { return 8 / sizeof(T); }
-template <typename T> constexpr int channels_of() { return kLanes * vec_of<T>(); }
+
+// How a workgroup lies on its tile: `lanes` threads side by side on a step with
+// vectors of `bytes`, kBlock / lanes of them one after another in time, `steps`
+// steps each.
+template <int LANES, int BYTES, int STEPS> struct Layout {
+  static constexpr int lanes = LANES, steps = STEPS, slices = kBlock / LANES;
+  static constexpr int tile = slices * STEPS;  // steps of a workgroup
+  template <typename T> static constexpr int vec() { return BYTES / (int)sizeof(T); }
+  template <typename T> static constexpr int channels() { return LANES * vec<T>(); }
+};
+typedef Layout<16, 8, 8> ForwardLong;    // 256 steps, 128 bytes of channels
+typedef Layout<32, 8, 8> ForwardWide;    // 128 steps, 256 bytes
+typedef Layout<8, 16, 4> BackwardLong;   // 256 steps, 128 bytes
+typedef Layout<32, 16, 4> BackwardWide;  // 64 steps, 512 bytes
+constexpr int kShortBytes = 8;           // of the vectors where a thread has all steps
 
 // Steps of a (batch, steps, dim) array: adjacent channels, any other strides.
 template <typename T> struct Steps {
@@ -167,10 +177,11 @@ __device__ A look_back(const Look &lk, long long base, long long t, int ch, bool
 }
 
 // One step's factor and addend.
-template <bool LOGITS, typename A> __device__ __forceinline__ void factor(A g, A x, A &f, A &u) {
+template <typename T, bool LOGITS, typename A>
+__device__ __forceinline__ void factor(A g, A x, A &f, A &u) {
   if constexpr (LOGITS) {
     A r;
-    mmpn::sigmoid_pair(g, f, r);
+    mmpn::sigmoid_pair<T>(g, f, r);
     u = r * x;
   } else {
     f = g;
@@ -187,14 +198,21 @@ template <typename T, int V> __device__ __forceinline__ Vec<T, V> load_some(cons
   return v;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) {
+__device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count, bool stream = false) {
   if (count >= V) {
-    mmpn::store_vec<T, V>(p, v);
+    if (stream) mmpn::store_vec<T, V, true>(p, v);
+    else mmpn::store_vec<T, V>(p, v);
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k)
       if (k < count) p[k] = v.e[k];
   }
+}
+
+// Whether the results' steps are whole lines of 128 bytes: then their stores go
+// past the caches.  A line that two workgroups write has to wait for both in one.
+template <typename T> __device__ __forceinline__ bool lines_of(int dim) {
+  return (dim * (int)sizeof(T)) % 128 == 0;
 }
 
 // Where a workgroup is: `groups` sequences times channel groups, and in each
@@ -216,11 +234,11 @@ __device__ __forceinline__ Place place(long long tiles, long long groups, int cg
 
 // Joins the slices' (A, B), which sa and sb hold: each becomes that of all
 // slices before it, and the tile's is returned.  A channel a lane.
-template <typename A, int CH>
+template <typename A, int CH, int SLICES>
 __device__ __forceinline__ void join_slices(A *sa, A *sb, int ch, A &ta, A &tb) {
   A pa = 1, pb = 0;
 #pragma unroll 8
-  for (int s = 0; s < kSlices; ++s) {
+  for (int s = 0; s < SLICES; ++s) {
     const A a = sa[s * CH + ch], b = sb[s * CH + ch];
     sa[s * CH + ch] = pa;
     sb[s * CH + ch] = pb;
@@ -231,18 +249,20 @@ __device__ __forceinline__ void join_slices(A *sa, A *sb, int ch, A &ta, A &tb) 
   tb = pb;
 }
 
-template <typename T, bool LOGITS, int W>
+template <typename T, bool LOGITS, typename L>
 __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
     long long steps, int dim, long long tiles, long long groups, int cgroups, Steps<T> gate,
     Steps<T> x, const typename Wide<T>::type *__restrict__ initial, T *__restrict__ h,
     typename Wide<T>::type *__restrict__ final_, Look lk) {
   typedef typename Wide<T>::type A;
-  constexpr int V = vec_of<T>(), CH = channels_of<T>();
+  constexpr int V = L::template vec<T>(), CH = L::template channels<T>();
+  constexpr int kSteps = L::steps, kSlices = L::slices, kTile = L::tile;
   __shared__ A sa[kSlices * CH], sb[kSlices * CH], sh[CH];
   const Place pl = place(tiles, groups, cgroups);
-  const int tid = threadIdx.x, c = (tid & (kLanes - 1)) * V, s = tid / kLanes;
+  const int tid = threadIdx.x, c = (tid & (L::lanes - 1)) * V, s = tid / L::lanes;
   const int ch = pl.group * CH + c;  // the thread's first channel
   const int count = dim - ch;
+  const bool stream = lines_of<T>(dim);
   const long long t0 = pl.t * kTile + s * kSteps;
   const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
   const T *px = x.p + pl.seq * x.sb + t0 * x.st + ch;
@@ -266,7 +286,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-      for (int k = 0; k < V; ++k) factor<LOGITS>((A)g[i].e[k], (A)v[i].e[k], f[i][k], u[i][k]);
+      for (int k = 0; k < V; ++k) factor<T, LOGITS>((A)g[i].e[k], (A)v[i].e[k], f[i][k], u[i][k]);
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) {
@@ -280,17 +300,17 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
     sb[s * CH + c + k] = b;
   }
   __syncthreads();
-  if (tid < 64) {
+  if (tid < (CH < 64 ? 64 : CH)) {
     const int my = tid < CH ? tid : CH - 1;
     const bool on = tid < CH && pl.group * CH + tid < dim;
     const long long at = pl.seq * dim + pl.group * CH + tid;
     A a, b;
-    if (tid < CH) join_slices<A, CH>(sa, sb, tid, a, b);
+    if (tid < CH) join_slices<A, CH, kSlices>(sa, sb, tid, a, b);
     A state = on && initial ? initial[at] : (A)0;
     if (tiles > 1) {
       if (on && pl.t > 0 && pl.t + 1 < tiles) publish<A, CH>(lk, pl.base + pl.t, my, 1, a, b);
       if (pl.t > 0)
-        state = look_back<A, CH, W>(
+        state = look_back<A, CH, kLook>(
             lk, pl.base, pl.t, my, on, state, [&](long long j, A &ja, A &jb) {
               ja = 1;
               jb = 0;
@@ -302,7 +322,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
                 for (int i = 0; i < kSteps; ++i) {
                   const long long r = w * kSteps + i;
                   A ff, uu;
-                  factor<LOGITS>((A)qg[r * gate.st], (A)qx[r * x.st], ff, uu);
+                  factor<T, LOGITS>((A)qg[r * gate.st], (A)qx[r * x.st], ff, uu);
                   wa = ff * wa;
                   wb = mmpn::fma_of(ff, wb, uu);
                 }
@@ -330,7 +350,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
       st[k] = mmpn::fma_of(f[i][k], st[k], u[i][k]);
       o.e[k] = (T)st[k];
     }
-    store_some<T, V>(ph + (long long)i * dim, o, count);
+    store_some<T, V>(ph + (long long)i * dim, o, count, stream);
   }
   if (t0 < steps && t0 + kSteps >= steps)
 #pragma unroll
@@ -339,19 +359,21 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
 }
 
 // Backwards: tile 0 holds the last steps, a thread's first step is its latest.
-template <typename T, bool LOGITS, int W>
+template <typename T, bool LOGITS, typename L>
 __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
     long long steps, int dim, long long tiles, long long groups, int cgroups, Steps<T> grad,
     Steps<T> gate, Steps<T> x, Steps<T> h, const typename Wide<T>::type *__restrict__ initial,
     const typename Wide<T>::type *__restrict__ grad_final, T *__restrict__ grad_gate,
     T *__restrict__ grad_x, typename Wide<T>::type *__restrict__ grad_initial, Look lk) {
   typedef typename Wide<T>::type A;
-  constexpr int V = vec_of<T>(), CH = channels_of<T>();
+  constexpr int V = L::template vec<T>(), CH = L::template channels<T>();
+  constexpr int kSteps = L::steps, kSlices = L::slices, kTile = L::tile;
   __shared__ A sa[kSlices * CH], sb[kSlices * CH], sh[CH];
   const Place pl = place(tiles, groups, cgroups);
-  const int tid = threadIdx.x, c = (tid & (kLanes - 1)) * V, s = tid / kLanes;
+  const int tid = threadIdx.x, c = (tid & (L::lanes - 1)) * V, s = tid / L::lanes;
   const int ch = pl.group * CH + c;
   const int count = dim - ch;
+  const bool stream = lines_of<T>(dim);
   const long long t0 = steps - 1 - (pl.t * kTile + s * kSteps);  // the thread's latest step
   const T *pd = grad.p + pl.seq * grad.sb + t0 * grad.st + ch;
   const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
@@ -392,7 +414,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       A f, u;
-      factor<LOGITS>((A)g.e[k], (A)0, f, u);
+      factor<T, LOGITS>((A)g.e[k], (A)0, f, u);
       pa[k] = f * pa[k];
       pb[k] = f * ((A)d.e[k] + pb[k]);
     }
@@ -403,17 +425,17 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
     sb[s * CH + c + k] = pb[k];
   }
   __syncthreads();
-  if (tid < 64) {
+  if (tid < (CH < 64 ? 64 : CH)) {
     const int my = tid < CH ? tid : CH - 1;
     const bool on = tid < CH && pl.group * CH + tid < dim;
     const long long at = pl.seq * dim + pl.group * CH + tid;
     A a, b;
-    if (tid < CH) join_slices<A, CH>(sa, sb, tid, a, b);
+    if (tid < CH) join_slices<A, CH, kSlices>(sa, sb, tid, a, b);
     A state = on && grad_final ? grad_final[at] : (A)0;
     if (tiles > 1) {
       if (on && pl.t > 0 && pl.t + 1 < tiles) publish<A, CH>(lk, pl.base + pl.t, my, 1, a, b);
       if (pl.t > 0)
-        state = look_back<A, CH, W>(
+        state = look_back<A, CH, kLook>(
             lk, pl.base, pl.t, my, on, state, [&](long long j, A &ja, A &jb) {
               ja = 1;
               jb = 0;
@@ -426,7 +448,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
                 for (int i = 0; i < kSteps; ++i) {
                   const long long r = w * kSteps + i;
                   A ff, uu;
-                  factor<LOGITS>((A)qg[-r * gate.st], (A)0, ff, uu);
+                  factor<T, LOGITS>((A)qg[-r * gate.st], (A)0, ff, uu);
                   wa = ff * wa;
                   wb = ff * ((A)qd[-r * grad.st] + wb);
                 }
@@ -461,7 +483,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
       const A dd = (A)d.e[k] + carry[k];
       if constexpr (LOGITS) {
         A f, u;
-        mmpn::sigmoid_pair((A)g.e[k], f, u);
+        mmpn::sigmoid_pair<T>((A)g.e[k], f, u);
         const A du = dd * u;
         og.e[k] = (T)(du * f * (hb - (A)v.e[k]));
         ox.e[k] = (T)du;
@@ -472,8 +494,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
         carry[k] = (A)g.e[k] * dd;
       }
     }
-    store_some<T, V>(grad_gate + o0 - (long long)i * dim, og, count);
-    store_some<T, V>(grad_x + o0 - (long long)i * dim, ox, count);
+    store_some<T, V>(grad_gate + o0 - (long long)i * dim, og, count, stream);
+    store_some<T, V>(grad_x + o0 - (long long)i * dim, ox, count, stream);
   }
   if (t0 >= 0 && t0 < kSteps)
 #pragma unroll
@@ -509,7 +531,7 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_short(
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       A f, u;
-      factor<LOGITS>((A)g.e[k], (A)v.e[k], f, u);
+      factor<T, LOGITS>((A)g.e[k], (A)v.e[k], f, u);
       s.e[k] = mmpn::fma_of(f, s.e[k], u);
       o.e[k] = (T)s.e[k];
     }
@@ -552,7 +574,7 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
       const A dd = (A)d.e[k] + carry.e[k];
       if constexpr (LOGITS) {
         A f, u;
-        mmpn::sigmoid_pair((A)g.e[k], f, u);
+        mmpn::sigmoid_pair<T>((A)g.e[k], f, u);
         const A du = dd * u;
         og.e[k] = (T)(du * f * (hb - (A)v.e[k]));
         ox.e[k] = (T)du;
@@ -573,27 +595,30 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
 // Up to this many steps a thread goes through them; a tile's threads would
 // mostly have none.
 constexpr int64_t kShort = 16;
-constexpr int kLook = 8;
+
+// Where there are few groups of channels, their chains of tiles take the time:
+// long tiles.  From this many groups of the wide layouts on, those are quicker.
+constexpr int64_t kForwardWide = 64, kBackwardWide = 16;
 
 // The tiles of a call, and their descriptors.
 struct Plan {
   int64_t tiles, groups;
   int cgroups;
 };
-template <typename T> Plan plan(int64_t batch, int64_t steps, int64_t dim) {
+template <typename T, typename L> Plan plan(int64_t batch, int64_t steps, int64_t dim) {
   Plan p;
-  p.tiles = mmpi::ceil_div(steps, kTile);
-  p.cgroups = (int)mmpi::ceil_div(dim, channels_of<T>());
+  p.tiles = mmpi::ceil_div(steps, L::tile);
+  p.cgroups = (int)mmpi::ceil_div(dim, L::template channels<T>());
   p.groups = batch * p.cgroups;
   return p;
 }
-template <typename T> int look_of(const Plan &p, Look *lk) {
+template <typename T, typename L> int look_of(const Plan &p, Look *lk) {
   typedef typename Wide<T>::type A;
   *lk = Look{nullptr, 0, 0, 0};
   if (p.tiles == 1) return MMP_OK;
   int st = MMP_OK;
   lk->desc = (unsigned long long *)mmpi::scratch(
-      mmpi::SCRATCH_RECUR_TILES, 8ull * words_of<A>() * channels_of<T>() * p.tiles * p.groups, &st);
+      mmpi::SCRATCH_RECUR_TILES, 8ull * words_of<A>() * L::template channels<T>() * p.tiles * p.groups, &st);
   if (st) return st;
   const mmpi::WaitParams w = mmpi::wait_params();
   lk->gen = mmpi::next_generation();
@@ -621,7 +646,7 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
     typedef typename Wide<T>::type A;
     const Steps<T> sg{(const T *)gate, gate_sb, gate_st}, sx{(const T *)x, x_sb, x_st};
     if (steps <= kShort) {
-      constexpr int V = vec_of<T>();
+      constexpr int V = kShortBytes / sizeof(T);
       const int64_t vecs = mmpi::ceil_div(dim, V), n = batch * vecs;
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
@@ -632,18 +657,24 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
                          (const A *)initial, (T *)h, (A *)final_);
       return mmpi::check_launch("mmp_recurrence(short)");
     }
-    const Plan p = plan<T>(batch, steps, dim);
-    if (!mmpi::grid_fits(p.groups * p.tiles, kBlock))
-      return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many tiles");
-    std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
-    Look lk;
-    if (int st = look_of<T>(p, &lk)) return st;
-    auto kernel = logits ? k_recur_tiles<T, true, kLook> : k_recur_tiles<T, false, kLook>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
-                       mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
-                       (long long)p.groups, p.cgroups, sg, sx, (const A *)initial, (T *)h,
-                       (A *)final_, lk);
-    return mmpi::check_launch("mmp_recurrence");
+    const int64_t wide = plan<T, ForwardWide>(batch, steps, dim).groups;
+    auto launch = [&](auto layout) -> int {
+      typedef decltype(layout) L;
+      const Plan p = plan<T, L>(batch, steps, dim);
+      if (!mmpi::grid_fits(p.groups * p.tiles, kBlock))
+        return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many tiles");
+      std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
+      Look lk;
+      if (int st = look_of<T, L>(p, &lk)) return st;
+      auto kernel = logits ? k_recur_tiles<T, true, L> : k_recur_tiles<T, false, L>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
+                         mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
+                         (long long)p.groups, p.cgroups, sg, sx, (const A *)initial, (T *)h,
+                         (A *)final_, lk);
+      return mmpi::check_launch("mmp_recurrence");
+    };
+    const bool one_tile = steps > ForwardWide::tile && steps <= ForwardLong::tile;
+    return wide >= kForwardWide && !one_tile ? launch(ForwardWide()) : launch(ForwardLong());
   })
 }
 
@@ -666,7 +697,7 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
     const Steps<T> sd{(const T *)grad, grad_sb, grad_st}, sg{(const T *)gate, gate_sb, gate_st};
     const Steps<T> sx{(const T *)x, x_sb, x_st}, sh{(const T *)h, h_sb, h_st};
     if (steps <= kShort) {
-      constexpr int V = vec_of<T>();
+      constexpr int V = kShortBytes / sizeof(T);
       const int64_t vecs = mmpi::ceil_div(dim, V), n = batch * vecs;
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
@@ -678,17 +709,23 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
                          (A *)grad_initial);
       return mmpi::check_launch("mmp_recurrence_grad(short)");
     }
-    const Plan p = plan<T>(batch, steps, dim);
-    if (!mmpi::grid_fits(p.groups * p.tiles, kBlock))
-      return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many tiles");
-    std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
-    Look lk;
-    if (int st = look_of<T>(p, &lk)) return st;
-    auto kernel = logits ? k_recur_grad_tiles<T, true, kLook> : k_recur_grad_tiles<T, false, kLook>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
-                       mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
-                       (long long)p.groups, p.cgroups, sd, sg, sx, sh, (const A *)initial,
-                       (const A *)grad_final, (T *)grad_gate, (T *)grad_x, (A *)grad_initial, lk);
-    return mmpi::check_launch("mmp_recurrence_grad");
+    const int64_t wide = plan<T, BackwardWide>(batch, steps, dim).groups;
+    auto launch = [&](auto layout) -> int {
+      typedef decltype(layout) L;
+      const Plan p = plan<T, L>(batch, steps, dim);
+      if (!mmpi::grid_fits(p.groups * p.tiles, kBlock))
+        return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many tiles");
+      std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
+      Look lk;
+      if (int st = look_of<T, L>(p, &lk)) return st;
+      auto kernel = logits ? k_recur_grad_tiles<T, true, L> : k_recur_grad_tiles<T, false, L>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
+                         mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
+                         (long long)p.groups, p.cgroups, sd, sg, sx, sh, (const A *)initial,
+                         (const A *)grad_final, (T *)grad_gate, (T *)grad_x, (A *)grad_initial,
+                         lk);
+      return mmpi::check_launch("mmp_recurrence_grad");
+    };
+    return wide >= kBackwardWide ? launch(BackwardWide()) : launch(BackwardLong());
   })
 }
