@@ -147,7 +147,8 @@ __global__ __launch_bounds__(kSplitBlock) void k_split_count(S src, unsigned til
 
 // Places the entries by digit, otherwise in order; first[d] is where digit d
 // begins, and first[256] the number of all.  Every workgroup adds up the
-// counts of the tiles before its own, four threads a digit.
+// counts of the tiles before its own, four threads a digit; a single one has
+// no others (count is NULL).
 template <typename S>
 __global__ __launch_bounds__(kSplitBlock) void k_split(S src, unsigned tile_len, int shift,
                                                        const unsigned *__restrict__ count,
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(kSplitBlock) void k_split(S src, unsigned tile_len,
   unsigned from = blockIdx.x * tile_len + wave * piece;
   from = from < n ? from : n;
   const unsigned to = n - from < piece ? n : from + piece;
-  {
+  if (count) {
     const int d = tid & (kDigits - 1);
     unsigned before = 0, total = 0;
 #pragma unroll 16
@@ -181,9 +182,13 @@ __global__ __launch_bounds__(kSplitBlock) void k_split(S src, unsigned tile_len,
     const bool there = i0 + lane < to && src.get(i0 + lane, e);
     tally(next[wave], there, e.row >> shift & (kDigits - 1), 8);
   }
+  if (!count) __syncthreads();
   unsigned total = 0, incl = 0;
   if (tid < kDigits) {
-    for (int k = 0; k < kEach; ++k) total += sums[1][k][tid];
+    if (count)
+      for (int k = 0; k < kEach; ++k) total += sums[1][k][tid];
+    else
+      for (int w = 0; w < kSplitWaves; ++w) total += next[w][tid];
     incl = total;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -200,7 +205,8 @@ __global__ __launch_bounds__(kSplitBlock) void k_split(S src, unsigned tile_len,
       first[tid] = at;
       if (tid == kDigits - 1) first[kDigits] = at + total;
     }
-    for (int k = 0; k < kEach; ++k) at += sums[0][k][tid];
+    if (count)
+      for (int k = 0; k < kEach; ++k) at += sums[0][k][tid];
 #pragma unroll
     for (int w = 0; w < kSplitWaves; ++w) {
       const unsigned c = next[w][tid];
@@ -485,6 +491,71 @@ __global__ __launch_bounds__(kBlock) void k_row_sums(
   }
 }
 
+// Few tokens, two a lane: every row looks for its own among them, and no order
+// is made (whose four launches take 17 us, one 5).
+constexpr int kFew = 128, kFewRows = 4;
+template <typename T, typename I, int V>
+__global__ __launch_bounds__(kBlock) void k_row_sums_few(const I *__restrict__ tokens, int n,
+                                                         const T *__restrict__ grad,
+                                                         long long stride, long long rows, int dim,
+                                                         int lanes, typename Wide<T>::type scale,
+                                                         T *__restrict__ out) {
+  typedef typename Wide<T>::type A;
+  const int wl = threadIdx.x & 63, lane = threadIdx.x & (lanes - 1);
+  const long long low = wl < n ? (long long)tokens[wl] : -1;
+  const long long high = wl + 64 < n ? (long long)tokens[wl + 64] : -1;
+  const int per = kBlock / lanes;
+  const long long v0 = (long long)blockIdx.x * per * kFewRows;
+  const int together = lanes < 64 ? 64 / lanes : 1;  // rows of a wave at once
+#pragma unroll 1
+  for (int r = 0; r < kFewRows; ++r) {
+    const long long v = v0 + r * per + threadIdx.x / lanes;
+    // the wave's first row of this turn, and the masks of each of its rows
+    const long long first = v0 + r * per + (threadIdx.x & ~63) / lanes;
+    unsigned long long mine[2] = {0, 0};
+    for (int k = 0; k < together; ++k) {
+      const unsigned long long a = __ballot(low == first + k), b = __ballot(high == first + k);
+      if (v == first + k) {
+        mine[0] = a;
+        mine[1] = b;
+      }
+    }
+    if (v >= rows) continue;
+    for (int c = lane * V; c < dim; c += lanes * V) {
+      const int at = c + V > dim ? dim - V : c;
+      A sum[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum[k] = 0;
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+        for (unsigned long long left = mine[part]; left;) {
+          constexpr int kLoads = 8;
+          Vec<T, V> x[kLoads];
+          bool there[kLoads];
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l) {
+            there[l] = left != 0;
+            if (there[l]) {
+              const int i = __ffsll((long long)left) - 1 + part * 64;
+              x[l] = mmpn::load_vec<T, V>(grad + (long long)i * stride + at);
+            }
+            left &= left - 1;
+          }
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l)
+            if (there[l]) {
+#pragma unroll
+              for (int k = 0; k < V; ++k) sum[k] += (A)x[l].e[k];
+            }
+        }
+      Vec<T, V> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) o.e[k] = (T)(sum[k] * scale);
+      mmpn::store_vec<T, V, true>(out + v * dim + at, o);
+    }
+  }
+}
+
 // The rows in windows, of those that begin in kLongWindows windows kLongCols
 // columns a workgroup, whose threads add up windows in kLongParts parts.
 constexpr int kLongWindows = 32, kLongCols = 64, kLongParts = 16;
@@ -569,15 +640,17 @@ int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *e
                  unsigned *first, Span *span, unsigned *order) {
   // up to 256 tiles of at least 1024 tokens, which every workgroup of k_split
   // adds up
-  const unsigned tile = n == 0 ? 1024 : (unsigned)(mmpi::ceil_div(mmpi::ceil_div(n, kMaxTiles), 1024) * 1024);
-  const unsigned tiles = n ? (unsigned)mmpi::ceil_div(n, tile) : 1;
+  const unsigned tile = (unsigned)(mmpi::ceil_div(mmpi::ceil_div(n, kMaxTiles), 1024) * 1024);
+  const unsigned tiles = (unsigned)mmpi::ceil_div(n, tile);
   auto pass = [&](auto src, int shift, Entry *out) -> int {
     typedef decltype(src) S;
-    hipLaunchKernelGGL((k_split_count<S>), dim3(tiles), dim3(kSplitBlock), 0, mmpi::stream(),
-                       src, tile, shift, count);
-    if (int st = mmpi::check_launch("mmp_embedding_grad(count)")) return st;
+    if (tiles > 1) {
+      hipLaunchKernelGGL((k_split_count<S>), dim3(tiles), dim3(kSplitBlock), 0, mmpi::stream(),
+                         src, tile, shift, count);
+      if (int st = mmpi::check_launch("mmp_embedding_grad(count)")) return st;
+    }
     hipLaunchKernelGGL((k_split<S>), dim3(tiles), dim3(kSplitBlock), 0, mmpi::stream(), src,
-                       tile, shift, (const unsigned *)count, first, out);
+                       tile, shift, tiles > 1 ? (const unsigned *)count : nullptr, first, out);
     return mmpi::check_launch("mmp_embedding_grad(split)");
   };
   if (rows <= (unsigned)kDigits * kGroupRows) {
@@ -610,41 +683,59 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
               double scale, T *out) {
   typedef typename Wide<T>::type A;
   constexpr int V = 16 / sizeof(T);
-  Temp order, spans, part, entries, counts;
-  const bool twice = rows > (int64_t)kDigits * kGroupRows;
-  if (int st = order.get((size_t)n * 4)) return st;
-  if (int st = spans.get((size_t)rows * sizeof(Span))) return st;
-  if (int st = entries.get((size_t)n * sizeof(Entry) * (twice ? 2 : 1))) return st;
-  const int64_t windows = n > kWindow ? mmpi::ceil_div(n, kWindow) : 0;
-  // counts of tiles, beginnings of groups, rows that begin in windows
-  if (int st = counts.get((size_t)(kMaxTiles * kDigits + kDigits + 1 + windows) * 4)) return st;
-  unsigned *count = (unsigned *)counts.p, *first = count + kMaxTiles * kDigits;
-  int *begins = (int *)(first + kDigits + 1);
-  Span *span = (Span *)spans.p;
-  if (int st = order_tokens<I>((unsigned)n, tokens, (unsigned)rows, (Entry *)entries.p,
-                               (Entry *)entries.p + n, count, first, span, (unsigned *)order.p))
-    return st;
   const int vec = dim >= V ? V : 1;
   const int lanes = row_lanes(dim, vec);
+  if (n <= kFew) {
+    const int64_t blocks = mmpi::ceil_div(rows, kBlock / lanes * kFewRows);
+    if (!mmpi::grid_fits(blocks, kBlock))
+      return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many rows");
+    auto kernel = vec == V ? k_row_sums_few<T, I, V> : k_row_sums_few<T, I, 1>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), tokens,
+                       (int)n, grad, (long long)stride, (long long)rows, dim, lanes, (A)scale, out);
+    return mmpi::check_launch("mmp_embedding_grad(few)");
+  }
+  const bool twice = rows > (int64_t)kDigits * kGroupRows;
+  const int64_t windows = mmpi::ceil_div(n, kWindow);
+  // One block for all: sums of windows, entries, places of rows, the order,
+  // rows that begin in windows, counts of tiles, beginnings of groups.
+  Temp temp;
+  size_t size = 0;
+  auto place = [&](size_t bytes) {
+    const size_t at = size;
+    size += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t at_part = place((size_t)windows * 2 * dim * sizeof(A));
+  const size_t at_entries = place((size_t)n * sizeof(Entry) * (twice ? 2 : 1));
+  const size_t at_span = place((size_t)rows * sizeof(Span));
+  const size_t at_order = place((size_t)n * 4), at_begins = place((size_t)windows * 4);
+  const size_t at_count = place(kMaxTiles * kDigits * 4), at_first = place((kDigits + 1) * 4);
+  if (int st = temp.get(size)) return st;
+  char *base = (char *)temp.p;
+  A *part = (A *)(base + at_part);
+  Entry *entries = (Entry *)(base + at_entries);
+  Span *span = (Span *)(base + at_span);
+  unsigned *order = (unsigned *)(base + at_order), *first = (unsigned *)(base + at_first);
+  int *begins = (int *)(base + at_begins);
+  if (int st = order_tokens<I>((unsigned)n, tokens, (unsigned)rows, entries, entries + n,
+                               (unsigned *)(base + at_count), first, span, order))
+    return st;
   const int64_t wblocks = mmpi::ceil_div(windows, kBlock / lanes);
   const int64_t blocks = mmpi::ceil_div(rows, kBlock / lanes * kRows) + wblocks;
   if (!mmpi::grid_fits(blocks, kBlock))
     return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many rows or tokens");
-  if (windows)
-    if (int st = part.get((size_t)windows * 2 * dim * sizeof(A))) return st;
   auto kernel = vec == V ? k_row_sums<T, I, V> : k_row_sums<T, I, 1>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), tokens, grad,
                      (long long)stride, (long long)rows, dim, lanes, (A)scale, (unsigned)wblocks,
                      (const Span *)span, (const unsigned *)first + kDigits,
-                     (const unsigned *)order.p, (A *)part.p, begins, out);
+                     (const unsigned *)order, part, begins, out);
   if (int st = mmpi::check_launch("mmp_embedding_grad")) return st;
-  if (!windows) return MMP_OK;
   const int64_t lblocks = mmpi::ceil_div(windows, kLongWindows) * mmpi::ceil_div(dim, kLongCols);
   if (!mmpi::grid_fits(lblocks, kBlock))
     return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many tokens and columns");
   hipLaunchKernelGGL((k_long_rows<T>), dim3((unsigned)lblocks), dim3(kBlock), 0, mmpi::stream(),
                      dim, (A)scale, (const Span *)span, (const unsigned *)first + kDigits,
-                     (const A *)part.p, (const int *)begins, out);
+                     (const A *)part, (const int *)begins, out);
   return mmpi::check_launch("mmp_embedding_grad(long)");
 }
 

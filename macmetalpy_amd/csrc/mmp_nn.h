@@ -87,9 +87,6 @@ __device__ __forceinline__ float exp_of(float x) {
 }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
-__device__ __forceinline__ float recip(float x) { return __builtin_amdgcn_rcpf(x); }
-__device__ __forceinline__ double recip(double x) { return 1.0 / x; }
-
 __device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
@@ -98,10 +95,23 @@ __device__ __forceinline__ double fma_of(double a, double b, double c) { return 
 // overflows, and u keeps its digits where f is near 1.  g was rounded to a T: of
 // a float16, whose 11 bits move exp(g) by more, the exponential is not corrected.
 template <typename T, typename A> __device__ __forceinline__ void sigmoid_pair(A g, A &f, A &u) {
-  A e;
-  if constexpr (sizeof(T) == 2) e = __builtin_amdgcn_exp2f((g < 0 ? g : -g) * 1.44269502f);
-  else e = exp_of(g < 0 ? g : -g);
-  const A r = recip(1 + e);
+  const A x = g < 0 ? g : -g;
+  A e, r;
+  if constexpr (sizeof(T) == 2) {
+    e = __builtin_amdgcn_exp2f(x * 1.44269502f);
+    r = __builtin_amdgcn_rcpf(1 + e);
+  } else if constexpr (sizeof(T) == 4) {
+    // The hardware's reciprocal is within a unit of the last place; the same
+    // error in every step would add up along a sequence, so one more step of
+    // Newton's iteration.
+    e = exp_of(x);
+    const A d = 1 + e;
+    r = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+  } else {
+    e = exp_of(x);
+    r = 1 / (1 + e);
+  }
   const A s = e * r;
   f = g < 0 ? s : r;
   u = g < 0 ? r : s;

@@ -88,15 +88,16 @@ __global__ __launch_bounds__(kBlock) void k_squares(Table t, long long chunk_len
   const Chunk<T> c(t, blockIdx.x, chunk_len);
   const T *x = c.x + c.head;
   double s = 0;
-  long long i0 = threadIdx.x;
-  for (; i0 + (kLoads - 1) * kBlock < c.vecs; i0 += kLoads * kBlock) {
+  for (long long i0 = threadIdx.x; i0 < c.vecs; i0 += kLoads * kBlock) {
     Vec<T, Chunk<T>::V> v[kLoads];
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) v[l] = mmpn::load_vec<T, Chunk<T>::V>(x + (i0 + l * kBlock) * Chunk<T>::V);
+    for (int l = 0; l < kLoads; ++l)
+      if (i0 + l * kBlock < c.vecs)
+        v[l] = mmpn::load_vec<T, Chunk<T>::V>(x + (i0 + l * kBlock) * Chunk<T>::V);
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) s += squares<T>(v[l]);
+    for (int l = 0; l < kLoads; ++l)
+      if (i0 + l * kBlock < c.vecs) s += squares<T>(v[l]);
   }
-  for (; i0 < c.vecs; i0 += kBlock) s += squares<T>(mmpn::load_vec<T, Chunk<T>::V>(x + i0 * Chunk<T>::V));
   // at most 7 elements before the vectors and 7 after them
   const long long rest = c.to - c.from - c.vecs * Chunk<T>::V;
   if (threadIdx.x < rest) {
@@ -107,31 +108,43 @@ __global__ __launch_bounds__(kBlock) void k_squares(Table t, long long chunk_len
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-template <typename N>
-__global__ __launch_bounds__(kNormBlock) void k_norm(const double *__restrict__ part, long long n,
-                                                     N *__restrict__ norm,
-                                                     double *__restrict__ full) {
-  __shared__ double lds[kNormBlock / 64];
+// The norm from the chunks' sums, in the same order wherever it is called.
+template <int BLOCK> __device__ __forceinline__ double norm_of(const double *part, int n, double *lds) {
   double s = 0;
 #pragma unroll 4
-  for (long long i = threadIdx.x; i < n; i += kNormBlock) s += part[i];
-  s = sqrt(block_sum<kNormBlock>(s, lds));
+  for (int i = threadIdx.x; i < n; i += BLOCK) s += part[i];
+  return sqrt(block_sum<BLOCK>(s, lds));
+}
+__device__ __forceinline__ void put_norm(void *norm, bool wide, double v) {
+  if (wide) *(double *)norm = v;
+  else *(float *)norm = (float)v;
+}
+
+template <int BLOCK>
+__global__ __launch_bounds__(BLOCK) void k_norm(const double *__restrict__ part, int n, bool wide,
+                                                void *__restrict__ norm, double *__restrict__ full) {
+  __shared__ double lds[BLOCK / 64];
+  const double s = norm_of<BLOCK>(part, n, lds);
   if (threadIdx.x == 0) {
-    *norm = (N)s;
+    put_norm(norm, wide, s);
     *full = s;
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_clip(Table t, long long chunk_len, double limit,
-                                                 const double *__restrict__ norm) {
+                                                 const double *__restrict__ part, int parts,
+                                                 bool wide, void *__restrict__ norm) {
   typedef typename Wide<T>::type A;
   constexpr int V = Chunk<T>::V;
   // backwards: what was summed last is the likeliest to be in a cache
   const Chunk<T> c(t, gridDim.x - 1 - blockIdx.x, chunk_len);
   const T *x = c.x + c.head;
   T *y0 = (T *)t.out[c.array] + c.from, *y = y0 + c.head;
-  const double n = *norm;
+  // few sums: every workgroup adds them up by itself; else *part is the norm
+  __shared__ double lds[kBlock / 64];
+  const double n = parts ? norm_of<kBlock>(part, parts, lds) : *part;
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) put_norm(norm, wide, n);
   // a norm that is NaN scales by NaN: a broken step shows
   const A by = (A)(n <= limit ? 1.0 : limit / n);
   if (by == 1 && y0 == c.x) return;  // in place, and nothing to change
@@ -141,16 +154,16 @@ __global__ __launch_bounds__(kBlock) void k_clip(Table t, long long chunk_len, d
     for (int k = 0; k < V; ++k) r.e[k] = (T)((A)v.e[k] * by);
     return r;
   };
-  long long i0 = threadIdx.x;
-  for (; i0 + (kLoads - 1) * kBlock < c.vecs; i0 += kLoads * kBlock) {
+  for (long long i0 = threadIdx.x; i0 < c.vecs; i0 += kLoads * kBlock) {
     Vec<T, V> v[kLoads];
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) v[l] = mmpn::load_vec<T, V, true>(x + (i0 + l * kBlock) * V);
+    for (int l = 0; l < kLoads; ++l)
+      if (i0 + l * kBlock < c.vecs) v[l] = mmpn::load_vec<T, V, true>(x + (i0 + l * kBlock) * V);
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) mmpn::store_vec<T, V, true>(y + (i0 + l * kBlock) * V, scaled(v[l]));
+    for (int l = 0; l < kLoads; ++l)
+      if (i0 + l * kBlock < c.vecs)
+        mmpn::store_vec<T, V, true>(y + (i0 + l * kBlock) * V, scaled(v[l]));
   }
-  for (; i0 < c.vecs; i0 += kBlock)
-    mmpn::store_vec<T, V, true>(y + i0 * V, scaled(mmpn::load_vec<T, V, true>(x + i0 * V)));
   const long long rest = c.to - c.from - c.vecs * V;
   if (threadIdx.x < rest) {
     const long long i = threadIdx.x < c.head ? threadIdx.x : threadIdx.x + c.vecs * V;
@@ -187,14 +200,19 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
       return mmpi::fail(MMP_E_ARG, "mmp_clip_norm: null pointer");
     total += sizes[i];
   }
-  // About 4096 chunks, of 16,384 elements at least and whole rounds of a workgroup's vectors.
-  int64_t chunk = mmpi::ceil_div(mmpi::ceil_div(total, 4096), 16384) * 16384;
-  if (chunk == 0) chunk = 16384;
+  // About 4096 chunks, of 4096 elements at least.
+  int64_t chunk = mmpi::ceil_div(mmpi::ceil_div(total, 4096), 4096) * 4096;
+  if (chunk == 0) chunk = 4096;
   int64_t chunks = 0;
   for (int64_t i = 0; i < count; ++i) chunks += mmpi::ceil_div(sizes[i], chunk);
   Temp part;
   if (int st = part.get((size_t)(chunks + 1) * 8)) return st;
   double *sums = (double *)part.p, *full = sums + chunks;
+  const bool wide = norm_dtype == MMP_F64;
+  if (chunks > 0x7fffffffLL) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_clip_norm: too many arrays");
+  // Up to this many sums the second pass adds them up without a launch between.
+  const bool few = chunks > 0 && chunks <= 1024 && outs;
+  void *norm_left = norm;  // to be written by the second pass's first launch
   // Arrays of one type are launched together, up to kArrays of them.
   for (int pass = 0; pass < 2; ++pass) {
     int64_t done = 0;
@@ -210,9 +228,11 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
                                sums + done);
           else
             hipLaunchKernelGGL((k_clip<T>), grid, block, 0, mmpi::stream(), t, (long long)chunk,
-                               limit, (const double *)full);
+                               limit, (const double *)(few ? sums : full), few ? (int)chunks : 0, wide,
+                               few ? norm_left : nullptr);
           break;
         })
+        if (pass == 1) norm_left = nullptr;
         done += of;
         of = 0;
         t.count = 0;
@@ -232,12 +252,13 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
         if (int st = launch()) return st;
     }
     if (pass == 1) break;
-    if (norm_dtype == MMP_F32)
-      hipLaunchKernelGGL((k_norm<float>), dim3(1), dim3(kNormBlock), 0, mmpi::stream(),
-                         (const double *)sums, (long long)chunks, (float *)norm, full);
+    if (few) continue;
+    if (chunks <= 1024)
+      hipLaunchKernelGGL((k_norm<kBlock>), dim3(1), dim3(kBlock), 0, mmpi::stream(),
+                         (const double *)sums, (int)chunks, wide, norm, full);
     else
-      hipLaunchKernelGGL((k_norm<double>), dim3(1), dim3(kNormBlock), 0, mmpi::stream(),
-                         (const double *)sums, (long long)chunks, (double *)norm, full);
+      hipLaunchKernelGGL((k_norm<kNormBlock>), dim3(1), dim3(kNormBlock), 0, mmpi::stream(),
+                         (const double *)sums, (int)chunks, wide, norm, full);
     if (int st = mmpi::check_launch("mmp_clip_norm(norm)")) return st;
     if (!outs) break;
   }
