@@ -68,13 +68,14 @@ template <typename T> struct Row {
     Words w = mmpn::words_of<T, V>(mmpn::load_vec<T, V, STREAM>(base + (long long)v * V));
     if (v == 0 || v == vecs - 1) {
       const Words fill = nothing();
+      const int first = head - v * V;  // the row's first element, as one of this vector
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         unsigned keep = 0;
 #pragma unroll
         for (int q = 0; q < (sizeof(T) == 2 ? 2 : 1); ++q) {
-          const long long c = (long long)v * V + (j * 4 + q * 2) / (int)sizeof(T) - head;
-          if (c >= 0 && c < classes) keep |= sizeof(T) == 2 ? 0xffffu << (16 * q) : 0xffffffffu;
+          const int k = (j * 4 + q * 2) / (int)sizeof(T);
+          if ((unsigned)(k - first) < (unsigned)classes) keep |= sizeof(T) == 2 ? 0xffffu << (16 * q) : 0xffffffffu;
         }
         w[j] = (w[j] & keep) | (fill[j] & ~keep);
       }
@@ -89,13 +90,12 @@ template <typename T> struct Row {
   }
   // vector v of the row g of the gradient
   __device__ __forceinline__ void store(T *g, int v, const Vec<T, V> &r) const {
-    T *p = g + ((long long)v * V - head);
+    const int first = head - v * V;
+    T *p = g - first;
     if (v == 0 || v == vecs - 1) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const long long c = (long long)v * V + k - head;
-        if (c >= 0 && c < classes) p[k] = r.e[k];
-      }
+      for (int k = 0; k < V; ++k)
+        if ((unsigned)(k - first) < (unsigned)classes) p[k] = r.e[k];
     } else {
       mmpn::store_vec<T, V, true>(p, r);
     }
@@ -377,10 +377,14 @@ template <typename T> int loss_impl(const Loss<T> &p) {
   // Vectors of a row wherever it begins: one more than fit its length.
   const int64_t vecs = p.classes / vec_of<T>() + 2;
   const int64_t cus = mmpi::cu_count();
-  // Parts of at least 16 KiB, for about two workgroups a CU.
+  // Few long rows in parts of at least 16 KiB, for about two workgroups a CU.  The
+  // two launches take 13 us (17 with the gradient; whole call, few rows), one
+  // workgroup for a row of so many 16-byte vectors (us; loss alone, with gradient):
+  // 4096 10, 13; 6250 12, 14; 12,500 18, 17 to 20; 32,500 32, 32.  With the
+  // gradient of 250 rows of 16,250 two parts a row take 40, one 32.
   int64_t parts = 2 * cus / p.rows;
   if (parts > vecs / 1024) parts = vecs / 1024;
-  if (parts >= 2) {
+  if (p.grad ? parts >= 3 && vecs >= 12288 : parts >= 2 && vecs >= 8192) {
     Temp part;
     if (int st = part.get((size_t)(p.rows * parts) * sizeof(Stat<A>))) return st;
     hipLaunchKernelGGL((k_loss_part<T>), dim3((unsigned)(p.rows * parts)), dim3(kPartBlock), 0,
@@ -395,8 +399,12 @@ template <typename T> int loss_impl(const Loss<T> &p) {
                          mmpi::stream(), p, (int)parts, (const Stat<A> *)part.p);
     return mmpi::check_launch("mmp_cross_entropy(join)");
   }
+  // Fewer threads to a row than a wave has, where they hold it: 60,000 rows of 250
+  // float16 with gradient 23 us with 16, 49 with 64; the loss alone 14 and 42.
   if (p.grad) {
     if (vecs <= 8 * 4) return launch_held<T, 8, 4>(p);
+    if (vecs <= 16 * 4) return launch_held<T, 16, 4>(p);
+    if (vecs <= 32 * 4) return launch_held<T, 32, 4>(p);
     if (vecs <= 64 * 4) return launch_held<T, 64, 4>(p);
     if (vecs <= 256 * 4) return launch_held<T, 256, 4>(p);
     if (vecs <= 512 * 4) return launch_held<T, 512, 4>(p);
@@ -408,8 +416,11 @@ template <typename T> int loss_impl(const Loss<T> &p) {
     return launch_pass<T, 1024, true>(p);
   }
   if (vecs <= 8 * 4) return launch_pass<T, 8, false>(p);
+  if (vecs <= 16 * 4) return launch_pass<T, 16, false>(p);
+  if (vecs <= 32 * 4) return launch_pass<T, 32, false>(p);
   if (vecs <= 64 * 16) return launch_pass<T, 64, false>(p);
-  return launch_pass<T, 256, false>(p);
+  if (vecs <= 6144) return launch_pass<T, 256, false>(p);
+  return launch_pass<T, 512, false>(p);
 }
 
 constexpr int64_t kMost = 0x7fffffffLL;

@@ -294,19 +294,28 @@ def cross_entropy_grad(logits, targets, weight=1.0):
 
 # ------------------------------------------------------------------ norm
 def _clip(arrays, limit, out):
-    arrays = [_floating(a, "every array") for a in arrays]
-    wide = _F64 if any(a._dtype == _F64 for a in arrays) else _F32
+    given, codes, sizes, ptrs, outs = [], [], [], [], None
+    for a in arrays:
+        a = _floating(a, "every array")
+        shape, dtype = a._shape, a._dtype
+        if a._strides != _c_contiguous_strides(shape):
+            a = a._contiguous_copy()
+        given.append(a)
+        codes.append(_CODE[dtype])
+        sizes.append(_prod(shape))
+        ptrs.append(a._buffer.ptr + a._offset * dtype.itemsize)
+    wide = _F64 if _CODE[_F64] in codes else _F32
     norm = _empty((), wide)
-    given = [_contiguous(a, a._dtype) for a in arrays]
     if limit is None:
-        outs = None
+        limit, out_ptrs = 0.0, None
     elif out is None:
-        outs = [_empty(a._shape, a._dtype) for a in arrays]
+        outs = [_empty(a._shape, a._dtype) for a in given]
+        out_ptrs = [o._buffer.ptr for o in outs]
     else:
         outs = list(out)
-        if len(outs) != len(arrays):
-            raise ValueError(f"out has {len(outs)} arrays for {len(arrays)}")
-        for a, o in zip(arrays, outs):
+        if len(outs) != len(given):
+            raise ValueError(f"out has {len(outs)} arrays for {len(given)}")
+        for a, o in zip(given, outs):
             if not isinstance(o, ndarray):
                 raise TypeError(f"out must hold device arrays, not {type(o).__name__}")
             if o._shape != a._shape or o._dtype != a._dtype:
@@ -316,10 +325,8 @@ def _clip(arrays, limit, out):
             if not o._is_c_contiguous():
                 raise ValueError("out must be contiguous")
             ew.flush_lazy(o._buffer)
-    HipBackend().clip_norm([_CODE[a._dtype] for a in given], [a.size for a in given],
-                           [a._ptr for a in given],
-                           None if outs is None else [o._ptr for o in outs],
-                           0.0 if limit is None else limit, _CODE[wide], norm._ptr)
+        out_ptrs = [o._ptr for o in outs]
+    HipBackend().clip_norm(codes, sizes, ptrs, out_ptrs, limit, _CODE[wide], norm._ptr)
     return outs, norm
 
 
