@@ -253,24 +253,53 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__
   const unsigned to = n - from < per ? n : from + per;
   unsigned *mine = next + wave * bins;
   __syncthreads();
-  constexpr int kLoads = 4;
-  for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
-    unsigned row[kLoads];
+  // Up to kKept entries a lane stay in registers, with their places among the
+  // wave's of their row: then the second time through has no chain of counters.
+  constexpr int kKept = 16, kLoads = 4;
+  const bool kept = per <= 64 * kKept;
+  Entry e[kKept];
+  unsigned place[kKept];
+  if (kept) {
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) {
-      const unsigned i = i0 + l * 64 + lane;
-      row[l] = entries[base + (i < to ? i : from)].row;
+    for (int l = 0; l < kKept; ++l) {
+      const unsigned i = from + l * 64 + lane;
+      e[l] = {0, 0};
+      if (i < to) e[l] = entries[base + i];
     }
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) tally(mine, i0 + l * 64 + lane < to, row[l] / kDigits, bits);
+    for (int l = 0; l < kKept; ++l) {
+      const bool there = from + l * 64 + lane < to;
+      const unsigned k = e[l].row / kDigits;
+      const unsigned long long same = lanes_alike(__ballot(there), k, bits);
+      const unsigned rank = lanes_below(same);
+      if (there) {
+        const unsigned o = mine[k];
+        place[l] = o + rank;
+        if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
+      }
+    }
+  } else {
+    for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
+      unsigned row[kLoads];
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) {
+        const unsigned i = i0 + l * 64 + lane;
+        row[l] = entries[base + (i < to ? i : from)].row;
+      }
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) tally(mine, i0 + l * 64 + lane < to, row[l] / kDigits, bits);
+    }
   }
   __syncthreads();
   // exclusive sums over the rows, neighbouring ones a thread's, and within a
   // row over the waves
   const unsigned mult = (bins + kGroupBlock - 1) / kGroupBlock;
   unsigned total = 0;
+  constexpr int kMostWaves = kGroupBlock / 64;
   for (unsigned k = tid * mult; k < (tid + 1) * mult && k < bins; ++k)
-    for (int w = 0; w < waves; ++w) total += next[w * bins + k];
+#pragma unroll
+    for (int w = 0; w < kMostWaves; ++w)
+      if (w < waves) total += next[w * bins + k];
   unsigned incl = total;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -283,14 +312,24 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__
   for (int w = 0; w < wave; ++w) at += part[w];
   for (unsigned k = tid * mult; k < (tid + 1) * mult && k < bins; ++k) {
     const unsigned begin = at, v = k * kDigits + blockIdx.x;
-    for (int w = 0; w < waves; ++w) {
-      const unsigned c = next[w * bins + k];
-      next[w * bins + k] = at;
-      at += c;
-    }
+    unsigned c[kMostWaves];
+#pragma unroll
+    for (int w = 0; w < kMostWaves; ++w) c[w] = w < waves ? next[w * bins + k] : 0;
+#pragma unroll
+    for (int w = 0; w < kMostWaves; ++w)
+      if (w < waves) {
+        next[w * bins + k] = at;
+        at += c[w];
+      }
     if (v < rows) span[v] = {begin, at};
   }
   __syncthreads();
+  if (kept) {
+#pragma unroll
+    for (int l = 0; l < kKept; ++l)
+      if (from + l * 64 + lane < to) order[mine[e[l].row / kDigits] + place[l]] = e[l].at;
+    return;
+  }
   for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
     Entry e[kLoads];
 #pragma unroll

@@ -406,7 +406,9 @@ template <typename T> int loss_impl(const Loss<T> &p) {
     if (vecs <= 16 * 4) return launch_held<T, 16, 4>(p);
     if (vecs <= 32 * 4) return launch_held<T, 32, 4>(p);
     if (vecs <= 64 * 4) return launch_held<T, 64, 4>(p);
+    if (vecs <= 64 * 8) return launch_held<T, 64, 8>(p);
     if (vecs <= 256 * 4) return launch_held<T, 256, 4>(p);
+    if (vecs <= 256 * 6) return launch_held<T, 256, 6>(p);
     if (vecs <= 512 * 4) return launch_held<T, 512, 4>(p);
     if (vecs <= 512 * 8) return launch_held<T, 512, 8>(p);
     if (vecs <= 512 * 12) return launch_held<T, 512, 12>(p);
