@@ -48,8 +48,10 @@ template <int LANES, int BYTES, int STEPS> struct Layout {
   template <typename T> static constexpr int vec() { return BYTES / (int)sizeof(T); }
   template <typename T> static constexpr int channels() { return LANES * vec<T>(); }
 };
-typedef Layout<16, 8, 8> ForwardLong;    // 256 steps, 128 bytes of channels
+typedef Layout<8, 8, 8> ForwardFew;      // 512 steps, 64 bytes of channels
+typedef Layout<16, 8, 8> ForwardLong;    // 256 steps, 128 bytes
 typedef Layout<32, 8, 8> ForwardWide;    // 128 steps, 256 bytes
+typedef Layout<4, 16, 4> BackwardFew;    // 512 steps, 64 bytes
 typedef Layout<8, 16, 4> BackwardLong;   // 256 steps, 128 bytes
 typedef Layout<32, 16, 4> BackwardWide;  // 64 steps, 512 bytes
 constexpr int kShortBytes = 8;           // of the vectors where a thread has all steps
@@ -596,9 +598,20 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
 // mostly have none.
 constexpr int64_t kShort = 16;
 
-// Where there are few groups of channels, their chains of tiles take the time:
-// long tiles.  From this many groups of the wide layouts on, those are quicker.
-constexpr int64_t kForwardWide = 64, kBackwardWide = 16;
+// Which layout.  A sequence's tiles wait for each other, about 0.4 us a tile, so
+// few groups of channels want long tiles; many want wide ones, whose loads
+// and stores use the memory better.  Forwards (us, float16 unless said; few / long
+// / wide layout): 1 x 50,000 x 100 37 / 59 / 113, 1 x 50,000 x 300 44 / 66, 1 x
+// 60,000 x 1024 120 / 100 / 140, 2 x 16,000 x 1024 - / 54 / 62, 8 x 4000 x 1024 -
+// / 51 / 52, 16 x 2000 x 1024 - / 51 / 50.5, 64 x 500 x 1024 - / 54 / 50, float32
+// 8 x 2000 x 1024 - / 50 / 46.  Backwards: 1 x 50,000 x 100 52 / 71 / 233, 1 x 50,000
+// x 300 90 / 86, 1 x 60,000 x 1024 239 / 181 / 291, 2 x 16,000 x 1024 - / 101 / 120,
+// 4 x 8000 x 1024 - / 101 / 105, 8 x 4000 x 1024 - / 101 / 97, 32 x 1000 x 1024 - /
+// 101 / 91, float32 3 x 1999 x 1001 - / 36 / 29.  Counted in groups of the wide layout, and of the long one for the few.
+// Steps that are one long tile and two wide ones take the long one: 256 x 256 x
+// 1024 89 / 94.
+constexpr int64_t kForwardWide = 64, kBackwardWide = 24;
+constexpr int64_t kForwardFew = 8, kBackwardFew = 4, kManyTiles = 8;
 
 // The tiles of a call, and their descriptors.
 struct Plan {
@@ -674,7 +687,10 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
       return mmpi::check_launch("mmp_recurrence");
     };
     const bool one_tile = steps > ForwardWide::tile && steps <= ForwardLong::tile;
-    return wide >= kForwardWide && !one_tile ? launch(ForwardWide()) : launch(ForwardLong());
+    if (wide >= kForwardWide && !one_tile) return launch(ForwardWide());
+    const Plan p = plan<T, ForwardLong>(batch, steps, dim);
+    return p.groups < kForwardFew && p.tiles >= kManyTiles ? launch(ForwardFew())
+                                                           : launch(ForwardLong());
   })
 }
 
@@ -726,6 +742,9 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
                          lk);
       return mmpi::check_launch("mmp_recurrence_grad");
     };
-    return wide >= kBackwardWide ? launch(BackwardWide()) : launch(BackwardLong());
+    if (wide >= kBackwardWide) return launch(BackwardWide());
+    const Plan p = plan<T, BackwardLong>(batch, steps, dim);
+    return p.groups < kBackwardFew && p.tiles >= kManyTiles ? launch(BackwardFew())
+                                                            : launch(BackwardLong());
   })
 }
