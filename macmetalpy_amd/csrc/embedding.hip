@@ -40,24 +40,25 @@ __global__ __launch_bounds__(kBlock) void k_embed(const I *__restrict__ tokens, 
                                                   T *__restrict__ out) {
   typedef typename Wide<T>::type A;
   const int per = kBlock / lanes;
-  const long long i = (long long)blockIdx.x * per + threadIdx.x / lanes;
-  if (i >= n) return;
-  const long long tok = (long long)tokens[i];
-  const bool there = tok >= 0 && tok < rows;
-  const T *src = table + (there ? tok : 0) * stride;
-  T *dst = out + i * dim;
-  for (int c = (threadIdx.x & (lanes - 1)) * V; c < dim; c += lanes * V) {
-    const int at = c + V > dim ? dim - V : c;
-    Vec<T, V> v;
-    if (there) {
-      v = mmpn::load_vec<T, V>(src + at);
+  for (long long i = (long long)blockIdx.x * per + threadIdx.x / lanes; i < n;
+       i += (long long)gridDim.x * per) {
+    const long long tok = (long long)tokens[i];
+    const bool there = tok >= 0 && tok < rows;
+    const T *src = table + (there ? tok : 0) * stride;
+    T *dst = out + i * dim;
+    for (int c = (threadIdx.x & (lanes - 1)) * V; c < dim; c += lanes * V) {
+      const int at = c + V > dim ? dim - V : c;
+      Vec<T, V> v;
+      if (there) {
+        v = mmpn::load_vec<T, V>(src + at);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v.e[k] = (T)((A)v.e[k] * scale);
-    } else {
+        for (int k = 0; k < V; ++k) v.e[k] = (T)((A)v.e[k] * scale);
+      } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k) v.e[k] = (T)0;
+        for (int k = 0; k < V; ++k) v.e[k] = (T)0;
+      }
+      mmpn::store_vec<T, V>(dst + at, v);
     }
-    mmpn::store_vec<T, V>(dst + at, v);
   }
 }
 
@@ -671,7 +672,7 @@ struct Temp {
   int get(size_t bytes) { return mmp_alloc(bytes ? bytes : 1, &p); }
 };
 
-constexpr int64_t kMost = 0x7fffffffLL;
+constexpr int64_t kMost = 0x7fff0000LL;  // room for a step past the end in 32 bits
 
 // Orders the tokens' positions by row; ea, eb: room for n entries each.
 template <typename I>
@@ -788,15 +789,14 @@ extern "C" int mmp_embedding(int dtype, int index_dtype, int64_t n, const void *
   if (n == 0 || dim == 0) return MMP_OK;
   if (!tokens || !out || (rows > 0 && !table))
     return mmpi::fail(MMP_E_ARG, "mmp_embedding: null pointer");
-  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding: rows of 2^31 or more");
+  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding: rows of 2^31 elements");
   MMP_DISPATCH_FLOAT(dtype, "mmp_embedding", {
     MMP_DISPATCH_INDEX(index_dtype, "mmp_embedding", {
       constexpr int V = 16 / sizeof(T);
       const int vec = dim >= V ? V : 1;
       const int lanes = row_lanes(dim, vec);
-      const int64_t blocks = mmpi::ceil_div(n, kBlock / lanes);
-      if (!mmpi::grid_fits(blocks, kBlock))
-        return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding: too many tokens");
+      int64_t blocks = mmpi::ceil_div(n, kBlock / lanes);
+      if (blocks > 1 << 22) blocks = 1 << 22;  // then a workgroup takes several turns
       auto kernel = vec == V ? k_embed<T, I, V> : k_embed<T, I, 1>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(),
                          (const I *)tokens, (long long)n, (const T *)table, (long long)rows,
@@ -817,7 +817,7 @@ extern "C" int mmp_embedding_grad(int dtype, int index_dtype, int64_t n, const v
   if (!out || (n > 0 && (!tokens || !grad)))
     return mmpi::fail(MMP_E_ARG, "mmp_embedding_grad: null pointer");
   if (dim > kMost || n > kMost || rows > kMost)
-    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: 2^31 tokens, rows or columns, or more");
+    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: 2^31 tokens, rows or columns");
   MMP_DISPATCH_FLOAT(dtype, "mmp_embedding_grad", {
     MMP_DISPATCH_INDEX(index_dtype, "mmp_embedding_grad", {
       return grad_impl<T, I>(n, (const I *)tokens, (const T *)grad, row_stride, rows, (int)dim,

@@ -352,13 +352,17 @@ __global__ __launch_bounds__(kPartBlock) void k_loss_join(Loss<T> p, int parts,
 }
 
 template <typename T, int L, int K> int launch_held(const Loss<T> &p) {
-  const unsigned blocks = (unsigned)mmpi::ceil_div(p.rows, block_of<L>() / L);
-  hipLaunchKernelGGL((k_loss_held<T, L, K>), dim3(blocks), dim3(block_of<L>()), 0, mmpi::stream(), p);
+  const int64_t blocks = mmpi::ceil_div(p.rows, block_of<L>() / L);
+  if (!mmpi::grid_fits(blocks, block_of<L>()))
+    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: too many rows");
+  hipLaunchKernelGGL((k_loss_held<T, L, K>), dim3((unsigned)blocks), dim3(block_of<L>()), 0, mmpi::stream(), p);
   return mmpi::check_launch("mmp_cross_entropy(held)");
 }
 template <typename T, int L, bool GRAD> int launch_pass(const Loss<T> &p) {
-  const unsigned blocks = (unsigned)mmpi::ceil_div(p.rows, block_of<L>() / L);
-  hipLaunchKernelGGL((k_loss_pass<T, L, GRAD>), dim3(blocks), dim3(block_of<L>()), 0,
+  const int64_t blocks = mmpi::ceil_div(p.rows, block_of<L>() / L);
+  if (!mmpi::grid_fits(blocks, block_of<L>()))
+    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: too many rows");
+  hipLaunchKernelGGL((k_loss_pass<T, L, GRAD>), dim3((unsigned)blocks), dim3(block_of<L>()), 0,
                      mmpi::stream(), p);
   return mmpi::check_launch("mmp_cross_entropy(pass)");
 }
@@ -425,7 +429,7 @@ template <typename T> int loss_impl(const Loss<T> &p) {
   return launch_pass<T, 512, false>(p);
 }
 
-constexpr int64_t kMost = 0x7fffffffLL;
+constexpr int64_t kMost = 0x7fff0000LL;  // room for a step past the end in 32 bits
 
 }  // namespace
 
@@ -439,8 +443,7 @@ extern "C" int mmp_cross_entropy(int dtype, int index_dtype, int64_t rows, int64
   if (!logits || !targets || !loss) return mmpi::fail(MMP_E_ARG, "mmp_cross_entropy: null pointer");
   if (index_dtype != MMP_I32 && index_dtype != MMP_I64)
     return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: index dtype code %d", index_dtype);
-  if (!mmpi::grid_fits(rows, 1024) || classes > kMost - 64)
-    return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: too many rows or classes");
+  if (classes > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: 2^31 classes");
   MMP_DISPATCH_FLOAT(dtype, "mmp_cross_entropy", {
     typedef typename Wide<T>::type A;
     return loss_impl<T>(Loss<T>{(const T *)logits, (long long)rows, (long long)row_stride,

@@ -214,7 +214,7 @@ __device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count, 
 // Whether the results' steps are whole lines of 128 bytes: then their stores go
 // past the caches.  A line that two workgroups write has to wait for both in one.
 template <typename T> __device__ __forceinline__ bool lines_of(int dim) {
-  return (dim * (int)sizeof(T)) % 128 == 0;
+  return ((unsigned)dim * (unsigned)sizeof(T)) % 128 == 0;
 }
 
 // Where a workgroup is: `groups` sequences times channel groups, and in each
@@ -640,7 +640,7 @@ template <typename T, typename L> int look_of(const Plan &p, Look *lk) {
   return MMP_OK;
 }
 
-constexpr int64_t kMost = 0x7fffffffLL;
+constexpr int64_t kMost = 0x7fff0000LL;  // room for a group past the end in 32 bits
 
 }  // namespace
 
@@ -654,7 +654,7 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
   if (batch == 0 || dim == 0) return MMP_OK;
   if (!final_ || (steps > 0 && (!gate || !x || !h)))
     return mmpi::fail(MMP_E_ARG, "mmp_recurrence: null pointer");
-  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: 2^31 channels or more");
+  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: 2^31 channels");
   MMP_DISPATCH_FLOAT(dtype, "mmp_recurrence", {
     typedef typename Wide<T>::type A;
     const Steps<T> sg{(const T *)gate, gate_sb, gate_st}, sx{(const T *)x, x_sb, x_st};
@@ -707,7 +707,7 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
   if (batch == 0 || dim == 0) return MMP_OK;
   if (!grad_initial || (steps > 0 && (!grad || !gate || !x || !h || !grad_gate || !grad_x)))
     return mmpi::fail(MMP_E_ARG, "mmp_recurrence_grad: null pointer");
-  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: 2^31 channels or more");
+  if (dim > kMost) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: 2^31 channels");
   MMP_DISPATCH_FLOAT(dtype, "mmp_recurrence_grad", {
     typedef typename Wide<T>::type A;
     const Steps<T> sd{(const T *)grad, grad_sb, grad_st}, sg{(const T *)gate, gate_sb, gate_st};

@@ -389,14 +389,38 @@ def test_recurrence_long_repeats():
             assert np.array_equal(a.get(), b.get())
 
 
+@pytest.mark.parametrize("logits", [True, False])
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+@pytest.mark.parametrize("shape", [(1, 5003, 30), (1, 5003, 95), (2, 2100, 700), (1, 1025, 1000),
+                                   (40, 700, 300), (100, 129, 257), (70, 200, 64), (9, 17, 513)],
+                         **by_name)
+def test_recurrence_layouts(shape, dt, logits):
+    """Few channels and many steps, many channels, and in between; sequences
+    that end inside a tile."""
+    g = np.random.default_rng(sum(shape) + 2)
+    gate, x, initial = _sequence(g, shape, dt, logits)
+    h, final = nn.gated_recurrence(cp.array(gate), cp.array(x), cp.array(initial), logits=logits)
+    want, last, bound, off = _recur(gate, x, initial, logits, E[dt])
+    near(h, want, bound, dt)
+    near(final, last, off, initial.dtype.type)
+    grad = g.standard_normal(shape).astype(dt)
+    end = g.standard_normal(initial.shape).astype(initial.dtype)
+    got = nn.gated_recurrence_grad(*map(cp.array, (grad, gate, x)), h, cp.array(initial),
+                                   cp.array(end), logits=logits)
+    for a, (w, lim), t in zip(got, _recur_grad(grad, gate, x, h.get(), initial, end, logits, E[dt]),
+                              (dt, dt, initial.dtype.type)):
+        near(a, w, lim, t)
+
+
 @pytest.mark.parametrize("dt", FLOATS, **by_name)
 def test_recurrence_without_predecessors(dt):
     """Tiles that find no earlier tile's state in time join its steps
     themselves: the same bits."""
     from macmetalpy_amd._backend import HipBackend
     g = np.random.default_rng(13)
-    for logits in (True, False):
-        gate, x, initial = _sequence(g, (2, 3001, 70), dt, logits)
+    for shape, logits in (((2, 4500, 70), True), ((2, 2100, 700), False), ((2, 2100, 700), True),
+                          ((40, 700, 300), False), ((40, 700, 300), True)):
+        gate, x, initial = _sequence(g, shape, dt, logits)
         args = [cp.array(a) for a in (gate, x, initial)]
         h, final = nn.gated_recurrence(*args, logits=logits)
         grads = nn.gated_recurrence_grad(args[1], args[0], args[1], h, args[2], logits=logits)
@@ -563,7 +587,7 @@ def _arrays(g, sizes, dts):
 
 
 @pytest.mark.parametrize("sizes", [(1,), (0, 5, 0), (3, 1, 4, 1, 5), (100_003, 7, 65_536), (70,) * 130,
-                                   (1_000_001, 4096, 4097, 4095, 1)], **by_name)
+                                   (3_000_001, 2_000_003), (1_000_001, 4096, 4097, 4095, 1)], **by_name)
 @pytest.mark.parametrize("dts", [(np.float16,), (np.float32,), (np.float64,),
                                  (np.float16, np.float32), (np.float32, np.float64, np.float16)],
                          ids=lambda d: "-".join(t.__name__ for t in d))
@@ -707,3 +731,25 @@ def test_mixed_types():
     lazy = cp.array(x) * 2.0  # an expression not evaluated yet
     near(nn.gated_recurrence(cp.array(gate), lazy)[0], _recur(gate, 2 * x, np.zeros((2, 6)), True, 0)[0],
          2 * bound, np.float32)
+
+
+def test_cross_entropy_many_short_rows():
+    rows = 5_000_000
+    x = cp.zeros((rows, 3), dtype=np.float32)
+    t = cp.full((rows,), 1, dtype=np.int32)
+    x[rows - 1, 1] = 2.0
+    loss, grad = nn.cross_entropy_grad(x, t)
+    loss = loss.get()
+    assert np.allclose(loss[:-1], np.log(3), rtol=1e-6)
+    assert np.isclose(loss[-1], np.log(2 + np.exp(2.0)) - 2, rtol=1e-6)
+    assert np.allclose(grad[rows - 2].get(), [1 / 3, -2 / 3, 1 / 3], rtol=1e-6)
+
+
+def test_embedding_many_tokens():
+    """More tokens than the launch has workgroups for at once."""
+    n, dim = (1 << 22) + 5, 1032
+    tok = cp.array((np.arange(n) % 7).astype(np.int32))
+    table = (np.arange(7 * dim) % 2003).astype(np.float16).reshape(7, dim)
+    got = nn.embedding(cp.array(table), tok)
+    for at in (0, n - 7, n - 6, n - 5, n - 4, n - 1):
+        assert np.array_equal(got[at].get(), table[at % 7])
