@@ -12,8 +12,12 @@
 // radix sort splits them by the low 8 bits of the row (tiles of the tokens
 // count and then place their own, in order): low ones, because the frequent
 // words of a vocabulary are neighbours, and one group of half the tokens would
-// be one workgroup's.  That orders a group's by row with counters in LDS.  More than 2^20
-// rows are too many for those: then every 8 bits of the row have a pass.
+// be one workgroup's.  That orders a group's by row with counters in LDS.  More
+// than 2^20 rows are too many for those, and of more than 2^17 tokens a workgroup
+// has too many: then every 8 bits of the row have a pass (8 columns; groups and
+// passes, of 60,000 rows: 60,000 tokens 59 and 70 us, 131,072 73 and 77, 262,144
+// 100 and 92, 524,288 132 and 107; of a million rows: 85 and 104, 108 and 109, 146
+// and 132, 207 and 159).
 //
 // Then a few lanes sum a row's positions.  Words' frequencies are skewed: a row
 // of more than kWindow positions is summed in windows of kWindow places of the
@@ -57,7 +61,7 @@ __global__ __launch_bounds__(kBlock) void k_embed(const I *__restrict__ tokens, 
 #pragma unroll
         for (int k = 0; k < V; ++k) v.e[k] = (T)0;
       }
-      mmpn::store_vec<T, V>(dst + at, v);
+      mmpn::store_vec<T, V, true>(dst + at, v);
     }
   }
 }
@@ -674,6 +678,11 @@ struct Temp {
 
 constexpr int64_t kMost = 0x7fff0000LL;  // room for a step past the end in 32 bits
 
+constexpr int64_t kGroupTokens = 1 << 17;
+inline bool in_groups(int64_t n, int64_t rows) {
+  return n <= kGroupTokens && rows <= (int64_t)kDigits * kGroupRows;
+}
+
 // Orders the tokens' positions by row; ea, eb: room for n entries each.
 template <typename I>
 int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *eb, unsigned *count,
@@ -693,7 +702,7 @@ int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *e
                        tile, shift, tiles > 1 ? (const unsigned *)count : nullptr, first, out);
     return mmpi::check_launch("mmp_embedding_grad(split)");
   };
-  if (rows <= (unsigned)kDigits * kGroupRows) {
+  if (in_groups(n, rows)) {
     if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
     const unsigned bins = (unsigned)mmpi::ceil_div(rows, kDigits);
     int bits = 0;
@@ -734,7 +743,6 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
                        (int)n, grad, (long long)stride, (long long)rows, dim, lanes, (A)scale, out);
     return mmpi::check_launch("mmp_embedding_grad(few)");
   }
-  const bool twice = rows > (int64_t)kDigits * kGroupRows;
   const int64_t windows = mmpi::ceil_div(n, kWindow);
   // One block for all: sums of windows, entries, places of rows, the order,
   // rows that begin in windows, counts of tiles, beginnings of groups.
@@ -746,7 +754,7 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
     return at;
   };
   const size_t at_part = place((size_t)windows * 2 * dim * sizeof(A));
-  const size_t at_entries = place((size_t)n * sizeof(Entry) * (twice ? 2 : 1));
+  const size_t at_entries = place((size_t)n * sizeof(Entry) * (in_groups(n, rows) ? 1 : 2));
   const size_t at_span = place((size_t)rows * sizeof(Span));
   const size_t at_order = place((size_t)n * 4), at_begins = place((size_t)windows * 4);
   const size_t at_count = place(kMaxTiles * kDigits * 4), at_first = place((kDigits + 1) * 4);

@@ -120,6 +120,20 @@ def test_embedding_grad_skewed():
     near(got, want, (count + 2) * E[np.float16] * size, np.float16)
 
 
+@pytest.mark.parametrize("rows,spread", [(1, 1), (3, 3), (257, 257), (70_001, 70_001), (70_001, 2),
+                                         (1_100_000, 1_100_000), (70_001, 0)])
+@pytest.mark.parametrize("n", [131_072, 200_003])
+def test_embedding_grad_many_tokens(n, rows, spread):
+    """On both sides of 2^17 tokens; spread 0: not one of them has a row."""
+    g = np.random.default_rng(n + rows + spread)
+    tok = g.integers(0, spread, n) * (rows // spread) if spread else np.full(n, -1)
+    tok[::13] = -1
+    grad = g.standard_normal((n, 3)).astype(np.float32)
+    want, size, count = _grad_want(grad, tok, rows, 0.5)
+    near(nn.embedding_grad(cp.array(grad), cp.array(tok), rows, scale=0.5), want,
+         (count + 2) * E[np.float32] * size, np.float32)
+
+
 def test_embedding_grad_views():
     g = np.random.default_rng(4)
     h = g.standard_normal((60, 50)).astype(np.float32)
