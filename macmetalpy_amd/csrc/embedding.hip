@@ -20,7 +20,7 @@
 // and 132, 207 and 159).
 //
 // Then a few lanes sum a row's positions.  Words' frequencies are skewed: a row
-// of more than kWindow positions is summed in windows of kWindow places of the
+// of more than a window's positions is summed in windows of places of the
 // order (a window holds the end of one such row and the beginning of another
 // at most), and the row's workgroup adds up the windows' sums.
 #include "mmp_nn.h"
@@ -67,7 +67,6 @@ __global__ __launch_bounds__(kBlock) void k_embed(const I *__restrict__ tokens, 
 }
 
 // ---------------------------------------------------------------- grouping
-constexpr int kWindow = 64;  // places of the order that are summed together
 constexpr int kDigits = 256, kMaxTiles = 256;
 constexpr int kSplitBlock = 1024, kSplitWaves = kSplitBlock / 64;
 
@@ -240,18 +239,28 @@ struct Span {
 };
 
 // Workgroup g orders group g, the rows v with v % 256 = g, by v / 256: order has
-// the positions, span the rows' places in it.
-constexpr int kGroupBlock = 1024, kGroupRows = 4096;
-__global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__ entries,
-                                                       const unsigned *__restrict__ first,
+// the positions, span the rows' places in it.  S is Entry, where k_split has
+// placed the group's at first[g], or the tokens' type: then every workgroup
+// looks for its own among all n tokens, at most 64 * kKept a wave, and
+// workgroup 0 writes first[256] (two launches less: 2000 tokens of 60,000 x 8
+// 34 to 19 us, 16,000 45 to 32).
+constexpr int kGroupBlock = 1024, kGroupRows = 4096, kKept = 16;
+template <typename S>
+__global__ __launch_bounds__(kGroupBlock) void k_group(const S *__restrict__ src, unsigned n,
+                                                       unsigned *__restrict__ first,
                                                        unsigned rows, unsigned bins, int bits,
                                                        int waves, Span *__restrict__ span,
                                                        unsigned *__restrict__ order) {
+  constexpr bool kSplit = __is_same(S, Entry);
   extern __shared__ unsigned next[];  // [waves][bins]
-  __shared__ unsigned part[kGroupBlock / 64];
+  __shared__ unsigned part[kGroupBlock / 64], low[kGroupBlock / 64], all[kGroupBlock / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (unsigned k = tid; k < waves * bins; k += kGroupBlock) next[k] = 0;
-  const unsigned base = first[blockIdx.x], n = first[blockIdx.x + 1] - base;
+  unsigned base = 0;
+  if constexpr (kSplit) {
+    base = first[blockIdx.x];
+    n = first[blockIdx.x + 1] - base;
+  }
   const unsigned per = (n + waves * 64 - 1) / (waves * 64) * 64;
   unsigned from = wave < waves ? wave * per : n;
   from = from < n ? from : n;
@@ -260,42 +269,70 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__
   __syncthreads();
   // Up to kKept entries a lane stay in registers, with their places among the
   // wave's of their row: then the second time through has no chain of counters.
-  constexpr int kKept = 16, kLoads = 4;
+  constexpr int kLoads = 4;
   const bool kept = per <= 64 * kKept;
   Entry e[kKept];
   unsigned place[kKept];
+  unsigned long long there[kKept];
   if (kept) {
+    unsigned lower = 0, valid = 0;
 #pragma unroll
     for (int l = 0; l < kKept; ++l) {
       const unsigned i = from + l * 64 + lane;
       e[l] = {0, 0};
-      if (i < to) e[l] = entries[base + i];
+      bool ok = i < to;
+      if constexpr (kSplit) {
+        if (ok) e[l] = src[base + i];
+      } else {
+        const long long t = ok ? (long long)src[i] : -1;
+        e[l] = {(unsigned)t, i};
+        ok = t >= 0 && t < (long long)rows;
+        const unsigned d = e[l].row % kDigits;
+        lower += (unsigned)__popcll(__ballot(ok && d < blockIdx.x));
+        valid += (unsigned)__popcll(__ballot(ok));
+        ok = ok && d == blockIdx.x;
+      }
+      there[l] = __ballot(ok);
     }
+    if constexpr (!kSplit)
+      if (lane == 0) {
+        low[wave] = lower;
+        all[wave] = valid;
+      }
 #pragma unroll
     for (int l = 0; l < kKept; ++l) {
-      const bool there = from + l * 64 + lane < to;
+      if (there[l] == 0) continue;
       const unsigned k = e[l].row / kDigits;
-      const unsigned long long same = lanes_alike(__ballot(there), k, bits);
+      const unsigned long long same = lanes_alike(there[l], k, bits);
       const unsigned rank = lanes_below(same);
-      if (there) {
+      if (there[l] >> lane & 1) {
         const unsigned o = mine[k];
         place[l] = o + rank;
         if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
       }
     }
-  } else {
+  } else if constexpr (kSplit) {
     for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
       unsigned row[kLoads];
 #pragma unroll
       for (int l = 0; l < kLoads; ++l) {
         const unsigned i = i0 + l * 64 + lane;
-        row[l] = entries[base + (i < to ? i : from)].row;
+        row[l] = src[base + (i < to ? i : from)].row;
       }
 #pragma unroll
       for (int l = 0; l < kLoads; ++l) tally(mine, i0 + l * 64 + lane < to, row[l] / kDigits, bits);
     }
   }
   __syncthreads();
+  if constexpr (!kSplit) {
+    unsigned valid = 0;
+#pragma unroll
+    for (int w = 0; w < kGroupBlock / 64; ++w) {
+      base += low[w];
+      valid += all[w];
+    }
+    if (blockIdx.x == 0 && tid == 0) first[kDigits] = valid;
+  }
   // exclusive sums over the rows, neighbouring ones a thread's, and within a
   // row over the waves
   const unsigned mult = (bins + kGroupBlock - 1) / kGroupBlock;
@@ -332,26 +369,28 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const Entry *__restrict__
   if (kept) {
 #pragma unroll
     for (int l = 0; l < kKept; ++l)
-      if (from + l * 64 + lane < to) order[mine[e[l].row / kDigits] + place[l]] = e[l].at;
+      if (there[l] >> lane & 1) order[mine[e[l].row / kDigits] + place[l]] = e[l].at;
     return;
   }
-  for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
-    Entry e[kLoads];
+  if constexpr (kSplit) {
+    for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
+      Entry x[kLoads];
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) {
-      const unsigned i = i0 + l * 64 + lane;
-      e[l] = entries[base + (i < to ? i : from)];
-    }
+      for (int l = 0; l < kLoads; ++l) {
+        const unsigned i = i0 + l * 64 + lane;
+        x[l] = src[base + (i < to ? i : from)];
+      }
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) {
-      const bool there = i0 + l * 64 + lane < to;
-      const unsigned k = e[l].row / kDigits;
-      const unsigned long long same = lanes_alike(__ballot(there), k, bits);
-      const unsigned rank = lanes_below(same);
-      if (there) {
-        const unsigned o = mine[k];
-        order[o + rank] = e[l].at;
-        if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
+      for (int l = 0; l < kLoads; ++l) {
+        const bool is = i0 + l * 64 + lane < to;
+        const unsigned k = x[l].row / kDigits;
+        const unsigned long long same = lanes_alike(__ballot(is), k, bits);
+        const unsigned rank = lanes_below(same);
+        if (is) {
+          const unsigned o = mine[k];
+          order[o + rank] = x[l].at;
+          if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
+        }
       }
     }
   }
@@ -419,23 +458,24 @@ __device__ __forceinline__ void add_rows(A (&sum)[V], const T *__restrict__ grad
   }
 }
 
-// Window w of the order: the sums of its pieces of rows of more than kWindow
+// Window w of the order: the sums of its pieces of rows of more than `window`
 // positions, part[2 w] of one that began before it and part[2 w + 1] of one
 // that begins in it; begins[w] is that row, or -1.
 template <typename T, typename I, int V>
 __device__ __forceinline__ void window_sums(const I *__restrict__ tokens, const T *__restrict__ grad,
                                             long long stride, unsigned total, int dim, int lanes,
-                                            unsigned w, const Span *__restrict__ span,
+                                            unsigned window, unsigned w,
+                                            const Span *__restrict__ span,
                                             const unsigned *__restrict__ order,
                                             typename Wide<T>::type *__restrict__ part,
                                             int *__restrict__ begins) {
   typedef typename Wide<T>::type A;
-  const unsigned p0 = w * kWindow, p1 = total - p0 < kWindow ? total : p0 + kWindow;
+  const unsigned p0 = w * window, p1 = total - p0 < window ? total : p0 + window;
 #pragma unroll 1
   for (int piece = 0; piece < 2; ++piece) {
     const long long r = (long long)tokens[order[piece ? p1 - 1 : p0]];
     const unsigned from = span[r].from, to = span[r].to;
-    const bool mine = to - from > kWindow && (from >= p0) == (piece == 1);
+    const bool mine = to - from > window && (from >= p0) == (piece == 1);
     if (piece == 1 && (threadIdx.x & (lanes - 1)) == 0) begins[w] = mine ? (int)r : -1;
     if (!mine) continue;
     for (int c = (threadIdx.x & (lanes - 1)) * V; c < dim; c += lanes * V) {
@@ -453,25 +493,75 @@ __device__ __forceinline__ void window_sums(const I *__restrict__ tokens, const 
   }
 }
 
+// A row of more than a window's positions that begins in the window, whole: the
+// workgroup's `lanes` threads side by side have some of its columns, and their
+// sums of parts of the row are added up in LDS.
+constexpr int kWholeLanes = 8, kWholeChunks = 64, kWholeTokens = 8192;
+template <typename T, typename I, int V>
+__device__ __forceinline__ void whole_row(const I *__restrict__ tokens, const T *__restrict__ grad,
+                                          long long stride, unsigned total, int dim, int lanes,
+                                          typename Wide<T>::type scale, unsigned window,
+                                          unsigned w, int chunk, int chunks,
+                                          const Span *__restrict__ span,
+                                          const unsigned *__restrict__ order, T *__restrict__ out) {
+  typedef typename Wide<T>::type A;
+  __shared__ A lds[kBlock * V];
+  const unsigned p0 = w * window;
+  if (p0 >= total) return;
+  const long long r = (long long)tokens[order[total - p0 < window ? total - 1 : p0 + window - 1]];
+  const unsigned from = span[r].from, to = span[r].to;
+  if (to - from <= window || from < p0) return;
+  const int slots = kBlock / lanes, slot = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+  const unsigned each = (to - from + slots - 1) / slots;
+  const unsigned f0 = from + slot * each < to ? from + slot * each : to;
+  const unsigned t0 = to - f0 < each ? to : f0 + each;
+  for (long long c0 = (long long)chunk * lanes * V; c0 < dim; c0 += (long long)chunks * lanes * V) {
+    const long long c = c0 + lane * V;
+    A sum[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] = 0;
+    if (c < dim)
+      add_rows<T, V, kInFlight, A>(sum, grad, stride, order, f0, t0, c + V > dim ? dim - V : (int)c);
+#pragma unroll
+    for (int k = 0; k < V; ++k) lds[threadIdx.x * V + k] = sum[k];
+    __syncthreads();
+    const int j = threadIdx.x;  // a column of the chunk
+    const long long cj = c0 + j / V * V;
+    if (j < lanes * V && cj < dim) {
+      A s = 0;
+      for (int o = 0; o < slots; ++o) s += lds[o * lanes * V + j];
+      out[r * dim + (cj + V > dim ? dim - V : cj) + j % V] = (T)(s * scale);
+    }
+    __syncthreads();
+  }
+}
+
 // The first `window_blocks` workgroups sum windows (the longest work starts
 // first).  The others have kRows rows of the gradient for `lanes` threads: those
 // of up to kFirst positions, most of them, are read all at once (one
 // after another they would wait for their order, then for their vectors), then
-// those of up to a window.
+// those of up to a window.  With WHOLE they are `chunks` workgroups a window, and
+// sum the long rows themselves.
 constexpr int kRows = 4, kFirst = 2;
-template <typename T, typename I, int V>
+template <typename T, typename I, int V, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void k_row_sums(
     const I *__restrict__ tokens, const T *__restrict__ grad, long long stride, long long rows,
-    int dim, int lanes, typename Wide<T>::type scale, unsigned window_blocks,
-    const Span *__restrict__ span, const unsigned *__restrict__ count,
+    int dim, int lanes, typename Wide<T>::type scale, unsigned window, unsigned window_blocks,
+    int chunks, const Span *__restrict__ span, const unsigned *__restrict__ count,
     const unsigned *__restrict__ order, typename Wide<T>::type *__restrict__ part,
     int *__restrict__ begins, T *__restrict__ out) {
   typedef typename Wide<T>::type A;
   const int per = kBlock / lanes, g = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
   if (blockIdx.x < window_blocks) {
+    if constexpr (WHOLE) {
+      whole_row<T, I, V>(tokens, grad, stride, *count, dim,
+                         lanes < kWholeLanes ? lanes : kWholeLanes, scale, window,
+                         blockIdx.x / chunks, blockIdx.x % chunks, chunks, span, order, out);
+      return;
+    }
     const unsigned w = blockIdx.x * per + g, total = *count;
-    if ((unsigned long long)w * kWindow < total)
-      window_sums<T, I, V>(tokens, grad, stride, total, dim, lanes, w, span, order, part,
+    if ((unsigned long long)w * window < total)
+      window_sums<T, I, V>(tokens, grad, stride, total, dim, lanes, window, w, span, order, part,
                               begins);
     return;
   }
@@ -481,7 +571,7 @@ __global__ __launch_bounds__(kBlock) void k_row_sums(
     unsigned id[kRows][kFirst];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      p[r] = {0, kWindow + 1};  // not one of these rows
+      p[r] = {0, window + 1};  // not one of these rows
       if (v + r < rows) p[r] = span[v + r];
     }
 #pragma unroll
@@ -520,7 +610,7 @@ __global__ __launch_bounds__(kBlock) void k_row_sums(
 #pragma unroll 1
   for (int r = 0; r < kRows && v + r < rows; ++r) {
     const unsigned from = span[v + r].from, to = span[v + r].to;
-    if (to - from <= kFirst || to - from > kWindow) continue;
+    if (to - from <= kFirst || to - from > window) continue;
     for (int c = lane * V; c < dim; c += lanes * V) {
       const int at = c + V > dim ? dim - V : c;
       A sum[V];
@@ -605,7 +695,7 @@ __global__ __launch_bounds__(kBlock) void k_row_sums_few(const I *__restrict__ t
 constexpr int kLongWindows = 32, kLongCols = 64, kLongParts = 16;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_long_rows(
-    int dim, typename Wide<T>::type scale, const Span *__restrict__ span,
+    int dim, typename Wide<T>::type scale, unsigned window, const Span *__restrict__ span,
     const unsigned *__restrict__ count, const typename Wide<T>::type *__restrict__ part,
     const int *__restrict__ begins, T *__restrict__ out) {
   typedef typename Wide<T>::type A;
@@ -620,7 +710,7 @@ __global__ __launch_bounds__(kBlock) void k_long_rows(
   if (threadIdx.x < 64) {
     const unsigned w = first + threadIdx.x;
     int v = -1;
-    if (threadIdx.x < kLongWindows && (unsigned long long)w * kWindow < *count) v = begins[w];
+    if (threadIdx.x < kLongWindows && (unsigned long long)w * window < *count) v = begins[w];
     const unsigned long long m = __ballot(v >= 0);
     if (v >= 0) row_of[threadIdx.x] = v;
     if (threadIdx.x == 0) there = m;
@@ -628,7 +718,7 @@ __global__ __launch_bounds__(kBlock) void k_long_rows(
   __syncthreads();
   for (unsigned long long left = there; left; left &= left - 1) {
     const long long v = row_of[__ffsll((long long)left) - 1];
-    const unsigned w0 = span[v].from / kWindow, w1 = (span[v].to - 1) / kWindow;
+    const unsigned w0 = span[v].from / window, w1 = (span[v].to - 1) / window;
     const unsigned each = (w1 - w0 + kLongParts) / kLongParts;
     const unsigned from = w0 + g * each, to = from + each < w1 + 1 ? from + each : w1 + 1;
     A sum[V];
@@ -683,6 +773,14 @@ inline bool in_groups(int64_t n, int64_t rows) {
   return n <= kGroupTokens && rows <= (int64_t)kDigits * kGroupRows;
 }
 
+// Waves of k_group that have counters, of 64 KiB at most.
+inline int group_waves(int64_t rows) {
+  return rows > 2048 * kDigits ? 4 : rows > 1024 * kDigits ? 8 : 16;
+}
+inline bool in_one(int64_t n, int64_t rows) {
+  return in_groups(n, rows) && n <= group_waves(rows) * 64 * kKept;
+}
+
 // Orders the tokens' positions by row; ea, eb: room for n entries each.
 template <typename I>
 int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *eb, unsigned *count,
@@ -703,14 +801,20 @@ int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *e
     return mmpi::check_launch("mmp_embedding_grad(split)");
   };
   if (in_groups(n, rows)) {
-    if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
     const unsigned bins = (unsigned)mmpi::ceil_div(rows, kDigits);
     int bits = 0;
     while ((bins - 1) >> bits) ++bits;
-    const int waves = bins > 2048 ? 4 : bins > 1024 ? 8 : 16;  // 64 KiB of counters at most
-    hipLaunchKernelGGL(k_group, dim3(rows < kDigits ? rows : kDigits), dim3(kGroupBlock),
-                       (unsigned)waves * bins * 4, mmpi::stream(), (const Entry *)ea,
-                       (const unsigned *)first, rows, bins, bits, waves, span, order);
+    const int waves = group_waves(rows);
+    const dim3 grid(rows < kDigits ? rows : kDigits);
+    const unsigned lds = (unsigned)waves * bins * 4;
+    if (in_one(n, rows)) {
+      hipLaunchKernelGGL((k_group<I>), grid, dim3(kGroupBlock), lds, mmpi::stream(), tokens, n,
+                         first, rows, bins, bits, waves, span, order);
+    } else {
+      if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
+      hipLaunchKernelGGL((k_group<Entry>), grid, dim3(kGroupBlock), lds, mmpi::stream(),
+                         (const Entry *)ea, n, first, rows, bins, bits, waves, span, order);
+    }
     return mmpi::check_launch("mmp_embedding_grad(group)");
   }
   if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
@@ -743,7 +847,6 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
                        (int)n, grad, (long long)stride, (long long)rows, dim, lanes, (A)scale, out);
     return mmpi::check_launch("mmp_embedding_grad(few)");
   }
-  const int64_t windows = mmpi::ceil_div(n, kWindow);
   // One block for all: sums of windows, entries, places of rows, the order,
   // rows that begin in windows, counts of tiles, beginnings of groups.
   Temp temp;
@@ -753,8 +856,19 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
     size += (bytes + 255) / 256 * 256;
     return at;
   };
-  const size_t at_part = place((size_t)windows * 2 * dim * sizeof(A));
-  const size_t at_entries = place((size_t)n * sizeof(Entry) * (in_groups(n, rows) ? 1 : 2));
+  // Long rows whole, by the launch that sums the others, where that is not too
+  // much for a few workgroups (us; whole, in windows; float16): 30,000 x 1024 by 2000
+  // tokens 30, 39, by 8192 42, 49, by 16,000 54, 56, two rows x 1024 by 4096 27, 27, by
+  // 8192 45, 29, by 16,384 85, 32, 200 x 8 by 16,000 25, 58.  Smaller windows are
+  // more work at once and more sums to add up (16, 32, 64 places): 5000 x 8 by 131,072
+  // 60, 72, 91, 60,000 x 128 56, 53, 58, 64,000 x 1024 129, 121, 121, 500 x 77 by
+  // 800,000 215, 157, 133.
+  const bool whole = in_one(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
+  const unsigned window = whole ? 16 : !in_groups(n, rows) ? 64 : lanes <= 8 ? 16 : 32;
+  const int64_t windows = mmpi::ceil_div(n, window);
+  const size_t at_part = place(whole ? 0 : (size_t)windows * 2 * dim * sizeof(A));
+  const size_t entry_lists = whole ? 0 : in_groups(n, rows) ? 1 : 2;
+  const size_t at_entries = place((size_t)n * sizeof(Entry) * entry_lists);
   const size_t at_span = place((size_t)rows * sizeof(Span));
   const size_t at_order = place((size_t)n * 4), at_begins = place((size_t)windows * 4);
   const size_t at_count = place(kMaxTiles * kDigits * 4), at_first = place((kDigits + 1) * 4);
@@ -768,21 +882,28 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
   if (int st = order_tokens<I>((unsigned)n, tokens, (unsigned)rows, entries, entries + n,
                                (unsigned *)(base + at_count), first, span, order))
     return st;
-  const int64_t wblocks = mmpi::ceil_div(windows, kBlock / lanes);
+  int64_t chunks = 1, wblocks = mmpi::ceil_div(windows, kBlock / lanes);
+  if (whole) {
+    chunks = mmpi::ceil_div(dim, (int64_t)(lanes < kWholeLanes ? lanes : kWholeLanes) * vec);
+    if (chunks > kWholeChunks) chunks = kWholeChunks;
+    wblocks = windows * chunks;
+  }
   const int64_t blocks = mmpi::ceil_div(rows, kBlock / lanes * kRows) + wblocks;
   if (!mmpi::grid_fits(blocks, kBlock))
     return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many rows or tokens");
-  auto kernel = vec == V ? k_row_sums<T, I, V> : k_row_sums<T, I, 1>;
+  auto kernel = whole ? (vec == V ? k_row_sums<T, I, V, true> : k_row_sums<T, I, 1, true>)
+                      : (vec == V ? k_row_sums<T, I, V, false> : k_row_sums<T, I, 1, false>);
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), tokens, grad,
-                     (long long)stride, (long long)rows, dim, lanes, (A)scale, (unsigned)wblocks,
-                     (const Span *)span, (const unsigned *)first + kDigits,
+                     (long long)stride, (long long)rows, dim, lanes, (A)scale, window,
+                     (unsigned)wblocks, (int)chunks, (const Span *)span, (const unsigned *)first + kDigits,
                      (const unsigned *)order, part, begins, out);
   if (int st = mmpi::check_launch("mmp_embedding_grad")) return st;
+  if (whole) return MMP_OK;
   const int64_t lblocks = mmpi::ceil_div(windows, kLongWindows) * mmpi::ceil_div(dim, kLongCols);
   if (!mmpi::grid_fits(lblocks, kBlock))
     return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_embedding_grad: too many tokens and columns");
   hipLaunchKernelGGL((k_long_rows<T>), dim3((unsigned)lblocks), dim3(kBlock), 0, mmpi::stream(),
-                     dim, (A)scale, (const Span *)span, (const unsigned *)first + kDigits,
+                     dim, (A)scale, window, (const Span *)span, (const unsigned *)first + kDigits,
                      (const A *)part, (const int *)begins, out);
   return mmpi::check_launch("mmp_embedding_grad(long)");
 }

@@ -134,6 +134,25 @@ def test_embedding_grad_many_tokens(n, rows, spread):
          (count + 2) * E[np.float32] * size, np.float32)
 
 
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+@pytest.mark.parametrize("n,rows,dim,spread", [
+    (16_384, 5, 40, 5), (16_385, 5, 40, 5), (17_000, 3, 1001, 3), (17_000, 700, 4097, 20),
+    (16_300, 9, 1001, 2), (20_000, 300, 1, 7), (12_000, 300, 1, 7), (8192, 270_000, 3, 3),
+    (8193, 270_000, 3, 3), (4096, 600_000, 2, 4096), (4097, 600_000, 2, 4096), (129, 256, 33, 1),
+    (129, 257, 8200, 1), (40_000, 600, 65, 600), (40_000, 600, 64, 3), (150_000, 600, 65, 9)])
+def test_embedding_grad_forms(dt, n, rows, dim, spread):
+    """Tokens that one workgroup's registers hold, and one more; rows of many
+    positions, whole and in windows."""
+    g = np.random.default_rng(n + dim)
+    tok = g.integers(0, spread, n) * (rows // spread) - 1  # -1 among them
+    grad = g.standard_normal((n, dim)).astype(dt)
+    want, size, count = _grad_want(grad, tok, rows, 2.0)
+    got = nn.embedding_grad(cp.array(grad), cp.array(tok), rows, scale=2.0)
+    near(got, want, (count + 2) * E[dt] * size, dt)
+    assert np.array_equal(nn.embedding_grad(cp.array(grad), cp.array(tok), rows, scale=2.0).get(),
+                          got.get())
+
+
 def test_embedding_grad_views():
     g = np.random.default_rng(4)
     h = g.standard_normal((60, 50)).astype(np.float32)
