@@ -53,11 +53,22 @@ __device__ __forceinline__ void store_vec(T *p, const Vec<T, N> &v) {
 // Vectors that are kept for a while are kept as words: as elements, a float16
 // vector that passes a branch takes a register for each of its halves.
 template <typename T, int N> __device__ __forceinline__ typename Vec<T, N>::Words words_of(const Vec<T, N> &v) {
-  static_assert(sizeof(T) * N % 4 == 0, "whole words");
-  return __builtin_bit_cast(typename Vec<T, N>::Words, v);
+  if constexpr (sizeof(T) * N < 4) {
+    typename Vec<T, N>::Words w = 0;
+    __builtin_memcpy(&w, &v, sizeof(v));
+    return w;
+  } else {
+    return __builtin_bit_cast(typename Vec<T, N>::Words, v);
+  }
 }
 template <typename T, int N> __device__ __forceinline__ Vec<T, N> elements_of(typename Vec<T, N>::Words w) {
-  return __builtin_bit_cast(Vec<T, N>, w);
+  if constexpr (sizeof(T) * N < 4) {
+    Vec<T, N> v;
+    __builtin_memcpy(&v, &w, sizeof(v));
+    return v;
+  } else {
+    return __builtin_bit_cast(Vec<T, N>, w);
+  }
 }
 
 // Words that the compiler takes for others from here on, so that it works out

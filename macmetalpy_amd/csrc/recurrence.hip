@@ -50,7 +50,9 @@ template <int LANES, int BYTES, int STEPS> struct Layout {
 };
 typedef Layout<8, 8, 8> ForwardFew;      // 512 steps, 64 bytes of channels
 typedef Layout<16, 8, 8> ForwardLong;    // 256 steps, 128 bytes
-typedef Layout<32, 8, 8> ForwardWide;    // 128 steps, 256 bytes
+template <typename T>                    // 128 steps, 256 bytes (512 in float32)
+using ForwardWide = Layout<32, sizeof(T) == 4 ? 16 : 8, 8>;
+typedef Layout<32, 16, 4> ForwardBrief;  // 64 steps, 512 bytes
 typedef Layout<4, 16, 4> BackwardFew;    // 512 steps, 64 bytes
 typedef Layout<8, 16, 4> BackwardLong;   // 256 steps, 128 bytes
 typedef Layout<32, 16, 4> BackwardWide;  // 64 steps, 512 bytes
@@ -200,15 +202,31 @@ template <typename T, int V> __device__ __forceinline__ Vec<T, V> load_some(cons
   return v;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count, bool stream = false) {
+__device__ __forceinline__ typename Vec<T, V>::Words load_words(const T *p) {
+  return mmpn::words_of<T, V>(mmpn::load_vec<T, V>(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void put(T *p, const Vec<T, V> &v, bool stream) {
+  if (stream) mmpn::store_vec<T, V, true>(p, v);
+  else mmpn::store_vec<T, V>(p, v);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) {
   if (count >= V) {
-    if (stream) mmpn::store_vec<T, V, true>(p, v);
-    else mmpn::store_vec<T, V>(p, v);
+    mmpn::store_vec<T, V, true>(p, v);
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k)
       if (k < count) p[k] = v.e[k];
   }
+}
+
+// The channel of a workgroup's column: a row's last vector ends with it (where it
+// is a vector's length at least), so that every vector is read and written
+// whole.  Some of its channels may be the vector before's too, with the same results.
+template <int V> __device__ __forceinline__ int channel_of(int column, int dim) {
+  const int first = column / V * V;
+  return (first + V > dim ? (dim > V ? dim - V : 0) : first) + column % V;
 }
 
 // Whether the results' steps are whole lines of 128 bytes: then their stores go
@@ -262,33 +280,36 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
   __shared__ A sa[kSlices * CH], sb[kSlices * CH], sh[CH];
   const Place pl = place(tiles, groups, cgroups);
   const int tid = threadIdx.x, c = (tid & (L::lanes - 1)) * V, s = tid / L::lanes;
-  const int ch = pl.group * CH + c;  // the thread's first channel
-  const int count = dim - ch;
-  const bool stream = lines_of<T>(dim);
+  const int ch = channel_of<V>(pl.group * CH + c, dim);  // the thread's first channel
+  const int count = pl.group * CH + c < dim ? dim - ch : 0;
   const long long t0 = pl.t * kTile + s * kSteps;
   const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
   const T *px = x.p + pl.seq * x.sb + t0 * x.st + ch;
   A f[kSteps][V], u[kSteps][V];
   {
-    Vec<T, V> g[kSteps], v[kSteps];
-    if (count >= V && t0 + kSteps <= steps) {
+    typename Vec<T, V>::Words g[kSteps], v[kSteps];
+    if (count >= V && t0 < steps) {  // steps past the end read the last, and are not used
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        g[i] = mmpn::load_vec<T, V>(pg + i * gate.st);
-        v[i] = mmpn::load_vec<T, V>(px + i * x.st);
+        g[i] = load_words<T, V>(pg);
+        v[i] = load_words<T, V>(px);
+        pg += t0 + i + 1 < steps ? gate.st : 0;
+        px += t0 + i + 1 < steps ? x.st : 0;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const int n = t0 + i < steps ? count : 0;
-        g[i] = load_some<T, V>(pg + i * gate.st, n);
-        v[i] = load_some<T, V>(px + i * x.st, n);
+        g[i] = mmpn::words_of<T, V>(load_some<T, V>(pg + i * gate.st, n));
+        v[i] = mmpn::words_of<T, V>(load_some<T, V>(px + i * x.st, n));
       }
     }
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+    for (int i = 0; i < kSteps; ++i) {
+      const Vec<T, V> gi = mmpn::elements_of<T, V>(g[i]), vi = mmpn::elements_of<T, V>(v[i]);
 #pragma unroll
-      for (int k = 0; k < V; ++k) factor<T, LOGITS>((A)g[i].e[k], (A)v[i].e[k], f[i][k], u[i][k]);
+      for (int k = 0; k < V; ++k) factor<T, LOGITS>((A)gi.e[k], (A)vi.e[k], f[i][k], u[i][k]);
+    }
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) {
@@ -304,8 +325,9 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
   __syncthreads();
   if (tid < (CH < 64 ? 64 : CH)) {
     const int my = tid < CH ? tid : CH - 1;
-    const bool on = tid < CH && pl.group * CH + tid < dim;
-    const long long at = pl.seq * dim + pl.group * CH + tid;
+    const int chan = channel_of<V>(pl.group * CH + my, dim);
+    const bool on = tid < CH && pl.group * CH + my / V * V < dim && chan < dim;
+    const long long at = pl.seq * dim + chan;
     A a, b;
     if (tid < CH) join_slices<A, CH, kSlices>(sa, sb, tid, a, b);
     A state = on && initial ? initial[at] : (A)0;
@@ -317,8 +339,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
               ja = 1;
               jb = 0;
               if (!on) return;
-              const T *qg = gate.p + pl.seq * gate.sb + j * kTile * gate.st + pl.group * CH + tid;
-              const T *qx = x.p + pl.seq * x.sb + j * kTile * x.st + pl.group * CH + tid;
+              const T *qg = gate.p + pl.seq * gate.sb + j * kTile * gate.st + chan;
+              const T *qx = x.p + pl.seq * x.sb + j * kTile * x.st + chan;
               for (int w = 0; w < kSlices; ++w) {
                 A wa = 1, wb = 0;
                 for (int i = 0; i < kSteps; ++i) {
@@ -352,7 +374,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
       st[k] = mmpn::fma_of(f[i][k], st[k], u[i][k]);
       o.e[k] = (T)st[k];
     }
-    store_some<T, V>(ph + (long long)i * dim, o, count, stream);
+    store_some<T, V>(ph + (long long)i * dim, o, count);
   }
   if (t0 < steps && t0 + kSteps >= steps)
 #pragma unroll
@@ -373,9 +395,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
   __shared__ A sa[kSlices * CH], sb[kSlices * CH], sh[CH];
   const Place pl = place(tiles, groups, cgroups);
   const int tid = threadIdx.x, c = (tid & (L::lanes - 1)) * V, s = tid / L::lanes;
-  const int ch = pl.group * CH + c;
-  const int count = dim - ch;
-  const bool stream = lines_of<T>(dim);
+  const int ch = channel_of<V>(pl.group * CH + c, dim);
+  const int count = pl.group * CH + c < dim ? dim - ch : 0;
   const long long t0 = steps - 1 - (pl.t * kTile + s * kSteps);  // the thread's latest step
   const T *pd = grad.p + pl.seq * grad.sb + t0 * grad.st + ch;
   const T *pg = gate.p + pl.seq * gate.sb + t0 * gate.st + ch;
@@ -383,16 +404,21 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
   const T *ph = h.p + pl.seq * h.sb + (t0 - 1) * h.st + ch;
   typedef typename Vec<T, V>::Words Words;
   Words wg[kSteps], wd[kSteps], wx[kSteps], wh[kSteps];
-  if (count >= V && t0 >= kSteps) {
+  if (count >= V && t0 >= 0) {  // steps before the first read it, and are not used
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      wg[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(pg - i * gate.st));
-      wd[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(pd - i * grad.st));
+      wg[i] = load_words<T, V>(pg);
+      wd[i] = load_words<T, V>(pd);
+      pg -= t0 > i ? gate.st : 0;
+      pd -= t0 > i ? grad.st : 0;
     }
+    if (t0 == 0) ph += h.st;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      if constexpr (LOGITS) wx[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(px - i * x.st));
-      wh[i] = mmpn::words_of<T, V>(mmpn::load_vec<T, V>(ph - i * h.st));
+      if constexpr (LOGITS) wx[i] = load_words<T, V>(px);
+      wh[i] = load_words<T, V>(ph);
+      px -= t0 > i ? x.st : 0;
+      ph -= t0 > i + 1 ? h.st : 0;
     }
   } else {
 #pragma unroll
@@ -429,8 +455,9 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
   __syncthreads();
   if (tid < (CH < 64 ? 64 : CH)) {
     const int my = tid < CH ? tid : CH - 1;
-    const bool on = tid < CH && pl.group * CH + tid < dim;
-    const long long at = pl.seq * dim + pl.group * CH + tid;
+    const int chan = channel_of<V>(pl.group * CH + my, dim);
+    const bool on = tid < CH && pl.group * CH + my / V * V < dim && chan < dim;
+    const long long at = pl.seq * dim + chan;
     A a, b;
     if (tid < CH) join_slices<A, CH, kSlices>(sa, sb, tid, a, b);
     A state = on && grad_final ? grad_final[at] : (A)0;
@@ -443,8 +470,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
               jb = 0;
               if (!on) return;
               const long long q = steps - 1 - j * kTile;
-              const T *qd = grad.p + pl.seq * grad.sb + q * grad.st + pl.group * CH + tid;
-              const T *qg = gate.p + pl.seq * gate.sb + q * gate.st + pl.group * CH + tid;
+              const T *qd = grad.p + pl.seq * grad.sb + q * grad.st + chan;
+              const T *qg = gate.p + pl.seq * gate.sb + q * gate.st + chan;
               for (int w = 0; w < kSlices; ++w) {
                 A wa = 1, wb = 0;
                 for (int i = 0; i < kSteps; ++i) {
@@ -496,8 +523,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
         carry[k] = (A)g.e[k] * dd;
       }
     }
-    store_some<T, V>(grad_gate + o0 - (long long)i * dim, og, count, stream);
-    store_some<T, V>(grad_x + o0 - (long long)i * dim, ox, count, stream);
+    store_some<T, V>(grad_gate + o0 - (long long)i * dim, og, count);
+    store_some<T, V>(grad_x + o0 - (long long)i * dim, ox, count);
   }
   if (t0 >= 0 && t0 < kSteps)
 #pragma unroll
@@ -506,7 +533,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
 }
 
 // Few steps: a thread per V channels goes through them.
-constexpr int kShortBlock = 256;
+constexpr int kShortBlock = 256, kAhead = 4, kAheadGrad = 2;
 template <typename T, bool LOGITS, int V>
 __global__ __launch_bounds__(kShortBlock) void k_recur_short(
     long long n, long long steps, int dim, int vecs, Steps<T> gate, Steps<T> x,
@@ -516,30 +543,55 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_short(
   const long long i = (long long)blockIdx.x * kShortBlock + threadIdx.x;
   if (i >= n) return;
   const long long b = i / vecs;
-  const int c = (int)(i - b * vecs) * V, count = dim - c;
+  // a row's last vector ends with it: some of its channels may be the vector
+  // before's too, with the same results
+  int c = (int)(i - b * vecs) * V;
+  c = c + V > dim ? dim - V : c;
+  const bool stream = lines_of<T>(dim);
   Vec<A, V> s;
   if (initial) {
-    s = load_some<A, V>(initial + b * dim + c, count);
+    s = mmpn::load_vec<A, V>(initial + b * dim + c);
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k) s.e[k] = 0;
   }
   const T *pg = gate.p + b * gate.sb + c, *px = x.p + b * x.sb + c;
   T *ph = h + b * steps * dim + c;
-  for (long long t = 0; t < steps; ++t) {
-    const Vec<T, V> g = load_some<T, V>(pg + t * gate.st, count);
-    const Vec<T, V> v = load_some<T, V>(px + t * x.st, count);
-    Vec<T, V> o;
+  typedef typename Vec<T, V>::Words Words;
+  Words g[kAhead], v[kAhead];
+  auto load = [&](long long t0) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      A f, u;
-      factor<T, LOGITS>((A)g.e[k], (A)v.e[k], f, u);
-      s.e[k] = mmpn::fma_of(f, s.e[k], u);
-      o.e[k] = (T)s.e[k];
+    for (int j = 0; j < kAhead; ++j)
+      if (t0 + j < steps) {
+        g[j] = load_words<T, V>(pg + (t0 + j) * gate.st);
+        v[j] = load_words<T, V>(px + (t0 + j) * x.st);
+      }
+  };
+  load(0);
+  for (long long t0 = 0; t0 < steps; t0 += kAhead) {
+    Words gn[kAhead], vn[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      gn[j] = g[j];
+      vn[j] = v[j];
     }
-    store_some<T, V>(ph + t * dim, o, count);
+    load(t0 + kAhead);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (t0 + j >= steps) break;
+      const Vec<T, V> gj = mmpn::elements_of<T, V>(gn[j]), vj = mmpn::elements_of<T, V>(vn[j]);
+      Vec<T, V> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        A f, u;
+        factor<T, LOGITS>((A)gj.e[k], (A)vj.e[k], f, u);
+        s.e[k] = mmpn::fma_of(f, s.e[k], u);
+        o.e[k] = (T)s.e[k];
+      }
+      put<T, V>(ph + (t0 + j) * dim, o, stream);
+    }
   }
-  store_some<A, V>(final_ + b * dim + c, s, count);
+  mmpn::store_vec<A, V>(final_ + b * dim + c, s);
 }
 
 template <typename T, bool LOGITS, int V>
@@ -552,51 +604,81 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
   const long long i = (long long)blockIdx.x * kShortBlock + threadIdx.x;
   if (i >= n) return;
   const long long b = i / vecs;
-  const int c = (int)(i - b * vecs) * V, count = dim - c;
+  // a row's last vector ends with it: some of its channels may be the vector
+  // before's too, with the same results
+  int c = (int)(i - b * vecs) * V;
+  c = c + V > dim ? dim - V : c;
+  const bool stream = lines_of<T>(dim);
   Vec<A, V> carry;
   if (grad_final) {
-    carry = load_some<A, V>(grad_final + b * dim + c, count);
+    carry = mmpn::load_vec<A, V>(grad_final + b * dim + c);
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k) carry.e[k] = 0;
   }
   const T *pd = grad.p + b * grad.sb + c, *pg = gate.p + b * gate.sb + c;
   const T *px = x.p + b * x.sb + c, *ph = h.p + b * h.sb + c;
-  for (long long t = steps - 1; t >= 0; --t) {
-    const Vec<T, V> d = load_some<T, V>(pd + t * grad.st, count);
-    const Vec<T, V> g = load_some<T, V>(pg + t * gate.st, count);
-    Vec<T, V> v, before;
-    if constexpr (LOGITS) v = load_some<T, V>(px + t * x.st, count);
-    before = load_some<T, V>(ph + (t - 1) * h.st, t > 0 ? count : 0);
-    Vec<T, V> og, ox;
+  typedef typename Vec<T, V>::Words Words;
+  Words d[kAheadGrad], g[kAheadGrad], v[kAheadGrad], p[kAheadGrad];
+  auto load = [&](long long t0) {  // t0 and the steps before it
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      A hb = (A)before.e[k];
-      if (t == 0 && initial && k < count) hb = initial[b * dim + c + k];
-      const A dd = (A)d.e[k] + carry.e[k];
-      if constexpr (LOGITS) {
-        A f, u;
-        mmpn::sigmoid_pair<T>((A)g.e[k], f, u);
-        const A du = dd * u;
-        og.e[k] = (T)(du * f * (hb - (A)v.e[k]));
-        ox.e[k] = (T)du;
-        carry.e[k] = f * dd;
-      } else {
-        og.e[k] = (T)(dd * hb);
-        ox.e[k] = (T)dd;
-        carry.e[k] = (A)g.e[k] * dd;
-      }
+    for (int j = 0; j < kAheadGrad; ++j) {
+      const long long t = t0 - j;
+      if (t < 0) break;
+      d[j] = load_words<T, V>(pd + t * grad.st);
+      g[j] = load_words<T, V>(pg + t * gate.st);
+      if constexpr (LOGITS) v[j] = load_words<T, V>(px + t * x.st);
+      if (t > 0) p[j] = load_words<T, V>(ph + (t - 1) * h.st);
     }
-    const long long o = (b * steps + t) * dim + c;
-    store_some<T, V>(grad_gate + o, og, count);
-    store_some<T, V>(grad_x + o, ox, count);
+  };
+  load(steps - 1);
+  for (long long t0 = steps - 1; t0 >= 0; t0 -= kAheadGrad) {
+    Words dn[kAheadGrad], gn[kAheadGrad], vn[kAheadGrad], pn[kAheadGrad];
+#pragma unroll
+    for (int j = 0; j < kAheadGrad; ++j) {
+      dn[j] = d[j];
+      gn[j] = g[j];
+      if constexpr (LOGITS) vn[j] = v[j];
+      pn[j] = p[j];
+    }
+    load(t0 - kAheadGrad);
+#pragma unroll
+    for (int j = 0; j < kAheadGrad; ++j) {
+      const long long t = t0 - j;
+      if (t < 0) break;
+      const Vec<T, V> dj = mmpn::elements_of<T, V>(dn[j]), gj = mmpn::elements_of<T, V>(gn[j]);
+      const Vec<T, V> pj = mmpn::elements_of<T, V>(pn[j]);
+      Vec<T, V> vj, og, ox;
+      if constexpr (LOGITS) vj = mmpn::elements_of<T, V>(vn[j]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        A hb = (A)pj.e[k];
+        if (t == 0) hb = initial ? initial[b * dim + c + k] : (A)0;
+        const A dd = (A)dj.e[k] + carry.e[k];
+        if constexpr (LOGITS) {
+          A f, u;
+          mmpn::sigmoid_pair<T>((A)gj.e[k], f, u);
+          const A du = dd * u;
+          og.e[k] = (T)(du * f * (hb - (A)vj.e[k]));
+          ox.e[k] = (T)du;
+          carry.e[k] = f * dd;
+        } else {
+          og.e[k] = (T)(dd * hb);
+          ox.e[k] = (T)dd;
+          carry.e[k] = (A)gj.e[k] * dd;
+        }
+      }
+      const long long o = (b * steps + t) * dim + c;
+      put<T, V>(grad_gate + o, og, stream);
+      put<T, V>(grad_x + o, ox, stream);
+    }
   }
-  store_some<A, V>(grad_initial + b * dim + c, carry, count);
+  mmpn::store_vec<A, V>(grad_initial + b * dim + c, carry);
 }
 
 // Up to this many steps a thread goes through them; a tile's threads would
 // mostly have none.
-constexpr int64_t kShort = 16;
+constexpr int64_t kShort = 16, kManyThreads = 65536;
 
 // Which layout.  A sequence's tiles wait for each other, about 0.4 us a tile, so
 // few groups of channels want long tiles; many want wide ones, whose loads
@@ -658,19 +740,21 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
   MMP_DISPATCH_FLOAT(dtype, "mmp_recurrence", {
     typedef typename Wide<T>::type A;
     const Steps<T> sg{(const T *)gate, gate_sb, gate_st}, sx{(const T *)x, x_sb, x_st};
-    if (steps <= kShort) {
-      constexpr int V = kShortBytes / sizeof(T);
-      const int64_t vecs = mmpi::ceil_div(dim, V), n = batch * vecs;
+    constexpr int kVec = kShortBytes / sizeof(T);
+    const int vec = dim >= kVec ? kVec : 1;
+    const int64_t vecs = mmpi::ceil_div(dim, vec), n = batch * vecs;
+    if (steps <= kShort || (n >= kManyThreads && steps > ForwardBrief::tile && steps <= ForwardLong::tile)) {
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many channels");
-      auto kernel = logits ? k_recur_short<T, true, V> : k_recur_short<T, false, V>;
+      auto kernel = vec == kVec ? (logits ? k_recur_short<T, true, kVec> : k_recur_short<T, false, kVec>)
+                                : (logits ? k_recur_short<T, true, 1> : k_recur_short<T, false, 1>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kShortBlock), 0, mmpi::stream(),
                          (long long)n, (long long)steps, (int)dim, (int)vecs, sg, sx,
                          (const A *)initial, (T *)h, (A *)final_);
       return mmpi::check_launch("mmp_recurrence(short)");
     }
-    const int64_t wide = plan<T, ForwardWide>(batch, steps, dim).groups;
+    const int64_t wide = plan<T, ForwardWide<T>>(batch, steps, dim).groups;
     auto launch = [&](auto layout) -> int {
       typedef decltype(layout) L;
       const Plan p = plan<T, L>(batch, steps, dim);
@@ -686,8 +770,9 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
                          (A *)final_, lk);
       return mmpi::check_launch("mmp_recurrence");
     };
-    const bool one_tile = steps > ForwardWide::tile && steps <= ForwardLong::tile;
-    if (wide >= kForwardWide && !one_tile) return launch(ForwardWide());
+    if (steps <= ForwardBrief::tile) return launch(ForwardBrief());
+    const bool one_tile = steps > ForwardWide<T>::tile && steps <= ForwardLong::tile;
+    if (wide >= kForwardWide && !one_tile) return launch(ForwardWide<T>());
     const Plan p = plan<T, ForwardLong>(batch, steps, dim);
     return p.groups < kForwardFew && p.tiles >= kManyTiles ? launch(ForwardFew())
                                                            : launch(ForwardLong());
@@ -713,12 +798,14 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
     const Steps<T> sd{(const T *)grad, grad_sb, grad_st}, sg{(const T *)gate, gate_sb, gate_st};
     const Steps<T> sx{(const T *)x, x_sb, x_st}, sh{(const T *)h, h_sb, h_st};
     if (steps <= kShort) {
-      constexpr int V = kShortBytes / sizeof(T);
-      const int64_t vecs = mmpi::ceil_div(dim, V), n = batch * vecs;
+      constexpr int kVec = kShortBytes / sizeof(T);
+      const int vec = dim >= kVec ? kVec : 1;
+      const int64_t vecs = mmpi::ceil_div(dim, vec), n = batch * vecs;
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many channels");
-      auto kernel = logits ? k_recur_grad_short<T, true, V> : k_recur_grad_short<T, false, V>;
+      auto kernel = vec == kVec ? (logits ? k_recur_grad_short<T, true, kVec> : k_recur_grad_short<T, false, kVec>)
+                                : (logits ? k_recur_grad_short<T, true, 1> : k_recur_grad_short<T, false, 1>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kShortBlock), 0, mmpi::stream(),
                          (long long)n, (long long)steps, (int)dim, (int)vecs, sd, sg, sx, sh,
                          (const A *)initial, (const A *)grad_final, (T *)grad_gate, (T *)grad_x,

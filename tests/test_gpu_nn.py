@@ -285,6 +285,26 @@ def test_recurrence_grad(shape, dt, logits):
         near(a, w, bound, t)
 
 
+@pytest.mark.parametrize("dt,shape", [
+    (np.float16, (300, 70, 1001)), (np.float32, (150, 70, 1001)), (np.float64, (66, 67, 1001)),
+    (np.float16, (300, 16, 1001)), (np.float16, (300, 15, 3)), (np.float16, (20, 64, 3)),
+    (np.float16, (20, 200, 7)), (np.float32, (20, 200, 1)), (np.float32, (20, 400, 1001)),
+    (np.float16, (40, 400, 1001)), (np.float64, (20, 300, 1001))], **by_name)
+def test_recurrence_many_sequences(dt, shape):
+    """Sequences enough for a thread to go through its channels' steps, odd rows."""
+    g = np.random.default_rng(shape[0])
+    gate, x, initial = _sequence(g, shape, dt, True)
+    h, final = nn.gated_recurrence(cp.array(gate), cp.array(x), cp.array(initial))
+    want, last, bound, off = _recur(gate, x, initial, True, E[dt])
+    near(h, want, bound, dt)
+    near(final, last, off, initial.dtype.type)
+    grad = g.standard_normal(shape).astype(dt)
+    got = nn.gated_recurrence_grad(*map(cp.array, (grad, gate, x)), h, cp.array(initial))
+    want = _recur_grad(grad, gate, x, h.get(), initial, 0 * initial, True, E[dt])
+    for a, (w, lim), t in zip(got, want, (dt, dt, initial.dtype.type)):
+        near(a, w, lim, t)
+
+
 @pytest.mark.parametrize("logits", [True, False])
 def test_recurrence_differences(logits):
     """The gradients against central differences of a weighted sum of outputs."""
