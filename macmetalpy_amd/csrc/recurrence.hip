@@ -13,11 +13,12 @@
 // Bound by memory: 3 arrays forwards, 6 (5 with factors) backwards.  Each is
 // read or written once.  n steps together are one step h -> A h + B, with A
 // the product of their factors and B what they make of h = 0, so time is cut
-// into tiles: a workgroup loads kTile steps of 64 channels (float16) into
-// registers, each thread joins kSteps steps of its own, the workgroup
-// joins its threads' (A, B) in LDS, and the tile's state before its first step
-// comes from the tiles before it by look-back; then each thread runs its steps
-// from its state and writes.
+// into tiles: a workgroup loads its steps of some channels into registers, each
+// thread joins the few steps of its own, the workgroup joins its threads'
+// (A, B) in LDS, and the tile's state before its first step comes from the tiles
+// before it by look-back; then each thread runs its steps from its state and
+// writes.  With few steps, or sequences enough to fill the device with a thread
+// for a few channels, a thread goes through the steps instead.
 //
 // Look-back: a tile publishes (A, B) and, as soon as it knows it, the state
 // after its last step.  It reads the kLook tiles before it until one of them
@@ -678,22 +679,40 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
 
 // Up to this many steps a thread goes through them; a tile's threads would
 // mostly have none.
-constexpr int64_t kShort = 16, kManyThreads = 65536;
+constexpr int64_t kShort = 16;
+// Forwards also up to 256 steps, where there are threads enough to keep the
+// memory busy and the tiles are as slow or waste more (us, float16, threads and
+// tiles): 253 x 170 x 1390 92 and 108, 256 x 256 x 1021 94 and 122, x 1024 84 and 85,
+// 200 x 128 x 1999 76 and 77; of 500 steps, 128 x 500 x 2048, 158 and 152; with half
+// as many threads 100 x 130 x 1999 51 and 56, 128 x 500 x 1024 128 and 79.  In float32
+// where the tiles are filled to two thirds at most: 200 x 130 x 3000 214 and 271,
+// 253 x 170 x 1390 165 and 172, 200 x 200 x 2000 226 and 188, 200 x 90 x 1999 114
+// and 92.  Backwards the tiles are as fast or faster at any length.
+constexpr int64_t kManyThreads = 65536;
+template <typename T> bool goes_through(int64_t steps, int64_t threads) {
+  const int64_t tile = ForwardWide<T>::tile;
+  if (threads < kManyThreads || steps <= ForwardBrief::tile || steps > 2 * tile) return false;
+  return sizeof(T) == 2 || 3 * steps <= 2 * mmpi::ceil_div(steps, tile) * tile;
+}
 
 // Which layout.  A sequence's tiles wait for each other, about 0.4 us a tile, so
 // few groups of channels want long tiles; many want wide ones, whose loads
 // and stores use the memory better.  Forwards (us, float16 unless said; few / long
-// / wide layout): 1 x 50,000 x 100 37 / 59 / 113, 1 x 50,000 x 300 44 / 66, 1 x
-// 60,000 x 1024 120 / 100 / 140, 2 x 16,000 x 1024 - / 54 / 62, 8 x 4000 x 1024 -
-// / 51 / 52, 16 x 2000 x 1024 - / 51 / 50.5, 64 x 500 x 1024 - / 54 / 50, float32
-// 8 x 2000 x 1024 - / 50 / 46.  Backwards: 1 x 50,000 x 100 52 / 71 / 233, 1 x 50,000
-// x 300 90 / 86, 1 x 60,000 x 1024 239 / 181 / 291, 2 x 16,000 x 1024 - / 101 / 120,
-// 4 x 8000 x 1024 - / 101 / 105, 8 x 4000 x 1024 - / 101 / 97, 32 x 1000 x 1024 - /
-// 101 / 91, float32 3 x 1999 x 1001 - / 36 / 29.  Counted in groups of the wide layout, and of the long one for the few.
-// Steps that are one long tile and two wide ones take the long one: 256 x 256 x
-// 1024 89 / 94.
-constexpr int64_t kForwardWide = 64, kBackwardWide = 24;
-constexpr int64_t kForwardFew = 8, kBackwardFew = 4, kManyTiles = 8;
+// / wide layout): 1 x 50,000 x 100 36 / 58 / 118, 1 x 50,000 x 300 43 / 65 / 116, 1
+// x 60,000 x 1024 116 / 99 / 126, 2 x 16,000 x 1024 60 / 43 / 52, 4 x 8000 x 1024
+// 59 / 41 / 45, 16 x 2000 x 1024 60 / 42 / 41, 64 x 500 x 1024 58 / 39.5 / 39;
+// float32 1 x 60,000 x 1024 215 / 164 / 163, 4 x 8000 x 1024 123 / 86 / 78, 3 x 1999
+// x 1001 37 / 28 / 19.5, 16 x 2000 x 1024 123 / 85 / 72.  Backwards: 1 x 50,000 x
+// 100 47 / 66 / 227, 1 x 50,000 x 300 84 / 77 / 212, 1 x 60,000 x 1024 233 / 173 /
+// 266, 2 x 16,000 x 1024 131 / 97 / 113, 4 x 8000 x 1024 134 / 98 / 94, 3 x 1999 x
+// 1001 43 / 32 / 27, 16 x 2000 x 1024 136 / 96 / 84; float32 1 x 50,000 x 100 55 / 65
+// / 230, 3 x 1999 x 1001 72 / 53 / 34.  Counted in groups of the wide layout, and of
+// the long one for the few.
+// Steps that are one long tile and two wide ones take the long one (256 x 256 x
+// 1024 86 / 94), but in float32 (160 / 147).  Up to 64 steps one tile of the brief
+// layout beats the others: 281 x 48 x 2851 60, 91 in wide ones, 100 x 30 x 1024 12, 16.
+template <typename T> constexpr int64_t kForwardWide = sizeof(T) == 4 ? 16 : 64;
+constexpr int64_t kBackwardWide = 12, kForwardFew = 8, kBackwardFew = 5, kManyTiles = 8;
 
 // The tiles of a call, and their descriptors.
 struct Plan {
@@ -743,7 +762,7 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
     constexpr int kVec = kShortBytes / sizeof(T);
     const int vec = dim >= kVec ? kVec : 1;
     const int64_t vecs = mmpi::ceil_div(dim, vec), n = batch * vecs;
-    if (steps <= kShort || (n >= kManyThreads && steps > ForwardBrief::tile && steps <= ForwardLong::tile)) {
+    if (steps <= kShort || goes_through<T>(steps, n)) {
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many channels");
@@ -771,8 +790,9 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
       return mmpi::check_launch("mmp_recurrence");
     };
     if (steps <= ForwardBrief::tile) return launch(ForwardBrief());
-    const bool one_tile = steps > ForwardWide<T>::tile && steps <= ForwardLong::tile;
-    if (wide >= kForwardWide && !one_tile) return launch(ForwardWide<T>());
+    const bool one_tile =
+        sizeof(T) != 4 && steps > ForwardWide<T>::tile && steps <= ForwardLong::tile;
+    if (wide >= kForwardWide<T> && !one_tile) return launch(ForwardWide<T>());
     const Plan p = plan<T, ForwardLong>(batch, steps, dim);
     return p.groups < kForwardFew && p.tiles >= kManyTiles ? launch(ForwardFew())
                                                            : launch(ForwardLong());
