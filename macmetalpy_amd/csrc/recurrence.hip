@@ -202,14 +202,9 @@ template <typename T, int V> __device__ __forceinline__ Vec<T, V> load_some(cons
   for (int k = 0; k < V; ++k) v.e[k] = k < count ? p[k] : (T)0;
   return v;
 }
-template <typename T, int V>
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ typename Vec<T, V>::Words load_words(const T *p) {
-  return mmpn::words_of<T, V>(mmpn::load_vec<T, V>(p));
-}
-template <typename T, int V>
-__device__ __forceinline__ void put(T *p, const Vec<T, V> &v, bool stream) {
-  if (stream) mmpn::store_vec<T, V, true>(p, v);
-  else mmpn::store_vec<T, V>(p, v);
+  return mmpn::words_of<T, V>(mmpn::load_vec<T, V, STREAM>(p));
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) {
@@ -228,12 +223,6 @@ __device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) 
 template <int V> __device__ __forceinline__ int channel_of(int column, int dim) {
   const int first = column / V * V;
   return (first + V > dim ? (dim > V ? dim - V : 0) : first) + column % V;
-}
-
-// Whether the results' steps are whole lines of 128 bytes: then their stores go
-// past the caches.  A line that two workgroups write has to wait for both in one.
-template <typename T> __device__ __forceinline__ bool lines_of(int dim) {
-  return ((unsigned)dim * (unsigned)sizeof(T)) % 128 == 0;
 }
 
 // Where a workgroup is: `groups` sequences times channel groups, and in each
@@ -270,7 +259,7 @@ __device__ __forceinline__ void join_slices(A *sa, A *sb, int ch, A &ta, A &tb) 
   tb = pb;
 }
 
-template <typename T, bool LOGITS, typename L>
+template <typename T, bool LOGITS, typename L, bool STREAM>
 __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
     long long steps, int dim, long long tiles, long long groups, int cgroups, Steps<T> gate,
     Steps<T> x, const typename Wide<T>::type *__restrict__ initial, T *__restrict__ h,
@@ -292,8 +281,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
     if (count >= V && t0 < steps) {  // steps past the end read the last, and are not used
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        g[i] = load_words<T, V>(pg);
-        v[i] = load_words<T, V>(px);
+        g[i] = load_words<T, V, STREAM>(pg);
+        v[i] = load_words<T, V, STREAM>(px);
         pg += t0 + i + 1 < steps ? gate.st : 0;
         px += t0 + i + 1 < steps ? x.st : 0;
       }
@@ -384,7 +373,7 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_tiles(
 }
 
 // Backwards: tile 0 holds the last steps, a thread's first step is its latest.
-template <typename T, bool LOGITS, typename L>
+template <typename T, bool LOGITS, typename L, bool STREAM>
 __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
     long long steps, int dim, long long tiles, long long groups, int cgroups, Steps<T> grad,
     Steps<T> gate, Steps<T> x, Steps<T> h, const typename Wide<T>::type *__restrict__ initial,
@@ -408,16 +397,16 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
   if (count >= V && t0 >= 0) {  // steps before the first read it, and are not used
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      wg[i] = load_words<T, V>(pg);
-      wd[i] = load_words<T, V>(pd);
+      wg[i] = load_words<T, V, STREAM>(pg);
+      wd[i] = load_words<T, V, STREAM>(pd);
       pg -= t0 > i ? gate.st : 0;
       pd -= t0 > i ? grad.st : 0;
     }
     if (t0 == 0) ph += h.st;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      if constexpr (LOGITS) wx[i] = load_words<T, V>(px);
-      wh[i] = load_words<T, V>(ph);
+      if constexpr (LOGITS) wx[i] = load_words<T, V, STREAM>(px);
+      wh[i] = load_words<T, V, STREAM>(ph);
       px -= t0 > i ? x.st : 0;
       ph -= t0 > i + 1 ? h.st : 0;
     }
@@ -548,7 +537,6 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_short(
   // before's too, with the same results
   int c = (int)(i - b * vecs) * V;
   c = c + V > dim ? dim - V : c;
-  const bool stream = lines_of<T>(dim);
   Vec<A, V> s;
   if (initial) {
     s = mmpn::load_vec<A, V>(initial + b * dim + c);
@@ -589,7 +577,7 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_short(
         s.e[k] = mmpn::fma_of(f, s.e[k], u);
         o.e[k] = (T)s.e[k];
       }
-      put<T, V>(ph + (t0 + j) * dim, o, stream);
+      mmpn::store_vec<T, V, true>(ph + (t0 + j) * dim, o);
     }
   }
   mmpn::store_vec<A, V>(final_ + b * dim + c, s);
@@ -609,7 +597,6 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
   // before's too, with the same results
   int c = (int)(i - b * vecs) * V;
   c = c + V > dim ? dim - V : c;
-  const bool stream = lines_of<T>(dim);
   Vec<A, V> carry;
   if (grad_final) {
     carry = mmpn::load_vec<A, V>(grad_final + b * dim + c);
@@ -670,8 +657,8 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
         }
       }
       const long long o = (b * steps + t) * dim + c;
-      put<T, V>(grad_gate + o, og, stream);
-      put<T, V>(grad_x + o, ox, stream);
+      mmpn::store_vec<T, V, true>(grad_gate + o, og);
+      mmpn::store_vec<T, V, true>(grad_x + o, ox);
     }
   }
   mmpn::store_vec<A, V>(grad_initial + b * dim + c, carry);
@@ -681,38 +668,51 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
 // mostly have none.
 constexpr int64_t kShort = 16;
 // Forwards also up to 256 steps, where there are threads enough to keep the
-// memory busy and the tiles are as slow or waste more (us, float16, threads and
-// tiles): 253 x 170 x 1390 92 and 108, 256 x 256 x 1021 94 and 122, x 1024 84 and 85,
-// 200 x 128 x 1999 76 and 77; of 500 steps, 128 x 500 x 2048, 158 and 152; with half
-// as many threads 100 x 130 x 1999 51 and 56, 128 x 500 x 1024 128 and 79.  In float32
-// where the tiles are filled to two thirds at most: 200 x 130 x 3000 214 and 271,
-// 253 x 170 x 1390 165 and 172, 200 x 200 x 2000 226 and 188, 200 x 90 x 1999 114
-// and 92.  Backwards the tiles are as fast or faster at any length.
+// memory busy: in float16 (us, threads and tiles) 256 x 256 x 1021 95 and 105, x 1024
+// 86 and 83, 200 x 200 x 2000 111 and 122, 200 x 128 x 1999 76 and 76; of 500 steps,
+// 128 x 500 x 2048, 156 and 148.  In all types, and for half as many threads, where
+// the tiles are filled to two thirds at most: 100 x 130 x 1999 32 and 57, 253 x 170
+// x 1390 92 and 107, float32 200 x 130 x 3000 221 and 266, but 200 x 200 x 2000 218
+// and 186, 200 x 90 x 1999 117 and 90.  Backwards the tiles are as fast at any length.
 constexpr int64_t kManyThreads = 65536;
 template <typename T> bool goes_through(int64_t steps, int64_t threads) {
   const int64_t tile = ForwardWide<T>::tile;
-  if (threads < kManyThreads || steps <= ForwardBrief::tile || steps > 2 * tile) return false;
-  return sizeof(T) == 2 || 3 * steps <= 2 * mmpi::ceil_div(steps, tile) * tile;
+  if (steps <= ForwardBrief::tile || steps > 2 * tile) return false;
+  if (3 * steps <= 2 * mmpi::ceil_div(steps, tile) * tile) return threads >= kManyThreads / 2;
+  return sizeof(T) == 2 && threads >= kManyThreads;
 }
+
+// Inputs of more than the last cache holds are read past it, if a step is in whole
+// lines (us; past it or not): 16 x 2048 x 2048 float16 82, 92, backwards 146, 160; of
+// less, 1 x 30,000 x 1024 50, 41; of lines that two workgroups read, backwards,
+// 1 x 60,000 x 500 152, 125.
+constexpr double kCaches = 256 << 20;
 
 // Which layout.  A sequence's tiles wait for each other, about 0.4 us a tile, so
 // few groups of channels want long tiles; many want wide ones, whose loads
 // and stores use the memory better.  Forwards (us, float16 unless said; few / long
-// / wide layout): 1 x 50,000 x 100 36 / 58 / 118, 1 x 50,000 x 300 43 / 65 / 116, 1
-// x 60,000 x 1024 116 / 99 / 126, 2 x 16,000 x 1024 60 / 43 / 52, 4 x 8000 x 1024
-// 59 / 41 / 45, 16 x 2000 x 1024 60 / 42 / 41, 64 x 500 x 1024 58 / 39.5 / 39;
-// float32 1 x 60,000 x 1024 215 / 164 / 163, 4 x 8000 x 1024 123 / 86 / 78, 3 x 1999
-// x 1001 37 / 28 / 19.5, 16 x 2000 x 1024 123 / 85 / 72.  Backwards: 1 x 50,000 x
-// 100 47 / 66 / 227, 1 x 50,000 x 300 84 / 77 / 212, 1 x 60,000 x 1024 233 / 173 /
-// 266, 2 x 16,000 x 1024 131 / 97 / 113, 4 x 8000 x 1024 134 / 98 / 94, 3 x 1999 x
-// 1001 43 / 32 / 27, 16 x 2000 x 1024 136 / 96 / 84; float32 1 x 50,000 x 100 55 / 65
-// / 230, 3 x 1999 x 1001 72 / 53 / 34.  Counted in groups of the wide layout, and of
-// the long one for the few.
-// Steps that are one long tile and two wide ones take the long one (256 x 256 x
-// 1024 86 / 94), but in float32 (160 / 147).  Up to 64 steps one tile of the brief
-// layout beats the others: 281 x 48 x 2851 60, 91 in wide ones, 100 x 30 x 1024 12, 16.
+// / wide layout): 1 x 50,000 x 100 36 / 58 / 111, 1 x 50,000 x 300 43 / 65 / 114, 1
+// x 60,000 x 1024 128 / 96 / 122, 2 x 16,000 x 1024 60 / 43 / 53, 4 x 8000 x 1024
+// 59 / 40 / 44, 16 x 2000 x 1024 58 / 41 / 41, 64 x 500 x 1024 58 / 40 / 39, 256 x 256
+// x 1021 168 / 123 / 105; float32 1 x 60,000 x 1024 254 / 157 / 146, 4 x 8000 x 1024
+// 145 / 82 / 73, 3 x 1999 x 1001 37 / 27 / 19, 16 x 2000 x 1024 147 / 82 / 69.
+// Backwards: 1 x 50,000 x 100 47 / 66 / 227, 1 x 50,000 x 300 85 / 78 / 218, 1 x
+// 60,000 x 1024 285 / 165 / 258, 2 x 16,000 x 1024 165 / 95 / 108, 4 x 8000 x 1024 167
+// / 94 / 89, 3 x 1999 x 1001 43 / 31 / 27, 16 x 2000 x 1024 163 / 91 / 80; float32
+// 1 x 50,000 x 100 56 / 65 / 214, 1 x 60,000 x 1024 560 / 291 / 302, 3 x 1999 x 1001
+// 71 / 53 / 34.  Counted in groups of the wide layout, and of the long one for the
+// few.  Up to 64 steps one tile of the brief layout beats the others: 281 x 48 x
+// 2851 60, 89 in wide ones, 100 x 30 x 1024 13, 17.
 template <typename T> constexpr int64_t kForwardWide = sizeof(T) == 4 ? 16 : 64;
 constexpr int64_t kBackwardWide = 12, kForwardFew = 8, kBackwardFew = 5, kManyTiles = 8;
+
+// Whether a call's inputs are read past the caches: more than those hold, in whole
+// lines.
+template <typename T>
+bool past_caches(int arrays, int64_t batch, int64_t steps, int64_t dim) {
+  return dim * (int64_t)sizeof(T) % 128 == 0 &&
+         (double)arrays * (double)batch * (double)steps * (double)dim * sizeof(T) > kCaches;
+}
 
 // The tiles of a call, and their descriptors.
 struct Plan {
@@ -732,7 +732,8 @@ template <typename T, typename L> int look_of(const Plan &p, Look *lk) {
   if (p.tiles == 1) return MMP_OK;
   int st = MMP_OK;
   lk->desc = (unsigned long long *)mmpi::scratch(
-      mmpi::SCRATCH_RECUR_TILES, 8ull * words_of<A>() * L::template channels<T>() * p.tiles * p.groups, &st);
+      mmpi::SCRATCH_RECUR_TILES,
+      8ull * words_of<A>() * L::template channels<T>() * p.tiles * p.groups, &st);
   if (st) return st;
   const mmpi::WaitParams w = mmpi::wait_params();
   lk->gen = mmpi::next_generation();
@@ -766,8 +767,9 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many channels");
-      auto kernel = vec == kVec ? (logits ? k_recur_short<T, true, kVec> : k_recur_short<T, false, kVec>)
-                                : (logits ? k_recur_short<T, true, 1> : k_recur_short<T, false, 1>);
+      auto kernel = vec == kVec
+                        ? (logits ? k_recur_short<T, true, kVec> : k_recur_short<T, false, kVec>)
+                        : (logits ? k_recur_short<T, true, 1> : k_recur_short<T, false, 1>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kShortBlock), 0, mmpi::stream(),
                          (long long)n, (long long)steps, (int)dim, (int)vecs, sg, sx,
                          (const A *)initial, (T *)h, (A *)final_);
@@ -782,7 +784,11 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
       std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
       Look lk;
       if (int st = look_of<T, L>(p, &lk)) return st;
-      auto kernel = logits ? k_recur_tiles<T, true, L> : k_recur_tiles<T, false, L>;
+      auto kernel = past_caches<T>(3, batch, steps, dim)
+                        ? (logits ? k_recur_tiles<T, true, L, true>
+                                  : k_recur_tiles<T, false, L, true>)
+                        : (logits ? k_recur_tiles<T, true, L, false>
+                                  : k_recur_tiles<T, false, L, false>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
                          mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
                          (long long)p.groups, p.cgroups, sg, sx, (const A *)initial, (T *)h,
@@ -790,9 +796,7 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
       return mmpi::check_launch("mmp_recurrence");
     };
     if (steps <= ForwardBrief::tile) return launch(ForwardBrief());
-    const bool one_tile =
-        sizeof(T) != 4 && steps > ForwardWide<T>::tile && steps <= ForwardLong::tile;
-    if (wide >= kForwardWide<T> && !one_tile) return launch(ForwardWide<T>());
+    if (wide >= kForwardWide<T>) return launch(ForwardWide<T>());
     const Plan p = plan<T, ForwardLong>(batch, steps, dim);
     return p.groups < kForwardFew && p.tiles >= kManyTiles ? launch(ForwardFew())
                                                            : launch(ForwardLong());
@@ -824,8 +828,9 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many channels");
-      auto kernel = vec == kVec ? (logits ? k_recur_grad_short<T, true, kVec> : k_recur_grad_short<T, false, kVec>)
-                                : (logits ? k_recur_grad_short<T, true, 1> : k_recur_grad_short<T, false, 1>);
+      auto kernel = vec == kVec
+                        ? (logits ? k_recur_grad_short<T, true, kVec> : k_recur_grad_short<T, false, kVec>)
+                        : (logits ? k_recur_grad_short<T, true, 1> : k_recur_grad_short<T, false, 1>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kShortBlock), 0, mmpi::stream(),
                          (long long)n, (long long)steps, (int)dim, (int)vecs, sd, sg, sx, sh,
                          (const A *)initial, (const A *)grad_final, (T *)grad_gate, (T *)grad_x,
@@ -841,7 +846,11 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
       std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
       Look lk;
       if (int st = look_of<T, L>(p, &lk)) return st;
-      auto kernel = logits ? k_recur_grad_tiles<T, true, L> : k_recur_grad_tiles<T, false, L>;
+      auto kernel = past_caches<T>(logits ? 6 : 5, batch, steps, dim)
+                        ? (logits ? k_recur_grad_tiles<T, true, L, true>
+                                  : k_recur_grad_tiles<T, false, L, true>)
+                        : (logits ? k_recur_grad_tiles<T, true, L, false>
+                                  : k_recur_grad_tiles<T, false, L, false>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kBlock), 0,
                          mmpi::stream(), (long long)steps, (int)dim, (long long)p.tiles,
                          (long long)p.groups, p.cgroups, sd, sg, sx, sh, (const A *)initial,

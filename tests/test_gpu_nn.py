@@ -306,6 +306,27 @@ def test_recurrence_many_sequences(dt, shape):
 
 
 @pytest.mark.parametrize("logits", [True, False])
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+def test_recurrence_past_the_caches(dt, logits):
+    """Arrays of more than 256 MiB, here one sequence that is every sequence."""
+    g = np.random.default_rng(21)
+    batch, steps, dim = (64, 700, 1024) if dt == np.float16 else (64, 350, 1024)
+    gate, x, initial = _sequence(g, (steps, dim), dt, logits)
+    grad = g.standard_normal((steps, dim)).astype(dt)
+    every = lambda a: cp.broadcast_to(cp.array(a), (batch,) + a.shape)  # noqa: E731
+    h, final = nn.gated_recurrence(every(gate), every(x), every(initial), logits=logits)
+    got = nn.gated_recurrence_grad(every(grad), every(gate), every(x), h, every(initial),
+                                   logits=logits)
+    want, last, bound, off = _recur(gate, x, initial, logits, E[dt])
+    wants = [(want, bound), (last, off)]
+    wants += _recur_grad(grad, gate, x, h[0].get(), initial, 0 * initial, logits, E[dt])
+    kinds = (dt, initial.dtype.type, dt, dt, initial.dtype.type)
+    for a, (w, lim), t in zip((h, final) + got, wants, kinds):
+        near(a[0], w, lim, t)
+        assert bool((a == a[:1]).all())
+
+
+@pytest.mark.parametrize("logits", [True, False])
 def test_recurrence_differences(logits):
     """The gradients against central differences of a weighted sum of outputs."""
     g = np.random.default_rng(8)
