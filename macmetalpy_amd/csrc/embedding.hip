@@ -691,8 +691,10 @@ __global__ __launch_bounds__(kBlock) void k_row_sums_few(const I *__restrict__ t
 }
 
 // The rows in windows, of those that begin in kLongWindows windows kLongCols
-// columns a workgroup, whose threads add up windows in kLongParts parts.
-constexpr int kLongWindows = 32, kLongCols = 64, kLongParts = 16;
+// columns a workgroup, whose threads add up windows in kLongParts parts.  Its rows
+// come one after another: with 32 windows a workgroup 478 x 113 by 59,961 tokens
+// take 4 us more.
+constexpr int kLongWindows = 8, kLongCols = 64, kLongParts = 16;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_long_rows(
     int dim, typename Wide<T>::type scale, unsigned window, const Span *__restrict__ span,
@@ -861,10 +863,10 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
   // tokens 30, 39, by 8192 42, 49, by 16,000 54, 56, two rows x 1024 by 4096 27, 27, by
   // 8192 45, 29, by 16,384 85, 32, 200 x 8 by 16,000 25, 58.  Smaller windows are
   // more work at once and more sums to add up (16, 32, 64 places): 5000 x 8 by 131,072
-  // 60, 72, 91, 60,000 x 128 56, 53, 58, 64,000 x 1024 129, 121, 121, 500 x 77 by
-  // 800,000 215, 157, 133.
+  // 60, 72, 91, 478 x 113 by 59,961 45, 58, -, 60,000 x 128 by 131,072 53, 51, 58, 64,000
+  // x 1024 129, 121, 121, 500 x 77 by 800,000 215, 157, 133.
   const bool whole = in_one(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
-  const unsigned window = whole ? 16 : !in_groups(n, rows) ? 64 : lanes <= 8 ? 16 : 32;
+  const unsigned window = whole ? 16 : !in_groups(n, rows) ? 64 : lanes <= 32 ? 16 : 32;
   const int64_t windows = mmpi::ceil_div(n, window);
   const size_t at_part = place(whole ? 0 : (size_t)windows * 2 * dim * sizeof(A));
   const size_t entry_lists = whole ? 0 : in_groups(n, rows) ? 1 : 2;
