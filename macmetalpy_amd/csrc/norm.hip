@@ -5,8 +5,14 @@
 //
 // Squares and sums are held in 64 bits: a float32 gradient's square can
 // overflow 32.  The arrays are cut into chunks; a workgroup sums one, and the
-// chunks' sums are added in their order by one workgroup, so the norm's bits
+// chunks' sums are added in their order by one workgroup (up to 1024 of them by
+// every workgroup of the second pass, which saves a launch), so the norm's bits
 // do not depend on timing.
+//
+// Bound by memory: the limit needs the norm first, so the arrays are read twice
+// and written once.  600,000,011 float16 in 60 arrays 632 us, 5.7 TB/s over the three:
+// 203 squares, 429 scaling, which goes backwards; 60,001 float32 in 40 arrays 4.4 and
+// 4.2, two launches.
 #include "mmp_nn.h"
 
 namespace {

@@ -20,6 +20,10 @@
 // writes.  With few steps, or sequences enough to fill the device with a thread
 // for a few channels, a thread goes through the steps instead.
 //
+// Measured, float16: 16 x 2048 x 2048 backwards 144 us, 5.6 TB/s, forwards 82, 4.9; one
+// sequence of 65,536 x 1024 104 us, 3.9 TB/s: its tiles wait for each other, and
+// only two workgroups a CU have room for what they hold meanwhile.
+//
 // Look-back: a tile publishes (A, B) and, as soon as it knows it, the state
 // after its last step.  It reads the kLook tiles before it until one of them
 // has that state and all after it have (A, B), and goes through those in
@@ -206,6 +210,7 @@ template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ typename Vec<T, V>::Words load_words(const T *p) {
   return mmpn::words_of<T, V>(mmpn::load_vec<T, V, STREAM>(p));
 }
+// Past the caches: 64 x 500 x 1024 float16 39 us, through them 46.
 template <typename T, int V>
 __device__ __forceinline__ void store_some(T *p, const Vec<T, V> &v, int count) {
   if (count >= V) {
@@ -522,7 +527,10 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
       if (k < count) grad_initial[pl.seq * dim + ch + k] = carry[k];
 }
 
-// Few steps: a thread per V channels goes through them.
+// A thread per V channels goes through the steps, with the next kAhead on their
+// way.  They are kept as words: float16 elements would be unpacked, and so waited
+// for, before those on hand are used (64 x 500 x 1024 544 us instead of 121).  One
+// step of 200 x 2048 float16 4 us, 253 x 170 x 1390 92 us, 3.9 TB/s.
 constexpr int kShortBlock = 256, kAhead = 4, kAheadGrad = 2;
 template <typename T, bool LOGITS, int V>
 __global__ __launch_bounds__(kShortBlock) void k_recur_short(
