@@ -500,9 +500,10 @@ int mmp_embedding(int dtype, int index_dtype, int64_t n, const void *tokens,
                   int64_t rows, int64_t dim, const void *table, int64_t row_stride,
                   double scale, void *out);
 
-/* out[v] = scale * the sum of grad[i] over the tokens i equal to v, in order
- * of i, v < rows; a token outside [0, rows) adds nothing.  n, rows and dim are
- * below 2^31.  Takes memory from the allocator for the call. */
+/* out[v] = scale * the sum of grad[i] over the tokens i equal to v, v < rows,
+ * added in an order that the tokens alone decide; a token outside [0, rows) adds
+ * nothing.  n, rows and dim are below 2^31.  Takes memory from the allocator for
+ * the call. */
 int mmp_embedding_grad(int dtype, int index_dtype, int64_t n, const void *tokens,
                        const void *grad, int64_t row_stride, int64_t rows,
                        int64_t dim, double scale, void *out);
@@ -529,7 +530,8 @@ int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t steps, int
 /* loss[r] = log(sum exp(x)) - x[targets[r]] (wide) of each row x of logits, and
  * where grad is not NULL grad[r] = w (softmax(x) - onehot(targets[r])) with
  * w = scale * weight[r] (wide; NULL for ones).  A target outside [0, classes)
- * gives a loss and a gradient of 0.  classes >= 1. */
+ * gives a loss and a gradient of 0.  classes >= 1.  Few long rows take memory
+ * from the allocator for the call. */
 int mmp_cross_entropy(int dtype, int index_dtype, int64_t rows, int64_t classes,
                       const void *logits, int64_t row_stride, const void *targets,
                       const void *weight, double scale, void *loss, void *grad);

@@ -1,11 +1,12 @@
 // embedding.hip -- rows of a table by tokens, scaled, and the gradient.
 //
 //   out[i]  = scale * table[tok[i]]
-//   grad[v] = scale * sum over i with tok[i] = v, in order of i, of g[i]
+//   grad[v] = scale * sum over i with tok[i] = v of g[i]
 //
 // A token outside [0, rows) is none: its output is zeros and it has no
 // gradient, so ragged batches can be filled up with -1.  Sums are held in 32
-// bits (64 for float64) and rounded once.
+// bits (64 for float64), added in an order that the tokens alone decide, and
+// rounded once.
 //
 // Both are bound by memory.  The gradient first brings the tokens' positions of
 // each row together, ascending, so that the sums keep their bits.  One pass of a
@@ -15,9 +16,9 @@
 // be one workgroup's.  That orders a group's by row with counters in LDS.  More
 // than 2^20 rows are too many for those, and of more than 2^17 tokens a workgroup
 // has too many: then every 8 bits of the row have a pass (8 columns; groups and
-// passes, of 60,000 rows: 60,000 tokens 59 and 70 us, 131,072 73 and 77, 262,144
-// 100 and 92, 524,288 132 and 107; of a million rows: 85 and 104, 108 and 109, 146
-// and 132, 207 and 159).
+// passes, of 60,000 rows: 60,000 tokens 42 and 51 us, 131,072 52 and 58, 200,000 61
+// and 67, 262,144 79 and 71, 524,288 118 and 94; of a million rows: 66 and 87, 87
+// and 92, 109 and 102, 122 and 110, 186 and 136).
 //
 // Then a few lanes sum a row's positions.  Words' frequencies are skewed: a row
 // of more than a window's positions is summed in windows of places of the
@@ -868,10 +869,11 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
   // tokens 30, 39, by 8192 42, 49, by 16,000 54, 56, two rows x 1024 by 4096 27, 27, by
   // 8192 45, 29, by 16,384 85, 32, 200 x 8 by 16,000 25, 58.  Smaller windows are
   // more work at once and more sums to add up (16, 32, 64 places): 5000 x 8 by 131,072
-  // 60, 72, 91, 478 x 113 by 59,961 45, 58, -, 60,000 x 128 by 131,072 53, 51, 58, 64,000
-  // x 1024 129, 121, 121, 500 x 77 by 800,000 215, 157, 133.
+  // 60, 69, 85, 478 x 113 by 59,961 45, 58, 72, 60,000 x 128 by 131,072 53, 50, 56, 64,000
+  // x 1024 132, 121, 120, 60,000 x 8 by 524,288 95, 92, 106, 500 x 77 by 800,000 213, 158,
+  // 133.
   const bool whole = in_one(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
-  const unsigned window = whole ? 16 : !in_groups(n, rows) ? 64 : lanes <= 32 ? 16 : 32;
+  const unsigned window = n > 1 << 19 ? 64 : whole || n * lanes <= 1 << 20 ? 16 : 32;
   const int64_t windows = mmpi::ceil_div(n, window);
   const size_t at_part = place(whole ? 0 : (size_t)windows * 2 * dim * sizeof(A));
   const size_t entry_lists = whole ? 0 : in_groups(n, rows) ? 1 : 2;

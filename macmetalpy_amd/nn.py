@@ -138,8 +138,8 @@ def embedding(table, tokens, scale=1.0) -> ndarray:
 def embedding_grad(grad, tokens, rows, scale=1.0) -> ndarray:
     """The gradient of :func:`embedding` with respect to its (rows, dim)
     table, whole: row v is ``scale`` times the sum of ``grad`` over the tokens
-    equal to v, in their order.  ``grad`` has shape ``tokens.shape + (dim,)``
-    and gives the type."""
+    equal to v, added in an order that the tokens alone decide.  ``grad`` has
+    shape ``tokens.shape + (dim,)`` and gives the type."""
     grad, tokens = _floating(grad, "grad"), _integers(tokens, "tokens")
     if grad.ndim == 0 or grad._shape[:-1] != tokens._shape:
         raise ValueError(f"grad of shape {grad._shape} does not fit tokens of shape "
