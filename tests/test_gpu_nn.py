@@ -289,7 +289,9 @@ def test_recurrence_grad(shape, dt, logits):
     (np.float16, (300, 70, 1001)), (np.float32, (150, 70, 1001)), (np.float64, (66, 67, 1001)),
     (np.float16, (300, 16, 1001)), (np.float16, (300, 15, 3)), (np.float16, (20, 64, 3)),
     (np.float16, (20, 200, 7)), (np.float32, (20, 200, 1)), (np.float32, (20, 400, 1001)),
-    (np.float16, (40, 400, 1001)), (np.float64, (20, 300, 1001))], **by_name)
+    (np.float16, (40, 400, 1001)), (np.float64, (20, 300, 1001)), (np.float16, (70, 700, 30)),
+    (np.float16, (30, 700, 65)), (np.float32, (70, 700, 15)), (np.float32, (70, 300, 64))],
+    **by_name)
 def test_recurrence_many_sequences(dt, shape):
     """Sequences enough for a thread to go through its channels' steps, odd rows."""
     g = np.random.default_rng(shape[0])
