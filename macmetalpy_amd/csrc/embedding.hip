@@ -826,8 +826,8 @@ int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *e
     return mmpi::check_launch("mmp_embedding_grad(group)");
   }
   if (int st = pass(Tokens<I>{tokens, n, rows}, 0, ea)) return st;
-  for (int shift = 8; (rows - 1) >> shift; shift += 8) {
-    if (int st = pass(Entries{ea, first + kDigits}, shift, eb)) return st;
+  for (int p = 1; p < mmpi::row_passes(rows); ++p) {
+    if (int st = pass(Entries{ea, first + kDigits}, 8 * p, eb)) return st;
     Entry *t = ea;
     ea = eb;
     eb = t;

@@ -14,6 +14,13 @@ enum { SCRATCH_REDUCE_PARTIALS = 0, SCRATCH_REDUCE_TICKETS = 1,
        SCRATCH_SCAN_COUNTER = 4, SCRATCH_REDUCE_PLAIN = 5, SCRATCH_RECUR_TILES = 6,
        SCRATCH_NSLOTS = 7 };
 
+// Passes of 8 bits each that order row numbers below `rows`, at most 2^32.
+inline int row_passes(long long rows) {
+  int passes = 1;
+  while ((rows - 1) >> (8 * passes)) ++passes;
+  return passes;
+}
+
 // HIP counts at most 2^32 - 1 work-items per grid dimension.
 inline bool grid_fits(long long blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
 
