@@ -539,8 +539,9 @@ int mmp_cross_entropy(int dtype, int index_dtype, int64_t rows, int64_t classes,
 /* norm = sqrt(sum of the squares of all `count` arrays of sizes[i] contiguous
  * elements of dtypes[i]), stored as norm_dtype (MMP_F32 or MMP_F64), summed in
  * double; where outs is not NULL, outs[i] = arrays[i] * min(1, limit / norm)
- * (outs[i] may be arrays[i]; NaN where the norm is NaN).  limit >= 0.  Takes
- * memory from the allocator for the call. */
+ * (outs[i] may be arrays[i], but MMP_E_ARG where an output overlaps a part of
+ * it or another array; NaN where the norm is NaN).  limit >= 0.  Takes memory
+ * from the allocator for the call. */
 int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *sizes,
                   const void *const *arrays, void *const *outs, double limit,
                   int norm_dtype, void *norm);

@@ -1,6 +1,7 @@
 // mmp_plan.h -- launch plans as plain host arithmetic: no HIP, so that the
 // rules can be compiled and tested without a device.
 #pragma once
+#include <algorithm>
 
 namespace mmpi {
 
@@ -19,6 +20,26 @@ inline int row_passes(long long rows) {
   int passes = 1;
   while ((rows - 1) >> (8 * passes)) ++passes;
   return passes;
+}
+
+// Memory that a call reads or writes.
+struct Extent {
+  unsigned long long from, to;  // addresses, the second past the end
+  bool written;
+};
+// Whether one of `n` extents is written and shares memory with another.  Sorts
+// them: behind the ends of all before it, and of the written ones, each needs one
+// look.
+inline bool written_overlap(Extent *e, long long n) {
+  std::sort(e, e + n, [](const Extent &a, const Extent &b) { return a.from < b.from; });
+  unsigned long long any = 0, written = 0;
+  for (long long i = 0; i < n; ++i) {
+    if (e[i].from == e[i].to) continue;
+    if (e[i].from < (e[i].written ? any : written)) return true;
+    any = any > e[i].to ? any : e[i].to;
+    if (e[i].written) written = written > e[i].to ? written : e[i].to;
+  }
+  return false;
 }
 
 // HIP counts at most 2^32 - 1 work-items per grid dimension.

@@ -13,6 +13,13 @@
 // and written once.  600,000,011 float16 in 60 arrays 632 us, 5.7 TB/s over the three:
 // 203 squares, 429 scaling, which goes backwards; 60,001 float32 in 40 arrays 4.4 and
 // 4.2, two launches.
+//
+// A chunk is read and written by its own workgroup, so an array may be scaled in
+// place, but memory that two of them share would be scaled once or twice, by
+// timing.  The host refuses that.
+#include <memory>
+#include <new>
+
 #include "mmp_nn.h"
 
 namespace {
@@ -185,6 +192,25 @@ struct Temp {
   int get(size_t bytes) { return mmp_alloc(bytes ? bytes : 1, &p); }
 };
 
+// Refuses outputs that share memory with another array's input or output, or
+// with a part of their own input.
+int check_outs(int64_t count, const int *dtypes, const int64_t *sizes, const void *const *arrays,
+               void *const *outs) {
+  std::unique_ptr<mmpi::Extent[]> extents(new (std::nothrow) mmpi::Extent[2 * count]);
+  if (!extents) return mmpi::fail(MMP_E_OOM, "mmp_clip_norm: %lld arrays", (long long)count);
+  int64_t n = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const unsigned long long in = (uintptr_t)arrays[i], out = (uintptr_t)outs[i];
+    const unsigned long long bytes =
+        (unsigned long long)sizes[i] * (dtypes[i] == MMP_F16 ? 2 : dtypes[i] == MMP_F32 ? 4 : 8);
+    extents[n++] = {out, out + bytes, true};
+    if (in != out) extents[n++] = {in, in + bytes, false};
+  }
+  if (mmpi::written_overlap(extents.get(), n))
+    return mmpi::fail(MMP_E_ARG, "mmp_clip_norm: an output overlaps another array");
+  return MMP_OK;
+}
+
 }  // namespace
 
 extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *sizes,
@@ -206,6 +232,8 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
       return mmpi::fail(MMP_E_ARG, "mmp_clip_norm: null pointer");
     total += sizes[i];
   }
+  if (outs && count > 0)
+    if (int st = check_outs(count, dtypes, sizes, arrays, outs)) return st;
   // About 4096 chunks, of 4096 elements at least.
   int64_t chunk = mmpi::ceil_div(mmpi::ceil_div(total, 4096), 4096) * 4096;
   if (chunk == 0) chunk = 4096;

@@ -341,7 +341,8 @@ def clip_by_global_norm(arrays, max_norm, out=None):
     """``(clipped, norm)``: the arrays scaled by ``min(1, max_norm / norm)``,
     a list in their order and types, and their :func:`global_norm` before.
     ``out`` is a list of arrays to write (the same arrays, to clip them in
-    place; otherwise none may overlap another).  A norm of NaN makes everything NaN."""
+    place; one that overlaps another array, as tied weights' gradients given
+    twice do, is an error).  A norm of NaN makes everything NaN."""
     limit = _scalar(max_norm, "max_norm")
     if not limit >= 0 or math.isnan(limit):
         raise ValueError(f"max_norm must not be negative or NaN: {max_norm}")

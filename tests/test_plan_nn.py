@@ -5,6 +5,7 @@ import os
 import shutil
 import subprocess
 
+import numpy as np
 import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "macmetalpy_amd",
@@ -13,6 +14,13 @@ SOURCE = r"""
 #include "mmp_plan.h"
 extern "C" {
 int t_row_passes(long long rows) { return mmpi::row_passes(rows); }
+// extents as triples (from, to, written)
+int t_overlap(const long long *e, int n) {
+  mmpi::Extent x[64];
+  for (int i = 0; i < n; ++i)
+    x[i] = {(unsigned long long)e[3 * i], (unsigned long long)e[3 * i + 1], e[3 * i + 2] != 0};
+  return mmpi::written_overlap(x, n);
+}
 }
 """
 
@@ -37,3 +45,19 @@ def test_row_passes_cover_the_rows_and_end(plans, rows):
     bits that they are held in."""
     got = plans.t_row_passes(ctypes.c_longlong(rows))
     assert got == max(1, -(-(rows - 1).bit_length() // 8)) <= 4
+
+
+def test_written_overlap(plans):
+    """Against every pair of extents, one of which is written."""
+    g = np.random.default_rng(5)
+    seen = [0, 0]
+    for _ in range(4000):
+        n = int(g.integers(1, 12))
+        at = g.integers(0, 60, n)
+        e = [(int(a), int(a + g.integers(0, 9)), int(g.integers(0, 2))) for a in at]
+        want = any((a[2] or b[2]) and max(a[0], b[0]) < min(a[1], b[1])
+                   for i, a in enumerate(e) for b in e[:i])
+        flat = (ctypes.c_longlong * (3 * n))(*[v for x in e for v in x])
+        assert plans.t_overlap(flat, n) == want, e
+        seen[want] += 1
+    assert min(seen) > 500
