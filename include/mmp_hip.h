@@ -489,9 +489,12 @@ int mmp_matmul_t(int dtype, int trans_a, int trans_b, int64_t batch, int64_t M,
 /* users write them with take, cumsum, max / sum and one reduction per      */
 /* array.  dtype: MMP_F16, MMP_F32 or MMP_F64; "wide" is double for MMP_F64 */
 /* and float otherwise, the type of sums, states and statistics.  Index     */
-/* dtypes: MMP_I32 or MMP_I64.  Outputs are contiguous; row strides, and    */
-/* sb / st, the strides of sequences and steps, are in elements, and the    */
-/* elements of a row or step are adjacent.                                  */
+/* dtypes: MMP_I32 or MMP_I64.  Outputs are contiguous and overlap neither  */
+/* inputs nor each other; row strides, and sb / st, the strides of          */
+/* sequences and steps, are in elements, and the elements of a row or step  */
+/* are adjacent.  While the stream is captured into a graph, calls that     */
+/* would take scratch memory fail with MMP_E_UNSUPPORTED: its replays       */
+/* outlive that memory.                                                     */
 /* ======================================================================== */
 
 /* out[i] = scale * table[tokens[i]], i < n, rows of dim elements; zeros for a
@@ -502,8 +505,8 @@ int mmp_embedding(int dtype, int index_dtype, int64_t n, const void *tokens,
 
 /* out[v] = scale * the sum of grad[i] over the tokens i equal to v, v < rows,
  * added in an order that the tokens alone decide; a token outside [0, rows) adds
- * nothing.  n, rows and dim are below 2^31.  Takes memory from the allocator for
- * the call. */
+ * nothing.  n, rows and dim are below 2^31.  More than 128 tokens take memory
+ * from the allocator for the call. */
 int mmp_embedding_grad(int dtype, int index_dtype, int64_t n, const void *tokens,
                        const void *grad, int64_t row_stride, int64_t rows,
                        int64_t dim, double scale, void *out);
@@ -511,14 +514,15 @@ int mmp_embedding_grad(int dtype, int index_dtype, int64_t n, const void *tokens
 /* h_t = f_t h_{t-1} + u_t along the steps of (batch, steps, dim) arrays, where
  * logits != 0 means f = 1 / (1 + exp(-gate)), u = (1 - f) x, and 0 f = gate,
  * u = x.  initial (h_{-1}; NULL for zeros) and final (the last state, or
- * initial where there are no steps) are (batch, dim) of the wide type. */
+ * initial where there are no steps) are (batch, dim) of the wide type.  Up to 16
+ * steps take no scratch memory, longer sequences may. */
 int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t steps, int64_t dim,
                    const void *gate, int64_t gate_sb, int64_t gate_st,
                    const void *x, int64_t x_sb, int64_t x_st,
                    const void *initial, void *h, void *final_state);
 
 /* Its gradient, from grad (of h), grad_final (of final; NULL for zeros), the
- * inputs and h. */
+ * inputs and h.  Up to 16 steps take no scratch memory, longer sequences may. */
 int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t steps, int64_t dim,
                         const void *grad, int64_t grad_sb, int64_t grad_st,
                         const void *gate, int64_t gate_sb, int64_t gate_st,
@@ -531,7 +535,7 @@ int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t steps, int
  * where grad is not NULL grad[r] = w (softmax(x) - onehot(targets[r])) with
  * w = scale * weight[r] (wide; NULL for ones).  A target outside [0, classes)
  * gives a loss and a gradient of 0.  classes >= 1.  Few long rows take memory
- * from the allocator for the call. */
+ * from the allocator for the call, except while the stream is captured. */
 int mmp_cross_entropy(int dtype, int index_dtype, int64_t rows, int64_t classes,
                       const void *logits, int64_t row_stride, const void *targets,
                       const void *weight, double scale, void *loss, void *grad);

@@ -765,15 +765,6 @@ inline int row_lanes(int64_t dim, int vec) {
   return lanes;
 }
 
-// Temporaries from the library's stream-ordered pool, released on scope exit.
-struct Temp {
-  void *p = nullptr;
-  ~Temp() {
-    if (p) (void)mmp_free(p);
-  }
-  int get(size_t bytes) { return mmp_alloc(bytes ? bytes : 1, &p); }
-};
-
 constexpr int64_t kMost = 0x7fff0000LL;  // room for a step past the end in 32 bits
 
 constexpr int64_t kGroupTokens = 1 << 17;
@@ -857,7 +848,7 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
   }
   // One block for all: sums of windows, entries, places of rows, the order,
   // rows that begin in windows, counts of tiles, beginnings of groups.
-  Temp temp;
+  mmpn::Temp temp;
   size_t size = 0;
   auto place = [&](size_t bytes) {
     const size_t at = size;
@@ -881,7 +872,7 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
   const size_t at_span = place((size_t)rows * sizeof(Span));
   const size_t at_order = place((size_t)n * 4), at_begins = place((size_t)windows * 4);
   const size_t at_count = place(kMaxTiles * kDigits * 4), at_first = place((kDigits + 1) * 4);
-  if (int st = temp.get(size)) return st;
+  if (int st = temp.get(size, "mmp_embedding_grad")) return st;
   char *base = (char *)temp.p;
   A *part = (A *)(base + at_part);
   Entry *entries = (Entry *)(base + at_entries);

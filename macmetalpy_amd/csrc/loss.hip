@@ -371,15 +371,6 @@ template <typename T, int L, bool GRAD> int launch_pass(const Loss<T> &p) {
   return mmpi::check_launch("mmp_cross_entropy(pass)");
 }
 
-// Temporaries from the library's stream-ordered pool, released on scope exit.
-struct Temp {
-  void *p = nullptr;
-  ~Temp() {
-    if (p) (void)mmp_free(p);
-  }
-  int get(size_t bytes) { return mmp_alloc(bytes ? bytes : 1, &p); }
-};
-
 template <typename T> int loss_impl(const Loss<T> &p) {
   typedef typename Wide<T>::type A;
   // Vectors of a row wherever it begins: one more than fit its length.
@@ -389,12 +380,13 @@ template <typename T> int loss_impl(const Loss<T> &p) {
   // two launches take 13 us (17 with the gradient; whole call, few rows), one
   // workgroup for a row of so many 16-byte vectors (us; loss alone, with gradient):
   // 4096 10, 13; 6250 12, 14; 12,500 18, 17 to 20; 32,500 32, 32.  With the
-  // gradient of 250 rows of 16,250 two parts a row take 40, one 32.
+  // gradient of 250 rows of 16,250 two parts a row take 40, one 32.  Never while the
+  // stream is captured, as the parts' statistics are in memory of this call.
   int64_t parts = 2 * cus / p.rows;
   if (parts > vecs / 1024) parts = vecs / 1024;
-  if (p.grad ? parts >= 3 && vecs >= 12288 : parts >= 2 && vecs >= 8192) {
-    Temp part;
-    if (int st = part.get((size_t)(p.rows * parts) * sizeof(Stat<A>))) return st;
+  if ((p.grad ? parts >= 3 && vecs >= 12288 : parts >= 2 && vecs >= 8192) && !mmpn::capturing()) {
+    mmpn::Temp part;
+    if (int st = part.get((size_t)(p.rows * parts) * sizeof(Stat<A>), "mmp_cross_entropy")) return st;
     hipLaunchKernelGGL((k_loss_part<T>), dim3((unsigned)(p.rows * parts)), dim3(kPartBlock), 0,
                        mmpi::stream(), p, (int)parts, (Stat<A> *)part.p);
     if (int st = mmpi::check_launch("mmp_cross_entropy(part)")) return st;

@@ -128,6 +128,31 @@ template <typename T, typename A> __device__ __forceinline__ void sigmoid_pair(A
   u = g < 0 ? r : s;
 }
 
+// Whether the library's stream is being captured into a graph.  Its replays
+// outlive the call: memory of the pool is another array's by then, and a tag
+// fixed at capture time no longer tells a replay's words from the ones before.
+inline bool capturing() {
+  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(mmpi::stream(), &s) == hipSuccess) return s != hipStreamCaptureStatusNone;
+  (void)hipGetLastError();
+  return true;
+}
+inline int refuse_capture(const char *what) {
+  return mmpi::fail(MMP_E_UNSUPPORTED, "%s: takes scratch memory, so it cannot be captured", what);
+}
+
+// Memory of the library's stream-ordered pool for the length of a call.
+struct Temp {
+  void *p = nullptr;
+  ~Temp() {
+    if (p) (void)mmp_free(p);
+  }
+  int get(size_t bytes, const char *what) {
+    if (capturing()) return refuse_capture(what);
+    return mmp_alloc(bytes ? bytes : 1, &p);
+  }
+};
+
 }  // namespace mmpn
 
 // Dispatch a floating dtype code onto a C++ type `T`.

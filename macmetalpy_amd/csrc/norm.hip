@@ -184,14 +184,6 @@ __global__ __launch_bounds__(kBlock) void k_clip(Table t, long long chunk_len, d
   }
 }
 
-struct Temp {
-  void *p = nullptr;
-  ~Temp() {
-    if (p) (void)mmp_free(p);
-  }
-  int get(size_t bytes) { return mmp_alloc(bytes ? bytes : 1, &p); }
-};
-
 // Refuses outputs that share memory with another array's input or output, or
 // with a part of their own input.
 int check_outs(int64_t count, const int *dtypes, const int64_t *sizes, const void *const *arrays,
@@ -239,8 +231,8 @@ extern "C" int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *si
   if (chunk == 0) chunk = 4096;
   int64_t chunks = 0;
   for (int64_t i = 0; i < count; ++i) chunks += mmpi::ceil_div(sizes[i], chunk);
-  Temp part;
-  if (int st = part.get((size_t)(chunks + 1) * 8)) return st;
+  mmpn::Temp part;
+  if (int st = part.get((size_t)(chunks + 1) * 8, "mmp_clip_norm")) return st;
   double *sums = (double *)part.p, *full = sums + chunks;
   const bool wide = norm_dtype == MMP_F64;
   if (chunks > 0x7fffffffLL) return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_clip_norm: too many arrays");

@@ -73,7 +73,9 @@ template <typename T> struct Steps {
 // a word with a tag above: generation << 2 | state, 1 for (A, B), 2 for the
 // state after the tile.  Words are written and read with relaxed atomics
 // and taken only where all tags of a channel agree and are this call's, so
-// they are never cleared and need no fence.
+// they are never cleared and need no fence.  The replays of a graph would all
+// have the tag of its capture and take the states of the replay before, so a
+// call of more than one tile refuses to be captured.
 struct Look {
   unsigned long long *desc;
   unsigned gen;       // this call's
@@ -743,10 +745,11 @@ template <typename T, typename L> Plan plan(int64_t batch, int64_t steps, int64_
   p.groups = batch * p.cgroups;
   return p;
 }
-template <typename T, typename L> int look_of(const Plan &p, Look *lk) {
+template <typename T, typename L> int look_of(const Plan &p, const char *what, Look *lk) {
   typedef typename Wide<T>::type A;
   *lk = Look{nullptr, 0, 0, 0};
   if (p.tiles == 1) return MMP_OK;
+  if (mmpn::capturing()) return mmpn::refuse_capture(what);
   int st = MMP_OK;
   lk->desc = (unsigned long long *)mmpi::scratch(
       mmpi::SCRATCH_RECUR_TILES,
@@ -800,7 +803,7 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many tiles");
       std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
       Look lk;
-      if (int st = look_of<T, L>(p, &lk)) return st;
+      if (int st = look_of<T, L>(p, "mmp_recurrence", &lk)) return st;
       auto kernel = past_caches<T>(3, batch, steps, dim)
                         ? (logits ? k_recur_tiles<T, true, L, true>
                                   : k_recur_tiles<T, false, L, true>)
@@ -864,7 +867,7 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence_grad: too many tiles");
       std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
       Look lk;
-      if (int st = look_of<T, L>(p, &lk)) return st;
+      if (int st = look_of<T, L>(p, "mmp_recurrence_grad", &lk)) return st;
       auto kernel = past_caches<T>(logits ? 6 : 5, batch, steps, dim)
                         ? (logits ? k_recur_grad_tiles<T, true, L, true>
                                   : k_recur_grad_tiles<T, false, L, true>)
