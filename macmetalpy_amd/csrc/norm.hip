@@ -161,6 +161,16 @@ __global__ __launch_bounds__(kBlock) void k_clip(Table t, long long chunk_len, d
   // a norm that is NaN scales by NaN: a broken step shows
   const A by = (A)(n <= limit ? 1.0 : limit / n);
   if (by == 1 && y0 == c.x) return;  // in place, and nothing to change
+  // A factor below the normal range has few bits or none, though its products
+  // need not be below: large elements, a small limit.  Those are divided and
+  // multiplied in 64 bits.  (float16 ones would all be 0.)
+  if constexpr (sizeof(T) > 2) {
+    if (limit > 0 && by < (A)(sizeof(T) == 4 ? 0x1p-126 : 0x1p-1022)) {
+      for (long long i = threadIdx.x; i < c.to - c.from; i += kBlock)
+        y0[i] = (T)((double)c.x[i] / n * limit);
+      return;
+    }
+  }
   auto scaled = [&](const Vec<T, V> &v) {
     Vec<T, V> r;
 #pragma unroll

@@ -54,3 +54,28 @@ def test_clip_refuses_outputs_that_overlap():
     parts = [a[:10], a[10:10], a[10:11], a[11:]]     # side by side, one of them empty
     nn.clip_by_global_norm(parts, 1.0, out=parts)
     assert np.allclose(a.get(), h / np.linalg.norm(h), rtol=1e-6)
+
+
+@pytest.mark.parametrize("dt,size,limits", [
+    (np.float32, 1e38, (1.0, 1e-2, 1e-3, 1e-5, 1e-20, 3e-36)),
+    (np.float64, 1e150, (1.0, 1e-150, 1e-160, 1e-200, 1e-290))],
+    ids=["float32", "float64"])
+def test_clip_factors_below_the_normal_range(dt, size, limits):
+    """limit / norm has few bits or none as a number of the arrays' type, the
+    results have all of theirs: a product of two factors of one rounding each."""
+    g = np.random.default_rng(60)
+    host = [(g.uniform(0.5, 1.0, n) * g.choice([-1, 1], n) * size).astype(dt) for n in (9001, 7, 1030)]
+    host[1][3] = 0.0
+    norm = np.sqrt(sum(((h.astype(np.float64) / size) ** 2).sum() for h in host))
+    for limit in limits:
+        clipped, got = nn.clip_by_global_norm([cp.array(h) for h in host], limit)
+        same = [cp.array(h) for h in host]
+        nn.clip_by_global_norm(same, limit, out=same)
+        if dt == np.float64:
+            assert np.isclose(float(got.get()), norm * size, rtol=1e-12)
+        for c, s, h in zip(clipped, same, host):
+            want = h.astype(np.float64) / size / norm * limit
+            off = np.abs(c.get().astype(np.float64) - want)
+            # the factor's rounding and the result's; the norm's sum of 10^4 squares
+            assert (off <= (2.5 * np.finfo(dt).eps + 1e-13) * np.abs(want)).all(), limit
+            assert np.array_equal(s.get(), c.get())
