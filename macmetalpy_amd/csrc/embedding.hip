@@ -70,7 +70,8 @@ __global__ __launch_bounds__(kBlock) void k_embed(const I *__restrict__ tokens, 
 }
 
 // ---------------------------------------------------------------- grouping
-constexpr int kDigits = 256, kMaxTiles = 256;
+using mmpi::kDigits;
+constexpr int kMaxTiles = 256;
 constexpr int kSplitBlock = 1024, kSplitWaves = kSplitBlock / 64;
 
 // A token's position and row.
@@ -248,7 +249,8 @@ struct Span {
 // looks for its own among all n tokens, at most 64 * kKept a wave, and
 // workgroup 0 writes first[256] (two launches less: 2000 tokens of 60,000 x 8
 // 34 to 19 us, 16,000 45 to 32).
-constexpr int kGroupBlock = 1024, kGroupRows = 4096, kKept = 16;
+using mmpi::kGroupBlock;
+using mmpi::kKept;
 template <typename S>
 __global__ __launch_bounds__(kGroupBlock) void k_group(const S *__restrict__ src, unsigned n,
                                                        unsigned *__restrict__ first,
@@ -256,7 +258,8 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const S *__restrict__ src
                                                        int waves, Span *__restrict__ span,
                                                        unsigned *__restrict__ order) {
   constexpr bool kSplit = __is_same(S, Entry);
-  extern __shared__ unsigned next[];  // [waves][bins]
+  // [waves][bins], 64 KiB at most; with the others up to 192 bytes more, of a CU's 160 KiB
+  extern __shared__ unsigned next[];
   __shared__ unsigned part[kGroupBlock / 64], low[kGroupBlock / 64], all[kGroupBlock / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (unsigned k = tid; k < waves * bins; k += kGroupBlock) next[k] = 0;
@@ -767,19 +770,6 @@ inline int row_lanes(int64_t dim, int vec) {
 
 constexpr int64_t kMost = 0x7fff0000LL;  // room for a step past the end in 32 bits
 
-constexpr int64_t kGroupTokens = 1 << 17;
-inline bool in_groups(int64_t n, int64_t rows) {
-  return n <= kGroupTokens && rows <= (int64_t)kDigits * kGroupRows;
-}
-
-// Waves of k_group that have counters, of 64 KiB at most.
-inline int group_waves(int64_t rows) {
-  return rows > 2048 * kDigits ? 4 : rows > 1024 * kDigits ? 8 : 16;
-}
-inline bool in_one(int64_t n, int64_t rows) {
-  return in_groups(n, rows) && n <= group_waves(rows) * 64 * kKept;
-}
-
 // Orders the tokens' positions by row; ea, eb: room for n entries each.
 template <typename I>
 int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *eb, unsigned *count,
@@ -799,14 +789,14 @@ int order_tokens(unsigned n, const I *tokens, unsigned rows, Entry *ea, Entry *e
                        tile, shift, tiles > 1 ? (const unsigned *)count : nullptr, first, out);
     return mmpi::check_launch("mmp_embedding_grad(split)");
   };
-  if (in_groups(n, rows)) {
-    const unsigned bins = (unsigned)mmpi::ceil_div(rows, kDigits);
+  if (mmpi::in_groups(n, rows)) {
+    const unsigned bins = (unsigned)mmpi::group_bins(rows);
     int bits = 0;
     while ((bins - 1) >> bits) ++bits;
-    const int waves = group_waves(rows);
+    const int waves = mmpi::group_waves(rows);
     const dim3 grid(rows < kDigits ? rows : kDigits);
     const unsigned lds = (unsigned)waves * bins * 4;
-    if (in_one(n, rows)) {
+    if (mmpi::in_one_group_pass(n, rows)) {
       hipLaunchKernelGGL((k_group<I>), grid, dim3(kGroupBlock), lds, mmpi::stream(), tokens, n,
                          first, rows, bins, bits, waves, span, order);
     } else {
@@ -863,11 +853,11 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
   // 60, 69, 85, 478 x 113 by 59,961 45, 58, 72, 60,000 x 128 by 131,072 53, 50, 56, 64,000
   // x 1024 132, 121, 120, 60,000 x 8 by 524,288 95, 92, 106, 500 x 77 by 800,000 213, 158,
   // 133.
-  const bool whole = in_one(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
+  const bool whole = mmpi::in_one_group_pass(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
   const unsigned window = n > 1 << 19 ? 64 : whole || n * lanes <= 1 << 20 ? 16 : 32;
   const int64_t windows = mmpi::ceil_div(n, window);
   const size_t at_part = place(whole ? 0 : (size_t)windows * 2 * dim * sizeof(A));
-  const size_t entry_lists = whole ? 0 : in_groups(n, rows) ? 1 : 2;
+  const size_t entry_lists = whole ? 0 : mmpi::in_groups(n, rows) ? 1 : 2;
   const size_t at_entries = place((size_t)n * sizeof(Entry) * entry_lists);
   const size_t at_span = place((size_t)rows * sizeof(Span));
   const size_t at_order = place((size_t)n * 4), at_begins = place((size_t)windows * 4);

@@ -22,6 +22,26 @@ inline int row_passes(long long rows) {
   return passes;
 }
 
+// Tokens ordered by row in groups of the rows with equal low 8 bits, a workgroup
+// a group: its rows are counted in LDS, by each of `waves` waves in counters of
+// its own, as many waves as have room in 64 KiB.  Too many rows or tokens for
+// that have a pass for every 8 bits instead (measured beside the kernels).
+constexpr int kDigits = 256, kGroupBlock = 1024;
+constexpr int kKept = 16;  // entries of a lane that stay in registers
+constexpr int kGroupRows = 4096;
+constexpr long long kGroupTokens = 1 << 17;
+inline bool in_groups(long long n, long long rows) {
+  return n <= kGroupTokens && rows <= (long long)kDigits * kGroupRows;
+}
+inline long long group_bins(long long rows) { return (rows + kDigits - 1) / kDigits; }
+inline int group_waves(long long rows) {
+  return rows > 2048 * kDigits ? 4 : rows > 1024 * kDigits ? 8 : 16;
+}
+// Whether a group's waves can look through all tokens and keep their own.
+inline bool in_one_group_pass(long long n, long long rows) {
+  return in_groups(n, rows) && n <= group_waves(rows) * 64 * kKept;
+}
+
 // Memory that a call reads or writes.
 struct Extent {
   unsigned long long from, to;  // addresses, the second past the end

@@ -79,3 +79,18 @@ def test_clip_factors_below_the_normal_range(dt, size, limits):
             # the factor's rounding and the result's; the norm's sum of 10^4 squares
             assert (off <= (2.5 * np.finfo(dt).eps + 1e-13) * np.abs(want)).all(), limit
             assert np.array_equal(s.get(), c.get())
+
+
+@pytest.mark.parametrize("rows", [1 << 18, (1 << 18) + 1, 1 << 19, (1 << 19) + 1, 1 << 20, (1 << 20) + 1])
+@pytest.mark.parametrize("n", [129, 4096, 4097, 8192, 8193, 16_384, 16_385, 1 << 17, (1 << 17) + 1])
+def test_embedding_grad_most_counters(rows, n):
+    """Rows that fill the counters of a workgroup, and one more; tokens on both
+    sides of what its waves keep and of the passes."""
+    g = np.random.default_rng(rows + n)
+    tok = g.integers(0, rows, n)
+    tok[::9] = rows - 1 - tok[::9] % 300
+    tok[::31] = 7
+    tok[:4] = [0, rows - 1, rows, -1]
+    grad = g.integers(-3, 4, (n, 2)).astype(np.float32)
+    got = nn.embedding_grad(cp.array(grad), cp.array(tok), rows).get()
+    assert np.array_equal(got, _sums(tok, grad, rows))

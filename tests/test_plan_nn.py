@@ -13,6 +13,10 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 SOURCE = r"""
 #include "mmp_plan.h"
 extern "C" {
+long long t_group_lds(long long rows) { return 4 * mmpi::group_bins(rows) * mmpi::group_waves(rows); }
+int t_groups(long long n, long long rows) {
+  return mmpi::in_groups(n, rows) + mmpi::in_one_group_pass(n, rows);
+}
 int t_row_passes(long long rows) { return mmpi::row_passes(rows); }
 // extents as triples (from, to, written)
 int t_overlap(const long long *e, int n) {
@@ -61,3 +65,20 @@ def test_written_overlap(plans):
         assert plans.t_overlap(flat, n) == want, e
         seen[want] += 1
     assert min(seen) > 500
+
+
+def test_group_counters_fit(plans):
+    """All row counts that are ordered in groups: counters of every row for each
+    wave within 64 KiB, and filling more than half of it where they are many."""
+    i64 = ctypes.c_longlong
+    plans.t_group_lds.restype = i64
+    for rows in {*range(1, 5000), *range(5000, (1 << 20) + 1, 509),
+                 *(b + k for b in (1 << 18, 1 << 19, 1 << 20) for k in (-257, -256, -1, 0, 1))}:
+        if plans.t_groups(i64(1), i64(rows)):
+            lds = plans.t_group_lds(i64(rows))
+            assert lds <= 64 << 10 and (lds > 32 << 10 or rows <= 1 << 17), rows
+    assert plans.t_groups(i64(1 << 17), i64(1 << 20)) == 1 and plans.t_groups(i64(1), i64(1 << 20)) == 2
+    assert not plans.t_groups(i64(1 << 17), i64((1 << 20) + 1))
+    assert not plans.t_groups(i64((1 << 17) + 1), i64(5))
+    for rows, most in ((1 << 18, 16_384), ((1 << 18) + 1, 8192), (1 << 19, 8192), ((1 << 19) + 1, 4096)):
+        assert plans.t_groups(i64(most), i64(rows)) == 2 and plans.t_groups(i64(most + 1), i64(rows)) == 1
