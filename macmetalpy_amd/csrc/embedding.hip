@@ -121,12 +121,35 @@ __device__ __forceinline__ unsigned long long lanes_alike(unsigned long long amo
   return among;
 }
 
+// Between one lane's access to its wave's counters and another lane's.  A wave's
+// LDS accesses run in their order, so this only keeps the compiler from moving
+// them: no instruction.
+__device__ __forceinline__ void lanes_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // counters[d] += 1 for every lane of `among`, in a wave's own counters.  Lanes with
 // one d are counted together: as atomics they would queue (131,072 equal tokens
 // 186 us in k_group).
 __device__ __forceinline__ void tally(unsigned *counters, bool there, unsigned d, int bits) {
   const unsigned long long same = lanes_alike(__ballot(there), d, bits);
   if (there && lanes_below(same) == 0) counters[d] += (unsigned)__popcll(same);
+  lanes_in_order();
+}
+
+// The place among the equal d that a lane's entry takes: counters[d], which goes up
+// by the lanes that have it, and the rank among those.
+__device__ __forceinline__ unsigned take_place(unsigned *counters, unsigned long long among, bool there,
+                                               unsigned d, int bits) {
+  const unsigned long long same = lanes_alike(among, d, bits);
+  const unsigned rank = lanes_below(same);
+  unsigned at = 0;
+  if (there) at = counters[d];
+  lanes_in_order();
+  if (there && rank == 0) counters[d] = at + (unsigned)__popcll(same);
+  lanes_in_order();
+  return at + rank;
 }
 
 // count[t][d]: entries of tile t with digit d = row >> shift & 255.  131,072 tokens
@@ -227,14 +250,9 @@ __global__ __launch_bounds__(kSplitBlock) void k_split(S src, unsigned tile_len,
   for (unsigned i0 = from; i0 < to; i0 += 64) {
     Entry e{0, 0};
     const bool there = i0 + lane < to && src.get(i0 + lane, e);
-    const unsigned d = e.row >> shift & (kDigits - 1);
-    const unsigned long long same = lanes_alike(__ballot(there), d, 8);
-    const unsigned rank = lanes_below(same);
-    if (there) {
-      const unsigned base = next[wave][d];
-      out[base + rank] = e;
-      if (rank == 0) next[wave][d] = base + (unsigned)__popcll(same);
-    }
+    const unsigned at =
+        take_place(next[wave], __ballot(there), there, e.row >> shift & (kDigits - 1), 8);
+    if (there) out[at] = e;
   }
 }
 
@@ -309,14 +327,7 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const S *__restrict__ src
 #pragma unroll
     for (int l = 0; l < kKept; ++l) {
       if (there[l] == 0) continue;
-      const unsigned k = e[l].row / kDigits;
-      const unsigned long long same = lanes_alike(there[l], k, bits);
-      const unsigned rank = lanes_below(same);
-      if (there[l] >> lane & 1) {
-        const unsigned o = mine[k];
-        place[l] = o + rank;
-        if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
-      }
+      place[l] = take_place(mine, there[l], there[l] >> lane & 1, e[l].row / kDigits, bits);
     }
   } else if constexpr (kSplit) {
     for (unsigned i0 = from; i0 < to; i0 += 64 * kLoads) {
@@ -390,14 +401,8 @@ __global__ __launch_bounds__(kGroupBlock) void k_group(const S *__restrict__ src
 #pragma unroll
       for (int l = 0; l < kLoads; ++l) {
         const bool is = i0 + l * 64 + lane < to;
-        const unsigned k = x[l].row / kDigits;
-        const unsigned long long same = lanes_alike(__ballot(is), k, bits);
-        const unsigned rank = lanes_below(same);
-        if (is) {
-          const unsigned o = mine[k];
-          order[o + rank] = x[l].at;
-          if (rank == 0) mine[k] = o + (unsigned)__popcll(same);
-        }
+        const unsigned at = take_place(mine, __ballot(is), is, x[l].row / kDigits, bits);
+        if (is) order[at] = x[l].at;
       }
     }
   }
