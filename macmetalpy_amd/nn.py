@@ -25,6 +25,7 @@ from . import _elementwise as ew
 from ._abi import DTYPE_CODES as _CODE
 from ._backend import HipBackend
 from ._native import empty as _empty
+from .manipulation import broadcast_to
 from .ndarray import ndarray, _c_contiguous_strides, _prod
 
 __all__ = ["embedding", "embedding_grad", "gated_recurrence", "gated_recurrence_grad",
@@ -257,7 +258,10 @@ def _loss(logits, targets, weight, want_grad):
     if classes == 0:
         raise ValueError("logits have no classes")
     wide, scale, each = _WIDE[dtype], 1.0, None
-    if isinstance(weight, (ndarray, np.ndarray)) and weight.ndim:
+    if isinstance(weight, ndarray) and weight.ndim == 0:
+        # one number on the device, for every row: reading it here would wait
+        each = _contiguous(broadcast_to(_device(weight), targets._shape), wide)
+    elif isinstance(weight, (ndarray, np.ndarray)) and weight.ndim:
         each = _floating(weight, "weight")
         if each._shape != targets._shape:
             raise ValueError(f"weight of shape {each._shape}: expected a number or "
@@ -288,7 +292,8 @@ def cross_entropy_grad(logits, targets, weight=1.0):
     """``(loss, grad)``: the losses of :func:`cross_entropy`, and the gradient
     of ``sum(weight * loss)`` with respect to the logits, in their type.
     ``weight`` is a number (``1 / n`` for a mean, times the factor by which
-    float16 training scales its loss) or one for each target."""
+    float16 training scales its loss), also as a device array of no axes, or
+    one for each target."""
     return _loss(logits, targets, weight, True)
 
 

@@ -94,3 +94,33 @@ def test_embedding_grad_most_counters(rows, n):
     grad = g.integers(-3, 4, (n, 2)).astype(np.float32)
     got = nn.embedding_grad(cp.array(grad), cp.array(tok), rows).get()
     assert np.array_equal(got, _sums(tok, grad, rows))
+
+
+# ------------------------------------------------------------------ loss
+@pytest.mark.parametrize("dt", [np.float16, np.float32, np.float64], ids=lambda t: t.__name__)
+def test_loss_weight_on_the_device_is_not_waited_for(dt, monkeypatch):
+    """A mean's weight that the device computed, as one number: used where it is."""
+    g = np.random.default_rng(70)
+    wide = np.float64 if dt == np.float64 else np.float32
+    x, t = cp.array(g.standard_normal((4, 5, 33)).astype(dt)), g.integers(-1, 33, (4, 5))
+    targets = cp.array(t)
+    factor = wide(1024.0 / (t >= 0).sum())
+    want = nn.cross_entropy_grad(x, targets, float(factor))
+    weights = [cp.array(np.array(factor)), 1024.0 / cp.sum((targets >= 0).astype(wide)),
+               cp.array(np.array(3, np.int32))]
+    cp.materialize(*weights)
+
+    def wait(self, *args):
+        raise AssertionError("a device array was read on the host")
+
+    with monkeypatch.context() as m:
+        for name in ("get", "__float__", "item"):
+            m.setattr(cp.ndarray, name, wait)
+        got = [nn.cross_entropy_grad(x, targets, w) for w in weights]
+        one = nn.cross_entropy_grad(x[0, 0], targets[0, 0], weights[0])
+        assert nn.cross_entropy_grad(x[:0], targets[:0], weights[0])[1].shape == (0, 5, 33)
+    for loss, grad in got[:2]:
+        assert grad.dtype == dt
+        assert np.array_equal(loss.get(), want[0].get()) and np.array_equal(grad.get(), want[1].get())
+    assert np.array_equal(got[2][1].get(), nn.cross_entropy_grad(x, targets, 3)[1].get())
+    assert np.array_equal(one[1].get(), want[1].get()[0, 0])
