@@ -211,19 +211,22 @@ bool cfg_flag(PyObject *name) {
   return v == Py_True;
 }
 
+constexpr long long kMostElements = 1LL << 59;  // their bytes are a positive number too
 bool shape_size(PyObject *shape, long long *n) {
   if (!PyTuple_CheckExact(shape)) return false;
   long long s = 1;
+  bool fits = true, none = false;
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(shape); ++i) {
     long long v = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
     if (v < 0) {
       PyErr_Clear();
       return false;
     }
-    s *= v;
+    none = none || v == 0;
+    fits = fits && !__builtin_mul_overflow(s, v, &s) && s <= kMostElements;
   }
-  *n = s;
-  return true;
+  *n = none ? 0 : s;
+  return none || fits;
 }
 
 PyObject *contig_strides(PyObject *shape) {
@@ -1633,7 +1636,13 @@ PyObject *gate_empty(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (same) dt = i;
   }
   if (dt < 0 || !shape_size(args[0], &n)) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "empty(shape tuple, dtype)");
+    bool ints = dt >= 0 && PyTuple_CheckExact(args[0]);
+    for (Py_ssize_t i = 0; ints && i < PyTuple_GET_SIZE(args[0]); ++i)
+      ints = PyLong_Check(PyTuple_GET_ITEM(args[0], i));
+    if (!PyErr_Occurred())
+      PyErr_Format(ints ? PyExc_MemoryError : PyExc_TypeError,
+                   ints ? "empty: no memory for an array of shape %R" : "empty(shape tuple, dtype)",
+                   nargs > 0 ? args[0] : Py_None);
     return nullptr;
   }
   if (!p_alloc) {
