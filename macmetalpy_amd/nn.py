@@ -112,9 +112,11 @@ def _steps(a):
 
 def _scalar(v, what) -> float:
     try:
-        return float(v)
+        if not isinstance(v, (str, bytes, bytearray)):  # float() reads those too
+            return float(v)
     except (TypeError, ValueError):
-        raise TypeError(f"{what} must be a number, not {type(v).__name__}") from None
+        pass
+    raise TypeError(f"{what} must be a number, not {type(v).__name__}")
 
 
 # ------------------------------------------------------------- embedding

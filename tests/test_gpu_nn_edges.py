@@ -124,3 +124,15 @@ def test_loss_weight_on_the_device_is_not_waited_for(dt, monkeypatch):
         assert np.array_equal(loss.get(), want[0].get()) and np.array_equal(grad.get(), want[1].get())
     assert np.array_equal(got[2][1].get(), nn.cross_entropy_grad(x, targets, 3)[1].get())
     assert np.array_equal(one[1].get(), want[1].get()[0, 0])
+
+
+# -------------------------------------------------------------- refusals
+@pytest.mark.parametrize("text", ["2", b"2", "nan", bytearray(b"2")])
+def test_numbers_as_text_are_refused(text):
+    f, i = cp.array(np.ones((3, 4), np.float32)), cp.array(np.zeros(3, np.int64))
+    for call, name in ((lambda: nn.embedding(f, i, scale=text), "scale"),
+                       (lambda: nn.embedding_grad(f, i, 5, scale=text), "scale"),
+                       (lambda: nn.cross_entropy_grad(f, i, text), "weight"),
+                       (lambda: nn.clip_by_global_norm([f], text), "max_norm")):
+        with pytest.raises(TypeError, match=name + " must be a number"):
+            call()
