@@ -103,8 +103,13 @@ __device__ __forceinline__ double fma_of(double a, double b, double c) { return 
 
 // f = 1 / (1 + exp(-g)) and u = 1 - f = 1 / (1 + exp(g)), each to its own
 // last places: the exponential's argument is never positive, so neither
-// overflows, and u keeps its digits where f is near 1.  g was rounded to a T: of
-// a float16, whose 11 bits move exp(g) by more, the exponential is not corrected.
+// overflows, and u keeps its digits where f is near 1.  g was rounded to a T: the
+// 11 bits of a float16 move exp(g) by a thousand times what the two corrections
+// below do, so there they are left out.  In units of 2^-24: f or u is off by up to 16
+// for |g| up to 20 (6 with them), by a factor that is the same in every step and does
+// not add up; what does, f + u - 1, holds a state of 1 within 2.0 / (1 - f) for every
+// float16 gate from -4 to 6 (1.96 with them).  They cost, forwards, 16 x 2048 x 2048 88 us
+// to 99, 253 x 170 x 1390 71 to 85, backwards 144 to 153.
 template <typename T, typename A> __device__ __forceinline__ void sigmoid_pair(A g, A &f, A &u) {
   const A x = g < 0 ? g : -g;
   A e, r;

@@ -136,3 +136,44 @@ def test_numbers_as_text_are_refused(text):
                        (lambda: nn.clip_by_global_norm([f], text), "max_norm")):
         with pytest.raises(TypeError, match=name + " must be a number"):
             call()
+
+
+# ------------------------------------------------------------ recurrence
+HALVES = np.arange(1 << 16, dtype=np.uint16).view(np.float16)
+
+
+def _gates(dt, low, high):
+    """Every float16 number between two, in type dt."""
+    with np.errstate(invalid="ignore"):
+        return HALVES[(HALVES >= low) & (HALVES <= high)].astype(dt)
+
+
+@pytest.mark.parametrize("dt", [np.float16, np.float32, np.float64], ids=lambda t: t.__name__)
+def test_recurrence_keeps_a_constant(dt):
+    """A state of 1 and inputs of 1 stay 1 whatever the gate, but for rounding,
+    however many calls follow each other.  With e the exponential, d = 1 + e is
+    rounded by E / (1 + e) at most, its reciprocal by E (1 + e) / 2, the product
+    of the two by E / 4 and the new state by E, together 2.75 E a step
+    (an error of e itself leaves f + u as it is); a step keeps f of the error before."""
+    e = 2.0 ** -53 if dt == np.float64 else 2.0 ** -24
+    gate = _gates(dt, -4, 6)
+    left = 1.0 / (1.0 + np.exp(gate.astype(np.float64)))  # 1 - f
+    gates = cp.array(np.broadcast_to(gate, (16, gate.size)).copy())
+    ones = cp.ones((16, gate.size), dtype=dt)
+    state = cp.ones((gate.size,), dtype=np.float64 if dt == np.float64 else np.float32)
+    for _ in range(64):
+        _, state = nn.gated_recurrence(gates, ones, state)
+    off = np.abs(state.get().astype(np.float64) - 1.0) * left / e
+    assert off.max() <= 2.8, off.max()
+
+
+@pytest.mark.parametrize("dt", [np.float32, np.float64], ids=lambda t: t.__name__)
+def test_recurrence_state_of_one_step(dt):
+    """From nothing and an input of 1 the state is 1 - f = e / (1 + e): e is rounded
+    by 3 E (the device's exponential by a unit, 2 E, its correction by E), d by E, its
+    reciprocal by E and the product by E."""
+    gate = _gates(dt, -20, 20)
+    want = 1.0 / (1.0 + np.exp(gate.astype(np.longdouble)))
+    _, final = nn.gated_recurrence(cp.array(gate.reshape(1, -1)), cp.ones((1, gate.size), dtype=dt))
+    off = np.abs(final.get() - want) / want / (2.0 ** -53 if dt == np.float64 else 2.0 ** -24)
+    assert float(off.max()) <= 6.1, off.max()
