@@ -504,7 +504,7 @@ int mmp_embedding(int dtype, int index_dtype, int64_t n, const void *tokens,
                   double scale, void *out);
 
 /* out[v] = scale * the sum of grad[i] over the tokens i equal to v, v < rows,
- * added in an order that the tokens alone decide; a token outside [0, rows) adds
+ * added in an order that tokens, dim and dtype decide; a token outside [0, rows) adds
  * nothing.  n, rows and dim are below 2^31.  More than 128 tokens take memory
  * from the allocator for the call. */
 int mmp_embedding_grad(int dtype, int index_dtype, int64_t n, const void *tokens,

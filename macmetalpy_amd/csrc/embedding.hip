@@ -5,8 +5,8 @@
 //
 // A token outside [0, rows) is none: its output is zeros and it has no
 // gradient, so ragged batches can be filled up with -1.  Sums are held in 32
-// bits (64 for float64), added in an order that the tokens alone decide, and
-// rounded once.
+// bits (64 for float64), added in an order that follows from the tokens, the width
+// and the type, not from timing, and rounded once.
 //
 // Both are bound by memory.  The gradient first brings the tokens' positions of
 // each row together, ascending, so that the sums keep their bits.  One pass of a

@@ -4,16 +4,20 @@ Embedding rows by tokens, a gated linear recurrence, the softmax cross
 entropy and the clipping of gradients by their global norm: with ``matmul``
 the parts of a training step of a recurrent language model, and, one step at a
 time, of its answers (``python -m macmetalpy_amd.recurrent_lm`` runs both).
-The reference has none of them.  Each is one call on device arrays that
-reads its inputs once (the norm's limit needs a second pass over the arrays);
-nothing is recorded or differentiated automatically, a gradient is a call of
-its own.
+The reference has none of them.  Each is one call on device arrays, most of
+which read their inputs once (the norm's limit needs a second pass over the
+arrays, and so does the gradient of a loss for rows too long for a workgroup's
+registers, or few and cut into parts); nothing is recorded or differentiated
+automatically, a gradient is a call of its own.
 
 float16, float32 and float64; sums, states and softmax statistics are held in
 float32 (float64 for float64), and results are rounded to the inputs' type
 once.  Nothing waits for the device: tokens and targets out of range are not
 errors but no tokens (zeros, no gradient), so batches can be filled up with
--1.  Equal inputs give equal bits.
+-1.  (``scale`` and ``max_norm`` are numbers of the host: one that is on the device
+is read, which waits.)  A call repeated gives the same bits, nothing depends on
+timing; losses and norms of the same values at another address modulo 16 may be
+added in another order.
 """
 from __future__ import annotations
 
@@ -141,8 +145,8 @@ def embedding(table, tokens, scale=1.0) -> ndarray:
 def embedding_grad(grad, tokens, rows, scale=1.0) -> ndarray:
     """The gradient of :func:`embedding` with respect to its (rows, dim)
     table, whole: row v is ``scale`` times the sum of ``grad`` over the tokens
-    equal to v, added in an order that the tokens alone decide.  ``grad`` has
-    shape ``tokens.shape + (dim,)`` and gives the type."""
+    equal to v, added in an order that the tokens, the width and the type decide.
+    ``grad`` has shape ``tokens.shape + (dim,)`` and gives the type."""
     grad, tokens = _floating(grad, "grad"), _integers(tokens, "tokens")
     if grad.ndim == 0 or grad._shape[:-1] != tokens._shape:
         raise ValueError(f"grad of shape {grad._shape} does not fit tokens of shape "
@@ -206,9 +210,10 @@ def gated_recurrence(gate, x, initial=None, *, logits=True):
     None; ``final`` the state after the last, in float32 (float64 for float64)
     and not rounded to the type of ``h``, to go on from: one new token a call
     is ``steps == 1``.  A gate of ``-inf`` (a factor of 0) starts a channel
-    anew.  Factors are multiplied up along many steps, so the products of
-    neighbouring ones have to stay in the type's range: use ones of at
-    most 1 in size."""
+    anew from any finite state.  Factors are multiplied up along many steps,
+    so the products of neighbouring ones have to stay in the type's range: use
+    ones of at most 1 in size.  A state that has become infinite may go on as
+    NaN, where such a product has become 0."""
     (gate, x), dtype = _sequences((("gate", gate), ("x", x)))
     steps, dim = x._shape[-2:]
     wide = _WIDE[dtype]
@@ -340,7 +345,8 @@ def _clip(arrays, limit, out):
 def global_norm(arrays) -> ndarray:
     """The square root of the sum of the squares of every element of every
     array, as a float32 scalar array (float64 if one of them is); squares are
-    summed in float64."""
+    summed in float64, where those of float64 elements from 1e154 on are
+    infinite."""
     return _clip(arrays, None, None)[1]
 
 
