@@ -108,8 +108,9 @@ __device__ __forceinline__ double fma_of(double a, double b, double c) { return 
 // below do, so there they are left out.  In units of 2^-24: f or u is off by up to 16
 // for |g| up to 20 (6 with them), by a factor that is the same in every step and does
 // not add up; what does, f + u - 1, holds a state of 1 within 2.0 / (1 - f) for every
-// float16 gate from -4 to 6 (1.96 with them).  They cost, forwards, 16 x 2048 x 2048 88 us
-// to 99, 253 x 170 x 1390 71 to 85, backwards 144 to 153.
+// float16 gate from -4 to 6 (1.96 with them).  They cost (us a call, on one set of
+// inputs), forwards, 16 x 2048 x 2048 88 to 99, 253 x 170 x 1390 71 to 85, backwards 144 to
+// 153.
 template <typename T, typename A> __device__ __forceinline__ void sigmoid_pair(A g, A &f, A &u) {
   const A x = g < 0 ? g : -g;
   A e, r;

@@ -42,7 +42,9 @@ using mmpn::Wide;
 constexpr int kBlock = 512;
 constexpr int kLook = 4;                 // tiles that look-back reads at once
 constexpr int kPolls = 256;
-constexpr int kWaves = 4;                // per SIMD: two workgroups a CU, so 128 registers
+// Per SIMD: two workgroups a CU, so 128 registers.  float64's gradient from logits
+// keeps 20 to 52 more in scratch (16 x 2048 x 512 153 us, 5.3 TB/s; from factors 114, 5.9).
+constexpr int kWaves = 4;
 
 // How a workgroup lies on its tile: `lanes` threads side by side on a step with
 // vectors of `bytes`, kBlock / lanes of them one after another in time, `steps`
@@ -532,7 +534,8 @@ __global__ __launch_bounds__(kBlock, kWaves) void k_recur_grad_tiles(
 // A thread per V channels goes through the steps, with the next kAhead on their
 // way.  They are kept as words: float16 elements would be unpacked, and so waited
 // for, before those on hand are used (64 x 500 x 1024 544 us instead of 121).  One
-// step of 200 x 2048 float16 4 us, 253 x 170 x 1390 92 us, 3.9 TB/s.
+// step of 200 x 2048 float16 4 us, 253 x 170 x 1390 92 us, 3.9 TB/s.  Backwards, one step
+// of 200 x 2048 4.2 us (float64 6.5), 16 steps 16 (48).
 constexpr int kShortBlock = 256, kAhead = 4, kAheadGrad = 2;
 template <typename T, bool LOGITS, int V>
 __global__ __launch_bounds__(kShortBlock) void k_recur_short(
