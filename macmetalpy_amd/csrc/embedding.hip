@@ -508,7 +508,8 @@ __device__ __forceinline__ void window_sums(const I *__restrict__ tokens, const 
 // A row of more than a window's positions that begins in the window, whole: the
 // workgroup's `lanes` threads side by side have some of its columns, and their
 // sums of parts of the row are added up in LDS.
-constexpr int kWholeLanes = 8, kWholeChunks = 64, kWholeTokens = 8192;
+using mmpi::kWholeLanes;
+constexpr int kWholeChunks = 64;
 template <typename T, typename I, int V>
 __device__ __forceinline__ void whole_row(const I *__restrict__ tokens, const T *__restrict__ grad,
                                           long long stride, unsigned total, int dim, int lanes,
@@ -850,16 +851,8 @@ int grad_impl(int64_t n, const I *tokens, const T *grad, int64_t stride, int64_t
     size += (bytes + 255) / 256 * 256;
     return at;
   };
-  // Long rows whole, by the launch that sums the others, where that is not too
-  // much for a few workgroups (us; whole, in windows; float16): 30,000 x 1024 by 2000
-  // tokens 30, 39, by 8192 42, 49, by 16,000 54, 56, two rows x 1024 by 4096 27, 27, by
-  // 8192 45, 29, by 16,384 85, 32, 200 x 8 by 16,000 25, 58.  Smaller windows are
-  // more work at once and more sums to add up (16, 32, 64 places): 5000 x 8 by 131,072
-  // 60, 69, 85, 478 x 113 by 59,961 45, 58, 72, 60,000 x 128 by 131,072 53, 50, 56, 64,000
-  // x 1024 132, 121, 120, 60,000 x 8 by 524,288 95, 92, 106, 500 x 77 by 800,000 213, 158,
-  // 133.
-  const bool whole = mmpi::in_one_group_pass(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
-  const unsigned window = n > 1 << 19 ? 64 : whole || n * lanes <= 1 << 20 ? 16 : 32;
+  const bool whole = mmpi::long_rows_whole(n, rows, lanes);
+  const unsigned window = (unsigned)mmpi::row_window(n, lanes, whole);
   const int64_t windows = mmpi::ceil_div(n, window);
   const size_t at_part = place(whole ? 0 : (size_t)windows * 2 * dim * sizeof(A));
   const size_t entry_lists = whole ? 0 : mmpi::in_groups(n, rows) ? 1 : 2;

@@ -20,6 +20,9 @@
 // Measured: 16,384 rows of 50,021 float16 with gradient 600 us, 5.5 TB/s; the loss
 // alone of 2047 rows of 100,003 float32 131 us, 6.3 TB/s; 50 rows of 32,000 float16
 // with gradient 8.5 us, a workgroup's chain of load, exponentials and store.
+#include <iterator>
+#include <utility>
+
 #include "mmp_nn.h"
 
 namespace {
@@ -375,58 +378,49 @@ template <typename T, int L, bool GRAD> int launch_pass(const Loss<T> &p) {
   return mmpi::check_launch("mmp_cross_entropy(pass)");
 }
 
+// The layouts of mmp_plan.h, by their numbers.
+template <typename T, size_t... I>
+int launch_held_of(const Loss<T> &p, const mmpi::LossPlan &plan, std::index_sequence<I...>) {
+  using mmpi::kLossHeld;
+  int st = MMP_OK;
+  const bool found =
+      ((plan.lanes == kLossHeld[I].lanes && plan.held == kLossHeld[I].held &&
+        ((st = launch_held<T, kLossHeld[I].lanes, kLossHeld[I].held>(p)), true)) || ...);
+  return found ? st : mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: no layout");
+}
+template <typename T, size_t... I>
+int launch_pass_of(const Loss<T> &p, const mmpi::LossPlan &plan, std::index_sequence<I...>) {
+  using mmpi::kLossPass;
+  int st = MMP_OK;
+  const bool found = ((plan.lanes == kLossPass[I].lanes &&
+                       ((st = launch_pass<T, kLossPass[I].lanes, false>(p)), true)) || ...);
+  return found ? st : mmpi::fail(MMP_E_UNSUPPORTED, "mmp_cross_entropy: no layout");
+}
+
 template <typename T> int loss_impl(const Loss<T> &p) {
   typedef typename Wide<T>::type A;
-  // Vectors of a row wherever it begins: one more than fit its length.
-  const int64_t vecs = p.classes / vec_of<T>() + 2;
-  const int64_t cus = mmpi::cu_count();
-  // Few long rows in parts of at least 16 KiB, for about two workgroups a CU.  The
-  // two launches take 13 us (17 with the gradient; whole call, few rows), one
-  // workgroup for a row of so many 16-byte vectors (us; loss alone, with gradient):
-  // 4096 10, 13; 6250 12, 14; 12,500 18, 17 to 20; 32,500 32, 32.  With the
-  // gradient of 250 rows of 16,250 two parts a row take 40, one 32.  Never while the
-  // stream is captured, as the parts' statistics are in memory of this call.
-  int64_t parts = 2 * cus / p.rows;
-  if (parts > vecs / 1024) parts = vecs / 1024;
-  if ((p.grad ? parts >= 3 && vecs >= 12288 : parts >= 2 && vecs >= 8192) && !mmpn::capturing()) {
+  // Whether the stream is captured is asked only where it matters.
+  mmpi::LossPlan plan = mmpi::loss_plan(p.grad != nullptr, sizeof(T), p.rows, p.classes, mmpi::cu_count(), true);
+  if (plan.parts && mmpn::capturing())
+    plan = mmpi::loss_plan(p.grad != nullptr, sizeof(T), p.rows, p.classes, mmpi::cu_count(), false);
+  if (const int parts = plan.parts) {
     mmpn::Temp part;
     if (int st = part.get((size_t)(p.rows * parts) * sizeof(Stat<A>), "mmp_cross_entropy")) return st;
     hipLaunchKernelGGL((k_loss_part<T>), dim3((unsigned)(p.rows * parts)), dim3(kPartBlock), 0,
-                       mmpi::stream(), p, (int)parts, (Stat<A> *)part.p);
+                       mmpi::stream(), p, parts, (Stat<A> *)part.p);
     if (int st = mmpi::check_launch("mmp_cross_entropy(part)")) return st;
     if (p.grad)
       hipLaunchKernelGGL((k_loss_join<T, true>), dim3((unsigned)(p.rows * parts)),
-                         dim3(kPartBlock), 0, mmpi::stream(), p, (int)parts,
-                         (const Stat<A> *)part.p);
+                         dim3(kPartBlock), 0, mmpi::stream(), p, parts, (const Stat<A> *)part.p);
     else
       hipLaunchKernelGGL((k_loss_join<T, false>), dim3((unsigned)p.rows), dim3(kPartBlock), 0,
-                         mmpi::stream(), p, (int)parts, (const Stat<A> *)part.p);
+                         mmpi::stream(), p, parts, (const Stat<A> *)part.p);
     return mmpi::check_launch("mmp_cross_entropy(join)");
   }
-  // Fewer threads to a row than a wave has, where they hold it: 60,000 rows of 250
-  // float16 with gradient 23 us with 16, 49 with 64; the loss alone 14 and 42.
-  if (p.grad) {
-    if (vecs <= 8 * 4) return launch_held<T, 8, 4>(p);
-    if (vecs <= 16 * 4) return launch_held<T, 16, 4>(p);
-    if (vecs <= 32 * 4) return launch_held<T, 32, 4>(p);
-    if (vecs <= 64 * 4) return launch_held<T, 64, 4>(p);
-    if (vecs <= 64 * 8) return launch_held<T, 64, 8>(p);
-    if (vecs <= 256 * 4) return launch_held<T, 256, 4>(p);
-    if (vecs <= 256 * 6) return launch_held<T, 256, 6>(p);
-    if (vecs <= 512 * 4) return launch_held<T, 512, 4>(p);
-    if (vecs <= 512 * 8) return launch_held<T, 512, 8>(p);
-    if (vecs <= 512 * 12) return launch_held<T, 512, 12>(p);
-    if (vecs <= 512 * 16) return launch_held<T, 512, 16>(p);
-    if (vecs <= 1024 * 12) return launch_held<T, 1024, 12>(p);
-    if (vecs <= 1024 * 16) return launch_held<T, 1024, 16>(p);
-    return launch_pass<T, 1024, true>(p);
-  }
-  if (vecs <= 8 * 4) return launch_pass<T, 8, false>(p);
-  if (vecs <= 16 * 4) return launch_pass<T, 16, false>(p);
-  if (vecs <= 32 * 4) return launch_pass<T, 32, false>(p);
-  if (vecs <= 64 * 16) return launch_pass<T, 64, false>(p);
-  if (vecs <= 6144) return launch_pass<T, 256, false>(p);
-  return launch_pass<T, 512, false>(p);
+  if (plan.held)
+    return launch_held_of(p, plan, std::make_index_sequence<std::size(mmpi::kLossHeld)>());
+  if (p.grad) return launch_pass<T, mmpi::kLossAgainLanes, true>(p);
+  return launch_pass_of(p, plan, std::make_index_sequence<std::size(mmpi::kLossPass)>());
 }
 
 constexpr int64_t kMost = 0x7fff0000LL;  // room for a step past the end in 32 bits

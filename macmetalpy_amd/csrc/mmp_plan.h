@@ -42,6 +42,22 @@ inline bool in_one_group_pass(long long n, long long rows) {
   return in_groups(n, rows) && n <= group_waves(rows) * 64 * kKept;
 }
 
+// Long rows whole, by the launch that sums the others, where that is not too
+// much for a few workgroups (`lanes` threads a row; us; whole, in windows; float16):
+// 30,000 x 1024 by 2000 tokens 30, 39, by 8192 42, 49, by 16,000 54, 56, two rows x 1024
+// by 4096 27, 27, by 8192 45, 29, by 16,384 85, 32, 200 x 8 by 16,000 25, 58.
+constexpr int kWholeLanes = 8, kWholeTokens = 8192;
+inline bool long_rows_whole(long long n, long long rows, int lanes) {
+  return in_one_group_pass(n, rows) && (n <= kWholeTokens || lanes <= kWholeLanes);
+}
+// Places of the order in a window.  Smaller windows are more work at once and more
+// sums to add up (us; 16, 32, 64 places): 5000 x 8 by 131,072 60, 69, 85, 478 x 113 by
+// 59,961 45, 58, 72, 60,000 x 128 by 131,072 53, 50, 56, 64,000 x 1024 132, 121, 120,
+// 60,000 x 8 by 524,288 95, 92, 106, 500 x 77 by 800,000 213, 158, 133.
+inline int row_window(long long n, int lanes, bool whole) {
+  return n > 1 << 19 ? 64 : whole || n * lanes <= 1 << 20 ? 16 : 32;
+}
+
 // Memory that a call reads or writes.
 struct Extent {
   unsigned long long from, to;  // addresses, the second past the end
@@ -318,6 +334,151 @@ inline int solve_block_waves(long long batch, int n, int nrhs, int elem, long lo
   int w = 8;
   while (w > 1 && w * here > (elem == 8 ? 10 : 20)) w /= 2;
   return want < w ? want : w;
+}
+
+// Recurrence: how a workgroup of kRecurBlock threads lies on a tile of time and
+// channels.  `lanes` threads side by side on a step with vectors of `bytes`, the
+// others of them one after another in time, `steps` steps each.
+constexpr int kRecurBlock = 512;
+struct RecurLayout {
+  int lanes, bytes, steps;
+  constexpr int tile() const { return kRecurBlock / lanes * steps; }  // steps
+  constexpr int channels(int elem) const { return lanes * (bytes / elem); }
+  long long groups(long long dim, int elem) const {
+    return (dim + channels(elem) - 1) / channels(elem);
+  }
+  long long tiles(long long n) const { return (n + tile() - 1) / tile(); }
+  // channels that its groups have room for
+  long long room(long long dim, int elem) const { return groups(dim, elem) * channels(elem); }
+};
+constexpr RecurLayout kForwardFew{8, 8, 8};      // 512 steps, 64 bytes of channels
+constexpr RecurLayout kForwardLong{16, 8, 8};    // 256 steps, 128 bytes
+constexpr RecurLayout kForwardWide{32, 8, 8};    // 128 steps, 256 bytes
+constexpr RecurLayout kForwardBrief{32, 16, 4};  // 64 steps, 512 bytes
+constexpr RecurLayout kBackwardFew{4, 16, 4};    // 512 steps, 64 bytes
+constexpr RecurLayout kBackwardLong{8, 16, 4};   // 256 steps, 128 bytes
+constexpr RecurLayout kBackwardWide{32, 16, 4};  // 64 steps, 512 bytes
+constexpr RecurLayout forward_wide(int elem) {  // 512 bytes in float32
+  return {kForwardWide.lanes, elem == 4 ? 16 : kForwardWide.bytes, kForwardWide.steps};
+}
+
+// Up to kShort steps a thread goes through them, with vectors of kShortBytes; a
+// tile's threads would mostly have none.
+constexpr int kShortBytes = 8, kShort = 16;
+// Forwards also up to 256 steps, where there are threads enough to keep the
+// memory busy: in float16 (us, threads and tiles) 256 x 256 x 1021 95 and 105, x 1024
+// 86 and 83, 200 x 200 x 2000 111 and 122, 200 x 128 x 1999 76 and 76; of 500 steps,
+// 128 x 500 x 2048, 156 and 148.  In all types, and for half as many threads, where
+// the tiles are filled to two thirds at most: 100 x 130 x 1999 32 and 57, 253 x 170
+// x 1390 92 and 107, float32 200 x 130 x 3000 221 and 266, but 200 x 200 x 2000 218
+// and 186, 200 x 90 x 1999 117 and 90.  Backwards the tiles are as fast at any length.
+constexpr long long kManyThreads = 65536;
+inline bool recur_goes_through(int elem, long long steps, long long threads) {
+  const RecurLayout wide = forward_wide(elem);
+  if (steps <= kForwardBrief.tile() || steps > 2 * wide.tile()) return false;
+  if (3 * steps <= 2 * wide.tiles(steps) * wide.tile()) return threads >= kManyThreads / 2;
+  return elem == 2 && threads >= kManyThreads;
+}
+
+// Which layout.  A sequence's tiles wait for each other, about 0.4 us a tile, so
+// few groups of channels want long tiles; many want wide ones, whose loads
+// and stores use the memory better.  Forwards (us, float16 unless said; few / long
+// / wide layout): 1 x 50,000 x 100 36 / 58 / 111, 1 x 50,000 x 300 43 / 65 / 114, 1
+// x 60,000 x 1024 128 / 96 / 122, 2 x 16,000 x 1024 60 / 43 / 53, 4 x 8000 x 1024
+// 59 / 40 / 44, 16 x 2000 x 1024 58 / 41 / 41, 64 x 500 x 1024 58 / 40 / 39, 256 x 256
+// x 1021 168 / 123 / 105; float32 1 x 60,000 x 1024 254 / 157 / 146, 4 x 8000 x 1024
+// 145 / 82 / 73, 3 x 1999 x 1001 37 / 27 / 19, 16 x 2000 x 1024 147 / 82 / 69.
+// Backwards: 1 x 50,000 x 100 47 / 66 / 227, 1 x 50,000 x 300 85 / 78 / 218, 1 x
+// 60,000 x 1024 285 / 165 / 258, 2 x 16,000 x 1024 165 / 95 / 108, 4 x 8000 x 1024 167
+// / 94 / 89, 3 x 1999 x 1001 43 / 31 / 27, 16 x 2000 x 1024 163 / 91 / 80; float32
+// 1 x 50,000 x 100 56 / 65 / 214, 1 x 60,000 x 1024 560 / 291 / 302, 3 x 1999 x 1001
+// 71 / 53 / 34.  Counted in groups of the wide layout, and of the long one for the
+// few.  Up to 64 steps one tile of the brief layout beats the others: 281 x 48 x
+// 2851 60, 89 in wide ones, 100 x 30 x 1024 13, 17.
+enum RecurForm { kRecurThreads, kRecurBrief, kRecurFew, kRecurLong, kRecurWide };
+// Whether the channel groups of a wide layout take less than twice the threads a step
+// of those of a narrower one: 300 x 2000 x 64 float16 backwards takes 277 us in wide
+// tiles, 98 in long ones; 100 x 1000 x 100 57 and 50, x 150 59 and 73; 300 x 2000 x 32
+// 83 in long ones, 60 in those of the few, x 40 (100 x 1000) 22 and 28.
+inline bool recur_fills(int elem, long long dim, RecurLayout wide, RecurLayout narrow) {
+  return wide.room(dim, elem) < 2 * narrow.room(dim, elem);
+}
+// wide_least: groups of the wide layout from which on it is taken; few_most: groups
+// of the long one below which there are few.
+inline RecurForm recur_tiles_form(int elem, long long batch, long long steps, long long dim,
+                                  RecurLayout few, RecurLayout longer, RecurLayout wide,
+                                  long long wide_least, long long few_most) {
+  constexpr int kManyTiles = 8;
+  if (batch * wide.groups(dim, elem) >= wide_least && recur_fills(elem, dim, wide, longer))
+    return kRecurWide;
+  const bool use_few = batch * longer.groups(dim, elem) < few_most
+                           ? longer.tiles(steps) >= kManyTiles
+                           : longer.tiles(steps) > 1 && !recur_fills(elem, dim, longer, few);
+  return use_few ? kRecurFew : kRecurLong;
+}
+inline RecurForm recur_form(int elem, long long batch, long long steps, long long dim) {
+  const long long vec = kShortBytes / elem, vecs = dim >= vec ? (dim + vec - 1) / vec : dim;
+  if (steps <= kShort || recur_goes_through(elem, steps, batch * vecs)) return kRecurThreads;
+  if (steps <= kForwardBrief.tile()) return kRecurBrief;
+  return recur_tiles_form(elem, batch, steps, dim, kForwardFew, kForwardLong, forward_wide(elem),
+                          elem == 4 ? 16 : 64, 8);
+}
+inline RecurForm recur_grad_form(int elem, long long batch, long long steps, long long dim) {
+  if (steps <= kShort) return kRecurThreads;
+  return recur_tiles_form(elem, batch, steps, dim, kBackwardFew, kBackwardLong, kBackwardWide, 12, 5);
+}
+
+// Whether `arrays` inputs and outputs of more than the last cache holds are read past
+// it: if a step is in whole lines (us; past it or not): 16 x 2048 x 2048 float16 82, 92,
+// backwards 146, 160; of less, 1 x 30,000 x 1024 50, 41; of lines that two workgroups
+// read, backwards, 1 x 60,000 x 500 152, 125.
+inline bool recur_past_caches(int arrays, int elem, long long batch, long long steps, long long dim) {
+  constexpr double kCaches = 256 << 20;
+  return dim * elem % 128 == 0 &&
+         (double)arrays * (double)batch * (double)steps * (double)dim * elem > kCaches;
+}
+
+// Cross entropy: `lanes` threads a row, which hold `held` vectors of 16 bytes each
+// between the statistics and the gradient, or 0: the row is read once, and for a
+// gradient again; or `parts` workgroups a row.
+struct LossPlan {
+  int lanes, held, parts;
+};
+// By the vectors that they have room for.  Fewer threads to a row than a wave has,
+// where they hold it: 60,000 rows of 250 float16 with gradient 23 us with 16, 49 with
+// 64; the loss alone 14 and 42.
+constexpr LossPlan kLossHeld[] = {{8, 4, 0},   {16, 4, 0},  {32, 4, 0},   {64, 4, 0},   {64, 8, 0},
+                                  {256, 4, 0}, {256, 6, 0}, {512, 4, 0},  {512, 8, 0},  {512, 12, 0},
+                                  {512, 16, 0}, {1024, 12, 0}, {1024, 16, 0}};
+constexpr int kLossAgainLanes = 1024;  // longer rows with a gradient
+// The loss alone: layouts and the vectors up to which each is taken, 0 for all.
+struct LossPass {
+  int lanes;
+  long long most;
+};
+constexpr LossPass kLossPass[] = {{8, 32}, {16, 64}, {32, 128}, {64, 1024}, {256, 6144}, {512, 0}};
+inline LossPlan loss_plan(bool grad, int elem, long long rows, long long classes, long long cus,
+                          bool may_split) {
+  // vectors of a row wherever it begins: one more than fit its length
+  const long long vecs = classes / (16 / elem) + 2;
+  // Few long rows in parts of at least 16 KiB, for about two workgroups a CU.  The
+  // two launches take 13 us (17 with the gradient; whole call, few rows), one
+  // workgroup for a row of so many 16-byte vectors (us; loss alone, with gradient):
+  // 4096 10, 13; 6250 12, 14; 12,500 18, 17 to 20; 32,500 32, 32.  With the
+  // gradient of 250 rows of 16,250 two parts a row take 40, one 32.  Never while the
+  // stream is captured, as the parts' statistics are in memory of this call.
+  long long parts = 2 * cus / rows;
+  if (parts > vecs / 1024) parts = vecs / 1024;
+  if (may_split && (grad ? parts >= 3 && vecs >= 12288 : parts >= 2 && vecs >= 8192))
+    return {0, 0, (int)parts};
+  if (grad) {
+    for (const LossPlan &p : kLossHeld)
+      if (vecs <= (long long)p.lanes * p.held) return p;
+    return {kLossAgainLanes, 0, 0};
+  }
+  for (const LossPass &p : kLossPass)
+    if (p.most == 0 || vecs <= p.most) return {p.lanes, 0, 0};
+  return {0, 0, 0};
 }
 
 }  // namespace mmpi

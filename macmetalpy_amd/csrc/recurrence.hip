@@ -39,7 +39,7 @@ namespace {
 using mmpn::Vec;
 using mmpn::Wide;
 
-constexpr int kBlock = 512;
+constexpr int kBlock = mmpi::kRecurBlock;
 constexpr int kLook = 4;                 // tiles that look-back reads at once
 constexpr int kPolls = 256;
 // Per SIMD: two workgroups a CU, so 128 registers.  float64's gradient from logits
@@ -55,15 +55,16 @@ template <int LANES, int BYTES, int STEPS> struct Layout {
   template <typename T> static constexpr int vec() { return BYTES / (int)sizeof(T); }
   template <typename T> static constexpr int channels() { return LANES * vec<T>(); }
 };
-typedef Layout<8, 8, 8> ForwardFew;      // 512 steps, 64 bytes of channels
-typedef Layout<16, 8, 8> ForwardLong;    // 256 steps, 128 bytes
-template <typename T>                    // 128 steps, 256 bytes (512 in float32)
-using ForwardWide = Layout<32, sizeof(T) == 4 ? 16 : 8, 8>;
-typedef Layout<32, 16, 4> ForwardBrief;  // 64 steps, 512 bytes
-typedef Layout<4, 16, 4> BackwardFew;    // 512 steps, 64 bytes
-typedef Layout<8, 16, 4> BackwardLong;   // 256 steps, 128 bytes
-typedef Layout<32, 16, 4> BackwardWide;  // 64 steps, 512 bytes
-constexpr int kShortBytes = 8;           // of the vectors where a thread has all steps
+template <const mmpi::RecurLayout &L> using LayoutOf = Layout<L.lanes, L.bytes, L.steps>;
+typedef LayoutOf<mmpi::kForwardFew> ForwardFew;
+typedef LayoutOf<mmpi::kForwardLong> ForwardLong;
+template <typename T>
+using ForwardWide = Layout<mmpi::kForwardWide.lanes, mmpi::forward_wide(sizeof(T)).bytes, mmpi::kForwardWide.steps>;
+typedef LayoutOf<mmpi::kForwardBrief> ForwardBrief;
+typedef LayoutOf<mmpi::kBackwardFew> BackwardFew;
+typedef LayoutOf<mmpi::kBackwardLong> BackwardLong;
+typedef LayoutOf<mmpi::kBackwardWide> BackwardWide;
+using mmpi::kShortBytes;
 
 // Steps of a (batch, steps, dim) array: adjacent channels, any other strides.
 template <typename T> struct Steps {
@@ -677,65 +678,6 @@ __global__ __launch_bounds__(kShortBlock) void k_recur_grad_short(
   mmpn::store_vec<A, V>(grad_initial + b * dim + c, carry);
 }
 
-// Up to this many steps a thread goes through them; a tile's threads would
-// mostly have none.
-constexpr int64_t kShort = 16;
-// Forwards also up to 256 steps, where there are threads enough to keep the
-// memory busy: in float16 (us, threads and tiles) 256 x 256 x 1021 95 and 105, x 1024
-// 86 and 83, 200 x 200 x 2000 111 and 122, 200 x 128 x 1999 76 and 76; of 500 steps,
-// 128 x 500 x 2048, 156 and 148.  In all types, and for half as many threads, where
-// the tiles are filled to two thirds at most: 100 x 130 x 1999 32 and 57, 253 x 170
-// x 1390 92 and 107, float32 200 x 130 x 3000 221 and 266, but 200 x 200 x 2000 218
-// and 186, 200 x 90 x 1999 117 and 90.  Backwards the tiles are as fast at any length.
-constexpr int64_t kManyThreads = 65536;
-template <typename T> bool goes_through(int64_t steps, int64_t threads) {
-  const int64_t tile = ForwardWide<T>::tile;
-  if (steps <= ForwardBrief::tile || steps > 2 * tile) return false;
-  if (3 * steps <= 2 * mmpi::ceil_div(steps, tile) * tile) return threads >= kManyThreads / 2;
-  return sizeof(T) == 2 && threads >= kManyThreads;
-}
-
-// Inputs of more than the last cache holds are read past it, if a step is in whole
-// lines (us; past it or not): 16 x 2048 x 2048 float16 82, 92, backwards 146, 160; of
-// less, 1 x 30,000 x 1024 50, 41; of lines that two workgroups read, backwards,
-// 1 x 60,000 x 500 152, 125.
-constexpr double kCaches = 256 << 20;
-
-// Which layout.  A sequence's tiles wait for each other, about 0.4 us a tile, so
-// few groups of channels want long tiles; many want wide ones, whose loads
-// and stores use the memory better.  Forwards (us, float16 unless said; few / long
-// / wide layout): 1 x 50,000 x 100 36 / 58 / 111, 1 x 50,000 x 300 43 / 65 / 114, 1
-// x 60,000 x 1024 128 / 96 / 122, 2 x 16,000 x 1024 60 / 43 / 53, 4 x 8000 x 1024
-// 59 / 40 / 44, 16 x 2000 x 1024 58 / 41 / 41, 64 x 500 x 1024 58 / 40 / 39, 256 x 256
-// x 1021 168 / 123 / 105; float32 1 x 60,000 x 1024 254 / 157 / 146, 4 x 8000 x 1024
-// 145 / 82 / 73, 3 x 1999 x 1001 37 / 27 / 19, 16 x 2000 x 1024 147 / 82 / 69.
-// Backwards: 1 x 50,000 x 100 47 / 66 / 227, 1 x 50,000 x 300 85 / 78 / 218, 1 x
-// 60,000 x 1024 285 / 165 / 258, 2 x 16,000 x 1024 165 / 95 / 108, 4 x 8000 x 1024 167
-// / 94 / 89, 3 x 1999 x 1001 43 / 31 / 27, 16 x 2000 x 1024 163 / 91 / 80; float32
-// 1 x 50,000 x 100 56 / 65 / 214, 1 x 60,000 x 1024 560 / 291 / 302, 3 x 1999 x 1001
-// 71 / 53 / 34.  Counted in groups of the wide layout, and of the long one for the
-// few.  Up to 64 steps one tile of the brief layout beats the others: 281 x 48 x
-// 2851 60, 89 in wide ones, 100 x 30 x 1024 13, 17.
-template <typename T> constexpr int64_t kForwardWide = sizeof(T) == 4 ? 16 : 64;
-constexpr int64_t kBackwardWide = 12, kForwardFew = 8, kBackwardFew = 5, kManyTiles = 8;
-
-// Whether the channel groups of a wide layout W take less than twice the threads a step
-// of those of N: 300 x 2000 x 64 float16 backwards takes 277 us in wide tiles, 98 in
-// long ones; 100 x 1000 x 100 57 and 50, x 150 59 and 73; 300 x 2000 x 32 83 in long
-// ones, 60 in those of the few, x 40 (100 x 1000) 22 and 28.
-template <typename T, typename W, typename N> bool fills(int64_t dim) {
-  constexpr int64_t w = W::template channels<T>(), n = N::template channels<T>();
-  return mmpi::ceil_div(dim, w) * w < 2 * mmpi::ceil_div(dim, n) * n;
-}
-
-// Whether a call's inputs are read past the caches: more than those hold, in whole
-// lines.
-template <typename T>
-bool past_caches(int arrays, int64_t batch, int64_t steps, int64_t dim) {
-  return dim * (int64_t)sizeof(T) % 128 == 0 &&
-         (double)arrays * (double)batch * (double)steps * (double)dim * sizeof(T) > kCaches;
-}
-
 // The tiles of a call, and their descriptors.
 struct Plan {
   int64_t tiles, groups;
@@ -786,7 +728,8 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
     constexpr int kVec = kShortBytes / sizeof(T);
     const int vec = dim >= kVec ? kVec : 1;
     const int64_t vecs = mmpi::ceil_div(dim, vec), n = batch * vecs;
-    if (steps <= kShort || goes_through<T>(steps, n)) {
+    const mmpi::RecurForm form = mmpi::recur_form(sizeof(T), batch, steps, dim);
+    if (form == mmpi::kRecurThreads) {
       const int64_t blocks = mmpi::ceil_div(n, kShortBlock);
       if (!mmpi::grid_fits(blocks, kShortBlock))
         return mmpi::fail(MMP_E_UNSUPPORTED, "mmp_recurrence: too many channels");
@@ -798,7 +741,6 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
                          (const A *)initial, (T *)h, (A *)final_);
       return mmpi::check_launch("mmp_recurrence(short)");
     }
-    const int64_t wide = plan<T, ForwardWide<T>>(batch, steps, dim).groups;
     auto launch = [&](auto layout) -> int {
       typedef decltype(layout) L;
       const Plan p = plan<T, L>(batch, steps, dim);
@@ -807,7 +749,7 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
       std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
       Look lk;
       if (int st = look_of<T, L>(p, "mmp_recurrence", &lk)) return st;
-      auto kernel = past_caches<T>(3, batch, steps, dim)
+      auto kernel = mmpi::recur_past_caches(3, sizeof(T), batch, steps, dim)
                         ? (logits ? k_recur_tiles<T, true, L, true>
                                   : k_recur_tiles<T, false, L, true>)
                         : (logits ? k_recur_tiles<T, true, L, false>
@@ -818,13 +760,12 @@ extern "C" int mmp_recurrence(int dtype, int logits, int64_t batch, int64_t step
                          (A *)final_, lk);
       return mmpi::check_launch("mmp_recurrence");
     };
-    if (steps <= ForwardBrief::tile) return launch(ForwardBrief());
-    if (wide >= kForwardWide<T> && fills<T, ForwardWide<T>, ForwardLong>(dim))
-      return launch(ForwardWide<T>());
-    const Plan p = plan<T, ForwardLong>(batch, steps, dim);
-    const bool few = p.groups < kForwardFew ? p.tiles >= kManyTiles
-                                            : p.tiles > 1 && !fills<T, ForwardLong, ForwardFew>(dim);
-    return few ? launch(ForwardFew()) : launch(ForwardLong());
+    switch (form) {
+      case mmpi::kRecurBrief: return launch(ForwardBrief());
+      case mmpi::kRecurWide: return launch(ForwardWide<T>());
+      case mmpi::kRecurFew: return launch(ForwardFew());
+      default: return launch(ForwardLong());
+    }
   })
 }
 
@@ -846,7 +787,8 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
     typedef typename Wide<T>::type A;
     const Steps<T> sd{(const T *)grad, grad_sb, grad_st}, sg{(const T *)gate, gate_sb, gate_st};
     const Steps<T> sx{(const T *)x, x_sb, x_st}, sh{(const T *)h, h_sb, h_st};
-    if (steps <= kShort) {
+    const mmpi::RecurForm form = mmpi::recur_grad_form(sizeof(T), batch, steps, dim);
+    if (form == mmpi::kRecurThreads) {
       constexpr int kVec = kShortBytes / sizeof(T);
       const int vec = dim >= kVec ? kVec : 1;
       const int64_t vecs = mmpi::ceil_div(dim, vec), n = batch * vecs;
@@ -862,7 +804,6 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
                          (A *)grad_initial);
       return mmpi::check_launch("mmp_recurrence_grad(short)");
     }
-    const int64_t wide = plan<T, BackwardWide>(batch, steps, dim).groups;
     auto launch = [&](auto layout) -> int {
       typedef decltype(layout) L;
       const Plan p = plan<T, L>(batch, steps, dim);
@@ -871,7 +812,7 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
       std::lock_guard<std::mutex> lock(mmpi::launch_mutex());
       Look lk;
       if (int st = look_of<T, L>(p, "mmp_recurrence_grad", &lk)) return st;
-      auto kernel = past_caches<T>(logits ? 6 : 5, batch, steps, dim)
+      auto kernel = mmpi::recur_past_caches(logits ? 6 : 5, sizeof(T), batch, steps, dim)
                         ? (logits ? k_recur_grad_tiles<T, true, L, true>
                                   : k_recur_grad_tiles<T, false, L, true>)
                         : (logits ? k_recur_grad_tiles<T, true, L, false>
@@ -883,12 +824,10 @@ extern "C" int mmp_recurrence_grad(int dtype, int logits, int64_t batch, int64_t
                          lk);
       return mmpi::check_launch("mmp_recurrence_grad");
     };
-    if (wide >= kBackwardWide && fills<T, BackwardWide, BackwardLong>(dim))
-      return launch(BackwardWide());
-    const Plan p = plan<T, BackwardLong>(batch, steps, dim);
-    const bool few = p.groups < kBackwardFew
-                         ? p.tiles >= kManyTiles
-                         : p.tiles > 1 && !fills<T, BackwardLong, BackwardFew>(dim);
-    return few ? launch(BackwardFew()) : launch(BackwardLong());
+    switch (form) {
+      case mmpi::kRecurWide: return launch(BackwardWide());
+      case mmpi::kRecurFew: return launch(BackwardFew());
+      default: return launch(BackwardLong());
+    }
   })
 }
