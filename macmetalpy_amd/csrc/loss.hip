@@ -400,9 +400,11 @@ int launch_pass_of(const Loss<T> &p, const mmpi::LossPlan &plan, std::index_sequ
 template <typename T> int loss_impl(const Loss<T> &p) {
   typedef typename Wide<T>::type A;
   // Whether the stream is captured is asked only where it matters.
-  mmpi::LossPlan plan = mmpi::loss_plan(p.grad != nullptr, sizeof(T), p.rows, p.classes, mmpi::cu_count(), true);
-  if (plan.parts && mmpn::capturing())
-    plan = mmpi::loss_plan(p.grad != nullptr, sizeof(T), p.rows, p.classes, mmpi::cu_count(), false);
+  auto plan_of = [&](bool may_split) {
+    return mmpi::loss_plan(p.grad != nullptr, sizeof(T), p.rows, p.classes, mmpi::cu_count(), may_split);
+  };
+  mmpi::LossPlan plan = plan_of(true);
+  if (plan.parts && mmpn::capturing()) plan = plan_of(false);
   if (const int parts = plan.parts) {
     mmpn::Temp part;
     if (int st = part.get((size_t)(p.rows * parts) * sizeof(Stat<A>), "mmp_cross_entropy")) return st;

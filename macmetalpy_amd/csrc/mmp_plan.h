@@ -447,8 +447,8 @@ struct LossPlan {
 // By the vectors that they have room for.  Fewer threads to a row than a wave has,
 // where they hold it: 60,000 rows of 250 float16 with gradient 23 us with 16, 49 with
 // 64; the loss alone 14 and 42.
-constexpr LossPlan kLossHeld[] = {{8, 4, 0},   {16, 4, 0},  {32, 4, 0},   {64, 4, 0},   {64, 8, 0},
-                                  {256, 4, 0}, {256, 6, 0}, {512, 4, 0},  {512, 8, 0},  {512, 12, 0},
+constexpr LossPlan kLossHeld[] = {{8, 4, 0},    {16, 4, 0},    {32, 4, 0},   {64, 4, 0}, {64, 8, 0},
+                                  {256, 4, 0},  {256, 6, 0},   {512, 4, 0},  {512, 8, 0}, {512, 12, 0},
                                   {512, 16, 0}, {1024, 12, 0}, {1024, 16, 0}};
 constexpr int kLossAgainLanes = 1024;  // longer rows with a gradient
 // The loss alone: layouts and the vectors up to which each is taken, 0 for all.

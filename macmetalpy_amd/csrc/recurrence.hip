@@ -59,7 +59,8 @@ template <const mmpi::RecurLayout &L> using LayoutOf = Layout<L.lanes, L.bytes, 
 typedef LayoutOf<mmpi::kForwardFew> ForwardFew;
 typedef LayoutOf<mmpi::kForwardLong> ForwardLong;
 template <typename T>
-using ForwardWide = Layout<mmpi::kForwardWide.lanes, mmpi::forward_wide(sizeof(T)).bytes, mmpi::kForwardWide.steps>;
+using ForwardWide = Layout<mmpi::kForwardWide.lanes, mmpi::forward_wide(sizeof(T)).bytes,
+                           mmpi::kForwardWide.steps>;
 typedef LayoutOf<mmpi::kForwardBrief> ForwardBrief;
 typedef LayoutOf<mmpi::kBackwardFew> BackwardFew;
 typedef LayoutOf<mmpi::kBackwardLong> BackwardLong;
