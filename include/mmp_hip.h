@@ -550,6 +550,28 @@ int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *sizes,
                   const void *const *arrays, void *const *outs, double limit,
                   int norm_dtype, void *norm);
 
+/* h = a(g) u with g = x W[:, :hidden], u = x W[:, hidden:], for (rows, dim) x
+ * and (dim, 2 hidden) weights W; activation a: 0 silu, 1 gelu (of the normal
+ * distribution's function), 2 sigmoid.  Row strides are at least the rows'
+ * lengths. */
+int mmp_gated_feed_forward(int dtype, int activation, int64_t rows, int64_t dim, int64_t hidden,
+                           const void *x, int64_t x_stride, const void *weights,
+                           int64_t w_stride, void *h);
+
+/* Its gradient, from grad (of h) and the inputs: grad_x (rows, dim) and
+ * grad_weights (dim, 2 hidden). */
+int mmp_gated_feed_forward_grad(int dtype, int activation, int64_t rows, int64_t dim,
+                                int64_t hidden, const void *grad, int64_t grad_stride,
+                                const void *x, int64_t x_stride, const void *weights,
+                                int64_t w_stride, void *grad_x, void *grad_weights);
+
+/* y[i] = (w >= round(2^32 rate) ? x[i] / (1 - rate) : 0) + residual[i] (NULL for
+ * none), w the word offset + *offset_at + i (offset_at: int64 on the device, NULL
+ * for 0) of the Philox4x32-10 stream of `seed`, whose words 4 j to 4 j + 3 have
+ * the counter j.  0 <= rate < 1. */
+int mmp_dropout(int dtype, int64_t n, const void *x, const void *residual, double rate,
+                uint64_t seed, uint64_t offset, const void *offset_at, void *y);
+
 /* ======================================================================== */
 /* Runtime compilation: replaces createLibraryFromString + setFunction +    */
 /* runFunction (_metal_backend.py:237-257, 313-357) for the fusion engine  */

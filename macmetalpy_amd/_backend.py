@@ -137,6 +137,12 @@ _SIGNATURES = {
     "mmp_cross_entropy": [_c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
                           ctypes.c_double, _c_vp, _c_vp],
     "mmp_clip_norm": [_c_i64, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_double, _c_int, _c_vp],
+    "mmp_gated_feed_forward": [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
+                               _c_vp],
+    "mmp_gated_feed_forward_grad": [_c_int, _c_int, _c_i64, _c_i64, _c_i64]
+                                   + [_c_vp, _c_i64] * 3 + [_c_vp] * 2,
+    "mmp_dropout": [_c_int, _c_i64, _c_vp, _c_vp, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64,
+                    _c_vp, _c_vp],
     "mmp_rtc_compile": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_c_vp)],
     "mmp_rtc_build": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _c_vp, _c_sz,
                       ctypes.POINTER(_c_sz)],
@@ -579,6 +585,22 @@ class HipBackend:
         if outs is None:
             at[3] = None
         _check(self._lib.mmp_clip_norm(len(sizes), *at, limit, norm_code, norm), "mmp_clip_norm")
+
+    def gated_feed_forward(self, dcode, activation, rows, dim, hidden, x, x_stride, weights,
+                           w_stride, h) -> None:
+        _check(self._lib.mmp_gated_feed_forward(dcode, activation, rows, dim, hidden, x, x_stride,
+                                                weights, w_stride, h), "mmp_gated_feed_forward")
+
+    def gated_feed_forward_grad(self, dcode, activation, rows, dim, hidden, grad, grad_stride, x,
+                                x_stride, weights, w_stride, grad_x, grad_weights) -> None:
+        _check(self._lib.mmp_gated_feed_forward_grad(dcode, activation, rows, dim, hidden, grad,
+                                                     grad_stride, x, x_stride, weights, w_stride,
+                                                     grad_x, grad_weights),
+               "mmp_gated_feed_forward_grad")
+
+    def dropout(self, dcode, n, x, residual, rate, seed, offset, offset_at, y) -> None:
+        _check(self._lib.mmp_dropout(dcode, n, x, residual, rate, seed, offset, offset_at, y),
+               "mmp_dropout")
 
     # ------------------------------------------ reference kernel interface
     def execute_kernel(self, shader_src: str, func_name, grid_size, buffers) -> None:

@@ -1,0 +1,124 @@
+// dropout.hip -- dropout whose mask is a function of a seed and a position.
+//
+//   y_i = (w_i >= t ? x_i / (1 - rate) : 0) + residual_i,   t = round(2^32 rate)
+//
+// with w_i word offset + i of the stream that the seed names: 32 bits of
+// Philox4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", 2011), whose block j, of words 4 j to 4 j + 3, has the counter
+// (j, 0) and the seed as its key, 64 bits each.  The gradient is the same call on
+// the gradient, so no mask is kept; neither does one depend on the type, the
+// layout or the launch.
+//
+// A round is two products of 32 x 32 to 64 bits, ten of them four words.
+#include "mmp_nn.h"
+
+namespace {
+
+using mmpn::Vec;
+using mmpn::Wide;
+
+struct Words {
+  unsigned w[4];
+};
+
+__device__ __forceinline__ Words philox(unsigned long long block, unsigned long long seed) {
+  unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = 0, c3 = 0;
+  unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const unsigned long long p = 0xD2511F53ull * c0, q = 0xCD9E8D57ull * c2;
+    c0 = (unsigned)(q >> 32) ^ c1 ^ k0;
+    c1 = (unsigned)q;
+    c2 = (unsigned)(p >> 32) ^ c3 ^ k1;
+    c3 = (unsigned)p;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return Words{{c0, c1, c2, c3}};
+}
+
+template <typename T> struct Drop {
+  typedef typename Wide<T>::type A;
+  const T *x, *residual;
+  T *y;
+  long long n;
+  unsigned long long seed, offset;
+  const long long *offset_at;  // added to offset, or null
+  unsigned threshold;
+  A scale;
+};
+
+template <typename T, bool ADD>
+__device__ __forceinline__ T drop(T x, T r, unsigned word, unsigned threshold, typename Wide<T>::type scale) {
+  typedef typename Wide<T>::type A;
+  const A y = word >= threshold ? (A)x * scale : (A)0;
+  if constexpr (ADD) return (T)(y + (A)r);
+  else return (T)y;
+}
+
+constexpr int kBlock = 256;
+template <typename T> constexpr int vec_of() { return sizeof(T) == 2 ? 8 : 4; }
+
+// V adjacent elements a thread.  Words in step with the vectors (LEAD 0) come in
+// whole blocks; otherwise the vector's first block starts before it.
+template <typename T, bool ADD>
+__global__ __launch_bounds__(kBlock) void k_dropout(Drop<T> p) {
+  constexpr int V = vec_of<T>();
+  const long long at = (blockIdx.x * (long long)kBlock + threadIdx.x) * V;
+  if (at >= p.n) return;
+  const unsigned long long first = p.offset + (p.offset_at ? (unsigned long long)*p.offset_at : 0ull) + at;
+  const int lead = (int)(first & 3);  // the same for all threads
+  unsigned w[V + 4];
+  const int blocks = lead ? V / 4 + 1 : V / 4;
+#pragma unroll
+  for (int b = 0; b < V / 4 + 1; ++b) {
+    if (b < blocks) {
+      const Words q = philox((first >> 2) + b, p.seed);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[4 * b + i] = q.w[i];
+    }
+  }
+  if (lead) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)  // down by lead words
+      if (lead >> s & 1)
+#pragma unroll
+        for (int i = 0; i + (1 << s) < V + 4; ++i) w[i] = w[i + (1 << s)];
+  }
+  if (at + V <= p.n) {
+    const Vec<T, V> x = mmpn::load_vec<T, V>(p.x + at);
+    Vec<T, V> r{}, y;
+    if constexpr (ADD) r = mmpn::load_vec<T, V>(p.residual + at);
+#pragma unroll
+    for (int i = 0; i < V; ++i) y.e[i] = drop<T, ADD>(x.e[i], r.e[i], w[i], p.threshold, p.scale);
+    mmpn::store_vec(p.y + at, y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (at + i < p.n) p.y[at + i] = drop<T, ADD>(p.x[at + i], ADD ? p.residual[at + i] : (T)0, w[i], p.threshold, p.scale);
+  }
+}
+
+}  // namespace
+
+extern "C" int mmp_dropout(int dtype, int64_t n, const void *x, const void *residual, double rate,
+                           uint64_t seed, uint64_t offset, const void *offset_at, void *y) {
+  const char *what = "mmp_dropout";
+  if (int st = mmpi::ensure_init()) return st;
+  if (n < 0) return mmpi::fail(MMP_E_ARG, "%s: negative extent", what);
+  if (!(rate >= 0.0 && rate < 1.0)) return mmpi::fail(MMP_E_ARG, "%s: rate outside [0, 1)", what);
+  if (n == 0) return MMP_OK;
+  if (!x || !y) return mmpi::fail(MMP_E_ARG, "%s: null pointer", what);
+  MMP_DISPATCH_FLOAT(dtype, "mmp_dropout", {
+    typedef typename Wide<T>::type A;
+    const int64_t blocks = mmpi::ceil_div(n, kBlock * vec_of<T>());
+    if (!mmpi::grid_fits(blocks, kBlock)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many elements", what);
+    const double t = __builtin_floor(rate * 4294967296.0 + 0.5);
+    const Drop<T> p{(const T *)x, (const T *)residual, (T *)y, (long long)n, seed, offset,
+                    (const long long *)offset_at, t > 4294967295.0 ? 4294967295u : (unsigned)t,
+                    (A)(1.0 / (1.0 - rate))};
+    if (residual) hipLaunchKernelGGL((k_dropout<T, true>), dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), p);
+    else hipLaunchKernelGGL((k_dropout<T, false>), dim3((unsigned)blocks), dim3(kBlock), 0, mmpi::stream(), p);
+    return mmpi::check_launch(what);
+  })
+}

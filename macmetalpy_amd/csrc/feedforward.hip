@@ -1,0 +1,629 @@
+// feedforward.hip -- the gated feed-forward product and its gradient.
+//
+//   g = x W[:, :hidden],  u = x W[:, hidden:],  h = a(g) u
+//
+// for rows x and one array W (dim, 2 hidden) of both projections; a is silu
+// (g f), gelu (g phi) or the sigmoid f.  The gradient works g and u out again
+// (a third more products, instead of 2 hidden values a row written, kept and
+// read) and forms D = [d u a'(g) | d a(g)], d the gradient of h; then
+// grad_x = D W^T and grad_W = x^T D.
+//
+// float16: all three products run on one kernel, k_prod16: tiles of 256 x 256 or
+// 128 x 128 outputs, operands copied HBM/L2 -> LDS, MFMA 16 x 16 x 32.  A tile of
+// the first holds 128 (64) columns of g and the same ones of u, the 16 wide
+// blocks of both side by side, so that the lane which has an element of g has
+// its u too and the activation is worked out on the accumulators; g and u are
+// never stored.  D is rounded to float16, as the gradient of a float16 product
+// is when a program forms it itself.
+#include <utility>
+
+#include "mmp_nn.h"
+
+namespace {
+
+using mmpn::Temp;
+using mmpn::Vec;
+using mmpn::Wide;
+
+enum { kSilu = 0, kGelu = 1, kSigmoid = 2 };
+
+__device__ __forceinline__ float erfc_of(float x) { return erfcf(x); }
+__device__ __forceinline__ double erfc_of(double x) { return erfc(x); }
+
+// a(g) and a'(g) in 32 bits (64 for float64).  With f = 1 / (1 + exp(-g)) and
+// rest = 1 - f: silu g f, f (1 + g rest); sigmoid f, f rest.  gelu g phi with
+// phi = erfc(-g / sqrt 2) / 2, which keeps its digits where phi is near 0, and
+// phi + g exp(-g^2 / 2) / sqrt(2 pi).
+template <typename T, int ACT, bool GRAD, typename A>
+__device__ __forceinline__ void activate(A g, A &a, A &da) {
+  if constexpr (ACT == kGelu) {
+    const A phi = (A)0.5 * erfc_of(g * (A)-0.70710678118654752440);
+    a = g * phi;
+    if constexpr (GRAD)
+      da = mmpn::fma_of(g * (A)0.39894228040143267794, mmpn::exp_of(g * g * (A)-0.5), phi);
+  } else {
+    A f, rest;
+    mmpn::sigmoid_pair<T>(g, f, rest);
+    if constexpr (ACT == kSilu) {
+      a = g * f;
+      if constexpr (GRAD) da = f * mmpn::fma_of(g, rest, (A)1);
+    } else {
+      a = f;
+      if constexpr (GRAD) da = f * rest;
+    }
+  }
+}
+
+// What becomes of a product's values, N adjacent columns of a row at a time.
+template <typename T> struct End {
+  typedef typename Wide<T>::type A;
+  T *out;
+  long long ldo;
+  const T *grad;  // of h
+  long long ldg;
+  int hidden, padded;  // columns of a projection, and of its part in D
+  bool whole;          // groups of four columns of `out` can be stored at once
+
+  template <int N> __device__ __forceinline__ void put(T *p, const T (&v)[N], int left) const {
+    if (whole && left >= N) {
+      Vec<T, N> w;
+#pragma unroll
+      for (int i = 0; i < N; ++i) w.e[i] = v[i];
+      mmpn::store_vec(p, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) p[i] = v[i];
+    }
+  }
+  // h = a(g) u
+  template <int ACT, int N>
+  __device__ __forceinline__ void forward(long long row, int col, const A (&g)[N], const A (&u)[N]) const {
+    T h[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      A a, da;
+      activate<T, ACT, false>(g[i], a, da);
+      h[i] = (T)(a * u[i]);
+    }
+    put(out + row * ldo + col, h, hidden - col);
+  }
+  // D = [d u a'(g) | d a(g)], zeros between the parts
+  template <int ACT, int N>
+  __device__ __forceinline__ void backward(long long row, int col, const A (&g)[N], const A (&u)[N]) const {
+    T dg[N], du[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      A a, da;
+      activate<T, ACT, true>(g[i], a, da);
+      const bool there = col + i < hidden;
+      const A d = there ? (A)grad[row * ldg + col + i] : (A)0;
+      dg[i] = there ? (T)(d * u[i] * da) : (T)0;
+      du[i] = there ? (T)(d * a) : (T)0;
+    }
+    put(out + row * ldo + col, dg, padded - col);
+    put(out + row * ldo + padded + col, du, padded - col);
+  }
+  // A column of the padded parts as one of the projections' own.
+  template <int N> __device__ __forceinline__ void plain(long long row, int col, const A (&v)[N], int cols) const {
+    T h[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = (T)v[i];
+    if (padded == hidden) return put(out + row * ldo + col, h, cols - col);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = col + i;
+      if (c < hidden) out[row * ldo + c] = h[i];
+      else if (c >= padded && c - padded < hidden) out[row * ldo + hidden + c - padded] = h[i];
+    }
+  }
+};
+
+enum { kForward = 0, kBackward = 1, kPlain = 2, kPartial = 3 };
+
+// ------------------------------------------------------------ float16 products
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16;
+
+__device__ __attribute__((aligned(16))) const unsigned kZeros[4] = {0, 0, 0, 0};
+
+// Rows of this many elements: a tile's offsets would pass 32 bits of bytes.
+constexpr long long kRow = 1LL << 21;
+
+struct Prod {
+  const u16 *a, *b;
+  long long lda, ldb;  // in elements, multiples of 8, below kRow
+  int m, n, k;         // n: columns, or the columns of a projection (paired)
+  int up;              // paired: from a column of g to the same one of u
+  int tiles_m, tiles_n, span;  // slabs of 64 to a part of k (blockIdx.y)
+  float *part;         // kPartial: (parts, m, n) or (parts, m, 2 n)
+};
+
+// Where a stage has its 16 byte chunks (k_prod16), and the eight k of half slab
+// `s` of one of the 16 m or n from `first` on.
+__device__ __forceinline__ int mn_slot(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int k_slot(int k, int width) {
+  return 2 * ((k & 3) | (((k >> 3) & 3) << 2)) & (width / 8 - 1);
+}
+template <bool ROWS_ARE_K, int W>
+__device__ __forceinline__ h8 fragment(const u16 *S, int first, int s, int lane) {
+  const int fr = lane & 15, grp = lane >> 4;
+  if constexpr (ROWS_ARE_K) {
+    const int col = first + 4 * (fr & 3), c8 = col >> 3, w = col & 7;
+    const int k1 = s * 32 + grp * 8 + (fr >> 2), k2 = k1 + 4;
+    typedef __attribute__((address_space(3))) s4 L;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(S + k1 * W + ((c8 ^ k_slot(k1, W)) << 3) + w));
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(S + k2 * W + ((c8 ^ k_slot(k2, W)) << 3) + w));
+    return __builtin_bit_cast(h8, (s8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  } else {
+    return *reinterpret_cast<const h8 *>(&S[(first + fr) * 64 + ((grp + 4 * s) ^ mn_slot(fr)) * 8]);
+  }
+}
+
+// 16 bytes a lane, global -> LDS: lane L's land at 16 L of `to`.
+__device__ __forceinline__ void copy16(const u16 *from, u16 *to) {
+  __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
+}
+
+// C = A B for operands whose rows are 16 byte aligned, any extents (the last
+// vector of a row may run into padding: zeros where it lies along k).
+//   AK / BK_: A (B) is stored with k along its rows' axis: a row of memory is one
+//   k and its elements are m (n).  Otherwise a row is one m (n).
+// A workgroup has a tile of 16 I WM x 16 J WN outputs, a wave of it 16 I x 16 J.
+// k goes by in slabs of 64 through two stages in LDS: while one feeds the
+// MFMAs the other is filled by copies that do not pass through registers.
+// Fragments are read half a slab ahead of the MFMAs that use them.
+//  * k along a row (128 bytes of a slab): 16 byte chunk c of row r lies at
+//    c ^ (r / 2 % 8), so that the 16 rows of a fragment spread over the banks.
+//  * m or n along a row: chunk c of row k at c ^ 2 (k % 4 + 4 (k / 8 % 4)); a
+//    lane gets its eight k of a column by two transposing reads, each of four
+//    rows.
+// The MFMA is issued as C^T = B^T A^T, so a lane has four adjacent columns.
+// Workgroups of an XCD (ids go round the eight) get tiles next to one another.
+template <int WM, int WN, int I, int J, bool AK, bool BK_, bool PAIR, int END, int ACT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_prod16(Prod p, End<mmp_half> end) {
+  constexpr int TM = 16 * I * WM, TN = 16 * J * WN, NW = WM * WN, BK = 64;
+  constexpr int PER = (TM + TN) / 8 / NW;  // copies of 1 KiB a wave and slab
+  static_assert(TN / 8 % PER == 0 && (!PAIR || J % 2 == 0), "");
+  __shared__ __attribute__((aligned(16))) u16 As0[TM * BK], As1[TM * BK];
+  __shared__ __attribute__((aligned(16))) u16 Bs0[TN * BK], Bs1[TN * BK];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  const int blocks = p.tiles_m * p.tiles_n;
+  int b = blockIdx.x;
+  {
+    const int xcd = b & 7, q = blocks >> 3, r = blocks & 7;
+    b = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
+  }
+  constexpr int GM = 4;
+  const int first = b / (GM * p.tiles_n) * GM, gm = min(p.tiles_m - first, GM);
+  const int rem = b - first * p.tiles_n;
+  const int tm = first + rem % gm, tn = rem / gm;
+  const int m0 = tm * TM, n0 = tn * (PAIR ? TN / 2 : TN);
+  const int nk = (p.k + BK - 1) / BK, kb = blockIdx.y * p.span, ke = min(nk, kb + p.span);
+
+  // Column of a 16 wide block of the tile that holds both projections.
+  auto column = [&](int chunk) {
+    if constexpr (!PAIR) return chunk * 8 + n0 < p.n ? chunk * 8 : 0;
+    const int cb = chunk >> 1, w = cb / J, j = cb % J;
+    const int c = (w * (J / 2) + j % (J / 2)) * 16 + (chunk & 1) * 8;
+    return (c + n0 < p.n ? c : 0) + (j / (J / 2)) * p.up;
+  };
+
+  const bool b_role = wave < TN / 8 / PER;
+  const u16 *base = b_role ? p.b + (BK_ ? (long long)n0 : n0 * p.ldb)
+                           : p.a + (AK ? (long long)m0 : m0 * p.lda);
+  const unsigned ld = (unsigned)(b_role ? p.ldb : p.lda);
+  const bool along_k = b_role ? BK_ : AK;  // rows are k
+  const long long step = along_k ? (long long)ld : 1;
+  const int at = b_role ? wave * PER : (wave - TN / 8 / PER) * PER;
+  unsigned off[PER];
+  int kof[PER];  // first k of this lane's chunk, in the slab
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    auto rows_k = [&](int width, auto col) {
+      const int per_row = width / 8, k = (at + i) * (64 / per_row) + lane / per_row;
+      kof[i] = k;
+      off[i] = (unsigned)k * ld + (unsigned)col((lane % per_row) ^ k_slot(k, width));
+    };
+    auto rows_mn = [&](int left) {
+      const int r = (at + i) * 8 + (lane >> 3), c = (lane & 7) ^ mn_slot(r);
+      kof[i] = c * 8;
+      off[i] = (unsigned)min(r, left - 1) * ld + (unsigned)c * 8;
+    };
+    if (b_role) {
+      if constexpr (BK_) rows_k(TN, column);
+      else rows_mn(p.n - n0);
+    } else {
+      if constexpr (AK) rows_k(TM, [&](int c) { return c * 8 + m0 < p.m ? c * 8 : 0; });
+      else rows_mn(p.m - m0);
+    }
+  }
+  auto issue = [&](u16 *A_, u16 *B_, int slab) {
+    const u16 *g = base + (long long)slab * BK * step;
+    u16 *dst = (b_role ? B_ : A_) + at * 512;
+    if ((slab + 1) * BK <= p.k) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        copy16(g + off[i], dst + i * 512);
+    } else {  // past the last k: zeros of both operands
+      const int left = p.k - slab * BK;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        copy16(kof[i] < left ? g + off[i] : (const u16 *)kZeros, dst + i * 512);
+    }
+  };
+
+  f4 acc[I][J];
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+
+  const int fr = lane & 15, grp = lane >> 4;
+  auto read_half = [&](const u16 *A_, const u16 *B_, int s, h8 (&af)[I], h8 (&bf)[J]) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      bf[j] = fragment<BK_, TN>(B_, (wn * J + j) * 16, s, lane);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+      af[i] = fragment<AK, TM>(A_, (wm * I + i) * 16, s, lane);
+  };
+  auto mfma_half = [&](const h8 (&af)[I], const h8 (&bf)[J]) {
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[j], af[i], acc[i][j], 0, 0, 0);
+  };
+  // A half slab's MFMAs with the reads of the next half one after each.
+  constexpr int READS = I * (AK ? 2 : 1) + J * (BK_ ? 2 : 1);
+  auto order = [&]() {
+#pragma unroll
+    for (int m = 0; m < I * J; ++m) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (m < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    // keeps the reads in their half
+    asm volatile("" ::: "memory");
+  };
+  // Before the barrier in the middle of a slab the MFMAs of its first half and
+  // the reads of its second; the barrier waits for this wave's copies, so the
+  // other stage is whole after it, and the stage just read is free for the slab
+  // two ahead.  Copies past the last slab fill it in again, unread.
+  h8 f0a[I], f0b[J], f1a[I], f1b[J];
+  issue(As0, Bs0, kb);
+  __syncthreads();
+  issue(As1, Bs1, min(kb + 1, ke - 1));
+  read_half(As0, Bs0, 0, f0a, f0b);
+  for (int kt = kb; kt < ke; kt += 2) {
+    mfma_half(f0a, f0b);
+    read_half(As0, Bs0, 1, f1a, f1b);
+    order();
+    __syncthreads();
+    issue(As0, Bs0, min(kt + 2, ke - 1));
+    mfma_half(f1a, f1b);
+    read_half(As1, Bs1, 0, f0a, f0b);
+    order();
+    if (kt + 1 < ke) {
+      mfma_half(f0a, f0b);
+      read_half(As1, Bs1, 1, f1a, f1b);
+      order();
+      __syncthreads();
+      issue(As1, Bs1, min(kt + 3, ke - 1));
+      mfma_half(f1a, f1b);
+      read_half(As0, Bs0, 0, f0a, f0b);
+      order();
+    }
+  }
+  __syncthreads();  // no copy into LDS may be in flight when the workgroup ends
+
+  constexpr int JN = PAIR ? J / 2 : J;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int row = m0 + (wm * I + i) * 16 + fr;
+    if (row >= p.m) continue;
+#pragma unroll
+    for (int j = 0; j < JN; ++j) {
+      const int col = n0 + (wn * JN + j) * 16 + grp * 4;
+      if (col >= p.n) continue;
+      float v[4], w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[r] = acc[i][j][r];
+        if constexpr (PAIR) w[r] = acc[i][j + J / 2][r];
+      }
+      if constexpr (END == kPartial) {
+        // (n columns or a multiple of 4 of them, so that vectors stay whole)
+        const int n4 = (p.n + 3) & ~3;
+        float *o = p.part + ((long long)blockIdx.y * p.m + row) * (PAIR ? 2 * n4 : n4) + col;
+        mmpn::store_vec(o, *reinterpret_cast<const Vec<float, 4> *>(v));
+        if constexpr (PAIR) mmpn::store_vec(o + n4, *reinterpret_cast<const Vec<float, 4> *>(w));
+      } else if constexpr (END == kForward) {
+        end.template forward<ACT>(row, col, v, w);
+      } else if constexpr (END == kBackward) {
+        end.template backward<ACT>(row, col, v, w);
+      } else {
+        end.plain(row, col, v, p.n);
+      }
+    }
+  }
+}
+
+// The parts of k added in order, four columns a thread.
+template <int END, int ACT>
+__global__ __launch_bounds__(256) void k_join16(const float *part, int parts, int m, int n, End<mmp_half> end) {
+  const int n4 = (n + 3) & ~3;
+  constexpr bool PAIR = END != kPlain;
+  const long long id = blockIdx.x * 256LL + threadIdx.x, row = id / (n4 / 4);
+  if (row >= m) return;
+  const int col = (int)(id - row * (n4 / 4)) * 4;
+  const long long width = PAIR ? 2 * n4 : n4;
+  float v[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
+  for (int z = 0; z < parts; ++z) {
+    const float *at = part + ((long long)z * m + row) * width + col;
+    const auto x = mmpn::load_vec<float, 4>(at);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += x.e[r];
+    if constexpr (PAIR) {
+      const auto y = mmpn::load_vec<float, 4>(at + n4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w[r] += y.e[r];
+    }
+  }
+  if constexpr (END == kForward) end.template forward<ACT>(row, col, v, w);
+  else if constexpr (END == kBackward) end.template backward<ACT>(row, col, v, w);
+  else end.plain(row, col, v, n);
+}
+
+// Rows of `panels` parts of `cols` elements, each part filled up with zeros to
+// `padded` (a multiple of 8): what k_prod16 takes, of rows that it cannot.
+__global__ __launch_bounds__(256) void k_padded(const mmp_half *src, long long ld, int rows, int panels,
+                                                int cols, int padded, mmp_half *dst) {
+  const int per = panels * padded / 8;
+  const long long id = blockIdx.x * 256LL + threadIdx.x, row = id / per;
+  if (row >= rows) return;
+  const int at = (int)(id - row * per) * 8, panel = at / padded, c = at - panel * padded;
+  const mmp_half *s = src + row * ld + (long long)panel * cols + c;
+  Vec<mmp_half, 8> v;
+  if (c + 8 <= cols) {
+    v = mmpn::load_vec<mmp_half, 8>(s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.e[i] = c + i < cols ? s[i] : (mmp_half)0;
+  }
+  mmpn::store_vec(dst + row * per * 8 + at, v);
+}
+
+// ---------------------------------------------------- float32 and float64: ends
+// Both projections (rows, 2 hidden) into h, or in place into D.
+template <typename T, int ACT, bool GRAD>
+__global__ __launch_bounds__(256) void k_ends(const T *both, long long rows, End<T> end) {
+  typedef typename Wide<T>::type A;
+  const long long id = blockIdx.x * 256LL + threadIdx.x, row = id / end.hidden;
+  if (row >= rows) return;
+  const int col = (int)(id - row * end.hidden);
+  const T *at = both + row * 2 * end.hidden + col;
+  const A g[1] = {at[0]}, u[1] = {at[end.hidden]};
+  if constexpr (GRAD) end.template backward<ACT>(row, col, g, u);
+  else end.template forward<ACT>(row, col, g, u);
+}
+
+// ------------------------------------------------------------------- host side
+bool aligned(const void *p, int bytes) { return (uintptr_t)p % bytes == 0; }
+
+// f(std::integral_constant<int, ACT>) of the activation's code.
+template <typename F> int with_activation(int act, F f) {
+  switch (act) {
+    case kSilu: return f(std::integral_constant<int, kSilu>());
+    case kGelu: return f(std::integral_constant<int, kGelu>());
+    default: return f(std::integral_constant<int, kSigmoid>());
+  }
+}
+
+int threads_of(long long n, const char *what, unsigned *blocks) {
+  const int64_t b = mmpi::ceil_div(n, 256);
+  if (!mmpi::grid_fits(b, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many elements", what);
+  *blocks = (unsigned)b;
+  return MMP_OK;
+}
+
+template <bool AK, bool BK_, bool PAIR, int END, int ACT>
+int launch16(int tile, dim3 grid, const Prod &p, const End<mmp_half> &end, const char *what) {
+  if (tile == 256)
+    hipLaunchKernelGGL((k_prod16<2, 4, 8, 4, AK, BK_, PAIR, END, ACT>), grid, dim3(512), 0, mmpi::stream(), p, end);
+  else
+    hipLaunchKernelGGL((k_prod16<2, 2, 4, 4, AK, BK_, PAIR, END, ACT>), grid, dim3(256), 0, mmpi::stream(), p, end);
+  return mmpi::check_launch(what);
+}
+
+template <bool AK, bool BK_, bool PAIR, int END, int ACT>
+int prod16(Prod p, const End<mmp_half> &end, const char *what) {
+  if (p.lda >= kRow || p.ldb >= kRow)
+    return mmpi::fail(MMP_E_UNSUPPORTED, "%s: float16 rows of 2^21 elements", what);
+  const int slabs = (p.k + 63) / 64;
+  mmpi::Prod16Plan plan = mmpi::prod16_plan(p.m, PAIR ? 2LL * p.n : p.n, slabs, mmpi::cu_count());
+  if (plan.parts > 1 && mmpn::capturing()) plan.parts = 1;
+  const int tile_n = PAIR ? plan.tile / 2 : plan.tile;
+  p.tiles_m = (p.m + plan.tile - 1) / plan.tile;
+  p.tiles_n = (p.n + tile_n - 1) / tile_n;
+  p.span = (slabs + plan.parts - 1) / plan.parts;
+  const int parts = (slabs + p.span - 1) / p.span;
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  if (!mmpi::grid_fits(tiles, 512)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many tiles", what);
+  const dim3 grid((unsigned)tiles, (unsigned)parts);
+  Temp part;
+  const int n4 = (p.n + 3) & ~3;
+  if (parts > 1) {
+    if (int st = part.get((size_t)parts * p.m * (PAIR ? 2 * n4 : n4) * sizeof(float), what)) return st;
+    p.part = (float *)part.p;
+    if (int st = launch16<AK, BK_, PAIR, kPartial, 0>(plan.tile, grid, p, end, what)) return st;
+    unsigned blocks;
+    if (int st = threads_of((long long)p.m * (n4 / 4), what, &blocks)) return st;
+    hipLaunchKernelGGL((k_join16<END, ACT>), dim3(blocks), dim3(256), 0, mmpi::stream(), p.part, parts, p.m, p.n, end);
+    return mmpi::check_launch(what);
+  }
+  return launch16<AK, BK_, PAIR, END, ACT>(plan.tile, grid, p, end, what);
+}
+
+// A matrix as k_prod16 takes it: itself, or a copy with padded rows.
+struct Operand {
+  const mmp_half *p;
+  long long ld;
+  Temp copy;
+  int get(const mmp_half *src, long long ld_src, int rows, int panels, int cols, int padded, const char *what) {
+    p = src;
+    ld = ld_src;
+    if (cols == padded && ld % 8 == 0 && ld < kRow && aligned(p, 16)) return MMP_OK;
+    if (int st = copy.get((size_t)rows * panels * padded * 2, what)) return st;
+    ld = (long long)panels * padded;
+    p = (const mmp_half *)copy.p;
+    unsigned blocks;
+    if (int st = threads_of(rows * (ld / 8), what, &blocks)) return st;
+    hipLaunchKernelGGL(k_padded, dim3(blocks), dim3(256), 0, mmpi::stream(), src, ld_src, rows, panels, cols, padded, (mmp_half *)copy.p);
+    return mmpi::check_launch(what);
+  }
+};
+
+int padded_of(int n) { return (n + 7) & ~7; }
+
+template <typename T> struct Call {
+  const char *what;
+  int act, rows, dim, hidden;
+  const T *x, *w, *grad;
+  long long ldx, ldw, ldg;
+  T *h, *grad_x, *grad_w;
+};
+
+int forward16(const Call<mmp_half> &c) {
+  Operand x, w;
+  const int hp = padded_of(c.hidden);
+  if (int st = x.get(c.x, c.ldx, c.rows, 1, c.dim, padded_of(c.dim), c.what)) return st;
+  if (int st = w.get(c.w, c.ldw, c.dim, 2, c.hidden, hp, c.what)) return st;
+  const Prod p{(const u16 *)x.p, (const u16 *)w.p, x.ld, w.ld, c.rows, c.hidden, c.dim, hp, 0, 0, 0, nullptr};
+  const End<mmp_half> end{c.h, c.hidden, nullptr, 0, c.hidden, c.hidden, c.hidden % 4 == 0};
+  return with_activation(c.act, [&](auto act) {
+    return prod16<false, true, true, kForward, act.value>(p, end, c.what);
+  });
+}
+
+int backward16(const Call<mmp_half> &c) {
+  Operand x, w;
+  Temp d;
+  const int hp = padded_of(c.hidden);
+  if (int st = x.get(c.x, c.ldx, c.rows, 1, c.dim, padded_of(c.dim), c.what)) return st;
+  if (int st = w.get(c.w, c.ldw, c.dim, 2, c.hidden, hp, c.what)) return st;
+  if (int st = d.get((size_t)c.rows * 2 * hp * 2, c.what)) return st;
+  const u16 *xp = (const u16 *)x.p, *wp = (const u16 *)w.p, *dp = (const u16 *)d.p;
+  const long long ldd = 2LL * hp;
+  const End<mmp_half> to_d{(mmp_half *)d.p, ldd, c.grad, c.ldg, c.hidden, hp, true};
+  int st = with_activation(c.act, [&](auto act) {
+    return prod16<false, true, true, kBackward, act.value>(
+        Prod{xp, wp, x.ld, w.ld, c.rows, hp, c.dim, hp, 0, 0, 0, nullptr}, to_d, c.what);
+  });
+  if (st) return st;
+  const End<mmp_half> to_x{c.grad_x, c.dim, nullptr, 0, c.dim, c.dim, c.dim % 4 == 0};
+  st = prod16<false, false, false, kPlain, 0>(Prod{dp, wp, ldd, w.ld, c.rows, c.dim, 2 * hp, 0, 0, 0, 0, nullptr},
+                                              to_x, c.what);
+  if (st) return st;
+  const End<mmp_half> to_w{c.grad_w, 2LL * c.hidden, nullptr, 0, c.hidden, hp, c.hidden % 2 == 0};
+  return prod16<true, true, false, kPlain, 0>(Prod{xp, dp, x.ld, ldd, c.dim, 2 * hp, c.rows, 0, 0, 0, 0, nullptr},
+                                              to_w, c.what);
+}
+
+template <typename T> int dtype_of() { return sizeof(T) == 4 ? MMP_F32 : MMP_F64; }
+
+template <typename T, bool GRAD> int ends(const Call<T> &c, const T *both, const End<T> &end) {
+  unsigned blocks;
+  if (int st = threads_of((long long)c.rows * c.hidden, c.what, &blocks)) return st;
+  return with_activation(c.act, [&](auto act) {
+    hipLaunchKernelGGL((k_ends<T, act.value, GRAD>), dim3(blocks), dim3(256), 0, mmpi::stream(), both, (long long)c.rows, end);
+    return mmpi::check_launch(c.what);
+  });
+}
+
+template <typename T> int forward(const Call<T> &c) {
+  if constexpr (sizeof(T) == 2) {
+    return forward16(c);
+  } else {
+    Temp both;
+    if (int st = both.get((size_t)c.rows * 2 * c.hidden * sizeof(T), c.what)) return st;
+    if (int st = mmp_matmul(dtype_of<T>(), 1, c.rows, 2LL * c.hidden, c.dim, c.x, c.ldx, 0, c.w, c.ldw, 0, both.p, 2LL * c.hidden, 0))
+      return st;
+    return ends<T, false>(c, (const T *)both.p, End<T>{c.h, c.hidden, nullptr, 0, c.hidden, c.hidden, true});
+  }
+}
+
+template <typename T> int backward(const Call<T> &c) {
+  if constexpr (sizeof(T) == 2) {
+    return backward16(c);
+  } else {
+    Temp d;
+    const long long ldd = 2LL * c.hidden;
+    if (int st = d.get((size_t)c.rows * ldd * sizeof(T), c.what)) return st;
+    if (int st = mmp_matmul(dtype_of<T>(), 1, c.rows, ldd, c.dim, c.x, c.ldx, 0, c.w, c.ldw, 0, d.p, ldd, 0)) return st;
+    if (int st = ends<T, true>(c, (const T *)d.p, End<T>{(T *)d.p, ldd, c.grad, c.ldg, c.hidden, c.hidden, true}))
+      return st;
+    if (int st = mmp_matmul_t(dtype_of<T>(), 0, 1, 1, c.rows, c.dim, ldd, d.p, ldd, 0, c.w, c.ldw, 0, c.grad_x, c.dim, 0))
+      return st;
+    return mmp_matmul_t(dtype_of<T>(), 1, 0, 1, c.dim, ldd, c.rows, c.x, c.ldx, 0, d.p, ldd, 0, c.grad_w, ldd, 0);
+  }
+}
+
+int zeros(int dtype, int64_t n, void *p) {
+  const double zero = 0.0;
+  return n ? mmp_fill(dtype, n, &zero, p) : MMP_OK;
+}
+
+int check(const char *what, int act, int64_t rows, int64_t dim, int64_t hidden) {
+  if (int st = mmpi::ensure_init()) return st;
+  if (rows < 0 || dim < 0 || hidden < 0) return mmpi::fail(MMP_E_ARG, "%s: negative extent", what);
+  if (act < kSilu || act > kSigmoid) return mmpi::fail(MMP_E_ARG, "%s: activation code %d", what, act);
+  // room for a tile past the end in 32 bits
+  if (rows > 0x7fff0000LL || dim > 0x7fff0000LL || hidden > 0x3fff0000LL)
+    return mmpi::fail(MMP_E_UNSUPPORTED, "%s: extent past 2^31", what);
+  return MMP_OK;
+}
+
+}  // namespace
+
+extern "C" int mmp_gated_feed_forward(int dtype, int activation, int64_t rows, int64_t dim, int64_t hidden,
+                                      const void *x, int64_t x_stride, const void *weights,
+                                      int64_t w_stride, void *h) {
+  const char *what = "mmp_gated_feed_forward";
+  if (int st = check(what, activation, rows, dim, hidden)) return st;
+  if (rows == 0 || hidden == 0) return MMP_OK;
+  if (!h || (dim && (!x || !weights))) return mmpi::fail(MMP_E_ARG, "%s: null pointer", what);
+  if (dim == 0) return zeros(dtype, rows * hidden, h);  // u is 0
+  MMP_DISPATCH_FLOAT(dtype, "mmp_gated_feed_forward", {
+    return forward<T>(Call<T>{what, activation, (int)rows, (int)dim, (int)hidden, (const T *)x,
+                              (const T *)weights, nullptr, (long long)x_stride, (long long)w_stride, 0,
+                              (T *)h, nullptr, nullptr});
+  })
+}
+
+extern "C" int mmp_gated_feed_forward_grad(int dtype, int activation, int64_t rows, int64_t dim,
+                                           int64_t hidden, const void *grad, int64_t grad_stride,
+                                           const void *x, int64_t x_stride, const void *weights,
+                                           int64_t w_stride, void *grad_x, void *grad_weights) {
+  const char *what = "mmp_gated_feed_forward_grad";
+  if (int st = check(what, activation, rows, dim, hidden)) return st;
+  if (dim == 0) return MMP_OK;
+  if ((rows && !grad_x) || (hidden && !grad_weights)) return mmpi::fail(MMP_E_ARG, "%s: null pointer", what);
+  if (rows == 0 || hidden == 0) {
+    if (int st = zeros(dtype, rows * dim, grad_x)) return st;
+    return zeros(dtype, 2 * dim * hidden, grad_weights);
+  }
+  if (!grad || !x || !weights) return mmpi::fail(MMP_E_ARG, "%s: null pointer", what);
+  MMP_DISPATCH_FLOAT(dtype, "mmp_gated_feed_forward_grad", {
+    return backward<T>(Call<T>{what, activation, (int)rows, (int)dim, (int)hidden, (const T *)x,
+                               (const T *)weights, (const T *)grad, (long long)x_stride,
+                               (long long)w_stride, (long long)grad_stride, nullptr, (T *)grad_x,
+                               (T *)grad_weights});
+  })
+}

@@ -273,6 +273,31 @@ inline GemmPlan gemm_plan(long long batch, int M, int N, int K, int elem, bool m
   return best;
 }
 
+// Tile and k ranges of the feed-forward products' float16 kernel (k_prod16):
+// 256 wide tiles, one workgroup a CU, or 128 wide ones, two; a tile's slab of 64
+// deep, its start and its end in us, and what a second launch that adds ranges
+// up costs.
+struct Prod16Plan {
+  int tile;
+  int parts;  // ranges of k
+  double us;
+};
+inline Prod16Plan prod16_plan(long long m, long long n, int slabs, double cus) {
+  Prod16Plan best{128, 1, 1e30};
+  for (int tile = 256; tile >= 128; tile /= 2) {
+    const double tiles = (double)((m + tile - 1) / tile) * (double)((n + tile - 1) / tile);
+    const double per_cu = tile == 256 ? 1 : 2;
+    for (int s = 1; s <= 64; s *= 2) {
+      if (s > 1 && (slabs / s < 4 || tiles * s > 2 * cus * per_cu)) break;
+      double t = tile == 256 ? rounds_us(tiles * s, 1, (slabs + s - 1) / s, 5.0, 1.75, 1.75, cus)
+                             : rounds_us(tiles * s, 2, (slabs + s - 1) / s, 3.5, 0.6, 0.75, cus);
+      if (s > 1) t += 4.0 + 2e-6 * s * (double)m * (double)n * 4 / 5.0;
+      if (t < best.us * 0.98) best = Prod16Plan{tile, s, t};
+    }
+  }
+  return best;
+}
+
 // Rows from which unaligned ones, each longer than a tile, are scanned by a
 // workgroup each instead of in tiles that look back.  What a row's waves walk
 // is paid in latency, so fewer rows need more bytes a step.  40,000,000

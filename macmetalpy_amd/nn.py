@@ -33,6 +33,7 @@ from .manipulation import broadcast_to
 from .ndarray import ndarray, _c_contiguous_strides, _prod
 
 __all__ = ["embedding", "embedding_grad", "gated_recurrence", "gated_recurrence_grad",
+           "gated_feed_forward", "gated_feed_forward_grad", "dropout",
            "cross_entropy", "cross_entropy_grad", "global_norm", "clip_by_global_norm"]
 
 _F32, _F64, _I32, _I64 = (np.dtype(t) for t in (np.float32, np.float64, np.int32, np.int64))
@@ -253,6 +254,128 @@ def gated_recurrence_grad(grad, gate, x, h, initial=None, grad_final=None, *, lo
                                      _ptr(grad_final), grad_gate._ptr, grad_x._ptr,
                                      grad_initial._ptr)
     return grad_gate, grad_x, grad_initial
+
+
+# ---------------------------------------------------------- feed-forward
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
+
+
+def _matrix(a):
+    """_rows of an array whose rows do not overlap, as products take them."""
+    width, rows = a._shape[-1], _prod(a._shape[:-1])
+    a, stride = _rows(a)
+    if stride < width and rows > 1:
+        return a._contiguous_copy(), width
+    return a, max(stride, width)
+
+
+def _gated(x, weights, activation):
+    x, weights = _floating(x, "x"), _floating(weights, "weights")
+    if x.ndim == 0 or weights.ndim != 2 or weights._shape[0] != x._shape[-1]:
+        raise ValueError(f"weights of shape {weights._shape} do not fit x of shape {x._shape}: "
+                         f"expected x's last axis and both projections' columns")
+    if weights._shape[1] % 2:
+        raise ValueError(f"weights of shape {weights._shape}: two projections have an even number "
+                         f"of columns")
+    if not isinstance(activation, str) or activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, not {activation!r}")
+    return x, weights, _ACTIVATIONS[activation]
+
+
+def gated_feed_forward(x, weights, activation="silu") -> ndarray:
+    """``a(x @ weights[:, :hidden]) * (x @ weights[:, hidden:])`` of (..., dim)
+    rows ``x`` and one (dim, 2 * hidden) array of both projections: (..., hidden).
+    ``activation`` is a: ``"silu"`` g / (1 + exp(-g)), ``"gelu"`` g times the
+    normal distribution's function of g, ``"sigmoid"`` 1 / (1 + exp(-g)).  The
+    projections are summed, activated and multiplied in float32 (float64 for
+    float64) and never stored."""
+    x, weights, act = _gated(x, weights, activation)
+    dtype = x._dtype
+    if weights._dtype != dtype:
+        dtype = np.result_type(dtype, weights._dtype)
+        x, weights = _contiguous(x, dtype), _contiguous(weights, dtype)
+    dim, hidden = weights._shape[0], weights._shape[1] // 2
+    h = _empty(x._shape[:-1] + (hidden,), dtype)
+    if h.size:
+        x, ldx = _matrix(x)
+        weights, ldw = _matrix(weights)
+        HipBackend().gated_feed_forward(_CODE[dtype], act, _prod(x._shape[:-1]), dim, hidden,
+                                        x._ptr, ldx, weights._ptr, ldw, h._ptr)
+    return h
+
+
+def gated_feed_forward_grad(grad, x, weights, activation="silu"):
+    """``(grad_x, grad_weights)`` of :func:`gated_feed_forward`, from ``grad``
+    (of its result) and its inputs, in their type.  The projections are worked
+    out again; their own gradients are rounded to that type once, for the two
+    products that follow."""
+    x, weights, act = _gated(x, weights, activation)
+    grad = _floating(grad, "grad")
+    dim, hidden = weights._shape[0], weights._shape[1] // 2
+    if grad._shape != x._shape[:-1] + (hidden,):
+        raise ValueError(f"grad of shape {grad._shape}: expected {x._shape[:-1] + (hidden,)}")
+    dtype = x._dtype
+    if weights._dtype != dtype or grad._dtype != dtype:
+        dtype = np.result_type(dtype, weights._dtype, grad._dtype)
+        grad, x, weights = (_contiguous(a, dtype) for a in (grad, x, weights))
+    grad_x, grad_weights = _empty(x._shape, dtype), _empty(weights._shape, dtype)
+    if grad_x.size or grad_weights.size:
+        grad, ldg = _matrix(grad)
+        x, ldx = _matrix(x)
+        weights, ldw = _matrix(weights)
+        HipBackend().gated_feed_forward_grad(_CODE[dtype], act, _prod(x._shape[:-1]), dim, hidden,
+                                             grad._ptr, ldg, x._ptr, ldx, weights._ptr, ldw,
+                                             grad_x._ptr, grad_weights._ptr)
+    return grad_x, grad_weights
+
+
+# --------------------------------------------------------------- dropout
+def _whole(v, most, what) -> int:
+    if not isinstance(v, (int, np.integer)) or isinstance(v, bool):
+        raise TypeError(f"{what} must be an integer, not {type(v).__name__}")
+    if not 0 <= v < most:
+        raise ValueError(f"{what} must be in [0, {most}), not {v}")
+    return int(v)
+
+
+def dropout(x, rate, seed, offset=0, residual=None) -> ndarray:
+    """``x`` with elements set to 0 with probability ``rate`` and the others
+    divided by ``1 - rate``, added to ``residual`` (of x's shape and type) if
+    there is one.  Nothing is drawn and no mask is kept: element i, in the order
+    of a contiguous array, is dropped where word ``offset + i`` of the stream
+    that ``seed`` names (64 bits) is less than ``rate * 2**32``.  So the gradient
+    of x is the same call on the gradient, whatever the type or the layout, and a
+    part of an array is dropped as in the whole one with its own place as
+    ``offset``; other calls take other seeds, or offsets beyond each other's
+    elements.  ``offset`` may also be an integer array of no axes, used on the device.
+
+    The words are Philox4x32-10's (Salmon, Moraes, Dror and Shaw 2011): words 4 j
+    to 4 j + 3 have the counter j and the seed as the key."""
+    x = _floating(x, "x")
+    rate, dtype = _scalar(rate, "rate"), x._dtype
+    if not 0.0 <= rate < 1.0:
+        raise ValueError(f"rate must be in [0, 1), not {rate}")
+    seed, at = _whole(seed, 1 << 64, "seed"), None
+    if isinstance(offset, (ndarray, np.ndarray)):
+        at = _integers(offset, "offset")
+        if at.ndim:
+            raise ValueError(f"offset of shape {at._shape}: expected an integer or an array of "
+                             f"no axes")
+        at, offset = _contiguous(at, _I64), 0
+    else:
+        offset = _whole(offset, 1 << 63, "offset")
+    if residual is not None:
+        residual = _floating(residual, "residual")
+        if residual._shape != x._shape or residual._dtype != dtype:
+            raise ValueError(f"residual of shape {residual._shape} and type {residual._dtype}: "
+                             f"expected {x._shape} and {dtype}")
+        residual = _contiguous(residual, dtype)
+    x = _contiguous(x, dtype)
+    y = _empty(x._shape, dtype)
+    if y.size:
+        HipBackend().dropout(_CODE[dtype], y.size, x._ptr, _ptr(residual), rate, seed, offset,
+                             _ptr(at), y._ptr)
+    return y
 
 
 # ------------------------------------------------------------------ loss
