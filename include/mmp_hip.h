@@ -550,6 +550,24 @@ int mmp_clip_norm(int64_t count, const int *dtypes, const int64_t *sizes,
                   const void *const *arrays, void *const *outs, double limit,
                   int norm_dtype, void *norm);
 
+/* The gated delta rule: states S (dk x dv) of (batch, heads),
+ *   u_t = beta_t (v_t - a_t S_{t-1}^T k_t), S_t = a_t S_{t-1} + k_t u_t^T,
+ *   o_t = scale S_t^T q_t, a_t = exp(gate_t),
+ * with q, k (batch, steps, key_heads, dk), v (batch, steps, heads, dv), gate and
+ * beta (batch, steps, heads) of dtype or, where gate_wide (beta_wide) is set, of the
+ * wide type; sb, st and sh are the strides of sequences, steps and heads.
+ * heads is a multiple of key_heads, dk at most 256.  initial (NULL for zeros) and
+ * final are (batch, heads, dk, dv) of the wide type, o (batch, steps, heads, dv).
+ * Up to 8 steps take no scratch memory. */
+int mmp_delta_rule(int dtype, int64_t batch, int64_t steps, int64_t key_heads, int64_t heads,
+                   int64_t dk, int64_t dv,
+                   const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                   const void *k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                   const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                   const void *gate, int gate_wide, int64_t g_sb, int64_t g_st, int64_t g_sh,
+                   const void *beta, int beta_wide, int64_t b_sb, int64_t b_st, int64_t b_sh,
+                   const void *initial, double scale, void *o, void *final_state);
+
 /* h = a(g) u with g = x W[:, :hidden], u = x W[:, hidden:], for (rows, dim) x
  * and (dim, 2 hidden) weights W; activation a: 0 silu, 1 gelu (of the normal
  * distribution's function), 2 sigmoid.  Row strides are at least the rows'

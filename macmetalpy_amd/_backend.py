@@ -137,6 +137,9 @@ _SIGNATURES = {
     "mmp_cross_entropy": [_c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
                           ctypes.c_double, _c_vp, _c_vp],
     "mmp_clip_norm": [_c_i64, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_double, _c_int, _c_vp],
+    "mmp_delta_rule": [_c_int] + [_c_i64] * 6 + [_c_vp, _c_i64, _c_i64, _c_i64] * 3
+                      + [_c_vp, _c_int, _c_i64, _c_i64, _c_i64] * 2
+                      + [_c_vp, ctypes.c_double, _c_vp, _c_vp],
     "mmp_gated_feed_forward": [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
                                _c_vp],
     "mmp_gated_feed_forward_grad": [_c_int, _c_int, _c_i64, _c_i64, _c_i64]
@@ -585,6 +588,10 @@ class HipBackend:
         if outs is None:
             at[3] = None
         _check(self._lib.mmp_clip_norm(len(sizes), *at, limit, norm_code, norm), "mmp_clip_norm")
+
+    def delta_rule(self, *args) -> None:
+        """The arguments of mmp_delta_rule in its order."""
+        _check(self._lib.mmp_delta_rule(*args), "mmp_delta_rule")
 
     def gated_feed_forward(self, dcode, activation, rows, dim, hidden, x, x_stride, weights,
                            w_stride, h) -> None:

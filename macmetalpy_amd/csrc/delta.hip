@@ -1,0 +1,695 @@
+// delta.hip -- the gated delta rule: a recurrence whose state is a matrix.
+//
+// A head's state S (dk x dv), decayed by a_t = exp(gate_t), is corrected
+// towards the value v_t at the key k_t and read by the query q_t:
+//
+//   u_t = beta_t (v_t - a_t S_{t-1}^T k_t)
+//   S_t = a_t S_{t-1} + k_t u_t^T,   o_t = scale S_t^T q_t
+//
+// Few steps go one after another (k_delta_steps), each in one pass over a state
+// that stays in registers.  Otherwise steps go by in chunks of C, as matrix
+// products.  With D_ij = a_{j+1} .. a_i, c_i = a_1 .. a_i (from the chunk's start),
+// e_j = a_{j+1} .. a_C and S the state before the chunk,
+//
+//   (1 + A) U = R,   A_ij = beta_i D_ij k_i.k_j (j < i),   R = beta (V - c K S)
+//   O = scale (c Q S + P U),   P_ij = D_ij q_i.k_j (j <= i)
+//   S' = c_C S + K^T (e U)
+//
+// k_delta_within makes T = (1 + A)^-1 and scale P of all chunks at once;
+// k_delta_pass goes through the chunks of a head with the state in registers, a
+// wave for each 16 columns of it.  The columns of a state do not meet, so
+// a wave needs nothing of another but the keys, the queries, T and P, which a
+// workgroup has in LDS.
+//
+// A gate of -inf starts the state anew.  Logarithms are summed without such
+// steps, which are counted: a factor between two steps is 0 where their counts differ,
+// and no difference of infinities arises.  Sums of logarithms are in 64 bits, as
+// a factor's relative error is the absolute one of its logarithm.
+//
+// The state is 32 bits wide (64 for float64), and so is what goes into it: where
+// a float16 product needs a value that is no input, it takes it as two float16
+// numbers (mmp_mma.h).
+#include "mmp_mma.h"
+
+namespace {
+
+using mmpn::Temp;
+using mmpn::Vec;
+using mmpn::Wide;
+using mmpx::Mma;
+using mmpx::Two;
+
+// Steps of a chunk: the products within one grow with it, the passes through the
+// states fall; the matrix rate decides, 16 times less for 32 bits and 32 for 64.
+template <typename T> constexpr int chunk_of() { return sizeof(T) == 2 ? 64 : sizeof(T) == 4 ? 32 : 16; }
+template <typename T> constexpr int vec_of() { return 16 / sizeof(T); }
+
+// An array (batch, steps, heads, width) with adjacent elements, or (batch, steps,
+// heads) of gates, by its strides.
+template <typename T> struct Seq {
+  const T *p;
+  long long sb, st, sh;
+  __device__ __forceinline__ const T *at(int b, long long t, int h) const { return p + b * sb + t * st + h * sh; }
+};
+// Gates may be of the sequences' type or the wide one.
+template <typename T> struct Gate {
+  typedef typename Wide<T>::type A;
+  const void *p;
+  long long sb, st, sh;
+  int wide;
+  __device__ __forceinline__ A at(int b, long long t, int h) const {
+    const long long i = b * sb + t * st + h * sh;
+    return wide ? ((const A *)p)[i] : (A)((const T *)p)[i];
+  }
+};
+
+template <typename T> struct Delta {
+  typedef typename Wide<T>::type A;
+  Seq<T> q, k, v;
+  Gate<T> gate, beta;
+  int batch, heads, group, dk, dv;  // group: heads that share a key head
+  long long steps;
+  int chunks;
+  A scale;
+  T *within;  // of each chunk of each head: T, P (float16: T, its rest, P, its rest)
+  A *vecs;    // c, e and beta of each step of a chunk
+};
+template <typename T> constexpr int parts_of() { return Mma<T>::SPLIT ? 2 : 1; }
+
+// exp(g) is 0 in the wide type: such a step is counted as one of -inf.
+template <typename A> __device__ __forceinline__ bool starts_anew(A g) { return g < (sizeof(A) == 4 ? (A)-104 : (A)-746); }
+__device__ __forceinline__ float exp_any(float x) { return x > 80.0f ? expf(x) : mmpn::exp_of(x); }
+__device__ __forceinline__ double exp_any(double x) { return exp(x); }
+
+// W columns of ROWS rows of an array in registers, and on their way to LDS.
+template <typename T, int ROWS, int W, int THREADS> struct Tile {
+  static constexpr int V = vec_of<T>(), PER = W / V, N = (ROWS * PER + THREADS - 1) / THREADS;
+  typedef typename Vec<T, V>::Words Words;
+  Words w[N];
+  // rows from `rows` on and columns from `cols` on are zeros
+  __device__ __forceinline__ void fetch(const T *p, long long stride, int rows, int cols, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = i * THREADS + tid, r = id / PER, c = id % PER * V;
+      Vec<T, V> x{};
+      if (r < rows && r < ROWS) {
+        const T *at = p + r * stride + c;
+        if (c + V <= cols) {
+          x = mmpn::load_vec<T, V>(at);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < cols) x.e[e] = at[e];
+        }
+      }
+      w[i] = mmpn::words_of(x);
+    }
+  }
+  __device__ __forceinline__ void put(T *lds, int ld, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = i * THREADS + tid, r = id / PER, c = id % PER * V;
+      if (r < ROWS) *reinterpret_cast<Words *>(lds + r * ld + c) = w[i];
+    }
+  }
+};
+
+// ------------------------------------------------------------- within chunks
+// Workgroup: a chunk of a head.
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
+  typedef typename Wide<T>::type A;
+  typedef Mma<T> M;
+  typedef Mma<A> MA;
+  typedef typename M::Acc Acc;
+  typedef typename MA::Acc AccA;
+  constexpr int C = chunk_of<T>(), NT = C / 16, LD = DK + M::PAD, LA = C + MA::PAD;
+  constexpr int KEYS = 2 * C * LD * sizeof(T), INV = C * LA * sizeof(A);
+  __shared__ __attribute__((aligned(16))) char mem[KEYS > INV ? KEYS : INV];
+  T *Ks = (T *)mem, *Qs = Ks + C * LD;
+  A *Ts = (A *)mem;  // when the keys are done with
+  __shared__ __attribute__((aligned(16))) A As[C * LA], Td[C * (16 + MA::PAD)];
+  __shared__ double G[C];
+  __shared__ int R[C];
+  __shared__ A bet[C];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  const long long id = blockIdx.x, bh = id / p.chunks;
+  const int n = (int)(id - bh * p.chunks), b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
+  const long long t0 = (long long)n * C;
+  const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
+  T *out = p.within + id * (2 * parts_of<T>() * C * C);
+
+  {
+    Tile<T, C, DK, 256> k, q;
+    k.fetch(p.k.at(b, t0, h / p.group), p.k.st, left, p.dk, tid);
+    q.fetch(p.q.at(b, t0, h / p.group), p.q.st, left, p.dk, tid);
+    k.put(Ks, LD, tid);
+    q.put(Qs, LD, tid);
+  }
+  if (wave == 0) {  // logarithms summed up, fresh starts counted
+    const A gate = lane < left ? p.gate.at(b, t0 + lane, h) : (A)0;
+    const bool anew = starts_anew(gate);
+    const int count = __popcll(__ballot(anew) & ((2ull << lane) - 1));
+    double sum = anew ? 0.0 : (double)gate;
+#pragma unroll
+    for (int d = 1; d < C; d *= 2) {
+      const double up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
+    }
+    const double last = __shfl(sum, C - 1);
+    const int count_last = __shfl(count, C - 1);
+    if (lane < C) {
+      const A beta = lane < left ? p.beta.at(b, t0 + lane, h) : (A)0;
+      G[lane] = sum;
+      R[lane] = count;
+      bet[lane] = beta;
+      A *v = p.vecs + id * 3 * C;
+      v[lane] = count == 0 ? exp_any((A)sum) : (A)0;
+      v[C + lane] = count == count_last ? exp_any((A)(last - sum)) : (A)0;
+      v[2 * C + lane] = beta;
+    }
+  }
+  __syncthreads();
+
+  // tiles of K K^T to A and of Q K^T to P, transposed: a lane has row fr of a tile
+  for (int task = wave; task < 2 * NT; task += 4) {
+    const bool query = task >= NT;
+    const int rt = query ? 2 * NT - 1 - task : task, i = 16 * rt + fr;
+    const T *X = query ? Qs : Ks;
+    const double Gi = G[i];
+    const int Ri = R[i];
+    const A by = query ? p.scale : bet[i];
+    for (int jt = 0; jt < NT; ++jt) {
+      Acc acc{};
+      if (jt <= rt)
+#pragma unroll
+        for (int ks = 0; ks < DK; ks += M::K)
+          acc = M::mul(M::rows(Ks, LD, 16 * jt, ks, lane), M::rows(X, LD, 16 * rt, ks, lane), acc);
+      A v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + M::row(g, r);
+        const bool in = (query ? j <= i : j < i) && R[j] == Ri;
+        v[r] = in ? exp_any((A)(Gi - G[j])) * by * acc[r] : (A)0;
+      }
+      if (query) {
+        T *o = out + parts_of<T>() * C * C + i * C + 16 * jt;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const T hi = (T)v[r];
+          o[M::row(g, r)] = hi;
+          if constexpr (M::SPLIT) o[C * C + M::row(g, r)] = (T)(v[r] - (A)hi);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) As[i * LA + 16 * jt + M::row(g, r)] = v[r];
+      }
+    }
+  }
+  __syncthreads();
+
+  // T's blocks on the diagonal: column fr of block g by substitution
+  constexpr int LT = 16 + MA::PAD;
+  if (wave == 0 && g < NT) {
+    A x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      A s = i == fr ? (A)1 : (A)0;
+#pragma unroll
+      for (int j = 0; j < i; ++j) s = mmpn::fma_of(-As[(16 * g + i) * LA + 16 * g + j], x[j], s);
+      x[i] = s;
+      Td[(16 * g + i) * LT + fr] = s;
+    }
+  }
+  __syncthreads();
+  // and below it: T_ij = -T_ii sum over j <= m < i of A_im T_mj, a wave a column
+  if (wave < NT) {
+    const int j = wave;
+    AccA t[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      t[i] = AccA{};
+      if (i == j) {
+        t[i] = MA::cols(Td, LT, 16 * j, 0, lane);
+      } else if (i > j) {
+        AccA s{};
+#pragma unroll
+        for (int m = 0; m < NT; ++m)
+          if (m >= j && m < i) s = MA::mul(MA::rows(As, LA, 16 * i, 16 * m, lane), t[m], s);
+        s = MA::mul(MA::rows(Td, LT, 16 * i, 0, lane), s, AccA{});
+        t[i] = -s;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) Ts[(16 * i + MA::row(g, r)) * LA + 16 * j + fr] = t[i][r];
+    }
+  }
+  __syncthreads();
+  constexpr int V = vec_of<T>();
+  for (int at = tid; at < C * C / V; at += 256) {
+    const int i = at / (C / V), j = at % (C / V) * V;
+    Vec<T, V> hi, lo;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const A v = Ts[i * LA + j + e];
+      hi.e[e] = (T)v;
+      lo.e[e] = (T)(v - (A)hi.e[e]);
+    }
+    mmpn::store_vec(out + i * C + j, hi);
+    if constexpr (M::SPLIT) mmpn::store_vec(out + C * C + i * C + j, lo);
+  }
+}
+
+// --------------------------------------------------------- through the chunks
+// What a pass leaves for the gradient: of each chunk the state before it,
+// transposed (dv, DK), and U, transposed (dv, C), in the sequences' type.
+template <typename T> struct Pass {
+  typedef typename Wide<T>::type A;
+  const A *initial;
+  A *final;
+  T *o;
+  T *keep_s, *keep_u;
+  int tiles;  // workgroups a head
+};
+
+template <typename T> __device__ __forceinline__ void put4(T *p, const typename Wide<T>::type (&v)[4], int g) {
+  if constexpr (sizeof(T) == 8) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[g + 4 * r] = (T)v[r];
+  } else {
+    Vec<T, 4> w;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w.e[r] = (T)v[r];
+    mmpn::store_vec(p + 4 * g, w);
+  }
+}
+
+// Workgroup: NW waves with 16 columns each of a head's state (one without any only
+// helps with the copies).
+template <typename T, int DK, int NW, bool OUT, bool KEEP>
+__global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e) {
+  typedef typename Wide<T>::type A;
+  typedef Mma<T> M;
+  typedef typename M::Acc Acc;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, THREADS = 64 * NW;
+  constexpr int LD = DK + M::PAD, LC = C + M::PAD, LV = 16 * NW + M::PAD, DT = DK / 16;
+  __shared__ __attribute__((aligned(16))) T Ks[C * LD], Qs[OUT ? C * LD : 1], Th[C * LC],
+      Tl[M::SPLIT ? C * LC : 1], Ps[OUT ? C * LC : 1], Vs[C * LV];
+  __shared__ __attribute__((aligned(16))) A vecs[3 * C];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  const long long bh = blockIdx.x / e.tiles;
+  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
+  const int n0 = (int)(blockIdx.x - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;  // of the state
+  const bool there = col < p.dv;
+
+  Acc S[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * t + M::row(g, r);
+      S[t][r] = e.initial && there && i < p.dk ? e.initial[(bh * p.dk + i) * p.dv + col] : (A)0;
+    }
+
+  Tile<T, C, DK, THREADS> k, q;
+  Tile<T, C, C, THREADS> th, tl, ps;
+  Tile<T, C, 16 * NW, THREADS> v;
+  constexpr int NV = (3 * C + THREADS - 1) / THREADS;
+  A vec[NV];
+  // f(tile, its LDS, its row length there, from, stride, rows, columns) of each array
+  auto arrays = [&](int n, auto f) {
+    const long long t0 = (long long)n * C;
+    const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
+    const T *w = p.within + (bh * p.chunks + n) * (2 * parts_of<T>() * C * C);
+    f(k, Ks, LD, p.k.at(b, t0, h / p.group), p.k.st, left, p.dk);
+    if constexpr (OUT) f(q, Qs, LD, p.q.at(b, t0, h / p.group), p.q.st, left, p.dk);
+    f(th, Th, LC, w, C, C, C);
+    if constexpr (M::SPLIT) f(tl, Tl, LC, w + C * C, C, C, C);
+    if constexpr (OUT) f(ps, Ps, LC, w + parts_of<T>() * C * C, C, C, C);
+    f(v, Vs, LV, p.v.at(b, t0, h) + n0, p.v.st, left, p.dv - n0);
+  };
+  auto fetch_vecs = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * THREADS + tid < 3 * C) vec[i] = p.vecs[(bh * p.chunks + n) * 3 * C + i * THREADS + tid];
+  };
+  auto put_vecs = [&]() {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * THREADS + tid < 3 * C) vecs[i * THREADS + tid] = vec[i];
+  };
+  auto fetch = [&](int n) {
+    arrays(n, [&](auto &tile, T *, int, const T *from, long long stride, int rows, int cols) {
+      tile.fetch(from, stride, rows, cols, tid);
+    });
+    fetch_vecs(n);
+  };
+  auto put = [&]() {
+    arrays(0, [&](auto &tile, T *to, int ld, const T *, long long, int, int) { tile.put(to, ld, tid); });
+    put_vecs();
+  };
+  auto load = [&](int n) {
+    arrays(n, [&](auto &tile, T *to, int ld, const T *from, long long stride, int rows, int cols) {
+      tile.fetch(from, stride, rows, cols, tid);
+      tile.put(to, ld, tid);
+    });
+    fetch_vecs(n);
+    put_vecs();
+  };
+
+  auto chunk = [&](int n) {
+    const long long t0 = (long long)n * C;
+    const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
+
+    Two<T> s[DT / PT];
+#pragma unroll
+    for (int i = 0; i < DT / PT; ++i) s[i] = mmpx::operand<T>(S, i * PT);
+    if constexpr (KEEP) {
+      if (there) {
+        T *o = e.keep_s + ((bh * p.chunks + n) * p.dv + col) * DK;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const A w[4] = {S[t][0], S[t][1], S[t][2], S[t][3]};
+          put4<T>(o + 16 * t, w, g);
+        }
+      }
+    }
+    // R = beta (V - c K S)
+    Acc x[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      x[i] = Acc{};
+#pragma unroll
+      for (int d = 0; d < DT / PT; ++d) x[i] = mmpx::mul_two<T>(M::rows(Ks, LD, 16 * i, d * M::K, lane), s[d], x[i]);
+    }
+    Two<T> f[NT / PT], fe[NT / PT];
+#pragma unroll
+    for (int i = 0; i < NT; i += PT) {
+      const typename M::Frag value = M::cols(Vs, LV, 16 * i, 16 * wave, lane);
+      A r[M::E];
+#pragma unroll
+      for (int c = 0; c < M::E; ++c) {
+        const int at = 16 * (i + (c >> 2)) + M::row(g, c & 3);
+        r[c] = vecs[2 * C + at] * mmpn::fma_of(-vecs[at], x[i + (c >> 2)][c & 3], (A)value[c]);
+      }
+      f[i / PT] = mmpx::two_of<T>(r);
+    }
+    // U = T R
+    Acc u[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      u[i] = Acc{};
+#pragma unroll
+      for (int j = 0; j <= i / PT; ++j) {
+        Two<T> t;
+        t.hi = M::rows(Th, LC, 16 * i, j * M::K, lane);
+        if constexpr (M::SPLIT) t.lo = M::rows(Tl, LC, 16 * i, j * M::K, lane);
+        u[i] = mmpx::mul_twos<T>(t, f[j], u[i]);
+      }
+    }
+    if constexpr (KEEP) {
+      if (there) {
+        T *o = e.keep_u + ((bh * p.chunks + n) * p.dv + col) * C;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const A w[4] = {u[i][0], u[i][1], u[i][2], u[i][3]};
+          put4<T>(o + 16 * i, w, g);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i += PT) {
+      f[i / PT] = mmpx::operand<T>(u, i);
+      A w[M::E];
+#pragma unroll
+      for (int c = 0; c < M::E; ++c) w[c] = vecs[C + 16 * (i + (c >> 2)) + M::row(g, c & 3)] * u[i + (c >> 2)][c & 3];
+      fe[i / PT] = mmpx::two_of<T>(w);
+    }
+    // O, transposed: a lane has a step's columns row(g, .) of the wave's 16
+    if constexpr (OUT) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        Acc o{};
+#pragma unroll
+        for (int d = 0; d < DT / PT; ++d) o = mmpx::two_mul<T>(s[d], M::rows(Qs, LD, 16 * i, d * M::K, lane), o);
+        const A by = p.scale * vecs[16 * i + fr];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] *= by;
+#pragma unroll
+        for (int j = 0; j <= i / PT; ++j) o = mmpx::two_mul<T>(f[j], M::rows(Ps, LC, 16 * i, j * M::K, lane), o);
+        const int step = 16 * i + fr;
+        if (step < left) {
+          T *to = e.o + (((long long)b * p.steps + t0 + step) * p.heads + h) * p.dv + n0 + 16 * wave;
+          if (n0 + 16 * wave + 16 <= p.dv) {
+            const A w[4] = {o[0], o[1], o[2], o[3]};
+            put4<T>(to, w, g);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n0 + 16 * wave + M::row(g, r) < p.dv) to[M::row(g, r)] = (T)o[r];
+          }
+        }
+      }
+    }
+    // S' = c_C S + K^T (e U)
+    const A decay = vecs[C - 1];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][r] *= decay;
+#pragma unroll
+      for (int j = 0; j < NT / PT; ++j) S[t] = mmpx::mul_two<T>(M::cols(Ks, LD, j * M::K, 16 * t, lane), fe[j], S[t]);
+    }
+  };
+
+  // The next chunk is on its way in registers during the products of this one,
+  // where there are enough of them.
+  constexpr bool AHEAD = DK <= 128;
+  if constexpr (AHEAD) fetch(0);
+  for (int n = 0; n < p.chunks; ++n) {
+    if constexpr (AHEAD) {
+      put();
+      __syncthreads();
+      if (n + 1 < p.chunks) fetch(n + 1);
+    } else {
+      load(n);
+      __syncthreads();
+    }
+    if (n0 + 16 * wave < p.dv) chunk(n);
+    __syncthreads();
+  }
+  if (e.final && there)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * t + M::row(g, r);
+        if (i < p.dk) e.final[(bh * p.dk + i) * p.dv + col] = S[t][r];
+      }
+}
+
+// ------------------------------------------------------------- single steps
+// Workgroup: 32 columns of a head's state, in vectors of 4, the rows over 32
+// groups of 8 threads.  S^T k and S^T q are summed in one pass over the state, as
+// o = a S^T q + (k.q) u.
+template <typename T, int ROWS>
+__global__ __launch_bounds__(256) void k_delta_steps(Delta<T> p, Pass<T> e) {
+  typedef typename Wide<T>::type A;
+  constexpr int GROUPS = 32;  // state rows side by side; a thread has ROWS of them
+  __shared__ A ks[GROUPS * ROWS], qs[GROUPS * ROWS];
+  __shared__ A part[4][8][9], kqs[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c4 = tid & 7, row0 = tid >> 3;
+  const long long bh = blockIdx.x / e.tiles;
+  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
+  const int col = (int)(blockIdx.x - bh * e.tiles) * 32 + c4 * 4;
+  const int cols = p.dv - col;  // <= 0: none
+  A S[ROWS][4];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = row0 + GROUPS * i;
+    const A *at = e.initial + (bh * p.dk + r) * p.dv + col;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) S[i][c] = 0;
+    if (e.initial && r < p.dk) {
+      if (cols >= 4) {
+        const auto w = mmpn::load_vec<A, 4>(at);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) S[i][c] = w.e[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c < cols) S[i][c] = at[c];
+      }
+    }
+  }
+  for (int t = 0; t < (int)p.steps; ++t) {
+    for (int i = tid; i < GROUPS * ROWS; i += 256) {
+      ks[i] = i < p.dk ? (A)p.k.at(b, t, h / p.group)[i] : (A)0;
+      qs[i] = i < p.dk ? (A)p.q.at(b, t, h / p.group)[i] : (A)0;
+    }
+    const A gate = p.gate.at(b, t, h), beta = p.beta.at(b, t, h);
+    const A a = starts_anew(gate) ? (A)0 : exp_any(gate);
+    __syncthreads();
+    A x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0}, kq = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const A kv = ks[row0 + GROUPS * i], qv = qs[row0 + GROUPS * i];
+      kq = mmpn::fma_of(kv, qv, kq);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        S[i][c] *= a;
+        x[c] = mmpn::fma_of(kv, S[i][c], x[c]);
+        y[c] = mmpn::fma_of(qv, S[i][c], y[c]);
+      }
+    }
+#pragma unroll
+    for (int d = 8; d < 64; d *= 2) {  // the wave's eight rows
+      kq += __shfl_xor(kq, d);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        x[c] += __shfl_xor(x[c], d);
+        y[c] += __shfl_xor(y[c], d);
+      }
+    }
+    if (lane < 8) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        part[wave][c4][c] = x[c];
+        part[wave][c4][4 + c] = y[c];
+      }
+      if (lane == 0) kqs[wave] = kq;
+    }
+    __syncthreads();
+    kq = (kqs[0] + kqs[1]) + (kqs[2] + kqs[3]);
+    A u[4];
+    const T *v = p.v.at(b, t, h) + col;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const A xs = (part[0][c4][c] + part[1][c4][c]) + (part[2][c4][c] + part[3][c4][c]);
+      u[c] = c < cols ? beta * ((A)v[c] - xs) : (A)0;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const A kv = ks[row0 + GROUPS * i];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) S[i][c] = mmpn::fma_of(kv, u[c], S[i][c]);
+    }
+    if (tid < 8) {
+      T *o = e.o + (((long long)b * p.steps + t) * p.heads + h) * p.dv + col;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const A ys = (part[0][c4][4 + c] + part[1][c4][4 + c]) + (part[2][c4][4 + c] + part[3][c4][4 + c]);
+        if (c < cols) o[c] = (T)(p.scale * mmpn::fma_of(kq, u[c], ys));
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = row0 + GROUPS * i;
+    A *at = e.final + (bh * p.dk + r) * p.dv + col;
+    if (r < p.dk) {
+      if (cols >= 4) {
+        Vec<A, 4> w;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w.e[c] = S[i][c];
+        mmpn::store_vec(at, w);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c < cols) at[c] = S[i][c];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+constexpr const char *kWhat = "mmp_delta_rule";
+
+// f(std::integral_constant<int, DK>) of the keys' width, filled up.
+template <typename F> int with_width(int dk, F f) {
+  if (dk <= 64) return f(std::integral_constant<int, 64>());
+  if (dk <= 128) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 256>());
+}
+
+// Memory of the chunks' products.
+template <typename T> struct Chunks {
+  Temp within, vecs;
+  int get(Delta<T> &p, const char *what) {
+    constexpr int C = chunk_of<T>();
+    const int64_t n = (p.steps + C - 1) / C, all = n * p.batch * p.heads;
+    if (!mmpi::grid_fits(all, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many steps", what);
+    p.chunks = (int)n;
+    if (int st = within.get((size_t)all * 2 * parts_of<T>() * C * C * sizeof(T), what)) return st;
+    if (int st = vecs.get((size_t)all * 3 * C * sizeof(typename Wide<T>::type), what)) return st;
+    p.within = (T *)within.p;
+    p.vecs = (typename Wide<T>::type *)vecs.p;
+    return with_width(p.dk, [&](auto dk) {
+      hipLaunchKernelGGL((k_delta_within<T, dk.value>), dim3((unsigned)all), dim3(256), 0, mmpi::stream(), p);
+      return mmpi::check_launch(what);
+    });
+  }
+};
+
+template <typename T, bool OUT, bool KEEP> int pass(const Delta<T> &p, Pass<T> e, const char *what) {
+  constexpr int NW = 4;
+  e.tiles = (p.dv + 16 * NW - 1) / (16 * NW);
+  const int64_t blocks = (int64_t)p.batch * p.heads * e.tiles;
+  if (!mmpi::grid_fits(blocks, 64 * NW)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
+  return with_width(p.dk, [&](auto dk) {
+    hipLaunchKernelGGL((k_delta_pass<T, dk.value, NW, OUT, KEEP>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+    return mmpi::check_launch(what);
+  });
+}
+
+template <typename T> int forward(Delta<T> p, Pass<T> e) {
+  if (p.steps <= 8) {
+    e.tiles = (p.dv + 31) / 32;
+    const int64_t blocks = (int64_t)p.batch * p.heads * e.tiles;
+    if (!mmpi::grid_fits(blocks, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", kWhat);
+    const dim3 grid((unsigned)blocks);
+    if (p.dk <= 128) hipLaunchKernelGGL((k_delta_steps<T, 4>), grid, dim3(256), 0, mmpi::stream(), p, e);
+    else hipLaunchKernelGGL((k_delta_steps<T, 8>), grid, dim3(256), 0, mmpi::stream(), p, e);
+    return mmpi::check_launch(kWhat);
+  }
+  Chunks<T> chunks;
+  if (int st = chunks.get(p, kWhat)) return st;
+  return pass<T, true, false>(p, e, kWhat);
+}
+
+int check(const char *what, int64_t batch, int64_t steps, int64_t key_heads, int64_t heads, int64_t dk, int64_t dv) {
+  if (int st = mmpi::ensure_init()) return st;
+  if (batch < 0 || steps < 0 || key_heads < 0 || heads < 0 || dk < 0 || dv < 0)
+    return mmpi::fail(MMP_E_ARG, "%s: negative extent", what);
+  if (heads && (!key_heads || heads % key_heads))
+    return mmpi::fail(MMP_E_ARG, "%s: %lld heads for %lld key heads", what, (long long)heads, (long long)key_heads);
+  if (dk > 256) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: keys of more than 256 channels", what);
+  if (batch > 0x7fffffffLL || heads > 0x7fffffffLL || dv > (1 << 20) || steps > 0x7fff0000LL ||
+      (heads && batch > 0x7fffffffLL / heads))
+    return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many sequences, channels or steps", what);
+  return MMP_OK;
+}
+
+}  // namespace
+
+extern "C" int mmp_delta_rule(int dtype, int64_t batch, int64_t steps, int64_t key_heads, int64_t heads,
+                              int64_t dk, int64_t dv, const void *q, int64_t q_sb, int64_t q_st,
+                              int64_t q_sh, const void *k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                              const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                              const void *gate, int gate_wide, int64_t g_sb, int64_t g_st, int64_t g_sh,
+                              const void *beta, int beta_wide, int64_t b_sb, int64_t b_st,
+                              int64_t b_sh, const void *initial, double scale, void *o,
+                              void *final_state) {
+  if (int st = check(kWhat, batch, steps, key_heads, heads, dk, dv)) return st;
+  if (batch == 0 || heads == 0 || dv == 0) return MMP_OK;
+  if (dk && !final_state) return mmpi::fail(MMP_E_ARG, "%s: null pointer", kWhat);
+  if (steps && (!v || !o || !gate || !beta || (dk && (!q || !k)))) return mmpi::fail(MMP_E_ARG, "%s: null pointer", kWhat);
+  MMP_DISPATCH_FLOAT(dtype, "mmp_delta_rule", {
+    typedef typename Wide<T>::type A;
+    const Delta<T> p{{(const T *)q, q_sb, q_st, q_sh}, {(const T *)k, k_sb, k_st, k_sh}, {(const T *)v, v_sb, v_st, v_sh},
+                     {gate, g_sb, g_st, g_sh, gate_wide}, {beta, b_sb, b_st, b_sh, beta_wide},
+                     (int)batch, (int)heads, (int)(heads / key_heads), (int)dk, (int)dv, (long long)steps, 0, (A)scale,
+                     nullptr, nullptr};
+    return forward<T>(p, Pass<T>{(const A *)initial, (A *)final_state, (T *)o, nullptr, nullptr, 0});
+  })
+}

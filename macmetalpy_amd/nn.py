@@ -33,6 +33,7 @@ from .manipulation import broadcast_to
 from .ndarray import ndarray, _c_contiguous_strides, _prod
 
 __all__ = ["embedding", "embedding_grad", "gated_recurrence", "gated_recurrence_grad",
+           "gated_delta_rule",
            "gated_feed_forward", "gated_feed_forward_grad", "dropout",
            "cross_entropy", "cross_entropy_grad", "global_norm", "clip_by_global_norm"]
 
@@ -254,6 +255,100 @@ def gated_recurrence_grad(grad, gate, x, h, initial=None, grad_final=None, *, lo
                                      _ptr(grad_final), grad_gate._ptr, grad_x._ptr,
                                      grad_initial._ptr)
     return grad_gate, grad_x, grad_initial
+
+
+# ------------------------------------------------------------ delta rule
+_MOST_KEYS = 256
+
+
+def _strided(a):
+    """(array, (pointer, strides of its first three axes)), with adjacent
+    elements along a fourth."""
+    strides = a._strides
+    if len(strides) == 4 and a._shape[3] > 1 and strides[3] != 1:
+        a = a._contiguous_copy()
+        strides = a._strides
+    return a, (a._ptr,) + tuple(strides[:3])
+
+
+def _delta(q, k, v, gate, beta, initial, scale, grad=None):
+    """The checked arrays of a delta rule: a dict of them, its extents and type."""
+    named = [("q", q), ("k", k), ("v", v)] + ([] if grad is None else [("grad", grad)])
+    arrays = {n: _floating(a, n) for n, a in named}
+    for n, a in arrays.items():
+        if a.ndim != 4:
+            raise ValueError(f"{n} must have axes for the batch, steps, heads and channels: shape "
+                             f"{a._shape}")
+    q, v = arrays["q"], arrays["v"]
+    batch, steps, key_heads, dk = q._shape
+    heads, dv = v._shape[2:]
+    if arrays["k"]._shape != q._shape:
+        raise ValueError(f"k of shape {arrays['k']._shape} does not match q of shape {q._shape}")
+    if v._shape[:2] != (batch, steps):
+        raise ValueError(f"v of shape {v._shape} does not match q of shape {q._shape}")
+    if heads and (not key_heads or heads % key_heads):
+        raise ValueError(f"{heads} heads of v cannot share {key_heads} heads of q and k")
+    if dk > _MOST_KEYS:
+        raise ValueError(f"q and k have {dk} channels, more than {_MOST_KEYS}")
+    if grad is not None and arrays["grad"]._shape != v._shape:
+        raise ValueError(f"grad of shape {arrays['grad']._shape}: expected {v._shape}")
+    dtype = np.result_type(*(a._dtype for a in arrays.values()))
+    for n, a in arrays.items():
+        if a._dtype != dtype:
+            arrays[n] = _contiguous(a, dtype)
+    wide = _WIDE[dtype]
+    for n, a in (("gate", gate), ("beta", beta)):
+        a = _floating(a, n)
+        if a._shape != v._shape[:3]:
+            raise ValueError(f"{n} of shape {a._shape}: expected {v._shape[:3]}")
+        arrays[n] = a if a._dtype in (dtype, wide) else _contiguous(a, wide)
+    initial = _state(initial, (batch, heads, dk, dv), wide, "initial")
+    scale = dk ** -0.5 if scale is None and dk else 1.0 if scale is None else _scalar(scale, "scale")
+    return arrays, initial, scale, (batch, steps, key_heads, heads, dk, dv), dtype
+
+
+def _delta_inputs(arrays, names, wide):
+    """The arrays' addresses and strides in order, gates with whether they are
+    of the wide type, and the arrays that those are of."""
+    kept, at = [], []
+    for n in names:
+        a, where = _strided(arrays[n])
+        kept.append(a)
+        at += where[:1] + (int(a._dtype == wide),) + where[1:] if n in ("gate", "beta") else where
+    return kept, at
+
+
+def gated_delta_rule(q, k, v, gate, beta, initial=None, *, scale=None):
+    """``(o, final)`` of a recurrence whose state is a matrix that keys write
+    to and queries read from, each head by itself::
+
+        S_t = a_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - a_t S_{t-1}^T k_t),  a_t = exp(gate_t)
+        o_t = scale S_t^T q_t
+
+    ``q`` and ``k`` are (batch, steps, key heads, dk) with at most 256 channels,
+    ``v`` and ``o`` (batch, steps, heads, dv), ``gate`` and ``beta`` (batch,
+    steps, heads); heads are a multiple of the key heads, and head h reads key
+    head ``h // (heads // key_heads)``.  ``scale`` is ``dk ** -0.5`` if None.
+    ``initial`` is the state before the first step (batch, heads, dk, dv), zeros if
+    None; ``final`` the state after the last, in float32 (float64 for float64), to
+    go on from: one new token a call is ``steps == 1``.
+
+    ``gate`` holds logarithms of the decay, at most 0; ``-inf`` starts a head
+    anew from any finite state, and a step with a gate and a beta of 0 leaves the
+    state as it is, so packed and filled up sequences need no mask.  Use keys
+    with ``beta * sum(k * k)`` of at most 2: beyond that the recurrence itself
+    grows.  float16 holds a chunk's states, corrections and values in its range:
+    65504 is the most they may reach."""
+    arrays, initial, scale, (batch, steps, key_heads, heads, dk, dv), dtype = _delta(
+        q, k, v, gate, beta, initial, scale)
+    wide = _WIDE[dtype]
+    o = _empty((batch, steps, heads, dv), dtype)
+    final = _empty((batch, heads, dk, dv), wide)
+    if o.size or final.size:
+        kept, at = _delta_inputs(arrays, ("q", "k", "v", "gate", "beta"), wide)
+        HipBackend().delta_rule(_CODE[dtype], batch, steps, key_heads, heads, dk, dv, *at,
+                                _ptr(initial), scale, o._ptr, final._ptr)
+    return o, final
 
 
 # ---------------------------------------------------------- feed-forward
