@@ -568,6 +568,21 @@ int mmp_delta_rule(int dtype, int64_t batch, int64_t steps, int64_t key_heads, i
                    const void *beta, int beta_wide, int64_t b_sb, int64_t b_st, int64_t b_sh,
                    const void *initial, double scale, void *o, void *final_state);
 
+/* Its gradient, from grad (of o, as v is laid out, with strides), grad_final (of
+ * final; NULL for zeros) and the inputs: grad_q, grad_k, grad_v, grad_gate,
+ * grad_beta of their inputs' shapes and types, grad_initial as initial. */
+int mmp_delta_rule_grad(int dtype, int64_t batch, int64_t steps, int64_t key_heads, int64_t heads,
+                        int64_t dk, int64_t dv,
+                        const void *grad, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                        const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                        const void *k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                        const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                        const void *gate, int gate_wide, int64_t g_sb, int64_t g_st, int64_t g_sh,
+                        const void *beta, int beta_wide, int64_t b_sb, int64_t b_st, int64_t b_sh,
+                        const void *initial, const void *grad_final, double scale,
+                        void *grad_q, void *grad_k, void *grad_v, void *grad_gate,
+                        void *grad_beta, void *grad_initial);
+
 /* h = a(g) u with g = x W[:, :hidden], u = x W[:, hidden:], for (rows, dim) x
  * and (dim, 2 hidden) weights W; activation a: 0 silu, 1 gelu (of the normal
  * distribution's function), 2 sigmoid.  Row strides are at least the rows'

@@ -215,7 +215,7 @@ EXPORTS = (
     "mmp_lu", "mmp_lu_solve", "mmp_cholesky", "mmp_qr", "mmp_qr_q", "mmp_eigh", "mmp_svd",
     "mmp_embedding", "mmp_embedding_grad", "mmp_recurrence", "mmp_recurrence_grad",
     "mmp_cross_entropy", "mmp_clip_norm",
-    "mmp_delta_rule",
+    "mmp_delta_rule", "mmp_delta_rule_grad",
     "mmp_gated_feed_forward", "mmp_gated_feed_forward_grad", "mmp_dropout",
     "mmp_rtc_compile", "mmp_rtc_build", "mmp_rtc_launch", "mmp_rtc_launch_threads",
     "mmp_wait_status",

@@ -140,6 +140,9 @@ _SIGNATURES = {
     "mmp_delta_rule": [_c_int] + [_c_i64] * 6 + [_c_vp, _c_i64, _c_i64, _c_i64] * 3
                       + [_c_vp, _c_int, _c_i64, _c_i64, _c_i64] * 2
                       + [_c_vp, ctypes.c_double, _c_vp, _c_vp],
+    "mmp_delta_rule_grad": [_c_int] + [_c_i64] * 6 + [_c_vp, _c_i64, _c_i64, _c_i64] * 4
+                           + [_c_vp, _c_int, _c_i64, _c_i64, _c_i64] * 2
+                           + [_c_vp, _c_vp, ctypes.c_double] + [_c_vp] * 6,
     "mmp_gated_feed_forward": [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
                                _c_vp],
     "mmp_gated_feed_forward_grad": [_c_int, _c_int, _c_i64, _c_i64, _c_i64]
@@ -592,6 +595,10 @@ class HipBackend:
     def delta_rule(self, *args) -> None:
         """The arguments of mmp_delta_rule in its order."""
         _check(self._lib.mmp_delta_rule(*args), "mmp_delta_rule")
+
+    def delta_rule_grad(self, *args) -> None:
+        """The arguments of mmp_delta_rule_grad in its order."""
+        _check(self._lib.mmp_delta_rule_grad(*args), "mmp_delta_rule_grad")
 
     def gated_feed_forward(self, dcode, activation, rows, dim, hidden, x, x_stride, weights,
                            w_stride, h) -> None:

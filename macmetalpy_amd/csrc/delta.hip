@@ -114,6 +114,23 @@ template <typename T, int ROWS, int W, int THREADS> struct Tile {
   }
 };
 
+// A chunk's gates, by one wave (lane: a step): logarithms summed up without the
+// fresh starts, and those counted.
+template <int C, typename T>
+__device__ __forceinline__ void chunk_gates(const Delta<T> &p, int b, long long t0, int h, int left, int lane,
+                                            double &sum, int &count, bool &anew) {
+  typedef typename Wide<T>::type A;
+  const A gate = lane < left ? p.gate.at(b, t0 + lane, h) : (A)0;
+  anew = starts_anew(gate);
+  count = __popcll(__ballot(anew) & ((2ull << lane) - 1));
+  sum = anew ? 0.0 : (double)gate;
+#pragma unroll
+  for (int d = 1; d < C; d *= 2) {
+    const double up = __shfl_up(sum, d);
+    if (lane >= d) sum += up;
+  }
+}
+
 // ------------------------------------------------------------- within chunks
 // Workgroup: a chunk of a head.
 template <typename T, int DK>
@@ -147,15 +164,10 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
     q.put(Qs, LD, tid);
   }
   if (wave == 0) {  // logarithms summed up, fresh starts counted
-    const A gate = lane < left ? p.gate.at(b, t0 + lane, h) : (A)0;
-    const bool anew = starts_anew(gate);
-    const int count = __popcll(__ballot(anew) & ((2ull << lane) - 1));
-    double sum = anew ? 0.0 : (double)gate;
-#pragma unroll
-    for (int d = 1; d < C; d *= 2) {
-      const double up = __shfl_up(sum, d);
-      if (lane >= d) sum += up;
-    }
+    double sum;
+    int count;
+    bool anew;
+    chunk_gates<C>(p, b, t0, h, left, lane, sum, count, anew);
     const double last = __shfl(sum, C - 1);
     const int count_last = __shfl(count, C - 1);
     if (lane < C) {
@@ -194,11 +206,14 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
       }
       if (query) {
         T *o = out + parts_of<T>() * C * C + i * C + 16 * jt;
+        Vec<T, 4> hi;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) hi.e[r] = (T)v[r];
+        mmpx::settle(hi);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const T hi = (T)v[r];
-          o[M::row(g, r)] = hi;
-          if constexpr (M::SPLIT) o[C * C + M::row(g, r)] = (T)(v[r] - (A)hi);
+          o[M::row(g, r)] = hi.e[r];
+          if constexpr (M::SPLIT) o[C * C + M::row(g, r)] = (T)(v[r] - (A)hi.e[r]);
         }
       } else {
 #pragma unroll
@@ -249,11 +264,10 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
     const int i = at / (C / V), j = at % (C / V) * V;
     Vec<T, V> hi, lo;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const A v = Ts[i * LA + j + e];
-      hi.e[e] = (T)v;
-      lo.e[e] = (T)(v - (A)hi.e[e]);
-    }
+    for (int e = 0; e < V; ++e) hi.e[e] = (T)Ts[i * LA + j + e];
+    mmpx::settle(hi);
+#pragma unroll
+    for (int e = 0; e < V; ++e) lo.e[e] = (T)(Ts[i * LA + j + e] - (A)hi.e[e]);
     mmpn::store_vec(out + i * C + j, hi);
     if constexpr (M::SPLIT) mmpn::store_vec(out + C * C + i * C + j, lo);
   }
@@ -602,6 +616,534 @@ __global__ __launch_bounds__(256) void k_delta_steps(Delta<T> p, Pass<T> e) {
   }
 }
 
+// ---------------------------------------------------------------- the gradient
+//
+// With dO and the gradient dS' of the state after a chunk,
+//
+//   dU = scale P^T dO + e K dS',  dR = T^T dU,  dX = -beta c dR
+//   dS = c_C dS' + (scale c Q)^T dO + K^T dX
+//
+// which k_delta_back goes through from the last chunk to the first, as the
+// forward pass does.  The rest has no order (k_delta_grads): with
+// E = -(strictly lower dR U^T) D, F = scale (lower dO U^T) D and Z = -c dR S^T,
+//
+//   dQ = scale c dO S^T + F K,   dV = beta dR,   dbeta = dR.V + K.Z + (E K K^T)
+//   dK = beta Z + e U dS'^T + F^T Q + (beta E + (beta E)^T) K
+//
+// and a chunk's logarithms G_i = log c_i get what their factors' products give:
+//   dG = Q.(scale c dO S^T) + beta K.Z - K.(e U dS'^T) + (row - column sums of F Q K^T + beta E K K^T)
+//   dG_C += sum of K.(e U dS'^T) + c_C S.dS',
+// of which gate_t gets the sum from t on.
+template <typename T> struct Back {
+  typedef typename Wide<T>::type A;
+  Seq<T> grad;  // of o
+  const A *grad_final;
+  A *grad_initial;
+  const T *keep_s, *keep_u;  // as Pass leaves them
+  T *keep_d, *keep_r;        // the gradient of the state after each chunk, and dR, as they
+  T *grad_q, *grad_k, *grad_v;
+  void *grad_gate, *grad_beta;  // of the types of gate and beta
+  int tiles;
+};
+
+// Workgroup: as k_delta_pass.
+template <typename T, int DK, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e) {
+  typedef typename Wide<T>::type A;
+  typedef Mma<T> M;
+  typedef typename M::Acc Acc;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, THREADS = 64 * NW;
+  constexpr int LD = DK + M::PAD, LC = C + M::PAD, LV = 16 * NW + M::PAD, DT = DK / 16;
+  __shared__ __attribute__((aligned(16))) T Ks[C * LD], Qs[C * LD], Th[C * LC], Ph[C * LC],
+      Tl[M::SPLIT ? C * LC : 1], Pl[M::SPLIT ? C * LC : 1], Os[C * LV];
+  __shared__ __attribute__((aligned(16))) A vecs[3 * C];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  const long long bh = blockIdx.x / e.tiles;
+  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
+  const int n0 = (int)(blockIdx.x - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;
+  const bool there = col < p.dv;
+
+  Acc S[DT];  // the state's gradient
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * t + M::row(g, r);
+      S[t][r] = e.grad_final && there && i < p.dk ? e.grad_final[(bh * p.dk + i) * p.dv + col] : (A)0;
+    }
+
+  Tile<T, C, DK, THREADS> k, q;
+  Tile<T, C, C, THREADS> th, tl, ph, pl;
+  Tile<T, C, 16 * NW, THREADS> o;
+  constexpr int NV = (3 * C + THREADS - 1) / THREADS;
+  A vec[NV];
+  auto arrays = [&](int n, auto f) {
+    const long long t0 = (long long)n * C;
+    const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
+    const T *w = p.within + (bh * p.chunks + n) * (2 * parts_of<T>() * C * C);
+    f(k, Ks, LD, p.k.at(b, t0, h / p.group), p.k.st, left, p.dk);
+    f(q, Qs, LD, p.q.at(b, t0, h / p.group), p.q.st, left, p.dk);
+    f(th, Th, LC, w, C, C, C);
+    f(ph, Ph, LC, w + parts_of<T>() * C * C, C, C, C);
+    if constexpr (M::SPLIT) {
+      f(tl, Tl, LC, w + C * C, C, C, C);
+      f(pl, Pl, LC, w + 3 * C * C, C, C, C);
+    }
+    f(o, Os, LV, e.grad.at(b, t0, h) + n0, e.grad.st, left, p.dv - n0);
+  };
+  auto fetch_vecs = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * THREADS + tid < 3 * C) vec[i] = p.vecs[(bh * p.chunks + n) * 3 * C + i * THREADS + tid];
+  };
+  auto put_vecs = [&]() {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * THREADS + tid < 3 * C) vecs[i * THREADS + tid] = vec[i];
+  };
+  auto fetch = [&](int n) {
+    arrays(n, [&](auto &tile, T *, int, const T *from, long long stride, int rows, int cols) {
+      tile.fetch(from, stride, rows, cols, tid);
+    });
+    fetch_vecs(n);
+  };
+  auto put = [&]() {
+    arrays(0, [&](auto &tile, T *to, int ld, const T *, long long, int, int) { tile.put(to, ld, tid); });
+    put_vecs();
+  };
+  auto load = [&](int n) {
+    arrays(n, [&](auto &tile, T *to, int ld, const T *from, long long stride, int rows, int cols) {
+      tile.fetch(from, stride, rows, cols, tid);
+      tile.put(to, ld, tid);
+    });
+    fetch_vecs(n);
+    put_vecs();
+  };
+
+  auto chunk = [&](int n) {
+    Two<T> s[DT / PT];
+#pragma unroll
+    for (int i = 0; i < DT / PT; ++i) s[i] = mmpx::operand<T>(S, i * PT);
+    if (there) {
+      T *to = e.keep_d + ((bh * p.chunks + n) * p.dv + col) * DK;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const A w[4] = {S[t][0], S[t][1], S[t][2], S[t][3]};
+        put4<T>(to + 16 * t, w, g);
+      }
+    }
+    typename M::Frag go[NT / PT];
+#pragma unroll
+    for (int j = 0; j < NT / PT; ++j) go[j] = M::cols(Os, LV, j * M::K, 16 * wave, lane);
+    // dU
+    Acc u[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      u[i] = Acc{};
+#pragma unroll
+      for (int d = 0; d < DT / PT; ++d) u[i] = mmpx::mul_two<T>(M::rows(Ks, LD, 16 * i, d * M::K, lane), s[d], u[i]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) u[i][r] *= vecs[C + 16 * i + M::row(g, r)];
+#pragma unroll
+      for (int j = i / PT; j < NT / PT; ++j) {
+        Two<T> w;
+        w.hi = M::cols(Ph, LC, j * M::K, 16 * i, lane);
+        if constexpr (M::SPLIT) w.lo = M::cols(Pl, LC, j * M::K, 16 * i, lane);
+        u[i] = mmpx::two_mul<T>(w, go[j], u[i]);
+      }
+    }
+    Two<T> f[NT / PT];
+#pragma unroll
+    for (int j = 0; j < NT / PT; ++j) f[j] = mmpx::operand<T>(u, j * PT);
+    // dR
+    Acc x[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      x[i] = Acc{};
+#pragma unroll
+      for (int j = i / PT; j < NT / PT; ++j) {
+        Two<T> w;
+        w.hi = M::cols(Th, LC, j * M::K, 16 * i, lane);
+        if constexpr (M::SPLIT) w.lo = M::cols(Tl, LC, j * M::K, 16 * i, lane);
+        x[i] = mmpx::mul_twos<T>(w, f[j], x[i]);
+      }
+    }
+    if (there) {
+      T *to = e.keep_r + ((bh * p.chunks + n) * p.dv + col) * C;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const A w[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
+        put4<T>(to + 16 * i, w, g);
+      }
+    }
+    // dX and scale c dO
+    Two<T> fo[NT / PT];
+#pragma unroll
+    for (int j = 0; j < NT / PT; ++j) {
+      A wx[M::E], wo[M::E];
+#pragma unroll
+      for (int c = 0; c < M::E; ++c) {
+        const int at = 16 * (j * PT + (c >> 2)) + M::row(g, c & 3);
+        wx[c] = -vecs[2 * C + at] * vecs[at] * x[j * PT + (c >> 2)][c & 3];
+        wo[c] = p.scale * vecs[at] * (A)go[j][c];
+      }
+      f[j] = mmpx::two_of<T>(wx);
+      fo[j] = mmpx::two_of<T>(wo);
+    }
+    const A decay = vecs[C - 1];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][r] *= decay;
+#pragma unroll
+      for (int j = 0; j < NT / PT; ++j) {
+        S[t] = mmpx::mul_two<T>(M::cols(Ks, LD, j * M::K, 16 * t, lane), f[j], S[t]);
+        S[t] = mmpx::mul_two<T>(M::cols(Qs, LD, j * M::K, 16 * t, lane), fo[j], S[t]);
+      }
+    }
+  };
+
+  constexpr bool AHEAD = DK <= 128;
+  if constexpr (AHEAD)
+    if (p.chunks) fetch(p.chunks - 1);
+  for (int n = p.chunks - 1; n >= 0; --n) {
+    if constexpr (AHEAD) {
+      put();
+      __syncthreads();
+      if (n) fetch(n - 1);
+    } else {
+      load(n);
+      __syncthreads();
+    }
+    if (n0 + 16 * wave < p.dv) chunk(n);
+    __syncthreads();
+  }
+  if (there)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * t + M::row(g, r);
+        if (i < p.dk) e.grad_initial[(bh * p.dk + i) * p.dv + col] = S[t][r];
+      }
+}
+
+// Workgroup: a chunk of a key head, for the heads that share it one after another.
+template <typename T, int DK>
+__global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
+  typedef typename Wide<T>::type A;
+  typedef Mma<T> M;
+  typedef typename M::Acc Acc;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, V = vec_of<T>();
+  constexpr int VB = 32, KB = 64;  // channels of values and of keys at a time
+  constexpr int LD = DK + M::PAD, LC = C + M::PAD, LB = VB + M::PAD, LK = KB + M::PAD;
+  constexpr int TASKS = (2 * NT + 3) / 4;
+  static_assert(C * (VB / V) == 256, "a vector of the chunk's values for each thread");
+  __shared__ __attribute__((aligned(16))) T Ks[C * LD], Qs[C * LD], Fs[C * LC], Es[C * LC], Os[C * LB],
+      Us[VB * LC], Rs[VB * LC], Ss[VB * LK], Ds[VB * LK];
+  __shared__ double G[C];
+  __shared__ int R[C];
+  __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][4][16], rv[C], ek[C], sd[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  const int shared = p.group ? p.heads / p.group : e.tiles;  // key heads
+  const long long id = blockIdx.x, bk = id / p.chunks;
+  const int n = (int)(id - bk * p.chunks), b = (int)(bk / shared), kh = (int)(bk - (long long)b * shared);
+  const long long t0 = (long long)n * C;
+  const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
+
+  {
+    Tile<T, C, DK, 256> k, q;
+    k.fetch(p.k.at(b, t0, kh), p.k.st, left, p.dk, tid);
+    q.fetch(p.q.at(b, t0, kh), p.q.st, left, p.dk, tid);
+    k.put(Ks, LD, tid);
+    q.put(Qs, LD, tid);
+  }
+  // dQ and dK, transposed: a wave has rows 16 rt and NT tiles of columns from ct on of each 64
+  const int rt = wave % NT, ct = wave / NT * NT;
+  Acc dq[DK / KB][NT], dk[DK / KB][NT];
+#pragma unroll
+  for (int kb = 0; kb < DK / KB; ++kb)
+#pragma unroll
+    for (int c = 0; c < NT; ++c) dq[kb][c] = dk[kb][c] = Acc{};
+
+  for (int head = 0; head < p.group; ++head) {
+    const int h = kh * p.group + head;
+    const long long at = ((long long)b * p.heads + h) * p.chunks + n;
+    __syncthreads();  // the head before is done with LDS
+    double sum = 0;
+    int count = 0;
+    bool anew = false;
+    if (wave == 0) {
+      chunk_gates<C>(p, b, t0, h, left, lane, sum, count, anew);
+      if (lane < C) {
+        G[lane] = sum;
+        R[lane] = count;
+        cs[lane] = p.vecs[at * 3 * C + lane];
+        es[lane] = p.vecs[at * 3 * C + C + lane];
+        bet[lane] = p.vecs[at * 3 * C + 2 * C + lane];
+      }
+    }
+    // dO U^T and dR U^T, transposed; dV and dR.V on the way
+    Acc w[TASKS][NT];
+#pragma unroll
+    for (int k = 0; k < TASKS; ++k)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w[k][j] = Acc{};
+    A with_v = 0;
+    Tile<T, C, VB, 256> o;
+    Tile<T, VB, C, 256> u, r;
+    const int vi = tid / (VB / V), vn = tid % (VB / V) * V;  // this thread's step and channels
+    for (int v0 = 0; v0 < p.dv; v0 += VB) {
+      o.fetch(e.grad.at(b, t0, h) + v0, e.grad.st, left, p.dv - v0, tid);
+      u.fetch(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
+      r.fetch(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
+      if (v0) __syncthreads();
+      o.put(Os, LB, tid);
+      u.put(Us, LC, tid);
+      r.put(Rs, LC, tid);
+      __syncthreads();
+      if (vi < left) {
+        const A beta = bet[vi];
+        const T *v = p.v.at(b, t0 + vi, h) + v0 + vn;
+        T *to = e.grad_v + (((long long)b * p.steps + t0 + vi) * p.heads + h) * p.dv + v0 + vn;
+        const int cols_left = p.dv - v0 - vn;
+        Vec<T, V> x{}, y;
+        if (cols_left >= V) {
+          x = mmpn::load_vec<T, V>(v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i < cols_left) x.e[i] = v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const A d = (A)Rs[(vn + i) * LC + vi];
+          with_v = mmpn::fma_of(d, (A)x.e[i], with_v);
+          y.e[i] = (T)(beta * d);
+        }
+        if (cols_left >= V) {
+          mmpn::store_vec(to, y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i < cols_left) to[i] = y.e[i];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < TASKS; ++k) {
+        const int task = wave + 4 * k;
+        if (task >= 2 * NT) continue;
+        const bool query = task >= NT;
+        const int row = query ? 2 * NT - 1 - task : task;
+#pragma unroll
+        for (int d = 0; d < VB; d += M::K) {
+          const typename M::Frag x = query ? M::rows(Os, LB, 16 * row, d, lane) : M::cols(Rs, LC, d, 16 * row, lane);
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            if (j <= row) w[k][j] = M::mul(M::cols(Us, LC, d, 16 * j, lane), x, w[k][j]);
+        }
+      }
+    }
+    if (p.dv == 0) __syncthreads();
+#pragma unroll
+    for (int d = 1; d < VB / V; d *= 2) with_v += __shfl_xor(with_v, d);
+    if (tid % (VB / V) == 0) rv[vi] = with_v;
+    // F and beta E, and their products with Q K^T and K K^T summed up by rows and columns
+#pragma unroll
+    for (int k = 0; k < TASKS; ++k) {
+      const int task = wave + 4 * k;
+      if (task >= 2 * NT) continue;
+      const bool query = task >= NT;
+      const int row = query ? 2 * NT - 1 - task : task, i = 16 * row + fr;
+      const T *X = query ? Qs : Ks;
+      T *to = (query ? Fs : Es) + i * LC;
+      const double Gi = G[i];
+      const int Ri = R[i];
+      const A by = query ? p.scale : bet[i];
+      A sum_row = 0, sum_e = 0;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        Acc x{};
+        if (j <= row)
+#pragma unroll
+          for (int d = 0; d < DK; d += M::K) x = M::mul(M::rows(Ks, LD, 16 * j, d, lane), M::rows(X, LD, 16 * row, d, lane), x);
+        A sum_col[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int jj = 16 * j + M::row(g, c);
+          const bool in = (query ? jj <= i : jj < i) && R[jj] == Ri;
+          const A f = in ? (query ? w[k][j][c] : -w[k][j][c]) * exp_any((A)(Gi - G[jj])) : (A)0;
+          to[jj] = (T)(f * by);
+          const A m = in ? f * x[c] : (A)0;
+          sum_e += m;
+          sum_row = mmpn::fma_of(m, by, sum_row);
+          sum_col[c] = m * by;
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum_col[c] += __shfl_xor(sum_col[c], d);
+        if (fr == 0)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) cols[query][row][16 * j + M::row(g, c)] = sum_col[c];
+      }
+      sum_row += __shfl_xor(sum_row, 16);
+      sum_row += __shfl_xor(sum_row, 32);
+      sum_e += __shfl_xor(sum_e, 16);
+      sum_e += __shfl_xor(sum_e, 32);
+      if (g == 0) {
+        rows[query][i] = sum_row;
+        if (!query) ek[i] = sum_e;
+      }
+    }
+
+    // with the states: a 64 wide block of key channels at a time
+    const int i = 16 * rt + fr;
+    A q_s = 0, k_z = 0, k_d = 0, s_d = 0;
+    Tile<T, VB, KB, 256> st, dt;
+#pragma unroll
+    for (int kb = 0; kb < DK / KB; ++kb) {
+      Acc a[NT], z[NT], y[NT];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) a[c] = z[c] = y[c] = Acc{};
+      for (int v0 = 0; v0 < p.dv; v0 += VB) {
+        o.fetch(e.grad.at(b, t0, h) + v0, e.grad.st, left, p.dv - v0, tid);
+        u.fetch(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
+        r.fetch(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
+        st.fetch(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, tid);
+        dt.fetch(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, tid);
+        __syncthreads();
+        o.put(Os, LB, tid);
+        u.put(Us, LC, tid);
+        r.put(Rs, LC, tid);
+        st.put(Ss, LK, tid);
+        dt.put(Ds, LK, tid);
+#pragma unroll
+        for (int c = 0; c < st.N; ++c) {
+          const Vec<T, V> x = mmpn::elements_of<T, V>(st.w[c]), x2 = mmpn::elements_of<T, V>(dt.w[c]);
+#pragma unroll
+          for (int l = 0; l < V; ++l) s_d = mmpn::fma_of((A)x.e[l], (A)x2.e[l], s_d);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < VB; d += M::K) {
+          const typename M::Frag fo = M::rows(Os, LB, 16 * rt, d, lane), fr_ = M::cols(Rs, LC, d, 16 * rt, lane),
+                                 fu = M::cols(Us, LC, d, 16 * rt, lane);
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            const typename M::Frag fs = M::cols(Ss, LK, d, 16 * (ct + c), lane), fd = M::cols(Ds, LK, d, 16 * (ct + c), lane);
+            a[c] = M::mul(fs, fo, a[c]);
+            z[c] = M::mul(fs, fr_, z[c]);
+            y[c] = M::mul(fd, fu, y[c]);
+          }
+        }
+      }
+      if (p.dv == 0) __syncthreads();  // F and E are there
+      const A sc = p.scale * cs[i], cz = -cs[i], ce = es[i], beta = bet[i];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const int d0 = kb * KB + 16 * (ct + c);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+          const int d = d0 + M::row(g, l);
+          const A qv = (A)Qs[i * LD + d], kv = (A)Ks[i * LD + d];
+          const A av = sc * a[c][l], zv = cz * z[c][l], yv = ce * y[c][l];
+          q_s = mmpn::fma_of(qv, av, q_s);
+          k_z = mmpn::fma_of(kv, zv, k_z);
+          k_d = mmpn::fma_of(kv, yv, k_d);
+          dq[kb][c][l] += av;
+          dk[kb][c][l] += beta * zv + yv;
+        }
+#pragma unroll
+        for (int j = 0; j < NT / PT; ++j) {
+          const typename M::Frag kc = M::cols(Ks, LD, j * M::K, d0, lane), qc = M::cols(Qs, LD, j * M::K, d0, lane);
+          if (j <= rt / PT) {
+            dq[kb][c] = M::mul(kc, M::rows(Fs, LC, 16 * rt, j * M::K, lane), dq[kb][c]);
+            dk[kb][c] = M::mul(kc, M::rows(Es, LC, 16 * rt, j * M::K, lane), dk[kb][c]);
+          }
+          if (j >= rt / PT) {
+            dk[kb][c] = M::mul(kc, M::cols(Es, LC, j * M::K, 16 * rt, lane), dk[kb][c]);
+            dk[kb][c] = M::mul(qc, M::cols(Fs, LC, j * M::K, 16 * rt, lane), dk[kb][c]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) {
+      q_s += __shfl_xor(q_s, d);
+      k_z += __shfl_xor(k_z, d);
+      k_d += __shfl_xor(k_d, d);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) s_d += __shfl_xor(s_d, d);
+    if (g == 0) {
+      dots[0][wave][fr] = q_s;
+      dots[1][wave][fr] = k_z;
+      dots[2][wave][fr] = k_d;
+    }
+    if (lane == 0) sd[wave] = s_d;
+    __syncthreads();
+    if (wave == 0) {
+      double dG = 0, w_i = 0;
+      A dbeta = 0;
+      const int l = lane < C ? lane : 0;
+      double qs_i = 0, kz_i = 0;
+#pragma unroll
+      for (int part = 0; part < 4 / NT; ++part) {  // the waves that share rows
+        qs_i += dots[0][part * NT + l / 16][l % 16];
+        kz_i += dots[1][part * NT + l / 16][l % 16];
+        w_i += dots[2][part * NT + l / 16][l % 16];
+      }
+      if (lane < C) {
+        dG = qs_i + (double)bet[l] * kz_i - w_i + rows[0][l] + rows[1][l];
+        for (int row = l / 16; row < NT; ++row) dG -= (double)cols[0][row][l] + (double)cols[1][row][l];
+        dbeta = (A)(rv[l] + kz_i + ek[l]);
+      } else {
+        w_i = 0;
+      }
+      double all = w_i;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+      if (lane == C - 1) dG += all + (double)cs[C - 1] * ((double)sd[0] + sd[1] + sd[2] + sd[3]);
+#pragma unroll
+      for (int d = 1; d < C; d *= 2) {  // the sum from this step on
+        const double down = __shfl_down(dG, d);
+        if (lane + d < C) dG += down;
+      }
+      if (lane < left) {
+        const long long to = ((long long)b * p.steps + t0 + lane) * p.heads + h;
+        const A dg = anew ? (A)0 : (A)dG;
+        if (p.gate.wide) ((A *)e.grad_gate)[to] = dg;
+        else ((T *)e.grad_gate)[to] = (T)dg;
+        if (p.beta.wide) ((A *)e.grad_beta)[to] = dbeta;
+        else ((T *)e.grad_beta)[to] = (T)dbeta;
+      }
+    }
+  }
+  const int i = 16 * rt + fr;
+  if (i < left)
+#pragma unroll
+    for (int kb = 0; kb < DK / KB; ++kb)
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const int d0 = kb * KB + 16 * (ct + c);
+        const long long to = (((long long)b * p.steps + t0 + i) * shared + kh) * p.dk + d0;
+        if (d0 + 16 <= p.dk) {
+          const A x[4] = {dq[kb][c][0], dq[kb][c][1], dq[kb][c][2], dq[kb][c][3]};
+          const A y[4] = {dk[kb][c][0], dk[kb][c][1], dk[kb][c][2], dk[kb][c][3]};
+          put4<T>(e.grad_q + to, x, g);
+          put4<T>(e.grad_k + to, y, g);
+        } else {
+#pragma unroll
+          for (int l = 0; l < 4; ++l)
+            if (d0 + M::row(g, l) < p.dk) {
+              e.grad_q[to + M::row(g, l)] = (T)dq[kb][c][l];
+              e.grad_k[to + M::row(g, l)] = (T)dk[kb][c][l];
+            }
+        }
+      }
+}
+
 // ------------------------------------------------------------------ host side
 constexpr const char *kWhat = "mmp_delta_rule";
 
@@ -624,6 +1166,7 @@ template <typename T> struct Chunks {
     if (int st = vecs.get((size_t)all * 3 * C * sizeof(typename Wide<T>::type), what)) return st;
     p.within = (T *)within.p;
     p.vecs = (typename Wide<T>::type *)vecs.p;
+    if (!all) return MMP_OK;
     return with_width(p.dk, [&](auto dk) {
       hipLaunchKernelGGL((k_delta_within<T, dk.value>), dim3((unsigned)all), dim3(256), 0, mmpi::stream(), p);
       return mmpi::check_launch(what);
@@ -655,6 +1198,48 @@ template <typename T> int forward(Delta<T> p, Pass<T> e) {
   Chunks<T> chunks;
   if (int st = chunks.get(p, kWhat)) return st;
   return pass<T, true, false>(p, e, kWhat);
+}
+
+constexpr const char *kGradWhat = "mmp_delta_rule_grad";
+
+template <typename T> int backward(Delta<T> p, Back<T> e, int key_heads, const typename Wide<T>::type *initial) {
+  constexpr int C = chunk_of<T>(), NW = 4;
+  const char *what = kGradWhat;
+  Chunks<T> chunks;
+  if (p.heads)
+    if (int st = chunks.get(p, what)) return st;
+  Temp s, d, u, r;
+  const int DK = p.dk <= 64 ? 64 : p.dk <= 128 ? 128 : 256;
+  const size_t columns = (size_t)p.batch * p.heads * p.chunks * p.dv * sizeof(T);
+  if (columns) {
+    if (int st = s.get(columns * DK, what)) return st;
+    if (int st = d.get(columns * DK, what)) return st;
+    if (int st = u.get(columns * C, what)) return st;
+    if (int st = r.get(columns * C, what)) return st;
+    if (int st = pass<T, false, true>(p, Pass<T>{initial, nullptr, nullptr, (T *)s.p, (T *)u.p, 0}, what)) return st;
+  }
+  e.keep_s = (const T *)s.p;
+  e.keep_u = (const T *)u.p;
+  e.keep_d = (T *)d.p;
+  e.keep_r = (T *)r.p;
+  e.tiles = (p.dv + 16 * NW - 1) / (16 * NW);
+  const int64_t blocks = (int64_t)p.batch * p.heads * e.tiles;
+  if (!mmpi::grid_fits(blocks, 64 * NW)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
+  if (blocks)
+    if (int st = with_width(p.dk, [&](auto dk) {
+          hipLaunchKernelGGL((k_delta_back<T, dk.value, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+          return mmpi::check_launch(what);
+        }))
+      return st;
+  if (!p.steps) return MMP_OK;
+  p.chunks = (int)((p.steps + C - 1) / C);
+  e.tiles = key_heads;
+  const int64_t all = (int64_t)p.batch * key_heads * p.chunks;
+  if (!mmpi::grid_fits(all, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many steps", what);
+  return with_width(p.dk, [&](auto dk) {
+    hipLaunchKernelGGL((k_delta_grads<T, dk.value>), dim3((unsigned)all), dim3(256), 0, mmpi::stream(), p, e);
+    return mmpi::check_launch(what);
+  });
 }
 
 int check(const char *what, int64_t batch, int64_t steps, int64_t key_heads, int64_t heads, int64_t dk, int64_t dv) {
@@ -691,5 +1276,34 @@ extern "C" int mmp_delta_rule(int dtype, int64_t batch, int64_t steps, int64_t k
                      (int)batch, (int)heads, (int)(heads / key_heads), (int)dk, (int)dv, (long long)steps, 0, (A)scale,
                      nullptr, nullptr};
     return forward<T>(p, Pass<T>{(const A *)initial, (A *)final_state, (T *)o, nullptr, nullptr, 0});
+  })
+}
+
+extern "C" int mmp_delta_rule_grad(int dtype, int64_t batch, int64_t steps, int64_t key_heads,
+                                   int64_t heads, int64_t dk, int64_t dv, const void *grad,
+                                   int64_t o_sb, int64_t o_st, int64_t o_sh, const void *q,
+                                   int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k,
+                                   int64_t k_sb, int64_t k_st, int64_t k_sh, const void *v,
+                                   int64_t v_sb, int64_t v_st, int64_t v_sh, const void *gate,
+                                   int gate_wide, int64_t g_sb, int64_t g_st, int64_t g_sh,
+                                   const void *beta, int beta_wide, int64_t b_sb, int64_t b_st,
+                                   int64_t b_sh, const void *initial, const void *grad_final,
+                                   double scale, void *grad_q, void *grad_k, void *grad_v,
+                                   void *grad_gate, void *grad_beta, void *grad_initial) {
+  if (int st = check(kGradWhat, batch, steps, key_heads, heads, dk, dv)) return st;
+  if (batch == 0 || key_heads == 0) return MMP_OK;
+  if (steps && heads && (!gate || !beta || !grad_gate || !grad_beta || (dv && (!grad || !v || !grad_v))))
+    return mmpi::fail(MMP_E_ARG, "%s: null pointer", kGradWhat);
+  if ((steps && dk && (!q || !k || !grad_q || !grad_k)) || (heads && dk && dv && !grad_initial))
+    return mmpi::fail(MMP_E_ARG, "%s: null pointer", kGradWhat);
+  MMP_DISPATCH_FLOAT(dtype, "mmp_delta_rule_grad", {
+    typedef typename Wide<T>::type A;
+    const Delta<T> p{{(const T *)q, q_sb, q_st, q_sh}, {(const T *)k, k_sb, k_st, k_sh}, {(const T *)v, v_sb, v_st, v_sh},
+                     {gate, g_sb, g_st, g_sh, gate_wide}, {beta, b_sb, b_st, b_sh, beta_wide},
+                     (int)batch, (int)heads, (int)(heads / key_heads), (int)dk, (int)dv, (long long)steps, 0, (A)scale,
+                     nullptr, nullptr};
+    const Back<T> e{{(const T *)grad, o_sb, o_st, o_sh}, (const A *)grad_final, (A *)grad_initial, nullptr, nullptr, nullptr, nullptr,
+                    (T *)grad_q, (T *)grad_k, (T *)grad_v, grad_gate, grad_beta, 0};
+    return backward<T>(p, e, (int)key_heads, (const A *)initial);
   })
 }

@@ -98,17 +98,32 @@ template <> struct Mma<double> {
 // A value in 32 bits as two float16 operands, the value rounded and what that
 // left: 22 bits, and a product of two such values but for the product of their
 // small parts.  Other types hold their values as they are.
+//
+// The rounded value is made opaque before its rest is worked out: the compiler
+// may round a product to float16 in one step where it is stored and in two, by way
+// of 32 bits, where the rest needs it, and about one in 2^13 values then differs by a
+// unit that the rest does not hold.
 template <typename T> struct Two {
   typename Mma<T>::Frag hi, lo;
 };
+template <typename W> __device__ __forceinline__ void settle(W &w) {
+  static_assert(sizeof(W) % 4 == 0, "");
+  unsigned u[sizeof(W) / 4];
+  __builtin_memcpy(u, &w, sizeof(W));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(W) / 4; ++i) asm volatile("" : "+v"(u[i]));
+  __builtin_memcpy(&w, u, sizeof(W));
+}
 template <typename T> __device__ __forceinline__ Two<T> two_of(const typename Mma<T>::A (&v)[Mma<T>::E]) {
   Two<T> f;
 #pragma unroll
-  for (int e = 0; e < Mma<T>::E; ++e) {
-    f.hi[e] = (T)v[e];
-    if constexpr (Mma<T>::SPLIT) f.lo[e] = (T)(v[e] - (float)f.hi[e]);
+  for (int e = 0; e < Mma<T>::E; ++e) f.hi[e] = (T)v[e];
+  f.lo = f.hi;
+  if constexpr (Mma<T>::SPLIT) {
+    settle(f.hi);
+#pragma unroll
+    for (int e = 0; e < Mma<T>::E; ++e) f.lo[e] = (T)(v[e] - (float)f.hi[e]);
   }
-  if constexpr (!Mma<T>::SPLIT) f.lo = f.hi;
   return f;
 }
 // Tiles [first, first + K / 16) of accumulators as an operand, each value times `by`.

@@ -33,7 +33,7 @@ from .manipulation import broadcast_to
 from .ndarray import ndarray, _c_contiguous_strides, _prod
 
 __all__ = ["embedding", "embedding_grad", "gated_recurrence", "gated_recurrence_grad",
-           "gated_delta_rule",
+           "gated_delta_rule", "gated_delta_rule_grad",
            "gated_feed_forward", "gated_feed_forward_grad", "dropout",
            "cross_entropy", "cross_entropy_grad", "global_norm", "clip_by_global_norm"]
 
@@ -349,6 +349,29 @@ def gated_delta_rule(q, k, v, gate, beta, initial=None, *, scale=None):
         HipBackend().delta_rule(_CODE[dtype], batch, steps, key_heads, heads, dk, dv, *at,
                                 _ptr(initial), scale, o._ptr, final._ptr)
     return o, final
+
+
+def gated_delta_rule_grad(grad, q, k, v, gate, beta, initial=None, grad_final=None, *, scale=None):
+    """``(grad_q, grad_k, grad_v, grad_gate, grad_beta, grad_initial)`` of
+    :func:`gated_delta_rule`, from ``grad`` (of ``o``), its inputs and, where the
+    final state was used too, ``grad_final``.  The states are worked out again.
+    The first three have the sequences' type, the gates' gradients the gates'
+    (float32 or float64 where a gate had a type that is neither the sequences' nor
+    the states'), ``grad_initial`` the states'.  The gradient of a gate of ``-inf``
+    is 0.  float16 holds the gradients of a chunk's states in its range: scale the
+    loss so that they are well between 1e-4 and 65504."""
+    arrays, initial, scale, (batch, steps, key_heads, heads, dk, dv), dtype = _delta(
+        q, k, v, gate, beta, initial, scale, grad)
+    wide = _WIDE[dtype]
+    state_shape = (batch, heads, dk, dv)
+    grad_final = _state(grad_final, state_shape, wide, "grad_final")
+    kept, at = _delta_inputs(arrays, ("grad", "q", "k", "v", "gate", "beta"), wide)
+    grads = [_empty(a._shape, a._dtype) for a in kept[1:]] + [_empty(state_shape, wide)]
+    if any(g.size for g in grads):
+        HipBackend().delta_rule_grad(_CODE[dtype], batch, steps, key_heads, heads, dk, dv, *at,
+                                     _ptr(initial), _ptr(grad_final), scale,
+                                     *(g._ptr for g in grads))
+    return tuple(grads)
 
 
 # ---------------------------------------------------------- feed-forward

@@ -88,3 +88,68 @@ def test_delta_rule(dt, size):
         # an output of float16 has P's and T's own roundings too
         close(got_o, o, dt, U[dt], parts + (8 * U[dt] if dt == np.float16 else 0))
         close(got_s, S, wide, U[wide], parts)
+
+
+def rule_grad(grad, q, k, v, gate, beta, initial, grad_final, scale):
+    """The gradients by the chain rule of one step, from the last to the first, in 64 bits."""
+    batch, steps, heads, dv = v.shape
+    shared = k.shape[2]
+    group = heads // shared
+    grad, q, k, v, gate, beta = (x.astype(np.float64) for x in (grad, q, k, v, gate, beta))
+    q, k = np.repeat(q, group, 2), np.repeat(k, group, 2)
+    S = np.zeros((batch, heads, k.shape[3], dv)) if initial is None else initial.astype(np.float64)
+    seen = []
+    for t in range(steps):
+        a = np.exp(gate[:, t])[..., None, None]
+        faded = np.where(a == 0, 0.0, a * S)
+        miss = v[:, t] - (faded * k[:, t, :, :, None]).sum(2)
+        u = beta[:, t, :, None] * miss
+        S = faded + k[:, t, :, :, None] * u[:, :, None]
+        seen.append((faded, miss, u, S))
+    D = np.zeros_like(S) if grad_final is None else grad_final.astype(np.float64)
+    gq, gk, gv, gg, gb = (np.zeros(x.shape) for x in (q, k, v, gate, beta))
+    for t in reversed(range(steps)):
+        faded, miss, u, S = seen.pop()
+        go = scale * grad[:, t]
+        gq[:, t] = (S * go[:, :, None]).sum(3)
+        D = D + q[:, t, :, :, None] * go[:, :, None]
+        du = (D * k[:, t, :, :, None]).sum(2)
+        dm = beta[:, t, :, None] * du
+        gb[:, t] = (du * miss).sum(2)
+        gv[:, t] = dm
+        gk[:, t] = (D * u[:, :, None]).sum(3) - (faded * dm[:, :, None]).sum(3)
+        D = D - k[:, t, :, :, None] * dm[:, :, None]
+        gg[:, t] = (D * faded).sum((2, 3))
+        a = np.exp(gate[:, t])[..., None, None]
+        D = np.where(a == 0, 0.0, a * D)
+    join = lambda x: x.reshape(batch, steps, shared, group, -1).sum(3)  # noqa: E731
+    return join(gq), join(gk), gv, gg, gb, D
+
+
+def grads_close(got, want, dt, steps, dk, dv):
+    """As the outputs; every gradient of float16 has operands rounded to it (states, their
+    gradients, U and dR, P's and T's products): U each, of addends that are random in sign, 8 times
+    the root mean square for the largest element.  A gate's gradient sums those of dk dv products
+    and all later steps of its chunk and so may be larger than its parts' difference: their size
+    is taken from the sums' largest."""
+    wide = np.float64 if dt == np.float64 else np.float32
+    parts = parts_of(dt, steps, max(dk, dv)) * 2
+    loose = parts + (8 * 3 * U[dt] if dt == np.float16 else 0)
+    for i, (a, b) in enumerate(zip(got[:5], want[:5])):
+        close(a, b, dt, U[dt], loose * (8 if i == 3 else 2))
+    close(got[5], want[5], wide, U[wide], parts)
+
+
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_delta_rule_grad(dt, size):
+    g = np.random.default_rng(sum(size) + 1)
+    wide = np.float64 if dt == np.float64 else np.float32
+    for start, anew in ((False, 0.0), (True, 0.05)):
+        x = make(g, *size, dt, anew)
+        batch, steps, key_heads, heads, dk, dv = size
+        states = [g.standard_normal((batch, heads, dk, dv)).astype(wide) if start else None for _ in range(2)]
+        grad = g.standard_normal(x[2].shape).astype(dt)
+        want = rule_grad(grad, *x, *states, dk ** -0.5)
+        got = nn.gated_delta_rule_grad(cp.array(grad), *map(cp.array, x), *(None if s is None else cp.array(s) for s in states))
+        grads_close(got, want, dt, steps, dk, dv)
