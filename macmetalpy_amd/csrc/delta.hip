@@ -29,6 +29,8 @@
 // The state is 32 bits wide (64 for float64), and so is what goes into it: where
 // a float16 product needs a value that is no input, it takes it as two float16
 // numbers (mmp_mma.h).
+#include <type_traits>
+
 #include "mmp_mma.h"
 
 namespace {
@@ -36,6 +38,7 @@ namespace {
 using mmpn::Temp;
 using mmpn::Vec;
 using mmpn::Wide;
+using mmpx::Lay;
 using mmpx::Mma;
 using mmpx::Two;
 
@@ -74,6 +77,8 @@ template <typename T> struct Delta {
   T *within;  // of each chunk of each head: T, P (float16: T, its rest, P, its rest)
   A *vecs;    // c, e and beta of each step of a chunk
 };
+// Of a chunk's c, e and beta in LDS, with room for whole copies.
+template <typename T> constexpr int kVecs = 1024 / sizeof(typename Wide<T>::type);
 template <typename T> constexpr int parts_of() { return Mma<T>::SPLIT ? 2 : 1; }
 
 // exp(g) is 0 in the wide type: such a step is counted as one of -inf.
@@ -84,32 +89,41 @@ __device__ __forceinline__ double exp_any(double x) { return exp(x); }
 // W columns of ROWS rows of an array in registers, and on their way to LDS.
 template <typename T, int ROWS, int W, int THREADS> struct Tile {
   static constexpr int V = vec_of<T>(), PER = W / V, N = (ROWS * PER + THREADS - 1) / THREADS;
+  static constexpr int STEP = THREADS / PER;  // rows from one of a thread's vectors to its next
+  static constexpr bool WHOLE = ROWS % STEP == 0;
+  static_assert(THREADS % PER == 0, "");
   typedef typename Vec<T, V>::Words Words;
   Words w[N];
   // rows from `rows` on and columns from `cols` on are zeros
   __device__ __forceinline__ void fetch(const T *p, long long stride, int rows, int cols, int tid) {
+    const int r0 = tid / PER, c = tid % PER * V;
+    const T *at = p + r0 * stride + c;
+    if (WHOLE && rows >= ROWS && cols >= W) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int id = i * THREADS + tid, r = id / PER, c = id % PER * V;
-      Vec<T, V> x{};
-      if (r < rows && r < ROWS) {
-        const T *at = p + r * stride + c;
-        if (c + V <= cols) {
-          x = mmpn::load_vec<T, V>(at);
-        } else {
+      for (int i = 0; i < N; ++i) w[i] = mmpn::words_of(mmpn::load_vec<T, V>(at + i * STEP * stride));
+    } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (c + e < cols) x.e[e] = at[e];
+      for (int i = 0; i < N; ++i) {
+        Vec<T, V> x{};
+        if (i * STEP + r0 < rows && i * STEP + r0 < ROWS) {
+          const T *from = at + i * STEP * stride;
+          if (c + V <= cols) {
+            x = mmpn::load_vec<T, V>(from);
+          } else if (c < cols) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (c + e < cols) x.e[e] = from[e];
+          }
         }
+        w[i] = mmpn::words_of(x);
       }
-      w[i] = mmpn::words_of(x);
     }
   }
-  __device__ __forceinline__ void put(T *lds, int ld, int tid) const {
+  __device__ __forceinline__ void put(T *lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int id = i * THREADS + tid, r = id / PER, c = id % PER * V;
-      if (r < ROWS) *reinterpret_cast<Words *>(lds + r * ld + c) = w[i];
+      const int r = i * STEP + tid / PER;
+      if (WHOLE || r < ROWS) *reinterpret_cast<Words *>(lds + Lay<T, W>::at(r, tid % PER * V)) = w[i];
     }
   }
 };
@@ -131,6 +145,13 @@ __device__ __forceinline__ void chunk_gates(const Delta<T> &p, int b, long long 
   }
 }
 
+// A chunk's c, e and beta to LDS, by one wave: 1 KiB, of which what is beyond them
+// is the next chunk's or, after the last, room that is there.
+template <typename T>
+__device__ __forceinline__ void copy_vecs(const Delta<T> &p, long long chunk, typename Wide<T>::type *to, int lane) {
+  mmpx::copy16((const char *)(p.vecs + chunk * 3 * chunk_of<T>()) + 16 * lane, to);
+}
+
 // ------------------------------------------------------------- within chunks
 // Workgroup: a chunk of a head.
 template <typename T, int DK>
@@ -140,12 +161,12 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
   typedef Mma<A> MA;
   typedef typename M::Acc Acc;
   typedef typename MA::Acc AccA;
-  constexpr int C = chunk_of<T>(), NT = C / 16, LD = DK + M::PAD, LA = C + MA::PAD;
-  constexpr int KEYS = 2 * C * LD * sizeof(T), INV = C * LA * sizeof(A);
+  constexpr int C = chunk_of<T>(), NT = C / 16;
+  constexpr int KEYS = 2 * C * DK * sizeof(T), INV = C * C * sizeof(A);
   __shared__ __attribute__((aligned(16))) char mem[KEYS > INV ? KEYS : INV];
-  T *Ks = (T *)mem, *Qs = Ks + C * LD;
+  T *Ks = (T *)mem, *Qs = Ks + C * DK;
   A *Ts = (A *)mem;  // when the keys are done with
-  __shared__ __attribute__((aligned(16))) A As[C * LA], Td[C * (16 + MA::PAD)];
+  __shared__ __attribute__((aligned(16))) A As[C * C], Td[C * 16];
   __shared__ double G[C];
   __shared__ int R[C];
   __shared__ A bet[C];
@@ -160,8 +181,8 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
     Tile<T, C, DK, 256> k, q;
     k.fetch(p.k.at(b, t0, h / p.group), p.k.st, left, p.dk, tid);
     q.fetch(p.q.at(b, t0, h / p.group), p.q.st, left, p.dk, tid);
-    k.put(Ks, LD, tid);
-    q.put(Qs, LD, tid);
+    k.put(Ks, tid);
+    q.put(Qs, tid);
   }
   if (wave == 0) {  // logarithms summed up, fresh starts counted
     double sum;
@@ -196,7 +217,7 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
       if (jt <= rt)
 #pragma unroll
         for (int ks = 0; ks < DK; ks += M::K)
-          acc = M::mul(M::rows(Ks, LD, 16 * jt, ks, lane), M::rows(X, LD, 16 * rt, ks, lane), acc);
+          acc = M::mul(M::template rows<DK>(Ks, 16 * jt, ks, lane), M::template rows<DK>(X, 16 * rt, ks, lane), acc);
       A v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -217,23 +238,22 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
         }
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) As[i * LA + 16 * jt + M::row(g, r)] = v[r];
+        for (int r = 0; r < 4; ++r) As[Lay<A, C>::at(i, 16 * jt + M::row(g, r))] = v[r];
       }
     }
   }
   __syncthreads();
 
   // T's blocks on the diagonal: column fr of block g by substitution
-  constexpr int LT = 16 + MA::PAD;
   if (wave == 0 && g < NT) {
     A x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       A s = i == fr ? (A)1 : (A)0;
 #pragma unroll
-      for (int j = 0; j < i; ++j) s = mmpn::fma_of(-As[(16 * g + i) * LA + 16 * g + j], x[j], s);
+      for (int j = 0; j < i; ++j) s = mmpn::fma_of(-As[Lay<A, C>::at(16 * g + i, 16 * g + j)], x[j], s);
       x[i] = s;
-      Td[(16 * g + i) * LT + fr] = s;
+      Td[Lay<A, 16>::at(16 * g + i, fr)] = s;
     }
   }
   __syncthreads();
@@ -245,17 +265,17 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
     for (int i = 0; i < NT; ++i) {
       t[i] = AccA{};
       if (i == j) {
-        t[i] = MA::cols(Td, LT, 16 * j, 0, lane);
+        t[i] = MA::template cols<16>(Td, 16 * j, 0, lane);
       } else if (i > j) {
         AccA s{};
 #pragma unroll
         for (int m = 0; m < NT; ++m)
-          if (m >= j && m < i) s = MA::mul(MA::rows(As, LA, 16 * i, 16 * m, lane), t[m], s);
-        s = MA::mul(MA::rows(Td, LT, 16 * i, 0, lane), s, AccA{});
+          if (m >= j && m < i) s = MA::mul(MA::template rows<C>(As, 16 * i, 16 * m, lane), t[m], s);
+        s = MA::mul(MA::template rows<16>(Td, 16 * i, 0, lane), s, AccA{});
         t[i] = -s;
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) Ts[(16 * i + MA::row(g, r)) * LA + 16 * j + fr] = t[i][r];
+      for (int r = 0; r < 4; ++r) Ts[Lay<A, C>::at(16 * i + MA::row(g, r), 16 * j + fr)] = t[i][r];
     }
   }
   __syncthreads();
@@ -264,10 +284,10 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
     const int i = at / (C / V), j = at % (C / V) * V;
     Vec<T, V> hi, lo;
 #pragma unroll
-    for (int e = 0; e < V; ++e) hi.e[e] = (T)Ts[i * LA + j + e];
+    for (int e = 0; e < V; ++e) hi.e[e] = (T)Ts[Lay<A, C>::at(i, j + e)];
     mmpx::settle(hi);
 #pragma unroll
-    for (int e = 0; e < V; ++e) lo.e[e] = (T)(Ts[i * LA + j + e] - (A)hi.e[e]);
+    for (int e = 0; e < V; ++e) lo.e[e] = (T)(Ts[Lay<A, C>::at(i, j + e)] - (A)hi.e[e]);
     mmpn::store_vec(out + i * C + j, hi);
     if constexpr (M::SPLIT) mmpn::store_vec(out + C * C + i * C + j, lo);
   }
@@ -297,206 +317,315 @@ template <typename T> __device__ __forceinline__ void put4(T *p, const typename 
   }
 }
 
+// The tiles that make up operand f, rounded, where a lane's values are rows of a column.
+template <typename T, int N>
+__device__ __forceinline__ void put_tiles(T *p, const typename Mma<T>::Acc (&acc)[N], int f, int g) {
+  if constexpr (sizeof(T) == 2) {
+    Vec<T, 8> w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w.e[e] = (T)acc[2 * f + (e >> 2)][e & 3];
+    mmpn::store_vec(p + 8 * g, w);
+  } else {
+    const typename Wide<T>::type w[4] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3]};
+    put4<T>(p, w, g);
+  }
+}
+
+// LDS of a workgroup; and what a chunk takes of it.
+constexpr int kLds = 160 * 1024;
+template <typename T, int DK, int W, bool OUT> struct __attribute__((aligned(16))) PassStage {
+  static constexpr int C = chunk_of<T>();
+  T k[C * DK], th[C * C], v[C * W];
+  T q[OUT ? C * DK : 8], p[OUT ? C * C : 8], tl[Mma<T>::SPLIT ? C * C : 8];
+  typename Wide<T>::type vecs[kVecs<T>];
+};
+
+// Keeps reads of LDS before and after it apart; where keys are wide, registers are
+// too few to read ahead.
+template <int DK> __device__ __forceinline__ void in_place() {
+  if constexpr (DK <= 128) asm volatile("" ::: "memory");
+}
+
+// S += a b, a tile of it for each of a's first index.
+template <typename T, int DT, int NC>
+__device__ __forceinline__ void add_to(typename Mma<T>::Acc (&S)[DT], const typename Mma<T>::Frag (&a)[DT][NC],
+                                       const Two<T> (&b)[NC]) {
+#pragma unroll
+  for (int j = 0; j < NC; ++j)
+#pragma unroll
+    for (int part = Mma<T>::SPLIT ? 0 : 1; part < 2; ++part)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) S[t] = Mma<T>::mul(a[t][j], part ? b[j].hi : b[j].lo, S[t]);
+}
+
+template <int ROWS_, int COLS> struct Extent {
+  static constexpr int R = ROWS_, W = COLS;
+};
+
+// One chunk's arrays to LDS: by copies that nothing waits for yet, where their rows are
+// aligned, or through registers.
+template <typename T, bool COPIES, int NW, typename F, typename S>
+__device__ __forceinline__ void load_arrays(const F &arrays, int n, S &to, int tid) {
+  arrays(n, to, [&](T *lds, const T *from, long long stride, int rows, int cols, auto extent) __attribute__((always_inline)) {
+    constexpr int R = decltype(extent)::R, W = decltype(extent)::W;
+    if constexpr (COPIES) {
+      mmpx::copy_tile<T, R, W, NW>(from, stride, rows, cols, lds, __builtin_amdgcn_readfirstlane(tid >> 6), tid & 63);
+    } else {
+      Tile<T, R, W, 64 * NW> tile;
+      tile.fetch(from, stride, rows, cols, tid);
+      tile.put(lds, tid);
+    }
+  });
+}
+
+// Chunks from, from + by .. of `count` one after another.  AHEAD: a chunk is copied to
+// one half of LDS while the one before is worked on in the other, `first` before
+// that copy begins and `work` during it.  (The compiler waits for all copies under
+// way at some reads of LDS, transposing ones, of which it cannot tell that they
+// read the other half: those belong in `first`.)
+template <bool AHEAD, typename S, typename S2, typename L, typename E, typename F>
+__device__ __forceinline__ void through(int from, int count, int by, S &one, S2 &two, const L &load, const E &first, const F &work) {
+  if constexpr (AHEAD) {
+    if (count > 0) load(from, one);
+    for (int i = 0; i < count; i += 2) {
+      __syncthreads();  // waits for the copies; and what the other half held is done with
+      first(one);
+      if (i + 1 < count) load(from + (i + 1) * by, two);
+      work(from + i * by, one);
+      if (i + 1 < count) {
+        __syncthreads();
+        first(two);
+        if (i + 2 < count) load(from + (i + 2) * by, one);
+        work(from + (i + 1) * by, two);
+      }
+    }
+  } else {
+    for (int i = 0; i < count; ++i) {
+      load(from + i * by, one);
+      __syncthreads();
+      first(one);
+      work(from + i * by, one);
+      __syncthreads();
+    }
+  }
+}
+
 // Workgroup: NW waves with 16 columns each of a head's state (one without any only
 // helps with the copies).
-template <typename T, int DK, int NW, bool OUT, bool KEEP>
+template <typename T, int DK, int NW, bool OUT, bool KEEP, bool ALIGNED>
 __global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
   typedef typename M::Acc Acc;
-  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, THREADS = 64 * NW;
-  constexpr int LD = DK + M::PAD, LC = C + M::PAD, LV = 16 * NW + M::PAD, DT = DK / 16;
-  __shared__ __attribute__((aligned(16))) T Ks[C * LD], Qs[OUT ? C * LD : 1], Th[C * LC],
-      Tl[M::SPLIT ? C * LC : 1], Ps[OUT ? C * LC : 1], Vs[C * LV];
-  __shared__ __attribute__((aligned(16))) A vecs[3 * C];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16;
+  constexpr int W = 16 * NW, DT = DK / 16;
+  typedef PassStage<T, DK, W, OUT> Stage;
+  constexpr bool AHEAD = ALIGNED && 2 * sizeof(Stage) <= kLds;
+  __shared__ Stage one;
+  __shared__ typename std::conditional<AHEAD, Stage, char>::type two;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, g = lane >> 4;
   const long long bh = blockIdx.x / e.tiles;
   const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
   const int n0 = (int)(blockIdx.x - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;  // of the state
   const bool there = col < p.dv;
+  const int kh = h / p.group;
 
   Acc S[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * t + M::row(g, r);
+      const int i = M::spot(t, M::row(g, r));
       S[t][r] = e.initial && there && i < p.dk ? e.initial[(bh * p.dk + i) * p.dv + col] : (A)0;
     }
 
-  Tile<T, C, DK, THREADS> k, q;
-  Tile<T, C, C, THREADS> th, tl, ps;
-  Tile<T, C, 16 * NW, THREADS> v;
-  constexpr int NV = (3 * C + THREADS - 1) / THREADS;
-  A vec[NV];
-  // f(tile, its LDS, its row length there, from, stride, rows, columns) of each array
-  auto arrays = [&](int n, auto f) {
+  // f(LDS, from, stride, rows, columns, their numbers in LDS) of each array of chunk n
+  auto arrays = [&](int n, Stage &to, auto f) __attribute__((always_inline)) {
     const long long t0 = (long long)n * C;
     const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
     const T *w = p.within + (bh * p.chunks + n) * (2 * parts_of<T>() * C * C);
-    f(k, Ks, LD, p.k.at(b, t0, h / p.group), p.k.st, left, p.dk);
-    if constexpr (OUT) f(q, Qs, LD, p.q.at(b, t0, h / p.group), p.q.st, left, p.dk);
-    f(th, Th, LC, w, C, C, C);
-    if constexpr (M::SPLIT) f(tl, Tl, LC, w + C * C, C, C, C);
-    if constexpr (OUT) f(ps, Ps, LC, w + parts_of<T>() * C * C, C, C, C);
-    f(v, Vs, LV, p.v.at(b, t0, h) + n0, p.v.st, left, p.dv - n0);
-  };
-  auto fetch_vecs = [&](int n) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < 3 * C) vec[i] = p.vecs[(bh * p.chunks + n) * 3 * C + i * THREADS + tid];
-  };
-  auto put_vecs = [&]() {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < 3 * C) vecs[i * THREADS + tid] = vec[i];
-  };
-  auto fetch = [&](int n) {
-    arrays(n, [&](auto &tile, T *, int, const T *from, long long stride, int rows, int cols) {
-      tile.fetch(from, stride, rows, cols, tid);
-    });
-    fetch_vecs(n);
-  };
-  auto put = [&]() {
-    arrays(0, [&](auto &tile, T *to, int ld, const T *, long long, int, int) { tile.put(to, ld, tid); });
-    put_vecs();
-  };
-  auto load = [&](int n) {
-    arrays(n, [&](auto &tile, T *to, int ld, const T *from, long long stride, int rows, int cols) {
-      tile.fetch(from, stride, rows, cols, tid);
-      tile.put(to, ld, tid);
-    });
-    fetch_vecs(n);
-    put_vecs();
+    f(to.k, p.k.at(b, t0, kh), p.k.st, left, p.dk, Extent<C, DK>());
+    if constexpr (OUT) f(to.q, p.q.at(b, t0, kh), p.q.st, left, p.dk, Extent<C, DK>());
+    f(to.th, w, C, C, C, Extent<C, C>());
+    if constexpr (M::SPLIT) f(to.tl, w + C * C, C, C, C, Extent<C, C>());
+    if constexpr (OUT) f(to.p, w + parts_of<T>() * C * C, C, C, C, Extent<C, C>());
+    f(to.v, p.v.at(b, t0, h) + n0, p.v.st, left, p.dv - n0, Extent<C, W>());
+    if (wave == 0) copy_vecs<T>(p, bh * p.chunks + n, to.vecs, lane);
   };
 
-  auto chunk = [&](int n) {
+  typedef typename M::Frag Frag;
+  constexpr int NF = DT / PT, NC = NT / PT;
+  Frag value[NC];
+  auto first = [&](const Stage &in) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) value[j] = M::template cols<W>(in.v, j * M::K, 16 * wave, lane);
+    in_place<DK>();
+  };
+  auto chunk = [&](int n, const Stage &in) __attribute__((always_inline)) {
+    const A *vecs = in.vecs;
     const long long t0 = (long long)n * C;
     const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
-
-    Two<T> s[DT / PT];
+    // Reads of LDS are kept a product ahead of the one that needs them (the empty
+    // asm holds them in their place), as there are no other waves to wait for them.
+    Frag kr[NT][NF], kc[DT][NC], tr[NT][NC], tl[NT][NC], qr[NT][NF], pr[NT][NC];
+    A cv[NT][4], ev[NT][4], bv[NT][4], co[NT];
 #pragma unroll
-    for (int i = 0; i < DT / PT; ++i) s[i] = mmpx::operand<T>(S, i * PT);
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int d = 0; d < NF; ++d) kr[i][d] = M::template tile_rows<DK>(in.k, i, d * M::K, lane);
+    in_place<DK>();
+    Two<T> s[NF];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) s[i] = mmpx::operand<T>(S, i * PT);
     if constexpr (KEEP) {
       if (there) {
         T *o = e.keep_s + ((bh * p.chunks + n) * p.dv + col) * DK;
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-          const A w[4] = {S[t][0], S[t][1], S[t][2], S[t][3]};
-          put4<T>(o + 16 * t, w, g);
-        }
+        for (int t = 0; t < NF; ++t) put_tiles<T>(o + t * M::K, S, t, g);
       }
     }
-    // R = beta (V - c K S)
-    Acc x[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      x[i] = Acc{};
-#pragma unroll
-      for (int d = 0; d < DT / PT; ++d) x[i] = mmpx::mul_two<T>(M::rows(Ks, LD, 16 * i, d * M::K, lane), s[d], x[i]);
-    }
-    Two<T> f[NT / PT], fe[NT / PT];
-#pragma unroll
-    for (int i = 0; i < NT; i += PT) {
-      const typename M::Frag value = M::cols(Vs, LV, 16 * i, 16 * wave, lane);
-      A r[M::E];
-#pragma unroll
-      for (int c = 0; c < M::E; ++c) {
-        const int at = 16 * (i + (c >> 2)) + M::row(g, c & 3);
-        r[c] = vecs[2 * C + at] * mmpn::fma_of(-vecs[at], x[i + (c >> 2)][c & 3], (A)value[c]);
-      }
-      f[i / PT] = mmpx::two_of<T>(r);
-    }
-    // U = T R
-    Acc u[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      u[i] = Acc{};
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j <= i / PT; ++j) {
-        Two<T> t;
-        t.hi = M::rows(Th, LC, 16 * i, j * M::K, lane);
-        if constexpr (M::SPLIT) t.lo = M::rows(Tl, LC, 16 * i, j * M::K, lane);
-        u[i] = mmpx::mul_twos<T>(t, f[j], u[i]);
+        tr[i][j] = M::template tile_rows<C>(in.th, i, j * M::K, lane);
+        if constexpr (M::SPLIT) tl[i][j] = M::template tile_rows<C>(in.tl, i, j * M::K, lane);
       }
-    }
-    if constexpr (KEEP) {
-      if (there) {
-        T *o = e.keep_u + ((bh * p.chunks + n) * p.dv + col) * C;
+    in_place<DK>();
+    // Products that add to the same tile are kept apart by others, as each waits for
+    // the one before.  K S, and Q S: transposed, a lane has a step's columns row(g, .) of the wave's 16
+    Acc x[NT], o[NT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const A w[4] = {u[i][0], u[i][1], u[i][2], u[i][3]};
-          put4<T>(o + 16 * i, w, g);
-        }
+    for (int i = 0; i < NT; ++i) x[i] = o[i] = Acc{};
+#pragma unroll
+    for (int d = 0; d < NF; ++d)
+#pragma unroll
+      for (int part = M::SPLIT ? 0 : 1; part < 2; ++part)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x[i] = M::mul(kr[i][d], part ? s[d].hi : s[d].lo, x[i]);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = M::spot(i, M::row(g, r));
+        cv[i][r] = vecs[at];
+        bv[i][r] = vecs[2 * C + at];
       }
-    }
-#pragma unroll
-    for (int i = 0; i < NT; i += PT) {
-      f[i / PT] = mmpx::operand<T>(u, i);
-      A w[M::E];
-#pragma unroll
-      for (int c = 0; c < M::E; ++c) w[c] = vecs[C + 16 * (i + (c >> 2)) + M::row(g, c & 3)] * u[i + (c >> 2)][c & 3];
-      fe[i / PT] = mmpx::two_of<T>(w);
-    }
-    // O, transposed: a lane has a step's columns row(g, .) of the wave's 16
+    const A decay = vecs[C - 1];
     if constexpr (OUT) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        Acc o{};
+        co[i] = p.scale * vecs[16 * i + fr];
 #pragma unroll
-        for (int d = 0; d < DT / PT; ++d) o = mmpx::two_mul<T>(s[d], M::rows(Qs, LD, 16 * i, d * M::K, lane), o);
-        const A by = p.scale * vecs[16 * i + fr];
+        for (int d = 0; d < NF; ++d) qr[i][d] = M::template rows<DK>(in.q, 16 * i, d * M::K, lane);
+      }
+      in_place<DK>();
+    }
+    // R = beta (V - c K S)
+    Two<T> f[NC], fe[NC];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] *= by;
+    for (int j = 0; j < NC; ++j) {
+      A r[M::E];
 #pragma unroll
-        for (int j = 0; j <= i / PT; ++j) o = mmpx::two_mul<T>(f[j], M::rows(Ps, LC, 16 * i, j * M::K, lane), o);
-        const int step = 16 * i + fr;
-        if (step < left) {
-          T *to = e.o + (((long long)b * p.steps + t0 + step) * p.heads + h) * p.dv + n0 + 16 * wave;
-          if (n0 + 16 * wave + 16 <= p.dv) {
-            const A w[4] = {o[0], o[1], o[2], o[3]};
-            put4<T>(to, w, g);
-          } else {
+      for (int c = 0; c < M::E; ++c) {
+        const int i = j * PT + (c >> 2);
+        r[c] = bv[i][c & 3] * mmpn::fma_of(-cv[i][c & 3], x[i][c & 3], (A)value[j][c]);
+      }
+      f[j] = mmpx::two_of<T>(r);
+    }
+    if constexpr (OUT) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (n0 + 16 * wave + M::row(g, r) < p.dv) to[M::row(g, r)] = (T)o[r];
-          }
-        }
+      for (int d = 0; d < NF; ++d)
+#pragma unroll
+        for (int part = M::SPLIT ? 0 : 1; part < 2; ++part)
+#pragma unroll
+          for (int i = 0; i < NT; ++i) o[i] = M::mul(part ? s[d].hi : s[d].lo, qr[i][d], o[i]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j <= i / PT; ++j) pr[i][j] = M::template rows<C>(in.p, 16 * i, j * M::K, lane);
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) kc[t][j] = M::template tile_cols<DK>(in.k, j * M::K, t, lane);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ev[i][r] = vecs[C + M::spot(i, M::row(g, r))];
+    in_place<DK>();
+    // U = T R
+    Acc u[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) u[i] = Acc{};
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int part = M::SPLIT ? 0 : 2; part < 3; ++part)
+#pragma unroll
+        for (int i = j * PT; i < NT; ++i)
+          u[i] = M::mul(part == 0 ? tl[i][j] : tr[i][j], part == 1 ? f[j].lo : f[j].hi, u[i]);
+    if constexpr (KEEP) {
+      if (there) {
+        T *to = e.keep_u + ((bh * p.chunks + n) * p.dv + col) * C;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) put_tiles<T>(to + j * M::K, u, j, g);
       }
     }
-    // S' = c_C S + K^T (e U)
-    const A decay = vecs[C - 1];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
+    for (int j = 0; j < NC; ++j) {
+      A w[M::E];
+#pragma unroll
+      for (int c = 0; c < M::E; ++c) w[c] = ev[j * PT + (c >> 2)][c & 3] * u[j * PT + (c >> 2)][c & 3];
+      fe[j] = mmpx::two_of<T>(w);
+      if constexpr (OUT) f[j] = mmpx::operand<T>(u, j * PT);
+    }
+    // S' = c_C S + K^T (e U)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[t][r] *= decay;
+    add_to<T>(S, kc, fe);
+    if constexpr (OUT) {
 #pragma unroll
-      for (int j = 0; j < NT / PT; ++j) S[t] = mmpx::mul_two<T>(M::cols(Ks, LD, j * M::K, 16 * t, lane), fe[j], S[t]);
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[i][r] *= co[i];
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int part = M::SPLIT ? 0 : 1; part < 2; ++part)
+#pragma unroll
+          for (int i = j * PT; i < NT; ++i) o[i] = M::mul(part ? f[j].hi : f[j].lo, pr[i][j], o[i]);
+      T *to = e.o + (((long long)b * p.steps + t0 + fr) * p.heads + h) * p.dv + n0 + 16 * wave;
+      const long long down = 16LL * p.heads * p.dv;
+      if (left == C && n0 + 16 * wave + 16 <= p.dv) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const A w[4] = {o[i][0], o[i][1], o[i][2], o[i][3]};
+          put4<T>(to + i * down, w, g);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * i + fr < left && n0 + 16 * wave + M::row(g, r) < p.dv) to[i * down + M::row(g, r)] = (T)o[i][r];
+      }
     }
   };
 
-  // The next chunk is on its way in registers during the products of this one,
-  // where there are enough of them.
-  constexpr bool AHEAD = DK <= 128;
-  if constexpr (AHEAD) fetch(0);
-  for (int n = 0; n < p.chunks; ++n) {
-    if constexpr (AHEAD) {
-      put();
-      __syncthreads();
-      if (n + 1 < p.chunks) fetch(n + 1);
-    } else {
-      load(n);
-      __syncthreads();
-    }
-    if (n0 + 16 * wave < p.dv) chunk(n);
-    __syncthreads();
-  }
+  const bool active = n0 + 16 * wave < p.dv;
+  through<AHEAD>(0, p.chunks, 1, one, two, [&](int n, Stage &to) __attribute__((always_inline)) { load_arrays<T, AHEAD, NW>(arrays, n, to, tid); },
+                 first, [&](int n, const Stage &in) __attribute__((always_inline)) {
+                   if (active) chunk(n, in);
+                 });
   if (e.final && there)
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = 16 * t + M::row(g, r);
+        const int i = M::spot(t, M::row(g, r));
         if (i < p.dk) e.final[(bh * p.dk + i) * p.dv + col] = S[t][r];
       }
 }
@@ -646,184 +775,190 @@ template <typename T> struct Back {
   int tiles;
 };
 
+template <typename T, int DK, int W> struct __attribute__((aligned(16))) BackStage {
+  static constexpr int C = chunk_of<T>();
+  T k[C * DK], q[C * DK], th[C * C], ph[C * C], o[C * W];
+  T tl[Mma<T>::SPLIT ? C * C : 8], pl[Mma<T>::SPLIT ? C * C : 8];
+  typename Wide<T>::type vecs[kVecs<T>];
+};
+
 // Workgroup: as k_delta_pass.
-template <typename T, int DK, int NW>
+template <typename T, int DK, int NW, bool ALIGNED>
 __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
   typedef typename M::Acc Acc;
-  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, THREADS = 64 * NW;
-  constexpr int LD = DK + M::PAD, LC = C + M::PAD, LV = 16 * NW + M::PAD, DT = DK / 16;
-  __shared__ __attribute__((aligned(16))) T Ks[C * LD], Qs[C * LD], Th[C * LC], Ph[C * LC],
-      Tl[M::SPLIT ? C * LC : 1], Pl[M::SPLIT ? C * LC : 1], Os[C * LV];
-  __shared__ __attribute__((aligned(16))) A vecs[3 * C];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16;
+  constexpr int W = 16 * NW, DT = DK / 16;
+  typedef BackStage<T, DK, W> Stage;
+  constexpr bool AHEAD = ALIGNED && 2 * sizeof(Stage) <= kLds;
+  __shared__ Stage one;
+  __shared__ typename std::conditional<AHEAD, Stage, char>::type two;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, g = lane >> 4;
   const long long bh = blockIdx.x / e.tiles;
   const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
   const int n0 = (int)(blockIdx.x - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;
   const bool there = col < p.dv;
+  const int kh = h / p.group;
 
   Acc S[DT];  // the state's gradient
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * t + M::row(g, r);
+      const int i = M::spot(t, M::row(g, r));
       S[t][r] = e.grad_final && there && i < p.dk ? e.grad_final[(bh * p.dk + i) * p.dv + col] : (A)0;
     }
 
-  Tile<T, C, DK, THREADS> k, q;
-  Tile<T, C, C, THREADS> th, tl, ph, pl;
-  Tile<T, C, 16 * NW, THREADS> o;
-  constexpr int NV = (3 * C + THREADS - 1) / THREADS;
-  A vec[NV];
-  auto arrays = [&](int n, auto f) {
+  auto arrays = [&](int n, Stage &to, auto f) __attribute__((always_inline)) {
     const long long t0 = (long long)n * C;
     const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
     const T *w = p.within + (bh * p.chunks + n) * (2 * parts_of<T>() * C * C);
-    f(k, Ks, LD, p.k.at(b, t0, h / p.group), p.k.st, left, p.dk);
-    f(q, Qs, LD, p.q.at(b, t0, h / p.group), p.q.st, left, p.dk);
-    f(th, Th, LC, w, C, C, C);
-    f(ph, Ph, LC, w + parts_of<T>() * C * C, C, C, C);
+    f(to.k, p.k.at(b, t0, kh), p.k.st, left, p.dk, Extent<C, DK>());
+    f(to.q, p.q.at(b, t0, kh), p.q.st, left, p.dk, Extent<C, DK>());
+    f(to.th, w, C, C, C, Extent<C, C>());
+    f(to.ph, w + parts_of<T>() * C * C, C, C, C, Extent<C, C>());
     if constexpr (M::SPLIT) {
-      f(tl, Tl, LC, w + C * C, C, C, C);
-      f(pl, Pl, LC, w + 3 * C * C, C, C, C);
+      f(to.tl, w + C * C, C, C, C, Extent<C, C>());
+      f(to.pl, w + 3 * C * C, C, C, C, Extent<C, C>());
     }
-    f(o, Os, LV, e.grad.at(b, t0, h) + n0, e.grad.st, left, p.dv - n0);
-  };
-  auto fetch_vecs = [&](int n) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < 3 * C) vec[i] = p.vecs[(bh * p.chunks + n) * 3 * C + i * THREADS + tid];
-  };
-  auto put_vecs = [&]() {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < 3 * C) vecs[i * THREADS + tid] = vec[i];
-  };
-  auto fetch = [&](int n) {
-    arrays(n, [&](auto &tile, T *, int, const T *from, long long stride, int rows, int cols) {
-      tile.fetch(from, stride, rows, cols, tid);
-    });
-    fetch_vecs(n);
-  };
-  auto put = [&]() {
-    arrays(0, [&](auto &tile, T *to, int ld, const T *, long long, int, int) { tile.put(to, ld, tid); });
-    put_vecs();
-  };
-  auto load = [&](int n) {
-    arrays(n, [&](auto &tile, T *to, int ld, const T *from, long long stride, int rows, int cols) {
-      tile.fetch(from, stride, rows, cols, tid);
-      tile.put(to, ld, tid);
-    });
-    fetch_vecs(n);
-    put_vecs();
+    f(to.o, e.grad.at(b, t0, h) + n0, e.grad.st, left, p.dv - n0, Extent<C, W>());
+    if (wave == 0) copy_vecs<T>(p, bh * p.chunks + n, to.vecs, lane);
   };
 
-  auto chunk = [&](int n) {
-    Two<T> s[DT / PT];
+  typedef typename M::Frag Frag;
+  constexpr int NF = DT / PT, NC = NT / PT;
+  Frag go[NC], pc[NT][NC], pl[NT][NC], tc[NT][NC], tl[NT][NC];
+  auto first = [&](const Stage &in) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < DT / PT; ++i) s[i] = mmpx::operand<T>(S, i * PT);
+    for (int j = 0; j < NC; ++j) go[j] = M::template cols<W>(in.o, j * M::K, 16 * wave, lane);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = i / PT; j < NC; ++j) {
+        pc[i][j] = M::template tile_cols<C>(in.ph, j * M::K, i, lane);
+        tc[i][j] = M::template tile_cols<C>(in.th, j * M::K, i, lane);
+        if constexpr (M::SPLIT) {
+          pl[i][j] = M::template tile_cols<C>(in.pl, j * M::K, i, lane);
+          tl[i][j] = M::template tile_cols<C>(in.tl, j * M::K, i, lane);
+        }
+      }
+    in_place<DK>();
+  };
+  auto chunk = [&](int n, const Stage &in) __attribute__((always_inline)) {
+    const A *vecs = in.vecs;
+    Frag kr[NT][NF], kc[DT][NC], qc[DT][NC];
+    A cv[NT][4], ev[NT][4], bv[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int d = 0; d < NF; ++d) kr[i][d] = M::template tile_rows<DK>(in.k, i, d * M::K, lane);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = M::spot(i, M::row(g, r));
+        cv[i][r] = vecs[at];
+        ev[i][r] = vecs[C + at];
+        bv[i][r] = vecs[2 * C + at];
+      }
+    const A decay = vecs[C - 1];
+    in_place<DK>();
+    Two<T> s[NF];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) s[i] = mmpx::operand<T>(S, i * PT);
     if (there) {
       T *to = e.keep_d + ((bh * p.chunks + n) * p.dv + col) * DK;
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const A w[4] = {S[t][0], S[t][1], S[t][2], S[t][3]};
-        put4<T>(to + 16 * t, w, g);
-      }
+      for (int t = 0; t < NF; ++t) put_tiles<T>(to + t * M::K, S, t, g);
     }
-    typename M::Frag go[NT / PT];
-#pragma unroll
-    for (int j = 0; j < NT / PT; ++j) go[j] = M::cols(Os, LV, j * M::K, 16 * wave, lane);
     // dU
     Acc u[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      u[i] = Acc{};
+    for (int i = 0; i < NT; ++i) u[i] = Acc{};
 #pragma unroll
-      for (int d = 0; d < DT / PT; ++d) u[i] = mmpx::mul_two<T>(M::rows(Ks, LD, 16 * i, d * M::K, lane), s[d], u[i]);
+    for (int d = 0; d < NF; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) u[i][r] *= vecs[C + 16 * i + M::row(g, r)];
+      for (int part = M::SPLIT ? 0 : 1; part < 2; ++part)
 #pragma unroll
-      for (int j = i / PT; j < NT / PT; ++j) {
-        Two<T> w;
-        w.hi = M::cols(Ph, LC, j * M::K, 16 * i, lane);
-        if constexpr (M::SPLIT) w.lo = M::cols(Pl, LC, j * M::K, 16 * i, lane);
-        u[i] = mmpx::two_mul<T>(w, go[j], u[i]);
-      }
+        for (int i = 0; i < NT; ++i) u[i] = M::mul(kr[i][d], part ? s[d].hi : s[d].lo, u[i]);
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) qc[t][j] = M::template tile_cols<DK>(in.q, j * M::K, t, lane);
+    in_place<DK>();
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) u[i][r] *= ev[i][r];
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int part = M::SPLIT ? 0 : 1; part < 2; ++part)
+#pragma unroll
+        for (int i = 0; i < (j + 1) * PT; ++i) u[i] = M::mul(part ? pc[i][j] : pl[i][j], go[j], u[i]);
+    // scale c dO, and what it gives the state
+    Two<T> f[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      A w[M::E];
+#pragma unroll
+      for (int c = 0; c < M::E; ++c) w[c] = p.scale * cv[j * PT + (c >> 2)][c & 3] * (A)go[j][c];
+      f[j] = mmpx::two_of<T>(w);
     }
-    Two<T> f[NT / PT];
 #pragma unroll
-    for (int j = 0; j < NT / PT; ++j) f[j] = mmpx::operand<T>(u, j * PT);
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][r] *= decay;
+    add_to<T>(S, qc, f);
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) kc[t][j] = M::template tile_cols<DK>(in.k, j * M::K, t, lane);
+    in_place<DK>();
+#pragma unroll
+    for (int j = 0; j < NC; ++j) f[j] = mmpx::operand<T>(u, j * PT);
     // dR
     Acc x[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      x[i] = Acc{};
+    for (int i = 0; i < NT; ++i) x[i] = Acc{};
 #pragma unroll
-      for (int j = i / PT; j < NT / PT; ++j) {
-        Two<T> w;
-        w.hi = M::cols(Th, LC, j * M::K, 16 * i, lane);
-        if constexpr (M::SPLIT) w.lo = M::cols(Tl, LC, j * M::K, 16 * i, lane);
-        x[i] = mmpx::mul_twos<T>(w, f[j], x[i]);
-      }
-    }
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int part = M::SPLIT ? 0 : 2; part < 3; ++part)
+#pragma unroll
+        for (int i = 0; i < (j + 1) * PT; ++i)
+          x[i] = M::mul(part == 0 ? tl[i][j] : tc[i][j], part == 1 ? f[j].lo : f[j].hi, x[i]);
     if (there) {
       T *to = e.keep_r + ((bh * p.chunks + n) * p.dv + col) * C;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const A w[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
-        put4<T>(to + 16 * i, w, g);
-      }
+      for (int j = 0; j < NC; ++j) put_tiles<T>(to + j * M::K, x, j, g);
     }
-    // dX and scale c dO
-    Two<T> fo[NT / PT];
+    // dX, and what it gives the state
 #pragma unroll
-    for (int j = 0; j < NT / PT; ++j) {
-      A wx[M::E], wo[M::E];
+    for (int j = 0; j < NC; ++j) {
+      A w[M::E];
 #pragma unroll
       for (int c = 0; c < M::E; ++c) {
-        const int at = 16 * (j * PT + (c >> 2)) + M::row(g, c & 3);
-        wx[c] = -vecs[2 * C + at] * vecs[at] * x[j * PT + (c >> 2)][c & 3];
-        wo[c] = p.scale * vecs[at] * (A)go[j][c];
+        const int i = j * PT + (c >> 2);
+        w[c] = -bv[i][c & 3] * cv[i][c & 3] * x[i][c & 3];
       }
-      f[j] = mmpx::two_of<T>(wx);
-      fo[j] = mmpx::two_of<T>(wo);
+      f[j] = mmpx::two_of<T>(w);
     }
-    const A decay = vecs[C - 1];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) S[t][r] *= decay;
-#pragma unroll
-      for (int j = 0; j < NT / PT; ++j) {
-        S[t] = mmpx::mul_two<T>(M::cols(Ks, LD, j * M::K, 16 * t, lane), f[j], S[t]);
-        S[t] = mmpx::mul_two<T>(M::cols(Qs, LD, j * M::K, 16 * t, lane), fo[j], S[t]);
-      }
-    }
+    add_to<T>(S, kc, f);
   };
 
-  constexpr bool AHEAD = DK <= 128;
-  if constexpr (AHEAD)
-    if (p.chunks) fetch(p.chunks - 1);
-  for (int n = p.chunks - 1; n >= 0; --n) {
-    if constexpr (AHEAD) {
-      put();
-      __syncthreads();
-      if (n) fetch(n - 1);
-    } else {
-      load(n);
-      __syncthreads();
-    }
-    if (n0 + 16 * wave < p.dv) chunk(n);
-    __syncthreads();
-  }
+  const bool active = n0 + 16 * wave < p.dv;
+  through<AHEAD>(p.chunks - 1, p.chunks, -1, one, two, [&](int n, Stage &to) __attribute__((always_inline)) { load_arrays<T, AHEAD, NW>(arrays, n, to, tid); },
+                 first, [&](int n, const Stage &in) __attribute__((always_inline)) {
+                   if (active) chunk(n, in);
+                 });
   if (there)
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = 16 * t + M::row(g, r);
+        const int i = M::spot(t, M::row(g, r));
         if (i < p.dk) e.grad_initial[(bh * p.dk + i) * p.dv + col] = S[t][r];
       }
 }
@@ -836,11 +971,10 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
   typedef typename M::Acc Acc;
   constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, V = vec_of<T>();
   constexpr int VB = 32, KB = 64;  // channels of values and of keys at a time
-  constexpr int LD = DK + M::PAD, LC = C + M::PAD, LB = VB + M::PAD, LK = KB + M::PAD;
   constexpr int TASKS = (2 * NT + 3) / 4;
   static_assert(C * (VB / V) == 256, "a vector of the chunk's values for each thread");
-  __shared__ __attribute__((aligned(16))) T Ks[C * LD], Qs[C * LD], Fs[C * LC], Es[C * LC], Os[C * LB],
-      Us[VB * LC], Rs[VB * LC], Ss[VB * LK], Ds[VB * LK];
+  __shared__ __attribute__((aligned(16))) T Ks[C * DK], Qs[C * DK], Fs[C * C], Es[C * C], Os[C * VB],
+      Us[VB * C], Rs[VB * C], Ss[VB * KB], Ds[VB * KB];
   __shared__ double G[C];
   __shared__ int R[C];
   __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][4][16], rv[C], ek[C], sd[4];
@@ -855,8 +989,8 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
     Tile<T, C, DK, 256> k, q;
     k.fetch(p.k.at(b, t0, kh), p.k.st, left, p.dk, tid);
     q.fetch(p.q.at(b, t0, kh), p.q.st, left, p.dk, tid);
-    k.put(Ks, LD, tid);
-    q.put(Qs, LD, tid);
+    k.put(Ks, tid);
+    q.put(Qs, tid);
   }
   // dQ and dK, transposed: a wave has rows 16 rt and NT tiles of columns from ct on of each 64
   const int rt = wave % NT, ct = wave / NT * NT;
@@ -898,9 +1032,9 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
       u.fetch(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
       r.fetch(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
       if (v0) __syncthreads();
-      o.put(Os, LB, tid);
-      u.put(Us, LC, tid);
-      r.put(Rs, LC, tid);
+      o.put(Os, tid);
+      u.put(Us, tid);
+      r.put(Rs, tid);
       __syncthreads();
       if (vi < left) {
         const A beta = bet[vi];
@@ -917,7 +1051,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const A d = (A)Rs[(vn + i) * LC + vi];
+          const A d = (A)Rs[Lay<T, C>::at(vn + i, vi)];
           with_v = mmpn::fma_of(d, (A)x.e[i], with_v);
           y.e[i] = (T)(beta * d);
         }
@@ -937,10 +1071,10 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         const int row = query ? 2 * NT - 1 - task : task;
 #pragma unroll
         for (int d = 0; d < VB; d += M::K) {
-          const typename M::Frag x = query ? M::rows(Os, LB, 16 * row, d, lane) : M::cols(Rs, LC, d, 16 * row, lane);
+          const typename M::Frag x = query ? M::template rows<VB>(Os, 16 * row, d, lane) : M::template cols<C>(Rs, d, 16 * row, lane);
 #pragma unroll
           for (int j = 0; j < NT; ++j)
-            if (j <= row) w[k][j] = M::mul(M::cols(Us, LC, d, 16 * j, lane), x, w[k][j]);
+            if (j <= row) w[k][j] = M::mul(M::template cols<C>(Us, d, 16 * j, lane), x, w[k][j]);
         }
       }
     }
@@ -956,7 +1090,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
       const bool query = task >= NT;
       const int row = query ? 2 * NT - 1 - task : task, i = 16 * row + fr;
       const T *X = query ? Qs : Ks;
-      T *to = (query ? Fs : Es) + i * LC;
+      T *to = query ? Fs : Es;
       const double Gi = G[i];
       const int Ri = R[i];
       const A by = query ? p.scale : bet[i];
@@ -966,14 +1100,14 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         Acc x{};
         if (j <= row)
 #pragma unroll
-          for (int d = 0; d < DK; d += M::K) x = M::mul(M::rows(Ks, LD, 16 * j, d, lane), M::rows(X, LD, 16 * row, d, lane), x);
+          for (int d = 0; d < DK; d += M::K) x = M::mul(M::template rows<DK>(Ks, 16 * j, d, lane), M::template rows<DK>(X, 16 * row, d, lane), x);
         A sum_col[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int jj = 16 * j + M::row(g, c);
           const bool in = (query ? jj <= i : jj < i) && R[jj] == Ri;
           const A f = in ? (query ? w[k][j][c] : -w[k][j][c]) * exp_any((A)(Gi - G[jj])) : (A)0;
-          to[jj] = (T)(f * by);
+          to[Lay<T, C>::at(i, jj)] = (T)(f * by);
           const A m = in ? f * x[c] : (A)0;
           sum_e += m;
           sum_row = mmpn::fma_of(m, by, sum_row);
@@ -1013,11 +1147,11 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         st.fetch(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, tid);
         dt.fetch(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, tid);
         __syncthreads();
-        o.put(Os, LB, tid);
-        u.put(Us, LC, tid);
-        r.put(Rs, LC, tid);
-        st.put(Ss, LK, tid);
-        dt.put(Ds, LK, tid);
+        o.put(Os, tid);
+        u.put(Us, tid);
+        r.put(Rs, tid);
+        st.put(Ss, tid);
+        dt.put(Ds, tid);
 #pragma unroll
         for (int c = 0; c < st.N; ++c) {
           const Vec<T, V> x = mmpn::elements_of<T, V>(st.w[c]), x2 = mmpn::elements_of<T, V>(dt.w[c]);
@@ -1027,11 +1161,11 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         __syncthreads();
 #pragma unroll
         for (int d = 0; d < VB; d += M::K) {
-          const typename M::Frag fo = M::rows(Os, LB, 16 * rt, d, lane), fr_ = M::cols(Rs, LC, d, 16 * rt, lane),
-                                 fu = M::cols(Us, LC, d, 16 * rt, lane);
+          const typename M::Frag fo = M::template rows<VB>(Os, 16 * rt, d, lane), fr_ = M::template cols<C>(Rs, d, 16 * rt, lane),
+                                 fu = M::template cols<C>(Us, d, 16 * rt, lane);
 #pragma unroll
           for (int c = 0; c < NT; ++c) {
-            const typename M::Frag fs = M::cols(Ss, LK, d, 16 * (ct + c), lane), fd = M::cols(Ds, LK, d, 16 * (ct + c), lane);
+            const typename M::Frag fs = M::template cols<KB>(Ss, d, 16 * (ct + c), lane), fd = M::template cols<KB>(Ds, d, 16 * (ct + c), lane);
             a[c] = M::mul(fs, fo, a[c]);
             z[c] = M::mul(fs, fr_, z[c]);
             y[c] = M::mul(fd, fu, y[c]);
@@ -1046,7 +1180,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
 #pragma unroll
         for (int l = 0; l < 4; ++l) {
           const int d = d0 + M::row(g, l);
-          const A qv = (A)Qs[i * LD + d], kv = (A)Ks[i * LD + d];
+          const A qv = (A)Qs[Lay<T, DK>::at(i, d)], kv = (A)Ks[Lay<T, DK>::at(i, d)];
           const A av = sc * a[c][l], zv = cz * z[c][l], yv = ce * y[c][l];
           q_s = mmpn::fma_of(qv, av, q_s);
           k_z = mmpn::fma_of(kv, zv, k_z);
@@ -1056,14 +1190,14 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         }
 #pragma unroll
         for (int j = 0; j < NT / PT; ++j) {
-          const typename M::Frag kc = M::cols(Ks, LD, j * M::K, d0, lane), qc = M::cols(Qs, LD, j * M::K, d0, lane);
+          const typename M::Frag kc = M::template cols<DK>(Ks, j * M::K, d0, lane), qc = M::template cols<DK>(Qs, j * M::K, d0, lane);
           if (j <= rt / PT) {
-            dq[kb][c] = M::mul(kc, M::rows(Fs, LC, 16 * rt, j * M::K, lane), dq[kb][c]);
-            dk[kb][c] = M::mul(kc, M::rows(Es, LC, 16 * rt, j * M::K, lane), dk[kb][c]);
+            dq[kb][c] = M::mul(kc, M::template rows<C>(Fs, 16 * rt, j * M::K, lane), dq[kb][c]);
+            dk[kb][c] = M::mul(kc, M::template rows<C>(Es, 16 * rt, j * M::K, lane), dk[kb][c]);
           }
           if (j >= rt / PT) {
-            dk[kb][c] = M::mul(kc, M::cols(Es, LC, j * M::K, 16 * rt, lane), dk[kb][c]);
-            dk[kb][c] = M::mul(qc, M::cols(Fs, LC, j * M::K, 16 * rt, lane), dk[kb][c]);
+            dk[kb][c] = M::mul(kc, M::template cols<C>(Es, j * M::K, 16 * rt, lane), dk[kb][c]);
+            dk[kb][c] = M::mul(qc, M::template cols<C>(Fs, j * M::K, 16 * rt, lane), dk[kb][c]);
           }
         }
       }
@@ -1154,6 +1288,17 @@ template <typename F> int with_width(int dk, F f) {
   return f(std::integral_constant<int, 256>());
 }
 
+// Whether whole 16 byte vectors make up the rows of the keys, the queries and `v`, as
+// copies take them.
+template <typename T> bool whole_vectors(const Seq<T> &s) {
+  constexpr int V = vec_of<T>();
+  return (uintptr_t)s.p % 16 == 0 && s.sb % V == 0 && s.st % V == 0 && s.sh % V == 0 && s.st >= 0 && s.st < (1 << 26);
+}
+template <typename T> bool copies(const Delta<T> &p, const Seq<T> &v) {
+  constexpr int V = vec_of<T>();
+  return p.dk % V == 0 && p.dv % V == 0 && whole_vectors(p.q) && whole_vectors(p.k) && whole_vectors(v);
+}
+
 // Memory of the chunks' products.
 template <typename T> struct Chunks {
   Temp within, vecs;
@@ -1163,7 +1308,7 @@ template <typename T> struct Chunks {
     if (!mmpi::grid_fits(all, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many steps", what);
     p.chunks = (int)n;
     if (int st = within.get((size_t)all * 2 * parts_of<T>() * C * C * sizeof(T), what)) return st;
-    if (int st = vecs.get((size_t)all * 3 * C * sizeof(typename Wide<T>::type), what)) return st;
+    if (int st = vecs.get((size_t)all * 3 * C * sizeof(typename Wide<T>::type) + 1024, what)) return st;
     p.within = (T *)within.p;
     p.vecs = (typename Wide<T>::type *)vecs.p;
     if (!all) return MMP_OK;
@@ -1180,7 +1325,11 @@ template <typename T, bool OUT, bool KEEP> int pass(const Delta<T> &p, Pass<T> e
   const int64_t blocks = (int64_t)p.batch * p.heads * e.tiles;
   if (!mmpi::grid_fits(blocks, 64 * NW)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
   return with_width(p.dk, [&](auto dk) {
-    hipLaunchKernelGGL((k_delta_pass<T, dk.value, NW, OUT, KEEP>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+    constexpr int DK = decltype(dk)::value;
+    if (copies(p, p.v))
+      hipLaunchKernelGGL((k_delta_pass<T, DK, NW, OUT, KEEP, true>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+    else
+      hipLaunchKernelGGL((k_delta_pass<T, DK, NW, OUT, KEEP, false>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
     return mmpi::check_launch(what);
   });
 }
@@ -1227,7 +1376,11 @@ template <typename T> int backward(Delta<T> p, Back<T> e, int key_heads, const t
   if (!mmpi::grid_fits(blocks, 64 * NW)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
   if (blocks)
     if (int st = with_width(p.dk, [&](auto dk) {
-          hipLaunchKernelGGL((k_delta_back<T, dk.value, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+          constexpr int DK = decltype(dk)::value;
+          if (copies(p, e.grad))
+            hipLaunchKernelGGL((k_delta_back<T, DK, NW, true>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+          else
+            hipLaunchKernelGGL((k_delta_back<T, DK, NW, false>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
           return mmpi::check_launch(what);
         }))
       return st;

@@ -17,7 +17,7 @@
 // is when a program forms it itself.
 #include <utility>
 
-#include "mmp_nn.h"
+#include "mmp_mma.h"
 
 namespace {
 
@@ -122,13 +122,11 @@ template <typename T> struct End {
 enum { kForward = 0, kBackward = 1, kPlain = 2, kPartial = 3 };
 
 // ------------------------------------------------------------ float16 products
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef short s8 __attribute__((ext_vector_type(8)));
+using mmpx::f4;
+using mmpx::h8;
+using mmpx::s4;
+using mmpx::s8;
 typedef unsigned short u16;
-
-__device__ __attribute__((aligned(16))) const unsigned kZeros[4] = {0, 0, 0, 0};
 
 // Rows of this many elements: a tile's offsets would pass 32 bits of bytes.
 constexpr long long kRow = 1LL << 21;
@@ -161,11 +159,6 @@ __device__ __forceinline__ h8 fragment(const u16 *S, int first, int s, int lane)
   } else {
     return *reinterpret_cast<const h8 *>(&S[(first + fr) * 64 + ((grp + 4 * s) ^ mn_slot(fr)) * 8]);
   }
-}
-
-// 16 bytes a lane, global -> LDS: lane L's land at 16 L of `to`.
-__device__ __forceinline__ void copy16(const u16 *from, u16 *to) {
-  __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
 }
 
 // C = A B for operands whose rows are 16 byte aligned, any extents (the last
@@ -250,12 +243,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod16(Prod p, End<mmp_half
     if ((slab + 1) * BK <= p.k) {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        copy16(g + off[i], dst + i * 512);
+        mmpx::copy16(g + off[i], dst + i * 512);
     } else {  // past the last k: zeros of both operands
       const int left = p.k - slab * BK;
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        copy16(kof[i] < left ? g + off[i] : (const u16 *)kZeros, dst + i * 512);
+        mmpx::copy16(kof[i] < left ? g + off[i] : (const u16 *)mmpx::kZeros, dst + i * 512);
     }
   };
 

@@ -3,12 +3,17 @@
 //
 // A lane (fr = lane % 16, g = lane / 16) has one row of the left operand, or one
 // column of the right one, and of an accumulator tile the column fr and the rows
-// row(g, r), r < 4.  The order of a product's k is free as long as both operands
-// agree, so the k that a lane feeds is chosen to be row(g, .): then a tile of
-// accumulators is a right operand as it is, without a move between lanes.
-// Swapping the operands gives the transposed tile, in which a lane has one row
-// and the columns row(g, .).
+// row(g, r), r < 4.  Swapping the operands gives the transposed tile, in which a lane
+// has one row and the columns row(g, .).
+//
+// Accumulators become the right operand of the next product as they are, without a
+// move between lanes: the order of a product's k is free as long as both operands
+// agree, and so is which rows make up a tile.  float16 feeds 8 adjacent k a lane, so
+// two tiles together take 32 rows, of which a lane group has 8 adjacent ones, four
+// in either; spot(t, i) is row i of tile t.
 #pragma once
+#include <type_traits>
+
 #include "mmp_nn.h"
 
 namespace mmpx {
@@ -19,6 +24,59 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 
+// Where element (r, c) of rows of W elements lies in LDS: 16 byte chunks of a row
+// change places by an order that the row gives.  Reads of one chunk of 16 rows, next to
+// one another or those of a tile (below), touch every bank once, and so do float32's
+// of 16 neighbouring elements of 4 rows; float16's transposing reads take two turns.
+template <typename T, int W> struct Lay {
+  static constexpr int V = 16 / (int)sizeof(T), PER = W / V;  // elements of a chunk, chunks of a row
+  static __device__ __forceinline__ int order(int r) {
+    if constexpr (sizeof(T) == 2) {
+      const int low = (r >> 3 & 1) | ((r >> 2 ^ r >> 4) & 1) << 1;
+      if constexpr (PER >= 16) return (r & 3) << 2 | low;
+      else if constexpr (PER == 8) return (r >> 1 & 1) << 2 | low;
+      else return r >> 2 & (PER - 1);
+    } else {
+      return PER >= 16 ? r & 15 : PER == 8 ? r >> 1 & 7 : r >> 2 & (PER - 1);
+    }
+  }
+  static __device__ __forceinline__ int at(int r, int c) { return r * W + ((c / V ^ order(r)) * V) + (c & (V - 1)); }
+};
+
+// 16 bytes a lane, global -> LDS, not through registers: lane L's land at 16 L of `to`.
+__device__ __forceinline__ void copy16(const void *from, void *to) {
+  __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
+}
+static __device__ __attribute__((aligned(16))) const unsigned kZeros[4] = {0, 0, 0, 0};
+
+// A tile of ROWS rows of W elements to LDS, by WAVES waves.  Rows from `rows` on and
+// columns from `cols` on (a multiple of a chunk) are zeros; rows 16 byte
+// aligned and fewer than 2^26 elements apart.
+template <typename T, int ROWS, int W, int WAVES>
+__device__ __forceinline__ void copy_tile(const T *p, long long stride, int rows, int cols, T *lds, int wave, int lane) {
+  typedef Lay<T, W> L;
+  constexpr int ALL = ROWS * L::PER / 64;
+  static_assert(ROWS * L::PER % 64 == 0, "");
+  constexpr int STEP = 64 * WAVES / L::PER;  // rows from one of a wave's copies to its next
+  static_assert(64 * WAVES % L::PER == 0, "");
+  const int r0 = (wave * 64 + lane) / L::PER, slot = (wave * 64 + lane) % L::PER;
+  const bool whole = rows >= ROWS && cols >= W;
+  auto copy = [&](auto guarded) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i * WAVES < ALL; ++i) {
+      const int part = i * WAVES + wave;
+      if (ALL % WAVES && part >= ALL) break;
+      const int c = (slot ^ L::order(r0 + i * STEP)) * L::V;
+      const T *from = p + i * STEP * stride + ((unsigned)r0 * (unsigned)stride + (unsigned)c);
+      if constexpr (decltype(guarded)::value)
+        if (r0 + i * STEP >= rows || c >= cols) from = (const T *)kZeros;
+      copy16(from, lds + part * 64 * L::V);
+    }
+  };
+  if (whole) copy(std::false_type());
+  else copy(std::true_type());
+}
+
 template <typename T> struct Mma;
 
 // v_mfma_f32_16x16x32_f16: two tiles of accumulators make one operand.
@@ -26,27 +84,42 @@ template <> struct Mma<mmp_half> {
   typedef float A;
   typedef f4 Acc;
   typedef h8 Frag;
-  static constexpr int K = 32, E = 8, PAD = 8;
+  static constexpr int K = 32, E = 8;
   static constexpr bool SPLIT = true;
   static __device__ __forceinline__ int row(int g, int r) { return 4 * g + r; }
+  static __device__ __forceinline__ int spot(int t, int i) { return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3); }
   static __device__ __forceinline__ Acc mul(Frag a, Frag b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
-  // k along the rows of `m`: row first + fr, k from k0 on
-  static __device__ __forceinline__ Frag rows(const mmp_half *m, int ld, int first, int k0, int lane) {
-    const mmp_half *p = m + (first + (lane & 15)) * ld + k0 + 4 * (lane >> 4);
-    const s4 lo = *reinterpret_cast<const s4 *>(p), hi = *reinterpret_cast<const s4 *>(p + 16);
+  static __device__ __forceinline__ s4 transposed(const mmp_half *p) {
+    typedef __attribute__((address_space(3))) s4 L;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)p);
+  }
+  // k along the rows of `m`, W wide, from k0 on: row first + fr, or row fr of tile t
+  template <int W>
+  static __device__ __forceinline__ Frag rows(const mmp_half *m, int first, int k0, int lane) {
+    return *reinterpret_cast<const h8 *>(m + Lay<mmp_half, W>::at(first + (lane & 15), k0 + 8 * (lane >> 4)));
+  }
+  template <int W>
+  static __device__ __forceinline__ Frag tile_rows(const mmp_half *m, int t, int k0, int lane) {
+    return rows<W>(m, spot(t, lane & 15) - (lane & 15), k0, lane);
+  }
+  // k along the columns of `m`: column first + fr, or fr of tile t.  A transposing read
+  // gives element j of lane 4 a + b of a group of 16 element b of what lane a + 4 j addresses.
+  template <int W>
+  static __device__ __forceinline__ Frag four_cols(const mmp_half *m, int k0, int c, int lane) {
+    const int r = k0 + 8 * (lane >> 4) + (lane >> 2 & 3);
+    const s4 lo = transposed(m + Lay<mmp_half, W>::at(r, c));
+    const s4 hi = transposed(m + Lay<mmp_half, W>::at(r + 4, c));
     return __builtin_bit_cast(h8, (s8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   }
-  // k along the columns of `m`: column first + fr.  A transposing read gives
-  // element j of lane 4 a + b of a group of 16 element b of what lane a + 4 j addresses.
-  static __device__ __forceinline__ Frag cols(const mmp_half *m, int ld, int k0, int first, int lane) {
-    const int q = lane & 15;
-    const mmp_half *p = m + (k0 + 4 * (lane >> 4) + (q >> 2)) * ld + first + 4 * (q & 3);
-    typedef __attribute__((address_space(3))) s4 L;
-    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)p);
-    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(p + 16 * ld));
-    return __builtin_bit_cast(h8, (s8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  template <int W>
+  static __device__ __forceinline__ Frag cols(const mmp_half *m, int k0, int first, int lane) {
+    return four_cols<W>(m, k0, first + 4 * (lane & 3), lane);
+  }
+  template <int W>
+  static __device__ __forceinline__ Frag tile_cols(const mmp_half *m, int k0, int t, int lane) {
+    return four_cols<W>(m, k0, spot(t, 4 * (lane & 3)), lane);
   }
 };
 
@@ -55,20 +128,32 @@ template <> struct Mma<float> {
   typedef float A;
   typedef f4 Acc;
   typedef f4 Frag;
-  static constexpr int K = 16, E = 4, PAD = 4;
+  static constexpr int K = 16, E = 4;
   static constexpr bool SPLIT = false;
   static __device__ __forceinline__ int row(int g, int r) { return 4 * g + r; }
+  static __device__ __forceinline__ int spot(int t, int i) { return 16 * t + i; }
   static __device__ __forceinline__ Acc mul(Frag a, Frag b, Acc c) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ Frag rows(const float *m, int ld, int first, int k0, int lane) {
-    return *reinterpret_cast<const f4 *>(m + (first + (lane & 15)) * ld + k0 + 4 * (lane >> 4));
+  template <int W>
+  static __device__ __forceinline__ Frag rows(const float *m, int first, int k0, int lane) {
+    return *reinterpret_cast<const f4 *>(m + Lay<float, W>::at(first + (lane & 15), k0 + 4 * (lane >> 4)));
   }
-  static __device__ __forceinline__ Frag cols(const float *m, int ld, int k0, int first, int lane) {
-    const float *p = m + (k0 + 4 * (lane >> 4)) * ld + first + (lane & 15);
-    return Frag{p[0], p[ld], p[2 * ld], p[3 * ld]};
+  template <int W>
+  static __device__ __forceinline__ Frag cols(const float *m, int k0, int first, int lane) {
+    const int r = k0 + 4 * (lane >> 4), c = first + (lane & 15);
+    typedef Lay<float, W> L;
+    return Frag{m[L::at(r, c)], m[L::at(r + 1, c)], m[L::at(r + 2, c)], m[L::at(r + 3, c)]};
+  }
+  template <int W>
+  static __device__ __forceinline__ Frag tile_rows(const float *m, int t, int k0, int lane) {
+    return rows<W>(m, 16 * t, k0, lane);
+  }
+  template <int W>
+  static __device__ __forceinline__ Frag tile_cols(const float *m, int k0, int t, int lane) {
+    return cols<W>(m, k0, 16 * t, lane);
   }
 };
 
@@ -77,21 +162,34 @@ template <> struct Mma<double> {
   typedef double A;
   typedef d4 Acc;
   typedef d4 Frag;
-  static constexpr int K = 16, E = 4, PAD = 2;
+  static constexpr int K = 16, E = 4;
   static constexpr bool SPLIT = false;
   static __device__ __forceinline__ int row(int g, int r) { return g + 4 * r; }
+  static __device__ __forceinline__ int spot(int t, int i) { return 16 * t + i; }
   static __device__ __forceinline__ Acc mul(Frag a, Frag b, Acc c) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[t], b[t], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ Frag rows(const double *m, int ld, int first, int k0, int lane) {
-    const double *p = m + (first + (lane & 15)) * ld + k0 + (lane >> 4);
-    return Frag{p[0], p[4], p[8], p[12]};
+  template <int W>
+  static __device__ __forceinline__ Frag rows(const double *m, int first, int k0, int lane) {
+    const int r = first + (lane & 15), c = k0 + (lane >> 4);
+    typedef Lay<double, W> L;
+    return Frag{m[L::at(r, c)], m[L::at(r, c + 4)], m[L::at(r, c + 8)], m[L::at(r, c + 12)]};
   }
-  static __device__ __forceinline__ Frag cols(const double *m, int ld, int k0, int first, int lane) {
-    const double *p = m + (k0 + (lane >> 4)) * ld + first + (lane & 15);
-    return Frag{p[0], p[4 * ld], p[8 * ld], p[12 * ld]};
+  template <int W>
+  static __device__ __forceinline__ Frag cols(const double *m, int k0, int first, int lane) {
+    const int r = k0 + (lane >> 4), c = first + (lane & 15);
+    typedef Lay<double, W> L;
+    return Frag{m[L::at(r, c)], m[L::at(r + 4, c)], m[L::at(r + 8, c)], m[L::at(r + 12, c)]};
+  }
+  template <int W>
+  static __device__ __forceinline__ Frag tile_rows(const double *m, int t, int k0, int lane) {
+    return rows<W>(m, 16 * t, k0, lane);
+  }
+  template <int W>
+  static __device__ __forceinline__ Frag tile_cols(const double *m, int k0, int t, int lane) {
+    return cols<W>(m, k0, 16 * t, lane);
   }
 };
 
@@ -121,8 +219,12 @@ template <typename T> __device__ __forceinline__ Two<T> two_of(const typename Mm
   f.lo = f.hi;
   if constexpr (Mma<T>::SPLIT) {
     settle(f.hi);
+    // v - hi, exact, and its rounding in one instruction (the opaque factor keeps the
+    // compiler from making it two)
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
 #pragma unroll
-    for (int e = 0; e < Mma<T>::E; ++e) f.lo[e] = (T)(v[e] - (float)f.hi[e]);
+    for (int e = 0; e < Mma<T>::E; ++e) f.lo[e] = (T)__builtin_fmaf((float)f.hi[e], minus, v[e]);
   }
   return f;
 }
@@ -133,26 +235,6 @@ __device__ __forceinline__ Two<T> operand(const typename Mma<T>::Acc (&acc)[N], 
 #pragma unroll
   for (int e = 0; e < Mma<T>::E; ++e) v[e] = acc[first + (e >> 2)][e & 3];
   return two_of<T>(v);
-}
-// a (b.hi + b.lo) and (a.hi + a.lo)(b.hi + b.lo) but for a.lo b.lo.
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Acc mul_two(typename Mma<T>::Frag a, const Two<T> &b, typename Mma<T>::Acc c) {
-  if constexpr (Mma<T>::SPLIT) c = Mma<T>::mul(a, b.lo, c);
-  return Mma<T>::mul(a, b.hi, c);
-}
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Acc mul_twos(const Two<T> &a, const Two<T> &b, typename Mma<T>::Acc c) {
-  if constexpr (Mma<T>::SPLIT) {
-    c = Mma<T>::mul(a.lo, b.hi, c);
-    c = Mma<T>::mul(a.hi, b.lo, c);
-  }
-  return Mma<T>::mul(a.hi, b.hi, c);
-}
-// The transposed product's.
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Acc two_mul(const Two<T> &a, typename Mma<T>::Frag b, typename Mma<T>::Acc c) {
-  if constexpr (Mma<T>::SPLIT) c = Mma<T>::mul(a.lo, b, c);
-  return Mma<T>::mul(a.hi, b, c);
 }
 
 }  // namespace mmpx
