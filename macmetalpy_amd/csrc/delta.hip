@@ -152,38 +152,58 @@ __device__ __forceinline__ void copy_vecs(const Delta<T> &p, long long chunk, ty
   mmpx::copy16((const char *)(p.vecs + chunk * 3 * chunk_of<T>()) + 16 * lane, to);
 }
 
+// k from k0 on of row i of an array in memory, as Mma::rows gives them of LDS; zeros
+// beyond its rows and columns.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag row_of(const T *p, long long stride, int i, int rows, int k0, int cols, int g) {
+  constexpr int E = Mma<T>::E;
+  const T *at = p + i * stride;
+  typename Mma<T>::Frag f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = (T)0;
+  if (i >= rows) return f;
+  if constexpr (sizeof(T) == 8) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (k0 + g + 4 * e < cols) f[e] = at[k0 + g + 4 * e];
+  } else {
+    const int c = k0 + E * g;
+    if (c + E <= cols) return __builtin_bit_cast(typename Mma<T>::Frag, mmpn::words_of(mmpn::load_vec<T, E>(at + c)));
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (c + e < cols) f[e] = at[c + e];
+  }
+  return f;
+}
+
 // ------------------------------------------------------------- within chunks
 // Workgroup: a chunk of a head.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
+__global__ __launch_bounds__(256, DK <= 128 ? 4 : 2) void k_delta_within(Delta<T> p) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
   typedef Mma<A> MA;
   typedef typename M::Acc Acc;
   typedef typename MA::Acc AccA;
   constexpr int C = chunk_of<T>(), NT = C / 16;
-  constexpr int KEYS = 2 * C * DK * sizeof(T), INV = C * C * sizeof(A);
+  constexpr int KEYS = C * DK * sizeof(T), INV = C * C * sizeof(A);
   __shared__ __attribute__((aligned(16))) char mem[KEYS > INV ? KEYS : INV];
-  T *Ks = (T *)mem, *Qs = Ks + C * DK;
+  T *Ks = (T *)mem;
   A *Ts = (A *)mem;  // when the keys are done with
   __shared__ __attribute__((aligned(16))) A As[C * C], Td[C * 16];
   __shared__ double G[C];
   __shared__ int R[C];
   __shared__ A bet[C];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
-  const long long id = blockIdx.x, bh = id / p.chunks;
+  const long long id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x), bh = id / p.chunks;
   const int n = (int)(id - bh * p.chunks), b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
   const long long t0 = (long long)n * C;
   const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
   T *out = p.within + id * (2 * parts_of<T>() * C * C);
 
-  {
-    Tile<T, C, DK, 256> k, q;
-    k.fetch(p.k.at(b, t0, h / p.group), p.k.st, left, p.dk, tid);
-    q.fetch(p.q.at(b, t0, h / p.group), p.q.st, left, p.dk, tid);
-    k.put(Ks, tid);
-    q.put(Qs, tid);
-  }
+  const T *query_rows = p.q.at(b, t0, h / p.group);
+  Tile<T, C, DK, 256> keys;
+  keys.fetch(p.k.at(b, t0, h / p.group), p.k.st, left, p.dk, tid);
   if (wave == 0) {  // logarithms summed up, fresh starts counted
     double sum;
     int count;
@@ -202,22 +222,26 @@ __global__ __launch_bounds__(256) void k_delta_within(Delta<T> p) {
       v[2 * C + lane] = beta;
     }
   }
+  keys.put(Ks, tid);
   __syncthreads();
 
   // tiles of K K^T to A and of Q K^T to P, transposed: a lane has row fr of a tile
   for (int task = wave; task < 2 * NT; task += 4) {
     const bool query = task >= NT;
     const int rt = query ? 2 * NT - 1 - task : task, i = 16 * rt + fr;
-    const T *X = query ? Qs : Ks;
     const double Gi = G[i];
     const int Ri = R[i];
     const A by = query ? p.scale : bet[i];
+    // a wave alone needs its 16 queries: from memory as they are
+    typename M::Frag x[DK / M::K];
+#pragma unroll
+    for (int ks = 0; ks < DK / M::K; ++ks)
+      x[ks] = query ? row_of<T>(query_rows, p.q.st, i, left, ks * M::K, p.dk, g) : M::template rows<DK>(Ks, 16 * rt, ks * M::K, lane);
     for (int jt = 0; jt < NT; ++jt) {
       Acc acc{};
       if (jt <= rt)
 #pragma unroll
-        for (int ks = 0; ks < DK; ks += M::K)
-          acc = M::mul(M::template rows<DK>(Ks, 16 * jt, ks, lane), M::template rows<DK>(X, 16 * rt, ks, lane), acc);
+        for (int ks = 0; ks < DK / M::K; ++ks) acc = M::mul(M::template rows<DK>(Ks, 16 * jt, ks * M::K, lane), x[ks], acc);
       A v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -424,9 +448,10 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e
   __shared__ Stage one;
   __shared__ typename std::conditional<AHEAD, Stage, char>::type two;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, g = lane >> 4;
-  const long long bh = blockIdx.x / e.tiles;
+  const unsigned id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x);
+  const long long bh = id / e.tiles;
   const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
-  const int n0 = (int)(blockIdx.x - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;  // of the state
+  const int n0 = (int)(id - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;  // of the state
   const bool there = col < p.dv;
   const int kh = h / p.group;
 
@@ -795,9 +820,10 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
   __shared__ Stage one;
   __shared__ typename std::conditional<AHEAD, Stage, char>::type two;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, g = lane >> 4;
-  const long long bh = blockIdx.x / e.tiles;
+  const unsigned id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x);
+  const long long bh = id / e.tiles;
   const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
-  const int n0 = (int)(blockIdx.x - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;
+  const int n0 = (int)(id - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;
   const bool there = col < p.dv;
   const int kh = h / p.group;
 
@@ -980,7 +1006,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
   __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][4][16], rv[C], ek[C], sd[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
   const int shared = p.group ? p.heads / p.group : e.tiles;  // key heads
-  const long long id = blockIdx.x, bk = id / p.chunks;
+  const long long id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x), bk = id / p.chunks;
   const int n = (int)(id - bk * p.chunks), b = (int)(bk / shared), kh = (int)(bk - (long long)b * shared);
   const long long t0 = (long long)n * C;
   const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);

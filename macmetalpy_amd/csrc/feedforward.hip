@@ -188,11 +188,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod16(Prod p, End<mmp_half
   const int wm = wave / WN, wn = wave % WN;
 
   const int blocks = p.tiles_m * p.tiles_n;
-  int b = blockIdx.x;
-  {
-    const int xcd = b & 7, q = blocks >> 3, r = blocks & 7;
-    b = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
-  }
+  const int b = (int)mmpx::adjacent_on_xcd(blockIdx.x, blocks);
   constexpr int GM = 4;
   const int first = b / (GM * p.tiles_n) * GM, gm = min(p.tiles_m - first, GM);
   const int rem = b - first * p.tiles_n;

@@ -24,6 +24,13 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 
+// Workgroup ids go round the eight XCDs, each with a cache of its own: the place that
+// gives each XCD a run of adjacent ones.
+__device__ __forceinline__ unsigned adjacent_on_xcd(unsigned id, unsigned all) {
+  const unsigned xcd = id & 7, q = all >> 3, r = all & 7;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
+}
+
 // Where element (r, c) of rows of W elements lies in LDS: 16 byte chunks of a row
 // change places by an order that the row gives.  Reads of one chunk of 16 rows, next to
 // one another or those of a tile (below), touch every bank once, and so do float32's
