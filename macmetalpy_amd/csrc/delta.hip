@@ -989,42 +989,65 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
       }
 }
 
-// Workgroup: a chunk of a key head, for the heads that share it one after another.
-template <typename T, int DK>
-__global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
+// Where LDS addresses are worked out again: kept from one part of a kernel to the
+// next, and from round to round, they take more registers than there are.
+__device__ __forceinline__ void again(int &lane) { asm volatile("" : "+v"(lane)); }
+
+// Channels of values that k_delta_grads takes at a time, as LDS has room for.
+template <typename T, int DK> constexpr int kBlockOf = sizeof(T) == 2 ? (DK <= 128 ? 128 : 64) : sizeof(T) == 4 ? 32 : 16;
+
+// Workgroup: a chunk of a key head, for the heads that share it one after another;
+// eight waves.  dO, U and dR of a block of the values' channels are in LDS, the states
+// go by in blocks of key channels, the next on its way while one is worked on.
+template <typename T, int DK, bool ALIGNED>
+__global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
   typedef typename M::Acc Acc;
-  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, V = vec_of<T>();
-  constexpr int VB = 32, KB = 64;  // channels of values and of keys at a time
-  constexpr int TASKS = (2 * NT + 3) / 4;
-  static_assert(C * (VB / V) == 256, "a vector of the chunk's values for each thread");
-  __shared__ __attribute__((aligned(16))) T Ks[C * DK], Qs[C * DK], Fs[C * C], Es[C * C], Os[C * VB],
-      Us[VB * C], Rs[VB * C], Ss[VB * KB], Ds[VB * KB];
+  typedef typename M::Frag Frag;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, V = vec_of<T>(), NC = NT / PT;
+  constexpr int VB = kBlockOf<T, DK>, KB = DK < 128 / NT ? DK : 128 / NT, NK = DK / KB, NF = VB / M::K;
+  struct __attribute__((aligned(16))) States {
+    T s[VB * KB], d[VB * KB];
+  };
+  __shared__ __attribute__((aligned(16))) T Ks[C * DK], Qs[C * DK], Fs[C * C], Es[C * C], Os[C * VB], Us[VB * C], Rs[VB * C];
+  __shared__ States states[2];
   __shared__ double G[C];
   __shared__ int R[C];
-  __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][4][16], rv[C], ek[C], sd[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][8][16], rv[C], ek[C], sd[8];
+  const int tid = threadIdx.x;
+  int lane = tid & 63;
+  const int fr = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int shared = p.group ? p.heads / p.group : e.tiles;  // key heads
   const long long id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x), bk = id / p.chunks;
   const int n = (int)(id - bk * p.chunks), b = (int)(bk / shared), kh = (int)(bk - (long long)b * shared);
   const long long t0 = (long long)n * C;
   const int left = (int)(p.steps - t0 < C ? p.steps - t0 : C);
 
-  {
-    Tile<T, C, DK, 256> k, q;
-    k.fetch(p.k.at(b, t0, kh), p.k.st, left, p.dk, tid);
-    q.fetch(p.q.at(b, t0, kh), p.q.st, left, p.dk, tid);
-    k.put(Ks, tid);
-    q.put(Qs, tid);
-  }
-  // dQ and dK, transposed: a wave has rows 16 rt and NT tiles of columns from ct on of each 64
-  const int rt = wave % NT, ct = wave / NT * NT;
-  Acc dq[DK / KB][NT], dk[DK / KB][NT];
+  // an array of a caller's, whose rows may be of any kind
+  auto theirs = [&](T *lds, const T *from, long long stride, int cols_left, auto width) __attribute__((always_inline)) {
+    constexpr int W = decltype(width)::value;
+    if constexpr (ALIGNED) {
+      mmpx::copy_tile<T, C, W, 8>(from, stride, left, cols_left, lds, wave, lane);
+    } else {
+      Tile<T, C, W, 512> tile;
+      tile.fetch(from, stride, left, cols_left, tid);
+      tile.put(lds, tid);
+    }
+  };
+  theirs(Ks, p.k.at(b, t0, kh), p.k.st, p.dk, std::integral_constant<int, DK>());
+  theirs(Qs, p.q.at(b, t0, kh), p.q.st, p.dk, std::integral_constant<int, DK>());
+
+  // A wave has a tile (16 rows rt, 16 columns ct) of each block of dQ and dK, transposed.
+  const int rt = wave % NT, ct = wave / NT;
+  const bool active = ct < KB / 16;
+  Acc dq[NK], dk[NK];
 #pragma unroll
-  for (int kb = 0; kb < DK / KB; ++kb)
-#pragma unroll
-    for (int c = 0; c < NT; ++c) dq[kb][c] = dk[kb][c] = Acc{};
+  for (int kb = 0; kb < NK; ++kb) dq[kb] = dk[kb] = Acc{};
+  const bool query = wave >= NT;  // of the products dO U^T, or dR U^T
+  const int row = query ? 2 * NT - 1 - wave : wave;
+  const bool task = wave < 2 * NT;
 
   for (int head = 0; head < p.group; ++head) {
     const int h = kh * p.group + head;
@@ -1041,80 +1064,110 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         cs[lane] = p.vecs[at * 3 * C + lane];
         es[lane] = p.vecs[at * 3 * C + C + lane];
         bet[lane] = p.vecs[at * 3 * C + 2 * C + lane];
+        rv[lane] = 0;
       }
     }
-    // dO U^T and dR U^T, transposed; dV and dR.V on the way
-    Acc w[TASKS][NT];
+    Acc w[NT], a[NK], z[NK], y[NK];
 #pragma unroll
-    for (int k = 0; k < TASKS; ++k)
+    for (int j = 0; j < NT; ++j) w[j] = Acc{};
 #pragma unroll
-      for (int j = 0; j < NT; ++j) w[k][j] = Acc{};
-    A with_v = 0;
-    Tile<T, C, VB, 256> o;
-    Tile<T, VB, C, 256> u, r;
-    const int vi = tid / (VB / V), vn = tid % (VB / V) * V;  // this thread's step and channels
+    for (int kb = 0; kb < NK; ++kb) a[kb] = z[kb] = y[kb] = Acc{};
+    A s_d = 0;
     for (int v0 = 0; v0 < p.dv; v0 += VB) {
-      o.fetch(e.grad.at(b, t0, h) + v0, e.grad.st, left, p.dv - v0, tid);
-      u.fetch(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
-      r.fetch(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
+      auto copy_states = [&](int kb) __attribute__((always_inline)) {
+        mmpx::copy_tile<T, VB, KB, 8>(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, states[kb & 1].s, wave, lane);
+        mmpx::copy_tile<T, VB, KB, 8>(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, states[kb & 1].d, wave, lane);
+      };
+      again(lane);
       if (v0) __syncthreads();
-      o.put(Os, tid);
-      u.put(Us, tid);
-      r.put(Rs, tid);
+      theirs(Os, e.grad.at(b, t0, h) + v0, e.grad.st, p.dv - v0, std::integral_constant<int, VB>());
+      mmpx::copy_tile<T, VB, C, 8>(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, Us, wave, lane);
+      mmpx::copy_tile<T, VB, C, 8>(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, Rs, wave, lane);
+      copy_states(0);
       __syncthreads();
-      if (vi < left) {
-        const A beta = bet[vi];
-        const T *v = p.v.at(b, t0 + vi, h) + v0 + vn;
-        T *to = e.grad_v + (((long long)b * p.steps + t0 + vi) * p.heads + h) * p.dv + v0 + vn;
-        const int cols_left = p.dv - v0 - vn;
-        Vec<T, V> x{}, y;
-        if (cols_left >= V) {
-          x = mmpn::load_vec<T, V>(v);
-        } else {
+      // dV and dR.V: a vector of a step's channels a thread
+      for (int vec = tid; vec < C * VB / V; vec += 512) {
+        const int i = vec / (VB / V), c = vec % (VB / V) * V, have = p.dv - v0 - c;
+        A with_v = 0;
+        if (i < left) {
+          const A beta = bet[i];
+          const T *v = p.v.at(b, t0 + i, h) + v0 + c;
+          T *to = e.grad_v + (((long long)b * p.steps + t0 + i) * p.heads + h) * p.dv + v0 + c;
+          Vec<T, V> x{}, o;
+          if (have >= V) {
+            x = mmpn::load_vec<T, V>(v);
+          } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (i < cols_left) x.e[i] = v[i];
+            for (int l = 0; l < V; ++l)
+              if (l < have) x.e[l] = v[l];
+          }
+#pragma unroll
+          for (int l = 0; l < V; ++l) {
+            const A d = (A)Rs[Lay<T, C>::at(c + l, i)];
+            with_v = mmpn::fma_of(d, (A)x.e[l], with_v);
+            o.e[l] = (T)(beta * d);
+          }
+          if (have >= V) {
+            mmpn::store_vec(to, o);
+          } else {
+#pragma unroll
+            for (int l = 0; l < V; ++l)
+              if (l < have) to[l] = o.e[l];
+          }
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const A d = (A)Rs[Lay<T, C>::at(vn + i, vi)];
-          with_v = mmpn::fma_of(d, (A)x.e[i], with_v);
-          y.e[i] = (T)(beta * d);
-        }
-        if (cols_left >= V) {
-          mmpn::store_vec(to, y);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (i < cols_left) to[i] = y.e[i];
-        }
+        for (int d = 1; d < VB / V; d *= 2) with_v += __shfl_xor(with_v, d);
+        if (c == 0) rv[i] += with_v;
       }
+      // dO U^T and dR U^T, transposed
+      again(lane);
+      if (task)
 #pragma unroll
-      for (int k = 0; k < TASKS; ++k) {
-        const int task = wave + 4 * k;
-        if (task >= 2 * NT) continue;
-        const bool query = task >= NT;
-        const int row = query ? 2 * NT - 1 - task : task;
-#pragma unroll
-        for (int d = 0; d < VB; d += M::K) {
-          const typename M::Frag x = query ? M::template rows<VB>(Os, 16 * row, d, lane) : M::template cols<C>(Rs, d, 16 * row, lane);
+        for (int d = 0; d < NF; ++d) {
+          const Frag x = query ? M::template rows<VB>(Os, 16 * row, d * M::K, lane) : M::template cols<C>(Rs, d * M::K, 16 * row, lane);
 #pragma unroll
           for (int j = 0; j < NT; ++j)
-            if (j <= row) w[k][j] = M::mul(M::template cols<C>(Us, d, 16 * j, lane), x, w[k][j]);
+            if (j <= row) w[j] = M::mul(M::template cols<C>(Us, d * M::K, 16 * j, lane), x, w[j]);
         }
+      // the products with the states
+      again(lane);
+      Frag fo[NF], fd[NF], fu[NF];
+#pragma unroll
+      for (int d = 0; d < NF; ++d) {
+        fo[d] = M::template rows<VB>(Os, 16 * rt, d * M::K, lane);
+        fd[d] = M::template cols<C>(Rs, d * M::K, 16 * rt, lane);
+        fu[d] = M::template cols<C>(Us, d * M::K, 16 * rt, lane);
+      }
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb) {
+        if (kb) __syncthreads();
+        Frag s[NF], ds[NF];
+        if (active)
+#pragma unroll
+          for (int d = 0; d < NF; ++d) {
+            s[d] = M::template cols<KB>(states[kb & 1].s, d * M::K, 16 * ct, lane);
+            ds[d] = M::template cols<KB>(states[kb & 1].d, d * M::K, 16 * ct, lane);
+          }
+        asm volatile("" ::: "memory");  // reads first: copies under way would be waited for
+        if (kb + 1 < NK) copy_states(kb + 1);
+        if (active)
+#pragma unroll
+          for (int d = 0; d < NF; ++d) {
+            a[kb] = M::mul(s[d], fo[d], a[kb]);
+            z[kb] = M::mul(s[d], fd[d], z[kb]);
+            y[kb] = M::mul(ds[d], fu[d], y[kb]);
+            if (rt == 0)
+#pragma unroll
+              for (int l = 0; l < M::E; ++l) s_d = mmpn::fma_of((A)s[d][l], (A)ds[d][l], s_d);
+          }
       }
     }
     if (p.dv == 0) __syncthreads();
-#pragma unroll
-    for (int d = 1; d < VB / V; d *= 2) with_v += __shfl_xor(with_v, d);
-    if (tid % (VB / V) == 0) rv[vi] = with_v;
+    again(lane);
+
     // F and beta E, and their products with Q K^T and K K^T summed up by rows and columns
-#pragma unroll
-    for (int k = 0; k < TASKS; ++k) {
-      const int task = wave + 4 * k;
-      if (task >= 2 * NT) continue;
-      const bool query = task >= NT;
-      const int row = query ? 2 * NT - 1 - task : task, i = 16 * row + fr;
+    if (task) {
+      const int i = 16 * row + fr;
       const T *X = query ? Qs : Ks;
       T *to = query ? Fs : Es;
       const double Gi = G[i];
@@ -1132,7 +1185,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         for (int c = 0; c < 4; ++c) {
           const int jj = 16 * j + M::row(g, c);
           const bool in = (query ? jj <= i : jj < i) && R[jj] == Ri;
-          const A f = in ? (query ? w[k][j][c] : -w[k][j][c]) * exp_any((A)(Gi - G[jj])) : (A)0;
+          const A f = in ? (query ? w[j][c] : -w[j][c]) * exp_any((A)(Gi - G[jj])) : (A)0;
           to[Lay<T, C>::at(i, jj)] = (T)(f * by);
           const A m = in ? f * x[c] : (A)0;
           sum_e += m;
@@ -1156,74 +1209,46 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
         if (!query) ek[i] = sum_e;
       }
     }
+    __syncthreads();
 
-    // with the states: a 64 wide block of key channels at a time
-    const int i = 16 * rt + fr;
-    A q_s = 0, k_z = 0, k_d = 0, s_d = 0;
-    Tile<T, VB, KB, 256> st, dt;
-#pragma unroll
-    for (int kb = 0; kb < DK / KB; ++kb) {
-      Acc a[NT], z[NT], y[NT];
-#pragma unroll
-      for (int c = 0; c < NT; ++c) a[c] = z[c] = y[c] = Acc{};
-      for (int v0 = 0; v0 < p.dv; v0 += VB) {
-        o.fetch(e.grad.at(b, t0, h) + v0, e.grad.st, left, p.dv - v0, tid);
-        u.fetch(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
-        r.fetch(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, tid);
-        st.fetch(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, tid);
-        dt.fetch(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, tid);
-        __syncthreads();
-        o.put(Os, tid);
-        u.put(Us, tid);
-        r.put(Rs, tid);
-        st.put(Ss, tid);
-        dt.put(Ds, tid);
-#pragma unroll
-        for (int c = 0; c < st.N; ++c) {
-          const Vec<T, V> x = mmpn::elements_of<T, V>(st.w[c]), x2 = mmpn::elements_of<T, V>(dt.w[c]);
-#pragma unroll
-          for (int l = 0; l < V; ++l) s_d = mmpn::fma_of((A)x.e[l], (A)x2.e[l], s_d);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int d = 0; d < VB; d += M::K) {
-          const typename M::Frag fo = M::template rows<VB>(Os, 16 * rt, d, lane), fr_ = M::template cols<C>(Rs, d, 16 * rt, lane),
-                                 fu = M::template cols<C>(Us, d, 16 * rt, lane);
-#pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            const typename M::Frag fs = M::template cols<KB>(Ss, d, 16 * (ct + c), lane), fd = M::template cols<KB>(Ds, d, 16 * (ct + c), lane);
-            a[c] = M::mul(fs, fo, a[c]);
-            z[c] = M::mul(fs, fr_, z[c]);
-            y[c] = M::mul(fd, fu, y[c]);
-          }
-        }
-      }
-      if (p.dv == 0) __syncthreads();  // F and E are there
+    // dQ, dK and their products with Q and K that the gates get
+    again(lane);
+    A q_s = 0, k_z = 0, k_d = 0;
+    if (active) {
+      const int i = 16 * rt + fr;
       const A sc = p.scale * cs[i], cz = -cs[i], ce = es[i], beta = bet[i];
+      Frag fr_[NC], fc[NC], er[NC], ec[NC];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const int d0 = kb * KB + 16 * (ct + c);
+      for (int j = 0; j < NC; ++j) {
+        fr_[j] = M::template rows<C>(Fs, 16 * rt, j * M::K, lane);
+        er[j] = M::template rows<C>(Es, 16 * rt, j * M::K, lane);
+        fc[j] = M::template cols<C>(Fs, j * M::K, 16 * rt, lane);
+        ec[j] = M::template cols<C>(Es, j * M::K, 16 * rt, lane);
+      }
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb) {
+        const int d0 = kb * KB + 16 * ct;
 #pragma unroll
         for (int l = 0; l < 4; ++l) {
           const int d = d0 + M::row(g, l);
           const A qv = (A)Qs[Lay<T, DK>::at(i, d)], kv = (A)Ks[Lay<T, DK>::at(i, d)];
-          const A av = sc * a[c][l], zv = cz * z[c][l], yv = ce * y[c][l];
+          const A av = sc * a[kb][l], zv = cz * z[kb][l], yv = ce * y[kb][l];
           q_s = mmpn::fma_of(qv, av, q_s);
           k_z = mmpn::fma_of(kv, zv, k_z);
           k_d = mmpn::fma_of(kv, yv, k_d);
-          dq[kb][c][l] += av;
-          dk[kb][c][l] += beta * zv + yv;
+          dq[kb][l] += av;
+          dk[kb][l] += beta * zv + yv;
         }
 #pragma unroll
-        for (int j = 0; j < NT / PT; ++j) {
-          const typename M::Frag kc = M::template cols<DK>(Ks, j * M::K, d0, lane), qc = M::template cols<DK>(Qs, j * M::K, d0, lane);
+        for (int j = 0; j < NC; ++j) {
+          const Frag kc = M::template cols<DK>(Ks, j * M::K, d0, lane);
           if (j <= rt / PT) {
-            dq[kb][c] = M::mul(kc, M::template rows<C>(Fs, 16 * rt, j * M::K, lane), dq[kb][c]);
-            dk[kb][c] = M::mul(kc, M::template rows<C>(Es, 16 * rt, j * M::K, lane), dk[kb][c]);
+            dq[kb] = M::mul(kc, fr_[j], dq[kb]);
+            dk[kb] = M::mul(kc, er[j], dk[kb]);
           }
           if (j >= rt / PT) {
-            dk[kb][c] = M::mul(kc, M::template cols<C>(Es, j * M::K, 16 * rt, lane), dk[kb][c]);
-            dk[kb][c] = M::mul(qc, M::template cols<C>(Fs, j * M::K, 16 * rt, lane), dk[kb][c]);
+            dk[kb] = M::mul(kc, ec[j], dk[kb]);
+            dk[kb] = M::mul(M::template cols<DK>(Qs, j * M::K, d0, lane), fc[j], dk[kb]);
           }
         }
       }
@@ -1244,19 +1269,20 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
     if (lane == 0) sd[wave] = s_d;
     __syncthreads();
     if (wave == 0) {
-      double dG = 0, w_i = 0;
+      double dG = 0, w_i = 0, qs_i = 0, kz_i = 0, sd_all = 0;
       A dbeta = 0;
       const int l = lane < C ? lane : 0;
-      double qs_i = 0, kz_i = 0;
 #pragma unroll
-      for (int part = 0; part < 4 / NT; ++part) {  // the waves that share rows
+      for (int part = 0; part < 8 / NT; ++part) {  // the waves that share rows
         qs_i += dots[0][part * NT + l / 16][l % 16];
         kz_i += dots[1][part * NT + l / 16][l % 16];
         w_i += dots[2][part * NT + l / 16][l % 16];
       }
+#pragma unroll
+      for (int part = 0; part < 8; ++part) sd_all += sd[part];
       if (lane < C) {
         dG = qs_i + (double)bet[l] * kz_i - w_i + rows[0][l] + rows[1][l];
-        for (int row = l / 16; row < NT; ++row) dG -= (double)cols[0][row][l] + (double)cols[1][row][l];
+        for (int r = l / 16; r < NT; ++r) dG -= (double)cols[0][r][l] + (double)cols[1][r][l];
         dbeta = (A)(rv[l] + kz_i + ek[l]);
       } else {
         w_i = 0;
@@ -1264,7 +1290,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
       double all = w_i;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-      if (lane == C - 1) dG += all + (double)cs[C - 1] * ((double)sd[0] + sd[1] + sd[2] + sd[3]);
+      if (lane == C - 1) dG += all + (double)cs[C - 1] * sd_all;
 #pragma unroll
       for (int d = 1; d < C; d *= 2) {  // the sum from this step on
         const double down = __shfl_down(dG, d);
@@ -1280,28 +1306,27 @@ __global__ __launch_bounds__(256, 1) void k_delta_grads(Delta<T> p, Back<T> e) {
       }
     }
   }
+  if (p.group == 0) __syncthreads();  // no copy into LDS may be in flight when the workgroup ends
   const int i = 16 * rt + fr;
-  if (i < left)
+  if (active && i < left)
 #pragma unroll
-    for (int kb = 0; kb < DK / KB; ++kb)
+    for (int kb = 0; kb < NK; ++kb) {
+      const int d0 = kb * KB + 16 * ct;
+      const long long to = (((long long)b * p.steps + t0 + i) * shared + kh) * p.dk + d0;
+      if (d0 + 16 <= p.dk) {
+        const A x[4] = {dq[kb][0], dq[kb][1], dq[kb][2], dq[kb][3]};
+        const A u[4] = {dk[kb][0], dk[kb][1], dk[kb][2], dk[kb][3]};
+        put4<T>(e.grad_q + to, x, g);
+        put4<T>(e.grad_k + to, u, g);
+      } else {
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const int d0 = kb * KB + 16 * (ct + c);
-        const long long to = (((long long)b * p.steps + t0 + i) * shared + kh) * p.dk + d0;
-        if (d0 + 16 <= p.dk) {
-          const A x[4] = {dq[kb][c][0], dq[kb][c][1], dq[kb][c][2], dq[kb][c][3]};
-          const A y[4] = {dk[kb][c][0], dk[kb][c][1], dk[kb][c][2], dk[kb][c][3]};
-          put4<T>(e.grad_q + to, x, g);
-          put4<T>(e.grad_k + to, y, g);
-        } else {
-#pragma unroll
-          for (int l = 0; l < 4; ++l)
-            if (d0 + M::row(g, l) < p.dk) {
-              e.grad_q[to + M::row(g, l)] = (T)dq[kb][c][l];
-              e.grad_k[to + M::row(g, l)] = (T)dk[kb][c][l];
-            }
-        }
+        for (int l = 0; l < 4; ++l)
+          if (d0 + M::row(g, l) < p.dk) {
+            e.grad_q[to + M::row(g, l)] = (T)dq[kb][l];
+            e.grad_k[to + M::row(g, l)] = (T)dk[kb][l];
+          }
       }
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -1414,9 +1439,11 @@ template <typename T> int backward(Delta<T> p, Back<T> e, int key_heads, const t
   p.chunks = (int)((p.steps + C - 1) / C);
   e.tiles = key_heads;
   const int64_t all = (int64_t)p.batch * key_heads * p.chunks;
-  if (!mmpi::grid_fits(all, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many steps", what);
+  if (!mmpi::grid_fits(all, 512)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many steps", what);
   return with_width(p.dk, [&](auto dk) {
-    hipLaunchKernelGGL((k_delta_grads<T, dk.value>), dim3((unsigned)all), dim3(256), 0, mmpi::stream(), p, e);
+    constexpr int DK = decltype(dk)::value;
+    if (copies(p, e.grad)) hipLaunchKernelGGL((k_delta_grads<T, DK, true>), dim3((unsigned)all), dim3(512), 0, mmpi::stream(), p, e);
+    else hipLaunchKernelGGL((k_delta_grads<T, DK, false>), dim3((unsigned)all), dim3(512), 0, mmpi::stream(), p, e);
     return mmpi::check_launch(what);
   });
 }
