@@ -997,8 +997,8 @@ __device__ __forceinline__ void again(int &lane) { asm volatile("" : "+v"(lane))
 template <typename T, int DK> constexpr int kBlockOf = sizeof(T) == 2 ? (DK <= 128 ? 128 : 64) : sizeof(T) == 4 ? 32 : 16;
 
 // Workgroup: a chunk of a key head, for the heads that share it one after another;
-// eight waves.  dO, U and dR of a block of the values' channels are in LDS, the states
-// go by in blocks of key channels, the next on its way while one is worked on.
+// eight waves.  All that a block of the values' channels has goes to LDS at once,
+// one wait for 112 KiB (dO, U, dR and both states of 128 x 128 float16).
 template <typename T, int DK, bool ALIGNED>
 __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
   typedef typename Wide<T>::type A;
@@ -1007,11 +1007,10 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
   typedef typename M::Frag Frag;
   constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, V = vec_of<T>(), NC = NT / PT;
   constexpr int VB = kBlockOf<T, DK>, KB = DK < 128 / NT ? DK : 128 / NT, NK = DK / KB, NF = VB / M::K;
-  struct __attribute__((aligned(16))) States {
-    T s[VB * KB], d[VB * KB];
-  };
-  __shared__ __attribute__((aligned(16))) T Ks[C * DK], Qs[C * DK], Fs[C * C], Es[C * C], Os[C * VB], Us[VB * C], Rs[VB * C];
-  __shared__ States states[2];
+  __shared__ __attribute__((aligned(16))) T Ks[C * DK], Qs[C * DK], mem[3 * C * VB], Ss[NK][VB * KB], Ds[NK][VB * KB];
+  T *Os = mem, *Us = Os + C * VB, *Rs = Us + C * VB;
+  static_assert(3 * VB >= 2 * C, "");
+  T *Fs = mem, *Es = Fs + C * C;  // when those are done with
   __shared__ double G[C];
   __shared__ int R[C];
   __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][8][16], rv[C], ek[C], sd[8];
@@ -1074,37 +1073,48 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
     for (int kb = 0; kb < NK; ++kb) a[kb] = z[kb] = y[kb] = Acc{};
     A s_d = 0;
     for (int v0 = 0; v0 < p.dv; v0 += VB) {
-      auto copy_states = [&](int kb) __attribute__((always_inline)) {
-        mmpx::copy_tile<T, VB, KB, 8>(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, states[kb & 1].s, wave, lane);
-        mmpx::copy_tile<T, VB, KB, 8>(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, states[kb & 1].d, wave, lane);
-      };
       again(lane);
       if (v0) __syncthreads();
       theirs(Os, e.grad.at(b, t0, h) + v0, e.grad.st, p.dv - v0, std::integral_constant<int, VB>());
       mmpx::copy_tile<T, VB, C, 8>(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, Us, wave, lane);
       mmpx::copy_tile<T, VB, C, 8>(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, Rs, wave, lane);
-      copy_states(0);
-      __syncthreads();
-      // dV and dR.V: a vector of a step's channels a thread
-      for (int vec = tid; vec < C * VB / V; vec += 512) {
-        const int i = vec / (VB / V), c = vec % (VB / V) * V, have = p.dv - v0 - c;
-        A with_v = 0;
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb) {
+        mmpx::copy_tile<T, VB, KB, 8>(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, Ss[kb], wave, lane);
+        mmpx::copy_tile<T, VB, KB, 8>(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, Ds[kb], wave, lane);
+      }
+      // the values meanwhile, a vector of a step's channels a thread
+      constexpr int NV = (C * VB / V + 511) / 512;
+      Vec<T, V> value[NV];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int vec = tid + 512 * k, i = vec / (VB / V), c = vec % (VB / V) * V, have = p.dv - v0 - c;
+        value[k] = Vec<T, V>{};
         if (i < left) {
-          const A beta = bet[i];
           const T *v = p.v.at(b, t0 + i, h) + v0 + c;
-          T *to = e.grad_v + (((long long)b * p.steps + t0 + i) * p.heads + h) * p.dv + v0 + c;
-          Vec<T, V> x{}, o;
           if (have >= V) {
-            x = mmpn::load_vec<T, V>(v);
+            value[k] = mmpn::load_vec<T, V>(v);
           } else {
 #pragma unroll
             for (int l = 0; l < V; ++l)
-              if (l < have) x.e[l] = v[l];
+              if (l < have) value[k].e[l] = v[l];
           }
+        }
+      }
+      __syncthreads();
+      // dV and dR.V
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int vec = tid + 512 * k, i = vec / (VB / V), c = vec % (VB / V) * V, have = p.dv - v0 - c;
+        A with_v = 0;
+        if (i < left) {
+          const A beta = bet[i];
+          T *to = e.grad_v + (((long long)b * p.steps + t0 + i) * p.heads + h) * p.dv + v0 + c;
+          Vec<T, V> o;
 #pragma unroll
           for (int l = 0; l < V; ++l) {
             const A d = (A)Rs[Lay<T, C>::at(c + l, i)];
-            with_v = mmpn::fma_of(d, (A)x.e[l], with_v);
+            with_v = mmpn::fma_of(d, (A)value[k].e[l], with_v);
             o.e[l] = (T)(beta * d);
           }
           if (have >= V) {
@@ -1117,7 +1127,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
         }
 #pragma unroll
         for (int d = 1; d < VB / V; d *= 2) with_v += __shfl_xor(with_v, d);
-        if (c == 0) rv[i] += with_v;
+        if (c == 0 && i < C) rv[i] += with_v;
       }
       // dO U^T and dR U^T, transposed
       again(lane);
@@ -1138,31 +1148,21 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
         fd[d] = M::template cols<C>(Rs, d * M::K, 16 * rt, lane);
         fu[d] = M::template cols<C>(Us, d * M::K, 16 * rt, lane);
       }
+      if (active)
 #pragma unroll
-      for (int kb = 0; kb < NK; ++kb) {
-        if (kb) __syncthreads();
-        Frag s[NF], ds[NF];
-        if (active)
+        for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
           for (int d = 0; d < NF; ++d) {
-            s[d] = M::template cols<KB>(states[kb & 1].s, d * M::K, 16 * ct, lane);
-            ds[d] = M::template cols<KB>(states[kb & 1].d, d * M::K, 16 * ct, lane);
-          }
-        asm volatile("" ::: "memory");  // reads first: copies under way would be waited for
-        if (kb + 1 < NK) copy_states(kb + 1);
-        if (active)
-#pragma unroll
-          for (int d = 0; d < NF; ++d) {
-            a[kb] = M::mul(s[d], fo[d], a[kb]);
-            z[kb] = M::mul(s[d], fd[d], z[kb]);
-            y[kb] = M::mul(ds[d], fu[d], y[kb]);
+            const Frag s = M::template cols<KB>(Ss[kb], d * M::K, 16 * ct, lane), ds = M::template cols<KB>(Ds[kb], d * M::K, 16 * ct, lane);
+            a[kb] = M::mul(s, fo[d], a[kb]);
+            z[kb] = M::mul(s, fd[d], z[kb]);
+            y[kb] = M::mul(ds, fu[d], y[kb]);
             if (rt == 0)
 #pragma unroll
-              for (int l = 0; l < M::E; ++l) s_d = mmpn::fma_of((A)s[d][l], (A)ds[d][l], s_d);
+              for (int l = 0; l < M::E; ++l) s_d = mmpn::fma_of((A)s[l], (A)ds[l], s_d);
           }
-      }
     }
-    if (p.dv == 0) __syncthreads();
+    __syncthreads();  // F and E take the place of dO, U and dR
     again(lane);
 
     // F and beta E, and their products with Q K^T and K K^T summed up by rows and columns
