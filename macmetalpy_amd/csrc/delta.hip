@@ -989,6 +989,22 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
       }
 }
 
+// The sum over the 16 lanes of a row of lanes, in all of them.
+template <int CTRL> __device__ __forceinline__ float lanes_of_row(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL> __device__ __forceinline__ double lanes_of_row(double x) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = __builtin_amdgcn_mov_dpp((int)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+template <typename A> __device__ __forceinline__ A sum16(A x) {
+  x += lanes_of_row<0xB1>(x);   // the neighbour
+  x += lanes_of_row<0x4E>(x);   // the other two of four
+  x += lanes_of_row<0x141>(x);  // mirrored within eight
+  return x + lanes_of_row<0x140>(x);  // and within sixteen
+}
+
 // Where LDS addresses are worked out again: kept from one part of a kernel to the
 // next, and from round to round, they take more registers than there are.
 __device__ __forceinline__ void again(int &lane) { asm volatile("" : "+v"(lane)); }
@@ -1013,7 +1029,10 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
   T *Fs = mem, *Es = Fs + C * C;  // when those are done with
   __shared__ double G[C];
   __shared__ int R[C];
-  __shared__ A cs[C], es[C], bet[C], rows[2][C], cols[2][NT][C], dots[3][8][16], rv[C], ek[C], sd[8];
+  // tiles on and below the diagonal of a chunk's matrix, and those above it that float16's
+  // operands of two tiles reach: a wave has every fourth
+  constexpr int LOWER = NT * (NT + 1) / 2, TILES = LOWER + (PT == 2 ? NT / 2 : 0), MINE = (TILES + 3) / 4;
+  __shared__ A cs[C], es[C], bet[C], rows[2][LOWER][16], cols[2][LOWER][16], below[LOWER][16], dots[4][8][16], sd[8];
   const int tid = threadIdx.x;
   int lane = tid & 63;
   const int fr = lane & 15, g = lane >> 4;
@@ -1038,20 +1057,21 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
   theirs(Ks, p.k.at(b, t0, kh), p.k.st, p.dk, std::integral_constant<int, DK>());
   theirs(Qs, p.q.at(b, t0, kh), p.q.st, p.dk, std::integral_constant<int, DK>());
 
-  // A wave has a tile (16 rows rt, 16 columns ct) of each block of dQ and dK, transposed.
+  // A wave has a tile (16 rows rt, 16 columns ct) of each block of dQ and dK, transposed,
+  // and the rows rt of dV in every WAVES_A_ROW-th piece of M::K channels.
   const int rt = wave % NT, ct = wave / NT;
+  constexpr int WAVES_A_ROW = 8 / NT, MY_D = (NF + WAVES_A_ROW - 1) / WAVES_A_ROW;
   const bool active = ct < KB / 16;
   Acc dq[NK], dk[NK];
 #pragma unroll
   for (int kb = 0; kb < NK; ++kb) dq[kb] = dk[kb] = Acc{};
-  const bool query = wave >= NT;  // of the products dO U^T, or dR U^T
-  const int row = query ? 2 * NT - 1 - wave : wave;
-  const bool task = wave < 2 * NT;
+  const bool query = wave >= 4;  // of dO U^T, or dR U^T
+  auto row_of_tile = [](int t) { return t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3; };
 
   for (int head = 0; head < p.group; ++head) {
     const int h = kh * p.group + head;
     const long long at = ((long long)b * p.heads + h) * p.chunks + n;
-    __syncthreads();  // the head before is done with LDS
+    if (head == 0) __syncthreads();  // (later ones: only wave 0 may still be at the head before, with what it alone writes)
     double sum = 0;
     int count = 0;
     bool anew = false;
@@ -1063,82 +1083,44 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
         cs[lane] = p.vecs[at * 3 * C + lane];
         es[lane] = p.vecs[at * 3 * C + C + lane];
         bet[lane] = p.vecs[at * 3 * C + 2 * C + lane];
-        rv[lane] = 0;
       }
     }
-    Acc w[NT], a[NK], z[NK], y[NK];
+    Acc w[MINE], a[NK], z[NK], y[NK];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) w[j] = Acc{};
+    for (int m = 0; m < MINE; ++m) w[m] = Acc{};
 #pragma unroll
     for (int kb = 0; kb < NK; ++kb) a[kb] = z[kb] = y[kb] = Acc{};
-    A s_d = 0;
+    A s_d = 0, with_v = 0;
     for (int v0 = 0; v0 < p.dv; v0 += VB) {
       again(lane);
       if (v0) __syncthreads();
       theirs(Os, e.grad.at(b, t0, h) + v0, e.grad.st, p.dv - v0, std::integral_constant<int, VB>());
       mmpx::copy_tile<T, VB, C, 8>(e.keep_u + (at * p.dv + v0) * C, C, p.dv - v0, C, Us, wave, lane);
       mmpx::copy_tile<T, VB, C, 8>(e.keep_r + (at * p.dv + v0) * C, C, p.dv - v0, C, Rs, wave, lane);
-#pragma unroll
+#pragma unroll 1
       for (int kb = 0; kb < NK; ++kb) {
         mmpx::copy_tile<T, VB, KB, 8>(e.keep_s + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, Ss[kb], wave, lane);
         mmpx::copy_tile<T, VB, KB, 8>(e.keep_d + (at * p.dv + v0) * DK + kb * KB, DK, p.dv - v0, KB, Ds[kb], wave, lane);
       }
-      // the values meanwhile, a vector of a step's channels a thread
-      constexpr int NV = (C * VB / V + 511) / 512;
-      Vec<T, V> value[NV];
+      // meanwhile the values of the steps and channels of which this wave will have dR
+      const int step = 16 * rt + fr;
+      const T *v = p.v.at(b, t0, h) + v0;
+      Frag value[MY_D];
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int vec = tid + 512 * k, i = vec / (VB / V), c = vec % (VB / V) * V, have = p.dv - v0 - c;
-        value[k] = Vec<T, V>{};
-        if (i < left) {
-          const T *v = p.v.at(b, t0 + i, h) + v0 + c;
-          if (have >= V) {
-            value[k] = mmpn::load_vec<T, V>(v);
-          } else {
-#pragma unroll
-            for (int l = 0; l < V; ++l)
-              if (l < have) value[k].e[l] = v[l];
-          }
-        }
-      }
+      for (int d = 0; d < NF; ++d)
+        if (d % WAVES_A_ROW == ct) value[d / WAVES_A_ROW] = row_of<T>(v, p.v.st, step, left, d * M::K, p.dv - v0, g);
       __syncthreads();
-      // dV and dR.V
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int vec = tid + 512 * k, i = vec / (VB / V), c = vec % (VB / V) * V, have = p.dv - v0 - c;
-        A with_v = 0;
-        if (i < left) {
-          const A beta = bet[i];
-          T *to = e.grad_v + (((long long)b * p.steps + t0 + i) * p.heads + h) * p.dv + v0 + c;
-          Vec<T, V> o;
-#pragma unroll
-          for (int l = 0; l < V; ++l) {
-            const A d = (A)Rs[Lay<T, C>::at(c + l, i)];
-            with_v = mmpn::fma_of(d, (A)value[k].e[l], with_v);
-            o.e[l] = (T)(beta * d);
-          }
-          if (have >= V) {
-            mmpn::store_vec(to, o);
-          } else {
-#pragma unroll
-            for (int l = 0; l < V; ++l)
-              if (l < have) to[l] = o.e[l];
-          }
-        }
-#pragma unroll
-        for (int d = 1; d < VB / V; d *= 2) with_v += __shfl_xor(with_v, d);
-        if (c == 0 && i < C) rv[i] += with_v;
-      }
       // dO U^T and dR U^T, transposed
       again(lane);
-      if (task)
 #pragma unroll
-        for (int d = 0; d < NF; ++d) {
-          const Frag x = query ? M::template rows<VB>(Os, 16 * row, d * M::K, lane) : M::template cols<C>(Rs, d * M::K, 16 * row, lane);
+      for (int m = 0; m < MINE; ++m) {
+        const int t = (wave & 3) + 4 * m, row = row_of_tile(t), j = t - row * (row + 1) / 2;
+        if (t < LOWER)
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-            if (j <= row) w[j] = M::mul(M::template cols<C>(Us, d * M::K, 16 * j, lane), x, w[j]);
-        }
+          for (int d = 0; d < NF; ++d)
+            w[m] = M::mul(M::template cols<C>(Us, d * M::K, 16 * j, lane),
+                          query ? M::template rows<VB>(Os, 16 * row, d * M::K, lane) : M::template cols<C>(Rs, d * M::K, 16 * row, lane), w[m]);
+      }
       // the products with the states
       again(lane);
       Frag fo[NF], fd[NF], fu[NF];
@@ -1147,6 +1129,29 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
         fo[d] = M::template rows<VB>(Os, 16 * rt, d * M::K, lane);
         fd[d] = M::template cols<C>(Rs, d * M::K, 16 * rt, lane);
         fu[d] = M::template cols<C>(Us, d * M::K, 16 * rt, lane);
+      }
+      // dV and dR.V
+      const A beta = bet[step];
+#pragma unroll
+      for (int d = 0; d < NF; ++d) {
+        if (d % WAVES_A_ROW != ct) continue;
+        T *to = e.grad_v + (((long long)b * p.steps + t0 + step) * p.heads + h) * p.dv + v0 + d * M::K;
+        const int have = step < left ? p.dv - v0 - d * M::K : 0;
+        Vec<T, M::E> o;
+#pragma unroll
+        for (int l = 0; l < M::E; ++l) {
+          with_v = mmpn::fma_of((A)fd[d][l], (A)value[d / WAVES_A_ROW][l], with_v);
+          o.e[l] = (T)(beta * (A)fd[d][l]);
+        }
+        if (sizeof(T) < 8 && have >= M::K) {
+          mmpn::store_vec(to + M::E * g, o);
+        } else {
+#pragma unroll
+          for (int l = 0; l < M::E; ++l) {
+            const int c = sizeof(T) < 8 ? M::E * g + l : g + 4 * l;
+            if (c < have) to[c] = o.e[l];
+          }
+        }
       }
       if (active)
 #pragma unroll
@@ -1166,47 +1171,44 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
     again(lane);
 
     // F and beta E, and their products with Q K^T and K K^T summed up by rows and columns
-    if (task) {
-      const int i = 16 * row + fr;
-      const T *X = query ? Qs : Ks;
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      const int t = (wave & 3) + 4 * m;
       T *to = query ? Fs : Es;
-      const double Gi = G[i];
-      const int Ri = R[i];
-      const A by = query ? p.scale : bet[i];
-      A sum_row = 0, sum_e = 0;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
+      if (t < LOWER) {
+        const int row = row_of_tile(t), j = t - row * (row + 1) / 2, i = 16 * row + fr;
+        const T *X = query ? Qs : Ks;
+        const double Gi = G[i];
+        const int Ri = R[i];
+        const A by = query ? p.scale : bet[i];
         Acc x{};
-        if (j <= row)
 #pragma unroll
-          for (int d = 0; d < DK; d += M::K) x = M::mul(M::template rows<DK>(Ks, 16 * j, d, lane), M::template rows<DK>(X, 16 * row, d, lane), x);
-        A sum_col[4];
+        for (int d = 0; d < DK; d += M::K) x = M::mul(M::template rows<DK>(Ks, 16 * j, d, lane), M::template rows<DK>(X, 16 * row, d, lane), x);
+        A sum_row = 0, sum_e = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int jj = 16 * j + M::row(g, c);
           const bool in = (query ? jj <= i : jj < i) && R[jj] == Ri;
-          const A f = in ? (query ? w[j][c] : -w[j][c]) * exp_any((A)(Gi - G[jj])) : (A)0;
+          const A f = in ? (query ? w[m][c] : -w[m][c]) * exp_any((A)(Gi - G[jj])) : (A)0;
           to[Lay<T, C>::at(i, jj)] = (T)(f * by);
-          const A m = in ? f * x[c] : (A)0;
-          sum_e += m;
-          sum_row = mmpn::fma_of(m, by, sum_row);
-          sum_col[c] = m * by;
+          const A part = in ? f * x[c] : (A)0;
+          sum_e += part;
+          sum_row = mmpn::fma_of(part, by, sum_row);
+          const A sum_col = sum16(part * by);
+          if (fr == 0) cols[query][t][M::row(g, c)] = sum_col;
         }
+        sum_row += __shfl_xor(sum_row, 16);
+        sum_row += __shfl_xor(sum_row, 32);
+        sum_e += __shfl_xor(sum_e, 16);
+        sum_e += __shfl_xor(sum_e, 32);
+        if (g == 0) {
+          rows[query][t][fr] = sum_row;
+          if (!query) below[t][fr] = sum_e;
+        }
+      } else if (t < TILES) {
+        const int row = 2 * (t - LOWER);
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sum_col[c] += __shfl_xor(sum_col[c], d);
-        if (fr == 0)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) cols[query][row][16 * j + M::row(g, c)] = sum_col[c];
-      }
-      sum_row += __shfl_xor(sum_row, 16);
-      sum_row += __shfl_xor(sum_row, 32);
-      sum_e += __shfl_xor(sum_e, 16);
-      sum_e += __shfl_xor(sum_e, 32);
-      if (g == 0) {
-        rows[query][i] = sum_row;
-        if (!query) ek[i] = sum_e;
+        for (int c = 0; c < 4; ++c) to[Lay<T, C>::at(16 * row + fr, 16 * (row + 1) + M::row(g, c))] = (T)0;
       }
     }
     __syncthreads();
@@ -1258,6 +1260,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
       q_s += __shfl_xor(q_s, d);
       k_z += __shfl_xor(k_z, d);
       k_d += __shfl_xor(k_d, d);
+      with_v += __shfl_xor(with_v, d);
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) s_d += __shfl_xor(s_d, d);
@@ -1265,28 +1268,38 @@ __global__ __launch_bounds__(512, 2) void k_delta_grads(Delta<T> p, Back<T> e) {
       dots[0][wave][fr] = q_s;
       dots[1][wave][fr] = k_z;
       dots[2][wave][fr] = k_d;
+      dots[3][wave][fr] = with_v;
     }
     if (lane == 0) sd[wave] = s_d;
     __syncthreads();
     if (wave == 0) {
-      double dG = 0, w_i = 0, qs_i = 0, kz_i = 0, sd_all = 0;
+      double dG = 0, w_i = 0;
       A dbeta = 0;
-      const int l = lane < C ? lane : 0;
+      if (lane < C) {
+        const int mine = lane / 16, i = lane % 16;
+        double kz_i = 0, rest = 0;
 #pragma unroll
-      for (int part = 0; part < 8 / NT; ++part) {  // the waves that share rows
-        qs_i += dots[0][part * NT + l / 16][l % 16];
-        kz_i += dots[1][part * NT + l / 16][l % 16];
-        w_i += dots[2][part * NT + l / 16][l % 16];
+        for (int part = 0; part < 8 / NT; ++part) {  // the waves that share rows
+          dG += dots[0][part * NT + mine][i];
+          kz_i += dots[1][part * NT + mine][i];
+          w_i += dots[2][part * NT + mine][i];
+          rest += dots[3][part * NT + mine][i];
+        }
+        dG += (double)bet[lane] * kz_i - w_i;
+        for (int j = 0; j <= mine; ++j) {
+          const int t = mine * (mine + 1) / 2 + j;
+          dG += (double)rows[0][t][i] + (double)rows[1][t][i];
+          rest += below[t][i];
+        }
+        for (int r = mine; r < NT; ++r) {
+          const int t = r * (r + 1) / 2 + mine;
+          dG -= (double)cols[0][t][i] + (double)cols[1][t][i];
+        }
+        dbeta = (A)(rest + kz_i);
       }
+      double sd_all = 0;
 #pragma unroll
       for (int part = 0; part < 8; ++part) sd_all += sd[part];
-      if (lane < C) {
-        dG = qs_i + (double)bet[l] * kz_i - w_i + rows[0][l] + rows[1][l];
-        for (int r = l / 16; r < NT; ++r) dG -= (double)cols[0][r][l] + (double)cols[1][r][l];
-        dbeta = (A)(rv[l] + kz_i + ek[l]);
-      } else {
-        w_i = 0;
-      }
       double all = w_i;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
