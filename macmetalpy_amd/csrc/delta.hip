@@ -326,7 +326,12 @@ template <typename T> struct Pass {
   A *final;
   T *o;
   T *keep_s, *keep_u;
-  int tiles;  // workgroups a head
+  int tiles;  // workgroups a head and segment
+  // Segments of `span` chunks that run at once: `initial` holds the state before each
+  // (batch, heads, segments, dk, dv); a scan for them leaves of each the state that no
+  // state before it would end in, there, and what it makes of one (DK, DK).
+  int segments, span;
+  A *maps;
 };
 
 template <typename T> __device__ __forceinline__ void put4(T *p, const typename Wide<T>::type (&v)[4], int g) {
@@ -435,24 +440,29 @@ __device__ __forceinline__ void through(int from, int count, int by, S &one, S2 
 }
 
 // Workgroup: NW waves with 16 columns each of a head's state (one without any only
-// helps with the copies).
+// helps with the copies).  OUT: with the outputs; KEEP: with what the gradient needs;
+// neither: a scan of segments.
 template <typename T, int DK, int NW, bool OUT, bool KEEP, bool ALIGNED>
 __global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
   typedef typename M::Acc Acc;
-  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16;
-  constexpr int W = 16 * NW, DT = DK / 16;
+  constexpr int C = chunk_of<T>(), NT = C / 16, PT = M::K / 16, W = 16 * NW, DT = DK / 16;
   typedef PassStage<T, DK, W, OUT> Stage;
   constexpr bool AHEAD = ALIGNED && 2 * sizeof(Stage) <= kLds;
   __shared__ Stage one;
   __shared__ typename std::conditional<AHEAD, Stage, char>::type two;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, g = lane >> 4;
   const unsigned id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x);
-  const long long bh = id / e.tiles;
-  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
-  const int n0 = (int)(id - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;  // of the state
+  const long long bs = id / e.tiles, bh = bs / e.segments;
+  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads), segment = (int)(bs - bh * e.segments);
+  const int n0 = (int)(id - bs * e.tiles) * W, col = n0 + 16 * wave + fr;  // of the state
   const bool there = col < p.dv;
+  const int begin = segment * e.span, count = p.chunks - begin < e.span ? p.chunks - begin : e.span;
+  // A scan has a column for each key channel too, beyond those of the values: what
+  // becomes of a state with 1 in that channel, without values.
+  constexpr bool SCAN = !OUT && !KEEP;
+  const int key = col - (p.dv + W - 1) / W * W;
   const int kh = h / p.group;
 
   Acc S[DT];
@@ -461,7 +471,8 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = M::spot(t, M::row(g, r));
-      S[t][r] = e.initial && there && i < p.dk ? e.initial[(bh * p.dk + i) * p.dv + col] : (A)0;
+      if constexpr (SCAN) S[t][r] = i == key ? (A)1 : (A)0;
+      else S[t][r] = e.initial && there && i < p.dk ? e.initial[(bs * p.dk + i) * p.dv + col] : (A)0;
     }
 
   // f(LDS, from, stride, rows, columns, their numbers in LDS) of each array of chunk n
@@ -640,19 +651,79 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e
     }
   };
 
-  const bool active = n0 + 16 * wave < p.dv;
-  through<AHEAD>(0, p.chunks, 1, one, two, [&](int n, Stage &to) __attribute__((always_inline)) { load_arrays<T, AHEAD, NW>(arrays, n, to, tid); },
+  const bool active = n0 + 16 * wave < p.dv || (SCAN && key - fr >= 0 && key - fr < DK);
+  through<AHEAD>(begin, count, 1, one, two, [&](int n, Stage &to) __attribute__((always_inline)) { load_arrays<T, AHEAD, NW>(arrays, n, to, tid); },
                  first, [&](int n, const Stage &in) __attribute__((always_inline)) {
                    if (active) chunk(n, in);
                  });
-  if (e.final && there)
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = M::spot(t, M::row(g, r));
+      if constexpr (SCAN) {
+        if (there && i < p.dk) e.final[(bs * p.dk + i) * p.dv + col] = S[t][r];
+        if (key >= 0 && key < DK) e.maps[(bs * DK + i) * DK + key] = S[t][r];
+      } else {
+        if (e.final && segment == e.segments - 1 && there && i < p.dk) e.final[(bh * p.dk + i) * p.dv + col] = S[t][r];
+      }
+    }
+}
+
+// The states before (BACK: the gradients after) the segments of a head, from what a
+// scan found of each, by a wave for 16 columns: S' = M S + N, or D = M^T D' + L.
+template <typename T, int DK, bool BACK>
+__global__ __launch_bounds__(64) void k_delta_join(int dk, int dv, int tiles, int segments, const typename Wide<T>::type *maps,
+                                                   const typename Wide<T>::type *first, typename Wide<T>::type *states) {
+  typedef typename Wide<T>::type A;
+  typedef Mma<T> M;
+  typedef typename M::Acc Acc;
+  constexpr int DT = DK / 16, PT = M::K / 16, NF = DT / PT;
+  const int lane = threadIdx.x, fr = lane & 15, g = lane >> 4;
+  const long long bh = blockIdx.x / tiles;
+  const int col = (int)(blockIdx.x - bh * tiles) * 16 + fr;
+  const bool there = col < dv;
+  auto place = [&](long long base, int t, int r) { return (base * dk + M::spot(t, M::row(g, r))) * dv + col; };
+  auto in = [&](int t, int r) { return there && M::spot(t, M::row(g, r)) < dk; };
+  Acc S[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[t][r] = first && in(t, r) ? first[place(bh, t, r)] : (A)0;
+  for (int k = 0; k < segments; ++k) {
+    const long long at = bh * segments + (BACK ? segments - 1 - k : k);
+    const A *map = maps + at * DK * DK;
+    Two<T> s[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) s[f] = mmpx::operand<T>(S, f * PT);
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = M::spot(t, M::row(g, r));
-        if (i < p.dk) e.final[(bh * p.dk + i) * p.dv + col] = S[t][r];
+        const A was = S[t][r];
+        S[t][r] = in(t, r) ? states[place(at, t, r)] : (A)0;
+        if (in(t, r)) states[place(at, t, r)] = was;
       }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const int row = M::spot(t, fr);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        A v[M::E];
+#pragma unroll
+        for (int l = 0; l < M::E; ++l) {
+          const int c = M::spot(f * PT + (l >> 2), M::row(g, l & 3));
+          v[l] = BACK ? map[(long long)c * DK + row] : map[(long long)row * DK + c];
+        }
+        const Two<T> m = mmpx::two_of<T>(v);
+        if constexpr (M::SPLIT) {
+          S[t] = M::mul(m.lo, s[f].hi, S[t]);
+          S[t] = M::mul(m.hi, s[f].lo, S[t]);
+        }
+        S[t] = M::mul(m.hi, s[f].hi, S[t]);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------- single steps
@@ -798,6 +869,7 @@ template <typename T> struct Back {
   T *grad_q, *grad_k, *grad_v;
   void *grad_gate, *grad_beta;  // of the types of gate and beta
   int tiles;
+  int segments, span;  // as in Pass, with grad_final in the place of initial
 };
 
 template <typename T, int DK, int W> struct __attribute__((aligned(16))) BackStage {
@@ -807,8 +879,9 @@ template <typename T, int DK, int W> struct __attribute__((aligned(16))) BackSta
   typename Wide<T>::type vecs[kVecs<T>];
 };
 
-// Workgroup: as k_delta_pass.
-template <typename T, int DK, int NW, bool ALIGNED>
+// Workgroup: as k_delta_pass.  SCAN: only what a segment makes of no gradient after it,
+// to grad_initial (batch, heads, segments, dk, dv).
+template <typename T, int DK, int NW, bool SCAN, bool ALIGNED>
 __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
@@ -821,9 +894,10 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
   __shared__ typename std::conditional<AHEAD, Stage, char>::type two;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, g = lane >> 4;
   const unsigned id = mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x);
-  const long long bh = id / e.tiles;
-  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads);
-  const int n0 = (int)(id - bh * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;
+  const long long bs = id / e.tiles, bh = bs / e.segments;
+  const int b = (int)(bh / p.heads), h = (int)(bh - (long long)b * p.heads), segment = (int)(bs - bh * e.segments);
+  const int n0 = (int)(id - bs * e.tiles) * 16 * NW, col = n0 + 16 * wave + fr;
+  const int begin = segment * e.span, count = p.chunks - begin < e.span ? p.chunks - begin : e.span;
   const bool there = col < p.dv;
   const int kh = h / p.group;
 
@@ -833,7 +907,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = M::spot(t, M::row(g, r));
-      S[t][r] = e.grad_final && there && i < p.dk ? e.grad_final[(bh * p.dk + i) * p.dv + col] : (A)0;
+      S[t][r] = !SCAN && e.grad_final && there && i < p.dk ? e.grad_final[(bs * p.dk + i) * p.dv + col] : (A)0;
     }
 
   auto arrays = [&](int n, Stage &to, auto f) __attribute__((always_inline)) {
@@ -893,7 +967,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
     Two<T> s[NF];
 #pragma unroll
     for (int i = 0; i < NF; ++i) s[i] = mmpx::operand<T>(S, i * PT);
-    if (there) {
+    if (!SCAN && there) {
       T *to = e.keep_d + ((bh * p.chunks + n) * p.dv + col) * DK;
 #pragma unroll
       for (int t = 0; t < NF; ++t) put_tiles<T>(to + t * M::K, S, t, g);
@@ -955,7 +1029,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
 #pragma unroll
         for (int i = 0; i < (j + 1) * PT; ++i)
           x[i] = M::mul(part == 0 ? tl[i][j] : tc[i][j], part == 1 ? f[j].lo : f[j].hi, x[i]);
-    if (there) {
+    if (!SCAN && there) {
       T *to = e.keep_r + ((bh * p.chunks + n) * p.dv + col) * C;
 #pragma unroll
       for (int j = 0; j < NC; ++j) put_tiles<T>(to + j * M::K, x, j, g);
@@ -975,17 +1049,17 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_back(Delta<T> p, Back<T> e
   };
 
   const bool active = n0 + 16 * wave < p.dv;
-  through<AHEAD>(p.chunks - 1, p.chunks, -1, one, two, [&](int n, Stage &to) __attribute__((always_inline)) { load_arrays<T, AHEAD, NW>(arrays, n, to, tid); },
+  through<AHEAD>(begin + count - 1, count, -1, one, two, [&](int n, Stage &to) __attribute__((always_inline)) { load_arrays<T, AHEAD, NW>(arrays, n, to, tid); },
                  first, [&](int n, const Stage &in) __attribute__((always_inline)) {
                    if (active) chunk(n, in);
                  });
-  if (there)
+  if (there && (SCAN || segment == 0))
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = M::spot(t, M::row(g, r));
-        if (i < p.dk) e.grad_initial[(bh * p.dk + i) * p.dv + col] = S[t][r];
+        if (i < p.dk) e.grad_initial[((SCAN ? bs : bh) * p.dk + i) * p.dv + col] = S[t][r];
       }
 }
 
@@ -1383,20 +1457,60 @@ template <typename T> struct Chunks {
   }
 };
 
+constexpr int kWaves = 4;  // of a pass' workgroups
+constexpr int kColumns = 16 * kWaves;
+inline int column_tiles(int n) { return (n + kColumns - 1) / kColumns; }
+inline int width_of(int dk) { return dk <= 64 ? 64 : dk <= 128 ? 128 : 256; }
+
 template <typename T, bool OUT, bool KEEP> int pass(const Delta<T> &p, Pass<T> e, const char *what) {
-  constexpr int NW = 4;
-  e.tiles = (p.dv + 16 * NW - 1) / (16 * NW);
-  const int64_t blocks = (int64_t)p.batch * p.heads * e.tiles;
-  if (!mmpi::grid_fits(blocks, 64 * NW)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
+  e.tiles = column_tiles(p.dv) + (OUT || KEEP ? 0 : column_tiles(width_of(p.dk)));
+  const int64_t blocks = (int64_t)p.batch * p.heads * e.segments * e.tiles;
+  if (!mmpi::grid_fits(blocks, 64 * kWaves)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
   return with_width(p.dk, [&](auto dk) {
     constexpr int DK = decltype(dk)::value;
     if (copies(p, p.v))
-      hipLaunchKernelGGL((k_delta_pass<T, DK, NW, OUT, KEEP, true>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+      hipLaunchKernelGGL((k_delta_pass<T, DK, kWaves, OUT, KEEP, true>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, mmpi::stream(), p, e);
     else
-      hipLaunchKernelGGL((k_delta_pass<T, DK, NW, OUT, KEEP, false>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+      hipLaunchKernelGGL((k_delta_pass<T, DK, kWaves, OUT, KEEP, false>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, mmpi::stream(), p, e);
     return mmpi::check_launch(what);
   });
 }
+template <typename T, bool BACK>
+int join(const Delta<T> &p, int segments, const void *maps, const typename Wide<T>::type *first, void *states, const char *what) {
+  typedef typename Wide<T>::type A;
+  const int tiles = (p.dv + 15) / 16;
+  const int64_t blocks = (int64_t)p.batch * p.heads * tiles;
+  if (!mmpi::grid_fits(blocks, 64)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
+  return with_width(p.dk, [&](auto dk) {
+    hipLaunchKernelGGL((k_delta_join<T, decltype(dk)::value, BACK>), dim3((unsigned)blocks), dim3(64), 0, mmpi::stream(), p.dk, p.dv, tiles,
+                       segments, (const A *)maps, first, (A *)states);
+    return mmpi::check_launch(what);
+  });
+}
+
+// The segments that the chunks of too few heads are cut into, with the states before
+// each of them.
+template <typename T> struct Segments {
+  typedef typename Wide<T>::type A;
+  Temp states, maps;
+  int get(const Delta<T> &p, Pass<T> &e, const char *what) {
+    const int DK = width_of(p.dk);
+    const mmpi::DeltaPlan plan = mmpi::delta_plan((long long)p.batch * p.heads, column_tiles(p.dv), column_tiles(DK), p.chunks, mmpi::cu_count());
+    e.segments = plan.segments;
+    e.span = plan.span;
+    if (e.segments == 1) return MMP_OK;
+    const size_t all = (size_t)p.batch * p.heads * e.segments * sizeof(A);
+    if (int st = states.get(all * p.dk * p.dv, what)) return st;
+    if (int st = maps.get(all * DK * DK, what)) return st;
+    Pass<T> scan = e;
+    scan.final = (A *)states.p;
+    scan.maps = (A *)maps.p;
+    if (int st = pass<T, false, false>(p, scan, what)) return st;
+    if (int st = join<T, false>(p, e.segments, maps.p, e.initial, states.p, what)) return st;
+    e.initial = (const A *)states.p;
+    return MMP_OK;
+  }
+};
 
 template <typename T> int forward(Delta<T> p, Pass<T> e) {
   if (p.steps <= 8) {
@@ -1410,44 +1524,67 @@ template <typename T> int forward(Delta<T> p, Pass<T> e) {
   }
   Chunks<T> chunks;
   if (int st = chunks.get(p, kWhat)) return st;
+  Segments<T> segments;
+  if (int st = segments.get(p, e, kWhat)) return st;
   return pass<T, true, false>(p, e, kWhat);
 }
 
 constexpr const char *kGradWhat = "mmp_delta_rule_grad";
 
 template <typename T> int backward(Delta<T> p, Back<T> e, int key_heads, const typename Wide<T>::type *initial) {
-  constexpr int C = chunk_of<T>(), NW = 4;
+  typedef typename Wide<T>::type A;
+  constexpr int C = chunk_of<T>(), NW = kWaves;
   const char *what = kGradWhat;
   Chunks<T> chunks;
   if (p.heads)
     if (int st = chunks.get(p, what)) return st;
   Temp s, d, u, r;
-  const int DK = p.dk <= 64 ? 64 : p.dk <= 128 ? 128 : 256;
+  const int DK = width_of(p.dk);
+  Segments<T> segments;
+  Temp ends;
+  e.segments = 1;
+  e.span = p.chunks;
   const size_t columns = (size_t)p.batch * p.heads * p.chunks * p.dv * sizeof(T);
   if (columns) {
     if (int st = s.get(columns * DK, what)) return st;
     if (int st = d.get(columns * DK, what)) return st;
     if (int st = u.get(columns * C, what)) return st;
     if (int st = r.get(columns * C, what)) return st;
-    if (int st = pass<T, false, true>(p, Pass<T>{initial, nullptr, nullptr, (T *)s.p, (T *)u.p, 0}, what)) return st;
+    Pass<T> states{initial, nullptr, nullptr, (T *)s.p, (T *)u.p, 0, 1, p.chunks, nullptr};
+    if (int st = segments.get(p, states, what)) return st;
+    if (int st = pass<T, false, true>(p, states, what)) return st;
+    e.segments = states.segments;
+    e.span = states.span;
   }
   e.keep_s = (const T *)s.p;
   e.keep_u = (const T *)u.p;
   e.keep_d = (T *)d.p;
   e.keep_r = (T *)r.p;
-  e.tiles = (p.dv + 16 * NW - 1) / (16 * NW);
-  const int64_t blocks = (int64_t)p.batch * p.heads * e.tiles;
+  e.tiles = column_tiles(p.dv);
+  const int64_t blocks = (int64_t)p.batch * p.heads * e.segments * e.tiles;
   if (!mmpi::grid_fits(blocks, 64 * NW)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
-  if (blocks)
-    if (int st = with_width(p.dk, [&](auto dk) {
-          constexpr int DK = decltype(dk)::value;
-          if (copies(p, e.grad))
-            hipLaunchKernelGGL((k_delta_back<T, DK, NW, true>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
-          else
-            hipLaunchKernelGGL((k_delta_back<T, DK, NW, false>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
-          return mmpi::check_launch(what);
-        }))
-      return st;
+  auto back = [&](auto scan, const Back<T> &e) {
+    return with_width(p.dk, [&](auto dk) {
+      constexpr int DK = decltype(dk)::value;
+      constexpr bool SCAN = decltype(scan)::value;
+      if (copies(p, e.grad))
+        hipLaunchKernelGGL((k_delta_back<T, DK, NW, SCAN, true>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+      else
+        hipLaunchKernelGGL((k_delta_back<T, DK, NW, SCAN, false>), dim3((unsigned)blocks), dim3(64 * NW), 0, mmpi::stream(), p, e);
+      return mmpi::check_launch(what);
+    });
+  };
+  if (blocks) {
+    if (e.segments > 1) {
+      if (int st = ends.get((size_t)p.batch * p.heads * e.segments * p.dk * p.dv * sizeof(A), what)) return st;
+      Back<T> scan = e;
+      scan.grad_initial = (A *)ends.p;
+      if (int st = back(std::true_type(), scan)) return st;
+      if (int st = join<T, true>(p, e.segments, segments.maps.p, e.grad_final, ends.p, what)) return st;
+      e.grad_final = (const A *)ends.p;
+    }
+    if (int st = back(std::false_type(), e)) return st;
+  }
   if (!p.steps) return MMP_OK;
   p.chunks = (int)((p.steps + C - 1) / C);
   e.tiles = key_heads;
@@ -1494,7 +1631,7 @@ extern "C" int mmp_delta_rule(int dtype, int64_t batch, int64_t steps, int64_t k
                      {gate, g_sb, g_st, g_sh, gate_wide}, {beta, b_sb, b_st, b_sh, beta_wide},
                      (int)batch, (int)heads, (int)(heads / key_heads), (int)dk, (int)dv, (long long)steps, 0, (A)scale,
                      nullptr, nullptr};
-    return forward<T>(p, Pass<T>{(const A *)initial, (A *)final_state, (T *)o, nullptr, nullptr, 0});
+    return forward<T>(p, Pass<T>{(const A *)initial, (A *)final_state, (T *)o, nullptr, nullptr, 0, 1, 0, nullptr});
   })
 }
 
@@ -1522,7 +1659,7 @@ extern "C" int mmp_delta_rule_grad(int dtype, int64_t batch, int64_t steps, int6
                      (int)batch, (int)heads, (int)(heads / key_heads), (int)dk, (int)dv, (long long)steps, 0, (A)scale,
                      nullptr, nullptr};
     const Back<T> e{{(const T *)grad, o_sb, o_st, o_sh}, (const A *)grad_final, (A *)grad_initial, nullptr, nullptr, nullptr, nullptr,
-                    (T *)grad_q, (T *)grad_k, (T *)grad_v, grad_gate, grad_beta, 0};
+                    (T *)grad_q, (T *)grad_k, (T *)grad_v, grad_gate, grad_beta, 0, 1, 0};
     return backward<T>(p, e, (int)key_heads, (const A *)initial);
   })
 }

@@ -298,6 +298,30 @@ inline Prod16Plan prod16_plan(long long m, long long n, int slabs, double cus) {
   return best;
 }
 
+// Segments that the chunks of the delta rule's heads are cut into: a pass takes a
+// workgroup for 64 columns of a head's state and is a chain of `chunks`, so few
+// heads leave CUs idle.  Segments run at once from states that a scan finds, which
+// takes the columns of the values and of the keys, and a join that goes through
+// them.  Us a chunk: 3.4 with outputs, 2.4 in the scan; 3 a segment in the join.
+struct DeltaPlan {
+  int segments, span;  // chunks of each but the last
+};
+inline DeltaPlan delta_plan(long long heads, int value_tiles, int key_tiles, int chunks, double cus) {
+  DeltaPlan best{1, chunks > 0 ? chunks : 1};
+  if (heads < 1 || value_tiles < 1) return best;
+  auto rounds = [&](long long wgs) { return __builtin_ceil((double)wgs / cus); };
+  double us = 3.4 * chunks * rounds(heads * value_tiles);
+  for (int s = 2; s <= 64 && chunks / s >= 4; s *= 2) {
+    const int span = (chunks + s - 1) / s;
+    const double t = span * (3.4 * rounds(heads * value_tiles * s) + 2.4 * rounds(heads * (value_tiles + key_tiles) * s)) + 3.0 * s + 10.0;
+    if (t < 0.95 * us) {
+      us = t;
+      best = DeltaPlan{(chunks + span - 1) / span, span};
+    }
+  }
+  return best;
+}
+
 // Rows from which unaligned ones, each longer than a tile, are scanned by a
 // workgroup each instead of in tiles that look back.  What a row's waves walk
 // is paid in latency, so fewer rows need more bytes a step.  40,000,000
