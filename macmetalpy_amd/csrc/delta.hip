@@ -671,58 +671,80 @@ __global__ __launch_bounds__(64 * NW, 1) void k_delta_pass(Delta<T> p, Pass<T> e
 }
 
 // The states before (BACK: the gradients after) the segments of a head, from what a
-// scan found of each, by a wave for 16 columns: S' = M S + N, or D = M^T D' + L.
+// scan found of each: S' = M S + N, or D = M^T D' + L.  Workgroup: 16 columns, a wave for
+// 16 rows; what the next segment needs of M and N is on its way meanwhile.
 template <typename T, int DK, bool BACK>
-__global__ __launch_bounds__(64) void k_delta_join(int dk, int dv, int tiles, int segments, const typename Wide<T>::type *maps,
-                                                   const typename Wide<T>::type *first, typename Wide<T>::type *states) {
+__global__ __launch_bounds__(4 * DK) void k_delta_join(int dk, int dv, int tiles, int segments, const typename Wide<T>::type *maps,
+                                                       const typename Wide<T>::type *first, typename Wide<T>::type *states) {
   typedef typename Wide<T>::type A;
   typedef Mma<T> M;
   typedef typename M::Acc Acc;
-  constexpr int DT = DK / 16, PT = M::K / 16, NF = DT / PT;
-  const int lane = threadIdx.x, fr = lane & 15, g = lane >> 4;
+  constexpr int PT = M::K / 16, NF = DK / M::K;
+  __shared__ __attribute__((aligned(16))) T high[2][16 * DK], low[2][M::SPLIT ? 16 * DK : 8];  // S, a column a row
+  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4;
+  const int t = __builtin_amdgcn_readfirstlane(tid >> 6);  // the tile of rows
   const long long bh = blockIdx.x / tiles;
   const int col = (int)(blockIdx.x - bh * tiles) * 16 + fr;
-  const bool there = col < dv;
-  auto place = [&](long long base, int t, int r) { return (base * dk + M::spot(t, M::row(g, r))) * dv + col; };
-  auto in = [&](int t, int r) { return there && M::spot(t, M::row(g, r)) < dk; };
-  Acc S[DT];
+  auto row = [&](int r) { return M::spot(t, M::row(g, r)); };
+  auto there = [&](int r) { return col < dv && row(r) < dk; };
+  auto place = [&](long long base, int r) { return (base * dk + row(r)) * dv + col; };
+  auto segment = [&](int k) { return bh * segments + (BACK ? segments - 1 - k : k); };
+
+  A m[NF][M::E];
+  Acc S, add;
+  auto fetch = [&](int k) {
+    const A *map = maps + segment(k) * DK * DK;
+    const int mine = M::spot(t, fr);
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+    for (int f = 0; f < NF; ++f)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) S[t][r] = first && in(t, r) ? first[place(bh, t, r)] : (A)0;
-  for (int k = 0; k < segments; ++k) {
-    const long long at = bh * segments + (BACK ? segments - 1 - k : k);
-    const A *map = maps + at * DK * DK;
-    Two<T> s[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) s[f] = mmpx::operand<T>(S, f * PT);
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const A was = S[t][r];
-        S[t][r] = in(t, r) ? states[place(at, t, r)] : (A)0;
-        if (in(t, r)) states[place(at, t, r)] = was;
+      for (int l = 0; l < M::E; ++l) {
+        const int c = M::spot(f * PT + (l >> 2), M::row(g, l & 3));
+        m[f][l] = BACK ? map[c * DK + mine] : map[mine * DK + c];
       }
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-      const int row = M::spot(t, fr);
+    for (int r = 0; r < 4; ++r) add[r] = there(r) ? states[place(segment(k), r)] : (A)0;
+  };
+  auto share = [&](int buf) {
+    Vec<T, 4> hi;
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        A v[M::E];
+    for (int r = 0; r < 4; ++r) hi.e[r] = (T)S[r];
+    mmpx::settle(hi);
 #pragma unroll
-        for (int l = 0; l < M::E; ++l) {
-          const int c = M::spot(f * PT + (l >> 2), M::row(g, l & 3));
-          v[l] = BACK ? map[(long long)c * DK + row] : map[(long long)row * DK + c];
-        }
-        const Two<T> m = mmpx::two_of<T>(v);
-        if constexpr (M::SPLIT) {
-          S[t] = M::mul(m.lo, s[f].hi, S[t]);
-          S[t] = M::mul(m.hi, s[f].lo, S[t]);
-        }
-        S[t] = M::mul(m.hi, s[f].hi, S[t]);
-      }
+    for (int r = 0; r < 4; ++r) {
+      high[buf][Lay<T, DK>::at(fr, row(r))] = hi.e[r];
+      if constexpr (M::SPLIT) low[buf][Lay<T, DK>::at(fr, row(r))] = (T)(S[r] - (A)hi.e[r]);
     }
+  };
+#pragma unroll
+  for (int r = 0; r < 4; ++r) S[r] = first && there(r) ? first[place(bh, r)] : (A)0;
+  // (where its registers are enough for both)
+  constexpr bool AHEAD = DK <= 128 && sizeof(A) == 4;
+  if constexpr (AHEAD) fetch(0);
+  share(0);
+  for (int k = 0; k < segments; ++k) {
+    if constexpr (!AHEAD) fetch(k);
+    Two<T> map[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) map[f] = mmpx::two_of<T>(m[f]);
+    Acc next = add;
+    __syncthreads();
+    if constexpr (AHEAD)
+      if (k + 1 < segments) fetch(k + 1);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const typename M::Frag hi = M::template rows<DK>(high[k & 1], 0, f * M::K, lane);
+      if constexpr (M::SPLIT) {
+        next = M::mul(map[f].lo, hi, next);
+        next = M::mul(map[f].hi, M::template rows<DK>(low[k & 1], 0, f * M::K, lane), next);
+      }
+      next = M::mul(map[f].hi, hi, next);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (there(r)) states[place(segment(k), r)] = S[r];
+    S = next;
+    share(k + 1 & 1);
   }
 }
 
@@ -1480,10 +1502,11 @@ int join(const Delta<T> &p, int segments, const void *maps, const typename Wide<
   typedef typename Wide<T>::type A;
   const int tiles = (p.dv + 15) / 16;
   const int64_t blocks = (int64_t)p.batch * p.heads * tiles;
-  if (!mmpi::grid_fits(blocks, 64)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
+  if (!mmpi::grid_fits(blocks, 1024)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many heads", what);
   return with_width(p.dk, [&](auto dk) {
-    hipLaunchKernelGGL((k_delta_join<T, decltype(dk)::value, BACK>), dim3((unsigned)blocks), dim3(64), 0, mmpi::stream(), p.dk, p.dv, tiles,
-                       segments, (const A *)maps, first, (A *)states);
+    constexpr int DK = decltype(dk)::value;
+    hipLaunchKernelGGL((k_delta_join<T, DK, BACK>), dim3((unsigned)blocks), dim3(4 * DK), 0, mmpi::stream(), p.dk, p.dv, tiles, segments,
+                       (const A *)maps, first, (A *)states);
     return mmpi::check_launch(what);
   });
 }
