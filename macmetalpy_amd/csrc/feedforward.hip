@@ -92,14 +92,22 @@ template <typename T> struct End {
   template <int ACT, int N>
   __device__ __forceinline__ void backward(long long row, int col, const A (&g)[N], const A (&u)[N]) const {
     T dg[N], du[N];
+    Vec<T, N> d{};
+    const T *from = grad + row * ldg + col;
+    if (col + N <= hidden) {
+      d = mmpn::load_vec<T, N>(from);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (col + i < hidden) d.e[i] = from[i];
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       A a, da;
       activate<T, ACT, true>(g[i], a, da);
       const bool there = col + i < hidden;
-      const A d = there ? (A)grad[row * ldg + col + i] : (A)0;
-      dg[i] = there ? (T)(d * u[i] * da) : (T)0;
-      du[i] = there ? (T)(d * a) : (T)0;
+      dg[i] = there ? (T)((A)d.e[i] * u[i] * da) : (T)0;
+      du[i] = there ? (T)((A)d.e[i] * a) : (T)0;
     }
     put(out + row * ldo + col, dg, padded - col);
     put(out + row * ldo + padded + col, du, padded - col);
