@@ -267,3 +267,27 @@ def test_dropout_rate():
     for rate in (0.05, 0.5, 0.8):
         gone = float((nn.dropout(cp.ones(n, dtype=np.float16), rate, 5).get() == 0).mean())
         assert abs(gone - rate) < 5 * (rate * (1 - rate) / n) ** 0.5
+
+
+def test_refusals():
+    z = lambda *s, dt=np.float32: cp.zeros(s, dtype=dt)  # noqa: E731
+    for x, w, act, error in ((z(3, 4), z(5, 6), "silu", ValueError), (z(3, 4), z(4, 5), "silu", ValueError),
+                             (z(3, 4), z(4, 6), "relu", ValueError), (z(3, 4), z(4, 6), None, ValueError),
+                             (z(3, 4, dt=np.int32), z(4, 6), "silu", TypeError), (z(3, 4), z(4), "silu", ValueError),
+                             (z(3, 4), z(2, 4, 6), "silu", ValueError), (cp.array(np.float32(1)), z(1, 2), "silu", ValueError)):
+        with pytest.raises(error):
+            nn.gated_feed_forward(x, w, act)
+        with pytest.raises(error):
+            nn.gated_feed_forward_grad(z(3, 3), x, w, act)
+    with pytest.raises(ValueError):
+        nn.gated_feed_forward_grad(z(3, 4), z(3, 4), z(4, 6))
+    x = z(3, 4)
+    for args, error in (((x, -0.1, 0), ValueError), ((x, 1.0, 0), ValueError), ((x, float("nan"), 0), ValueError),
+                        ((x, "0.1", 0), TypeError), ((x, 0.1, -1), ValueError), ((x, 0.1, 2 ** 64), ValueError),
+                        ((x, 0.1, 1.5), TypeError), ((x, 0.1, True), TypeError), ((x, 0.1, 0, -1), ValueError),
+                        ((x, 0.1, 0, 2 ** 63), ValueError), ((x, 0.1, 0, 1.0), TypeError),
+                        ((x, 0.1, 0, z(1, dt=np.int64)), ValueError), ((x, 0.1, 0, cp.array(np.array(1.0))), TypeError),
+                        ((x, 0.1, 0, 0, z(3, 5)), ValueError), ((x, 0.1, 0, 0, z(3, 4, dt=np.float16)), ValueError),
+                        ((z(3, dt=np.int32), 0.1, 0), TypeError)):
+        with pytest.raises(error):
+            nn.dropout(*args)

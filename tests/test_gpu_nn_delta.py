@@ -153,3 +153,185 @@ def test_delta_rule_grad(dt, size):
         want = rule_grad(grad, *x, *states, dk ** -0.5)
         got = nn.gated_delta_rule_grad(cp.array(grad), *map(cp.array, x), *(None if s is None else cp.array(s) for s in states))
         grads_close(got, want, dt, steps, dk, dv)
+
+
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+@pytest.mark.parametrize("size", [(1, 4160, 1, 1, 64, 33), (1, 2100, 2, 4, 130, 64), (2, 1500, 1, 1, 256, 16)], ids=str)
+def test_long_sequences(dt, size):
+    """Few heads and many chunks: segments that run at once, with and without fresh starts."""
+    if dt == np.float64:
+        size = (size[0], size[1] // 4) + size[2:]
+    g = np.random.default_rng(size[1])
+    wide = np.float64 if dt == np.float64 else np.float32
+    batch, steps, key_heads, heads, dk, dv = size
+    for anew in (0.0, 0.003):
+        x = make(g, *size, dt, anew)
+        # memories of some thousand steps: states pass many segments
+        x = x[:3] + ((x[3].astype(np.float64) * 1e-2).astype(dt),) + x[4:]
+        states = [g.standard_normal((batch, heads, dk, dv)).astype(wide) for _ in range(2)]
+        o, S = rule(*x, states[0], dk ** -0.5)
+        got_o, got_s = nn.gated_delta_rule(*map(cp.array, x), cp.array(states[0]))
+        parts = parts_of(dt, steps, dk) * 4
+        close(got_o, o, dt, U[dt], parts + (8 * U[dt] if dt == np.float16 else 0))
+        close(got_s, S, wide, U[wide], parts)
+        grad = g.standard_normal(x[2].shape).astype(dt)
+        want = rule_grad(grad, *x, *states, dk ** -0.5)
+        got = nn.gated_delta_rule_grad(cp.array(grad), *map(cp.array, x), *map(cp.array, states))
+        loose = parts + (8 * 3 * U[dt] if dt == np.float16 else 0)
+        for i in range(5):
+            close(got[i], want[i], dt, U[dt], loose * (8 if i == 3 else 2))
+        close(got[5], want[5], wide, U[wide], parts * 2)
+
+
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+@pytest.mark.parametrize("steps", [1, 6, 70])
+def test_views(dt, steps):
+    """Slices of one projection, reversed and broadcast arrays, gates of either type: the bits of
+    contiguous copies."""
+    g = np.random.default_rng(steps)
+    b, h, kh, dk, dv = 2, 4, 2, 16, 24
+    wide = np.float64 if dt == np.float64 else np.float32
+    parts = cp.array((g.standard_normal((b, steps, 2 * kh * dk + h * dv + 5)) * 0.2).astype(dt))
+    q = parts[..., :kh * dk].reshape((b, steps, kh, dk))
+    k = parts[..., kh * dk:2 * kh * dk].reshape((b, steps, kh, dk))
+    v = parts[..., 2 * kh * dk + 5:].reshape((b, steps, h, dv))
+    both = cp.array(g.standard_normal((2, h, steps, b)).astype(wide))
+    gate, beta = -cp.abs(both[0]).transpose((2, 1, 0)), cp.abs(both[1]).transpose((2, 1, 0)) * 0.3
+    grad = cp.array(g.standard_normal((b, steps, h, 2 * dv)).astype(dt))[..., ::2]
+    plain = lambda a: cp.array(np.ascontiguousarray(a.get()))  # noqa: E731
+    cases = [(q, k, v, gate, beta, grad), (q[::-1], k[:, ::-1], v, gate, beta, grad),
+             (cp.broadcast_to(q[:1], q.shape), k, cp.broadcast_to(v[:, :, :1], v.shape), gate, beta, grad)]
+    for q_, k_, v_, gate_, beta_, grad_ in cases:
+        got = nn.gated_delta_rule(q_, k_, v_, gate_, beta_)
+        want = nn.gated_delta_rule(*map(plain, (q_, k_, v_, gate_, beta_)))
+        for x, y in zip(got, want):
+            assert x.dtype == y.dtype and np.array_equal(x.get(), y.get())
+        got = nn.gated_delta_rule_grad(grad_, q_, k_, v_, gate_, beta_)
+        want = nn.gated_delta_rule_grad(*map(plain, (grad_, q_, k_, v_, gate_, beta_)))
+        assert [x.dtype for x in got] == [np.dtype(t) for t in (dt, dt, dt, wide, wide, wide)]
+        for x, y in zip(got, want):
+            assert np.array_equal(x.get(), y.get())
+
+
+@pytest.mark.parametrize("dt", FLOATS, **by_name)
+def test_steps_go_on(dt):
+    """Token by token, in pieces and at once: the states agree to their own roundings."""
+    g = np.random.default_rng(8)
+    x = make(g, 2, 100, 1, 2, 32, 24, dt)
+    parts = parts_of(dt, 100, 32) + (8 * U[dt] if dt == np.float16 else 0)
+    o, S = rule(*x, None, 32 ** -0.5)
+    for cuts in (range(0, 101), (0, 8, 17, 64, 100), (0, 99, 100)):
+        state, rows = None, []
+        for a, b in zip(cuts[:-1], cuts[1:]):
+            row, state = nn.gated_delta_rule(*(cp.array(np.ascontiguousarray(v[:, a:b])) for v in x), state)
+            rows.append(row.get())
+        close(cp.array(np.concatenate(rows, 1)), o, dt, U[dt], parts)
+        close(state, S, state.dtype.type, 0.0, parts)
+
+
+def test_padding_and_fresh_starts():
+    """Steps with a gate and a beta of 0 leave the state; a gate of -inf is as no state before."""
+    g = np.random.default_rng(9)
+    for dt in FLOATS:
+        x = make(g, 1, 90, 1, 1, 16, 16, dt, pad=20)
+        _, S = nn.gated_delta_rule(*map(cp.array, x))
+        _, T = nn.gated_delta_rule(*(cp.array(np.ascontiguousarray(v[:, :70])) for v in x))
+        wide = T.dtype.type
+        close(S, T.get().astype(np.float64), wide, 0.0, parts_of(dt, 70, 16))
+        x[3][:, 40] = -np.inf
+        start = cp.array(g.standard_normal((1, 1, 16, 16)).astype(wide))
+        o, S = nn.gated_delta_rule(*map(cp.array, x), start)
+        p, T = nn.gated_delta_rule(*(cp.array(np.ascontiguousarray(v[:, 40:])) for v in x))
+        close(S, T.get().astype(np.float64), wide, 0.0, parts_of(dt, 90, 16))
+        close(cp.array(np.ascontiguousarray(o.get()[:, 40:])), p.get().astype(np.float64), dt, 2 * U[dt],
+              parts_of(dt, 90, 16) + 8 * U[dt] * (dt == np.float16))
+        # outputs from the fresh start on alone: nothing before it has a gradient
+        grad = x[2].copy()
+        grad[:, :40] = 0
+        grads = nn.gated_delta_rule_grad(cp.array(grad), *map(cp.array, x), start)
+        assert not np.any(grads[0].get()[:, :40]) and not np.any(grads[2].get()[:, :40])
+        assert float(grads[3].get()[0, 40, 0]) == 0.0 and not np.any(grads[5].get())
+
+
+def test_empty():
+    for dt in FLOATS:
+        wide = np.float64 if dt == np.float64 else np.float32
+        z = lambda *s: cp.zeros(s, dtype=dt)  # noqa: E731
+        one = cp.ones((2, 3, 4, 5), dtype=wide)
+        o, S = nn.gated_delta_rule(z(2, 0, 1, 4), z(2, 0, 1, 4), z(2, 0, 3, 5), z(2, 0, 3), z(2, 0, 3), one)
+        assert o.shape == (2, 0, 3, 5) and np.array_equal(S.get(), one.get())
+        grads = nn.gated_delta_rule_grad(z(2, 0, 3, 5), z(2, 0, 1, 4), z(2, 0, 1, 4), z(2, 0, 3, 5), z(2, 0, 3), z(2, 0, 3), one, one)
+        assert np.array_equal(grads[5].get(), one.get())
+        for steps in (3, 20):
+            o, S = nn.gated_delta_rule(z(2, steps, 1, 0), z(2, steps, 1, 0), z(2, steps, 3, 5), z(2, steps, 3), z(2, steps, 3))
+            assert S.shape == (2, 3, 0, 5) and not np.any(o.get())
+            grads = nn.gated_delta_rule_grad(z(2, steps, 3, 5), z(2, steps, 1, 0), z(2, steps, 1, 0), z(2, steps, 3, 5), z(2, steps, 3), z(2, steps, 3))
+            assert not any(np.any(g.get()) for g in grads)
+            k = cp.ones((2, steps, 1, 4), dtype=dt)
+            o, S = nn.gated_delta_rule(k, k, z(2, steps, 3, 0), z(2, steps, 3), z(2, steps, 3))
+            assert o.shape == (2, steps, 3, 0) and S.shape == (2, 3, 4, 0)
+            grads = nn.gated_delta_rule_grad(z(2, steps, 3, 0), k, k, z(2, steps, 3, 0), z(2, steps, 3), z(2, steps, 3))
+            assert not any(np.any(g.get()) for g in grads)
+            o, S = nn.gated_delta_rule(k, k, z(2, steps, 0, 5), z(2, steps, 0), z(2, steps, 0))
+            assert o.shape == (2, steps, 0, 5)
+            grads = nn.gated_delta_rule_grad(z(2, steps, 0, 5), k, k, z(2, steps, 0, 5), z(2, steps, 0), z(2, steps, 0))
+            assert not np.any(grads[0].get()) and not np.any(grads[1].get())
+            assert nn.gated_delta_rule(z(0, steps, 1, 4), z(0, steps, 1, 4), z(0, steps, 2, 5), z(0, steps, 2), z(0, steps, 2))[0].size == 0
+
+
+def test_differences():
+    """The gradient against differences of the operator itself, in 64 bits."""
+    g = np.random.default_rng(11)
+    x = [a.astype(np.float64) for a in make(g, 1, 37, 1, 2, 6, 5, np.float64)]
+    states = [g.standard_normal((1, 2, 6, 5)) for _ in range(2)]
+    grad = g.standard_normal(x[2].shape)
+
+    def value(args):
+        o, S = nn.gated_delta_rule(*map(cp.array, args))
+        return float((o.get() * grad).sum() + (S.get() * states[1]).sum())
+
+    args = x + [states[0]]
+    grads = nn.gated_delta_rule_grad(cp.array(grad), *map(cp.array, args), cp.array(states[1]))
+    step = 1e-5
+    for i, a in enumerate(args):
+        d = g.standard_normal(a.shape)
+        move = lambda by: [b + by * d if j == i else b for j, b in enumerate(args)]  # noqa: E731
+        slope = (value(move(step)) - value(move(-step))) / (2 * step)
+        want = float((grads[i].get() * d).sum())
+        # third derivatives of order 1e4 times step^2 / 6, and 2^-53 of values of some 1e2 over step
+        assert abs(slope - want) <= 1e4 * step ** 2 + 1e2 * 2.0 ** -53 / step * 10
+
+
+def test_repeats():
+    """The same bits every time."""
+    g = np.random.default_rng(12)
+    for dt in FLOATS:
+        x = [cp.array(a) for a in make(g, 2, 700, 2, 4, 48, 40, dt, 0.01)]
+        first = nn.gated_delta_rule(*x) + nn.gated_delta_rule_grad(x[2], *x)
+        again = nn.gated_delta_rule(*x) + nn.gated_delta_rule_grad(x[2], *x)
+        assert all(np.array_equal(a.get(), b.get(), equal_nan=True) for a, b in zip(first, again))
+
+
+def test_refusals():
+    z = lambda *s, dt=np.float32: cp.zeros(s, dtype=dt)  # noqa: E731
+    q, v, g = z(2, 3, 2, 4), z(2, 3, 4, 5), z(2, 3, 4)
+    for bad, error in (((z(2, 3, 8), q, v, g, g), ValueError), ((q, z(2, 3, 2, 5), v, g, g), ValueError),
+                       ((q, q, z(2, 4, 4, 5), g, g), ValueError), ((q, q, z(2, 3, 3, 5), z(2, 3, 3), z(2, 3, 3)), ValueError),
+                       ((q, q, v, z(2, 3, 2), g), ValueError), ((q, q, v, g, z(2, 3)), ValueError),
+                       ((z(2, 3, 2, 257), z(2, 3, 2, 257), v, g, g), ValueError),
+                       ((q, q, v, g, cp.zeros((2, 3, 4), dtype=np.int32)), TypeError),
+                       ((z(2, 3, 0, 4), z(2, 3, 0, 4), v, g, g), ValueError),
+                       ((q, q, v, g, g, z(2, 4, 5, 4)), ValueError), ((q, q, v, g, g, None), None)):
+        if error is None:
+            nn.gated_delta_rule(*bad)
+            continue
+        with pytest.raises(error):
+            nn.gated_delta_rule(*bad)
+        with pytest.raises(error):
+            nn.gated_delta_rule_grad(v, *bad)
+    with pytest.raises(TypeError):
+        nn.gated_delta_rule(q, q, v, g, g, scale="1")
+    with pytest.raises(ValueError):
+        nn.gated_delta_rule_grad(q, q, q, v, g, g)
+    with pytest.raises(ValueError):
+        nn.gated_delta_rule_grad(v, q, q, v, g, g, None, z(2, 4, 4, 4))
