@@ -40,6 +40,7 @@ using mmpn::Vec;
 using mmpn::Wide;
 using mmpx::Lay;
 using mmpx::Mma;
+using mmpx::Tile;
 using mmpx::Two;
 
 // Steps of a chunk: the products within one grow with it, the passes through the
@@ -85,48 +86,6 @@ template <typename T> constexpr int parts_of() { return Mma<T>::SPLIT ? 2 : 1; }
 template <typename A> __device__ __forceinline__ bool starts_anew(A g) { return g < (sizeof(A) == 4 ? (A)-104 : (A)-746); }
 __device__ __forceinline__ float exp_any(float x) { return x > 80.0f ? expf(x) : mmpn::exp_of(x); }
 __device__ __forceinline__ double exp_any(double x) { return exp(x); }
-
-// W columns of ROWS rows of an array in registers, and on their way to LDS.
-template <typename T, int ROWS, int W, int THREADS> struct Tile {
-  static constexpr int V = vec_of<T>(), PER = W / V, N = (ROWS * PER + THREADS - 1) / THREADS;
-  static constexpr int STEP = THREADS / PER;  // rows from one of a thread's vectors to its next
-  static constexpr bool WHOLE = ROWS % STEP == 0;
-  static_assert(THREADS % PER == 0, "");
-  typedef typename Vec<T, V>::Words Words;
-  Words w[N];
-  // rows from `rows` on and columns from `cols` on are zeros
-  __device__ __forceinline__ void fetch(const T *p, long long stride, int rows, int cols, int tid) {
-    const int r0 = tid / PER, c = tid % PER * V;
-    const T *at = p + r0 * stride + c;
-    if (WHOLE && rows >= ROWS && cols >= W) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = mmpn::words_of(mmpn::load_vec<T, V>(at + i * STEP * stride));
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        Vec<T, V> x{};
-        if (i * STEP + r0 < rows && i * STEP + r0 < ROWS) {
-          const T *from = at + i * STEP * stride;
-          if (c + V <= cols) {
-            x = mmpn::load_vec<T, V>(from);
-          } else if (c < cols) {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-              if (c + e < cols) x.e[e] = from[e];
-          }
-        }
-        w[i] = mmpn::words_of(x);
-      }
-    }
-  }
-  __device__ __forceinline__ void put(T *lds, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = i * STEP + tid / PER;
-      if (WHOLE || r < ROWS) *reinterpret_cast<Words *>(lds + Lay<T, W>::at(r, tid % PER * V)) = w[i];
-    }
-  }
-};
 
 // A chunk's gates, by one wave (lane: a step): logarithms summed up without the
 // fresh starts, and those counted.

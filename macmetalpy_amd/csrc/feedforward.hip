@@ -148,6 +148,14 @@ struct Prod {
   float *part;         // kPartial: (parts, m, n) or (parts, m, 2 n)
 };
 
+// Tile b in an order that goes down four rows of tiles at a time: what runs together
+// on an XCD shares rows of the one operand and columns of the other in its cache.
+__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int &tm, int &tn) {
+  const int first = b / (4 * tiles_n) * 4, rows = min(tiles_m - first, 4), rest = b - first * tiles_n;
+  tm = first + rest % rows;
+  tn = rest / rows;
+}
+
 // Where a stage has its 16 byte chunks (k_prod16), and the eight k of half slab
 // `s` of one of the 16 m or n from `first` on.
 __device__ __forceinline__ int mn_slot(int r) { return (r >> 1) & 7; }
@@ -183,7 +191,6 @@ __device__ __forceinline__ h8 fragment(const u16 *S, int first, int s, int lane)
 //    lane gets its eight k of a column by two transposing reads, each of four
 //    rows.
 // The MFMA is issued as C^T = B^T A^T, so a lane has four adjacent columns.
-// Workgroups of an XCD (ids go round the eight) get tiles next to one another.
 template <int WM, int WN, int I, int J, bool AK, bool BK_, bool PAIR, int END, int ACT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod16(Prod p, End<mmp_half> end) {
   constexpr int TM = 16 * I * WM, TN = 16 * J * WN, NW = WM * WN, BK = 64;
@@ -196,11 +203,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod16(Prod p, End<mmp_half
   const int wm = wave / WN, wn = wave % WN;
 
   const int blocks = p.tiles_m * p.tiles_n;
-  const int b = (int)mmpx::adjacent_on_xcd(blockIdx.x, blocks);
-  constexpr int GM = 4;
-  const int first = b / (GM * p.tiles_n) * GM, gm = min(p.tiles_m - first, GM);
-  const int rem = b - first * p.tiles_n;
-  const int tm = first + rem % gm, tn = rem / gm;
+  int tm, tn;
+  tile_of((int)mmpx::adjacent_on_xcd(blockIdx.x, blocks), p.tiles_m, p.tiles_n, tm, tn);
   const int m0 = tm * TM, n0 = tn * (PAIR ? TN / 2 : TN);
   const int nk = (p.k + BK - 1) / BK, kb = blockIdx.y * p.span, ke = min(nk, kb + p.span);
 
@@ -353,22 +357,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod16(Prod p, End<mmp_half
 }
 
 // The parts of k added in order, four columns a thread.
-template <int END, int ACT>
-__global__ __launch_bounds__(256) void k_join16(const float *part, int parts, int m, int n, End<mmp_half> end) {
+template <typename T, int END, int ACT>
+__global__ __launch_bounds__(256) void k_join_parts(const typename Wide<T>::type *part, int parts, int m, int n, End<T> end) {
+  typedef typename Wide<T>::type A;
   const int n4 = (n + 3) & ~3;
   constexpr bool PAIR = END != kPlain;
   const long long id = blockIdx.x * 256LL + threadIdx.x, row = id / (n4 / 4);
   if (row >= m) return;
   const int col = (int)(id - row * (n4 / 4)) * 4;
   const long long width = PAIR ? 2 * n4 : n4;
-  float v[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
+  A v[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
   for (int z = 0; z < parts; ++z) {
-    const float *at = part + ((long long)z * m + row) * width + col;
-    const auto x = mmpn::load_vec<float, 4>(at);
+    const A *at = part + ((long long)z * m + row) * width + col;
+    const auto x = mmpn::load_vec<A, 4>(at);
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] += x.e[r];
     if constexpr (PAIR) {
-      const auto y = mmpn::load_vec<float, 4>(at + n4);
+      const auto y = mmpn::load_vec<A, 4>(at + n4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) w[r] += y.e[r];
     }
@@ -397,18 +402,133 @@ __global__ __launch_bounds__(256) void k_padded(const mmp_half *src, long long l
   mmpn::store_vec(dst + row * per * 8 + at, v);
 }
 
-// ---------------------------------------------------- float32 and float64: ends
-// Both projections (rows, 2 hidden) into h, or in place into D.
-template <typename T, int ACT, bool GRAD>
-__global__ __launch_bounds__(256) void k_ends(const T *both, long long rows, End<T> end) {
+// ------------------------------------------------- float32 and float64: projections
+template <typename T> struct Wides;
+template <int END, int ACT, typename T, int N>
+__device__ __forceinline__ void finish(const Wides<T> &p, const End<T> &end, int row, int col, const typename Wide<T>::type (&g)[N],
+                                       const typename Wide<T>::type (&u)[N]);
+
+template <typename T> struct Wides {
+  const T *x, *w;
+  long long ldx, ldw;
+  int m, n, k;  // n: columns of a projection
+  int tiles_n, span;  // slabs to a part of k (blockIdx.y)
+  typename Wide<T>::type *part;
+};
+
+// Both projections for 32 I rows and 32 J columns, any extents, alignment and strides;
+// a wave has 16 I x 16 J of either.  k goes by in slabs of 128 bytes through two
+// buffers in LDS, the next on its way in registers.  Products issued as
+// transposed ones, so that a lane has four columns of a row.
+template <typename T, int I, int J, int END, int ACT>
+__global__ __launch_bounds__(256, I == 1 ? 6 : 2) void k_projections(Wides<T> p, End<T> end) {
   typedef typename Wide<T>::type A;
-  const long long id = blockIdx.x * 256LL + threadIdx.x, row = id / end.hidden;
-  if (row >= rows) return;
-  const int col = (int)(id - row * end.hidden);
-  const T *at = both + row * 2 * end.hidden + col;
-  const A g[1] = {at[0]}, u[1] = {at[end.hidden]};
-  if constexpr (GRAD) end.template backward<ACT>(row, col, g, u);
-  else end.template forward<ACT>(row, col, g, u);
+  typedef mmpx::Mma<T> M;
+  constexpr int TM = 32 * I, TN = 32 * J, BK = 128 / sizeof(T);
+  __shared__ __attribute__((aligned(16))) T As[2][TM * BK], Gs[2][BK * TN], Us[2][BK * TN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
+  const int wm = wave >> 1, wn = wave & 1;
+  int tm, tn;
+  tile_of((int)mmpx::adjacent_on_xcd(blockIdx.x, gridDim.x), (p.m + TM - 1) / TM, p.tiles_n, tm, tn);
+  const int m0 = tm * TM, n0 = tn * TN;
+  const int nk = (p.k + BK - 1) / BK, kb = blockIdx.y * p.span, ke = min(nk, kb + p.span);
+  const T *x = p.x + m0 * p.ldx, *w = p.w + n0;
+  // slabs on their way in registers
+  constexpr int DEPTH = 2;
+  struct Slab {
+    mmpx::Tile<T, TM, BK, 256> a;
+    mmpx::Tile<T, BK, TN, 256> g, u;
+  } slab[DEPTH];
+  auto fetch = [&](Slab &s, int kt) __attribute__((always_inline)) {
+    const int k0 = kt * BK;
+    s.a.fetch(x + k0, p.ldx, p.m - m0, p.k - k0, tid);
+    s.g.fetch(w + k0 * p.ldw, p.ldw, p.k - k0, p.n - n0, tid);
+    s.u.fetch(w + k0 * p.ldw + p.n, p.ldw, p.k - k0, p.n - n0, tid);
+  };
+  auto put = [&](const Slab &s, int buf) __attribute__((always_inline)) {
+    s.a.put(As[buf], tid);
+    s.g.put(Gs[buf], tid);
+    s.u.put(Us[buf], tid);
+  };
+  typename M::Acc ag[I][J], au[I][J];
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j) ag[i][j] = au[i][j] = typename M::Acc{};
+  fetch(slab[0], kb);
+  put(slab[0], 0);
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (kb + 1 + d < ke) fetch(slab[d], kb + 1 + d);
+  __syncthreads();
+  for (int kt = kb; kt < ke; kt += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (kt + d >= ke) break;
+      const int cur = d & 1;  // (DEPTH is even)
+#pragma unroll
+      for (int k0 = 0; k0 < BK; k0 += M::K) {
+        typename M::Frag fa[I], fg[J], fu[J];
+#pragma unroll
+        for (int i = 0; i < I; ++i) fa[i] = M::template rows<BK>(As[cur], (wm * I + i) * 16, k0, lane);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          fg[j] = M::template cols<TN>(Gs[cur], k0, (wn * J + j) * 16, lane);
+          fu[j] = M::template cols<TN>(Us[cur], k0, (wn * J + j) * 16, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            ag[i][j] = M::mul(fg[j], fa[i], ag[i][j]);
+            au[i][j] = M::mul(fu[j], fa[i], au[i][j]);
+          }
+      }
+      if (kt + d + 1 < ke) put(slab[d], cur ^ 1);
+      if (kt + d + 1 + DEPTH < ke) fetch(slab[d], kt + d + 1 + DEPTH);
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int row = m0 + (wm * I + i) * 16 + fr;
+    if (row >= p.m) continue;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int first = n0 + (wn * J + j) * 16;
+      if constexpr (sizeof(T) == 4) {
+        const int col = first + 4 * g;
+        const A v[4] = {ag[i][j][0], ag[i][j][1], ag[i][j][2], ag[i][j][3]};
+        const A u[4] = {au[i][j][0], au[i][j][1], au[i][j][2], au[i][j][3]};
+        if (col < p.n) finish<END, ACT>(p, end, row, col, v, u);
+      } else {  // float64's accumulators have columns g + 4 r
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int col = first + g + 4 * r;
+          const A v[1] = {ag[i][j][r]}, u[1] = {au[i][j][r]};
+          if (col < p.n) finish<END, ACT>(p, end, row, col, v, u);
+        }
+      }
+    }
+  }
+}
+
+template <int END, int ACT, typename T, int N>
+__device__ __forceinline__ void finish(const Wides<T> &p, const End<T> &end, int row, int col, const typename Wide<T>::type (&g)[N],
+                                       const typename Wide<T>::type (&u)[N]) {
+  if constexpr (END == kPartial) {
+    const int n4 = (p.n + 3) & ~3;
+    auto *o = p.part + ((long long)blockIdx.y * p.m + row) * 2 * n4 + col;
+#pragma unroll
+    for (int r = 0; r < N; ++r) {  // (beyond the columns there is room)
+      o[r] = g[r];
+      o[n4 + r] = u[r];
+    }
+  } else if constexpr (END == kForward) {
+    end.template forward<ACT>(row, col, g, u);
+  } else {
+    end.template backward<ACT>(row, col, g, u);
+  }
 }
 
 // ------------------------------------------------------------------- host side
@@ -462,7 +582,7 @@ int prod16(Prod p, const End<mmp_half> &end, const char *what) {
     if (int st = launch16<AK, BK_, PAIR, kPartial, 0>(plan.tile, grid, p, end, what)) return st;
     unsigned blocks;
     if (int st = threads_of((long long)p.m * (n4 / 4), what, &blocks)) return st;
-    hipLaunchKernelGGL((k_join16<END, ACT>), dim3(blocks), dim3(256), 0, mmpi::stream(), p.part, parts, p.m, p.n, end);
+    hipLaunchKernelGGL((k_join_parts<mmp_half, END, ACT>), dim3(blocks), dim3(256), 0, mmpi::stream(), p.part, parts, p.m, p.n, end);
     return mmpi::check_launch(what);
   }
   return launch16<AK, BK_, PAIR, END, ACT>(plan.tile, grid, p, end, what);
@@ -535,25 +655,47 @@ int backward16(const Call<mmp_half> &c) {
 
 template <typename T> int dtype_of() { return sizeof(T) == 4 ? MMP_F32 : MMP_F64; }
 
-template <typename T, bool GRAD> int ends(const Call<T> &c, const T *both, const End<T> &end) {
-  unsigned blocks;
-  if (int st = threads_of((long long)c.rows * c.hidden, c.what, &blocks)) return st;
+template <typename T, int I, int J, int END, int ACT>
+int launch_projections(dim3 grid, const Wides<T> &p, const End<T> &end, const char *what) {
+  hipLaunchKernelGGL((k_projections<T, I, J, END, ACT>), grid, dim3(256), 0, mmpi::stream(), p, end);
+  return mmpi::check_launch(what);
+}
+template <typename T> int partial_projections(int rows, dim3 grid, const Wides<T> &p, const End<T> &end, const char *what) {
+  return rows == 128 ? launch_projections<T, 4, 2, kPartial, 0>(grid, p, end, what) : launch_projections<T, 1, 1, kPartial, 0>(grid, p, end, what);
+}
+template <typename T, int END> int projections(const Call<T> &c, const End<T> &end) {
+  typedef typename Wide<T>::type A;
+  constexpr int BK = 128 / sizeof(T);
+  const int slabs = (c.dim + BK - 1) / BK;
+  Wides<T> p{c.x, c.w, c.ldx, c.ldw, c.rows, c.hidden, c.dim, 0, 0, nullptr};
+  mmpi::ProjectionsPlan plan = mmpi::projections_plan((int)sizeof(T), p.m, p.n, slabs, mmpi::cu_count());
+  const int columns = plan.rows == 128 ? 64 : 32;
+  p.tiles_n = (c.hidden + columns - 1) / columns;
+  if (plan.parts > 1 && mmpn::capturing()) plan.parts = 1;
+  p.span = (slabs + plan.parts - 1) / plan.parts;
+  const int parts = (slabs + p.span - 1) / p.span;
+  const long long tiles = (long long)((p.m + plan.rows - 1) / plan.rows) * p.tiles_n;
+  if (!mmpi::grid_fits(tiles, 256)) return mmpi::fail(MMP_E_UNSUPPORTED, "%s: too many tiles", c.what);
+  const dim3 grid((unsigned)tiles, (unsigned)parts);
   return with_activation(c.act, [&](auto act) {
-    hipLaunchKernelGGL((k_ends<T, act.value, GRAD>), dim3(blocks), dim3(256), 0, mmpi::stream(), both, (long long)c.rows, end);
+    constexpr int ACT = decltype(act)::value;
+    if (parts == 1)
+      return plan.rows == 128 ? launch_projections<T, 4, 2, END, ACT>(grid, p, end, c.what) : launch_projections<T, 1, 1, END, ACT>(grid, p, end, c.what);
+    Temp part;
+    const int n4 = (p.n + 3) & ~3;
+    if (int st = part.get((size_t)parts * p.m * 2 * n4 * sizeof(A), c.what)) return st;
+    p.part = (A *)part.p;
+    if (int st = partial_projections<T>(plan.rows, grid, p, end, c.what)) return st;
+    unsigned blocks;
+    if (int st = threads_of((long long)p.m * (n4 / 4), c.what, &blocks)) return st;
+    hipLaunchKernelGGL((k_join_parts<T, END, ACT>), dim3(blocks), dim3(256), 0, mmpi::stream(), (const A *)part.p, parts, p.m, p.n, end);
     return mmpi::check_launch(c.what);
   });
 }
 
 template <typename T> int forward(const Call<T> &c) {
-  if constexpr (sizeof(T) == 2) {
-    return forward16(c);
-  } else {
-    Temp both;
-    if (int st = both.get((size_t)c.rows * 2 * c.hidden * sizeof(T), c.what)) return st;
-    if (int st = mmp_matmul(dtype_of<T>(), 1, c.rows, 2LL * c.hidden, c.dim, c.x, c.ldx, 0, c.w, c.ldw, 0, both.p, 2LL * c.hidden, 0))
-      return st;
-    return ends<T, false>(c, (const T *)both.p, End<T>{c.h, c.hidden, nullptr, 0, c.hidden, c.hidden, true});
-  }
+  if constexpr (sizeof(T) == 2) return forward16(c);
+  else return projections<T, kForward>(c, End<T>{c.h, c.hidden, nullptr, 0, c.hidden, c.hidden, c.hidden % 4 == 0});
 }
 
 template <typename T> int backward(const Call<T> &c) {
@@ -563,9 +705,7 @@ template <typename T> int backward(const Call<T> &c) {
     Temp d;
     const long long ldd = 2LL * c.hidden;
     if (int st = d.get((size_t)c.rows * ldd * sizeof(T), c.what)) return st;
-    if (int st = mmp_matmul(dtype_of<T>(), 1, c.rows, ldd, c.dim, c.x, c.ldx, 0, c.w, c.ldw, 0, d.p, ldd, 0)) return st;
-    if (int st = ends<T, true>(c, (const T *)d.p, End<T>{(T *)d.p, ldd, c.grad, c.ldg, c.hidden, c.hidden, true}))
-      return st;
+    if (int st = projections<T, kBackward>(c, End<T>{(T *)d.p, ldd, c.grad, c.ldg, c.hidden, c.hidden, c.hidden % 4 == 0})) return st;
     if (int st = mmp_matmul_t(dtype_of<T>(), 0, 1, 1, c.rows, c.dim, ldd, d.p, ldd, 0, c.w, c.ldw, 0, c.grad_x, c.dim, 0))
       return st;
     return mmp_matmul_t(dtype_of<T>(), 1, 0, 1, c.dim, ldd, c.rows, c.x, c.ldx, 0, d.p, ldd, 0, c.grad_w, ldd, 0);

@@ -84,6 +84,48 @@ __device__ __forceinline__ void copy_tile(const T *p, long long stride, int rows
   else copy(std::true_type());
 }
 
+// W columns of ROWS rows of an array in registers, and on their way to LDS.
+template <typename T, int ROWS, int W, int THREADS> struct Tile {
+  static constexpr int V = 16 / (int)sizeof(T), PER = W / V, N = (ROWS * PER + THREADS - 1) / THREADS;
+  static constexpr int STEP = THREADS / PER;  // rows from one of a thread's vectors to its next
+  static constexpr bool WHOLE = ROWS % STEP == 0;
+  static_assert(THREADS % PER == 0, "");
+  typedef typename mmpn::Vec<T, V>::Words Words;
+  Words w[N];
+  // rows from `rows` on and columns from `cols` on are zeros
+  __device__ __forceinline__ void fetch(const T *p, long long stride, int rows, int cols, int tid) {
+    const int r0 = tid / PER, c = tid % PER * V;
+    const T *at = p + r0 * stride + c;
+    if (WHOLE && rows >= ROWS && cols >= W) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = mmpn::words_of(mmpn::load_vec<T, V>(at + i * STEP * stride));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        mmpn::Vec<T, V> x{};
+        if (i * STEP + r0 < rows && i * STEP + r0 < ROWS) {
+          const T *from = at + i * STEP * stride;
+          if (c + V <= cols) {
+            x = mmpn::load_vec<T, V>(from);
+          } else if (c < cols) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (c + e < cols) x.e[e] = from[e];
+          }
+        }
+        w[i] = mmpn::words_of(x);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(T *lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * STEP + tid / PER;
+      if (WHOLE || r < ROWS) *reinterpret_cast<Words *>(lds + Lay<T, W>::at(r, tid % PER * V)) = w[i];
+    }
+  }
+};
+
 template <typename T> struct Mma;
 
 // v_mfma_f32_16x16x32_f16: two tiles of accumulators make one operand.

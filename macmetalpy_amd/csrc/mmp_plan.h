@@ -298,6 +298,32 @@ inline Prod16Plan prod16_plan(long long m, long long n, int slabs, double cus) {
   return best;
 }
 
+// Rows of a tile (128 by 64 columns of both projections, or 32 by 32) and k ranges of the
+// feed-forward product in float32 and float64; a slab of 128 bytes of k in us, the
+// bytes that tiles read at what they were seen to reach, TB/s.
+struct ProjectionsPlan {
+  int rows, parts;
+  double us;
+};
+inline ProjectionsPlan projections_plan(int elem, long long m, long long hidden, int slabs, double cus) {
+  ProjectionsPlan best{32, 1, 1e30};
+  for (int rows = 128; rows >= 32; rows /= 4) {
+    const bool large = rows == 128;
+    const int columns = large ? 64 : 32;
+    const double tiles = (double)((m + rows - 1) / rows) * (double)((hidden + columns - 1) / columns);
+    const double per_cu = large ? 2 : 6, shared = large ? 2.15 : 0.35, alone = large ? 4.0 : 1.6;
+    const double bytes = tiles * slabs * 128.0 * (rows + (large ? 128 : 64));
+    for (int s = 1; s <= 64; s *= 2) {
+      if (s > 1 && (slabs / s < 4 || tiles * s > 2 * cus * per_cu)) break;
+      double t = rounds_us(tiles * s, per_cu, (slabs + s - 1) / s, large ? 5.0 : 2.0, shared, alone, cus);
+      if (t < bytes / 6e6) t = bytes / 6e6;
+      if (s > 1) t += 4.0 + 2e-6 * s * (double)m * (double)hidden * 2 * elem / 5.0;
+      if (t < best.us * 0.98) best = ProjectionsPlan{rows, s, t};
+    }
+  }
+  return best;
+}
+
 // Segments that the chunks of the delta rule's heads are cut into: a pass takes a
 // workgroup for 64 columns of a head's state and is a chain of `chunks`, so few
 // heads leave CUs idle.  Segments run at once from states that a scan finds, which
