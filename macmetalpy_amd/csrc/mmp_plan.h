@@ -276,7 +276,10 @@ inline GemmPlan gemm_plan(long long batch, int M, int N, int K, int elem, bool m
 // Tile and k ranges of the feed-forward products' float16 kernel (k_prod16):
 // 256 wide tiles, one workgroup a CU, or 128 wide ones, two; a tile's slab of 64
 // deep, its start and its end in us, and what a second launch that adds ranges
-// up costs.
+// up costs.  Measured with 256 / 128 wide tiles, and 128 wide ones in 2 / 4 ranges, us,
+// rows x depth x hidden: 8 x 2048 x 5632 45 / 23 / 17 / 15, 64 x 1024 x 4096 25 / 12 /
+// 12 / 13, 512 x 1024 x 1024 27 / 12 / 15 / 14, 1024 x 1024 x 4096 31 / 23 / 52 / 63,
+// 1999 x 1008 x 2504 33 / 39 / 60 / 81, 2048 x 4096 x 4096 112 / 133 / 170 / 268.
 struct Prod16Plan {
   int tile;
   int parts;  // ranges of k
@@ -299,8 +302,12 @@ inline Prod16Plan prod16_plan(long long m, long long n, int slabs, double cus) {
 }
 
 // Rows of a tile (128 by 64 columns of both projections, or 32 by 32) and k ranges of the
-// feed-forward product in float32 and float64; a slab of 128 bytes of k in us, the
-// bytes that tiles read at what they were seen to reach, TB/s.
+// feed-forward product in float32 and float64; a slab of 128 bytes of k in us, and the
+// bytes that all tiles read, caches serving most, at 9 TB/s.  Measured in float32, large / small tiles and small
+// ones in 2 / 4 / 8 ranges, us, rows x depth x hidden: 515 x 771 x 1030 100 / 44 / 39 /
+// 37 / 41, 81 x 3849 x 3558 484 / 221 / 132 / 96 / 82, 4032 x 105 x 11,130 294 / 299 / 688,
+// 9123 x 145 x 176 21 / 19 / 36, 2048 cubed 282 / 355 / 359, 8 x 2048 x 2048 162 / 38 / 24
+// / 16 / 15.
 struct ProjectionsPlan {
   int rows, parts;
   double us;
@@ -316,7 +323,7 @@ inline ProjectionsPlan projections_plan(int elem, long long m, long long hidden,
     for (int s = 1; s <= 64; s *= 2) {
       if (s > 1 && (slabs / s < 4 || tiles * s > 2 * cus * per_cu)) break;
       double t = rounds_us(tiles * s, per_cu, (slabs + s - 1) / s, large ? 5.0 : 2.0, shared, alone, cus);
-      if (t < bytes / 6e6) t = bytes / 6e6;
+      if (t < bytes / 9e6) t = bytes / 9e6;
       if (s > 1) t += 4.0 + 2e-6 * s * (double)m * (double)hidden * 2 * elem / 5.0;
       if (t < best.us * 0.98) best = ProjectionsPlan{rows, s, t};
     }
@@ -329,6 +336,11 @@ inline ProjectionsPlan projections_plan(int elem, long long m, long long hidden,
 // heads leave CUs idle.  Segments run at once from states that a scan finds, which
 // takes the columns of the values and of the keys, and a join that goes through
 // them.  Us a chunk: 3.4 with outputs, 2.4 in the scan; 3 a segment in the join.
+// Measured in 1 / 2 / 4 / 8 / 16 / 32 segments, us, heads x chunks: 8 x 64 of 128 x 128
+// float16 218 / 200 / 125 / 94 / 105 / 152, 8 x 512 1726 / 1427 / 770 / 452 / 371 / 420,
+// 16 x 32 of 64 x 64 97 / 90 / 62 / 51 / 55 / 74, 64 x 16 78 / 117 / 139 / 188,
+// 5 x 25 of 72 x 100 float32 161 / 152 / 101 / 80 / 86 / 101, 1 x 32 of 256 x 256 float16
+// 222 / 200 / 146 / 157 / 207 / 329.
 struct DeltaPlan {
   int segments, span;  // chunks of each but the last
 };
@@ -337,7 +349,7 @@ inline DeltaPlan delta_plan(long long heads, int value_tiles, int key_tiles, int
   if (heads < 1 || value_tiles < 1) return best;
   auto rounds = [&](long long wgs) { return __builtin_ceil((double)wgs / cus); };
   double us = 3.4 * chunks * rounds(heads * value_tiles);
-  for (int s = 2; s <= 64 && chunks / s >= 4; s *= 2) {
+  for (int s = 2; s <= 64 && chunks / s >= 3; s *= 2) {
     const int span = (chunks + s - 1) / s;
     const double t = span * (3.4 * rounds(heads * value_tiles * s) + 2.4 * rounds(heads * (value_tiles + key_tiles) * s)) + 3.0 * s + 10.0;
     if (t < 0.95 * us) {
