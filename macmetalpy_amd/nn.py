@@ -1,9 +1,11 @@
 """``cp.nn``: the operators of sequence models, with their gradients.
 
-Embedding rows by tokens, a gated linear recurrence, the softmax cross
+Embedding rows by tokens, a gated linear recurrence, the gated delta rule (whose
+states are matrices), the gated feed-forward product, dropout, the softmax cross
 entropy and the clipping of gradients by their global norm: with ``matmul``
 the parts of a training step of a recurrent language model, and, one step at a
-time, of its answers (``python -m macmetalpy_amd.recurrent_lm`` runs both).
+time, of its answers (``python -m macmetalpy_amd.recurrent_lm`` and
+``macmetalpy_amd.delta_lm`` run both).
 The reference has none of them.  Each is one call on device arrays, most of
 which read their inputs once (the norm's limit needs a second pass over the
 arrays, and so does the gradient of a loss for rows too long for a workgroup's
@@ -335,7 +337,8 @@ def gated_delta_rule(q, k, v, gate, beta, initial=None, *, scale=None):
 
     ``gate`` holds logarithms of the decay, at most 0; ``-inf`` starts a head
     anew from any finite state, and a step with a gate and a beta of 0 leaves the
-    state as it is, so packed and filled up sequences need no mask.  Use keys
+    state as it is (with finite keys and values), so packed and filled up sequences
+    need no mask.  Use keys
     with ``beta * sum(k * k)`` of at most 2: beyond that the recurrence itself
     grows.  float16 holds a chunk's states, corrections and values in its range:
     65504 is the most they may reach."""

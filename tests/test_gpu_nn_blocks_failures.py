@@ -71,8 +71,9 @@ def _ffn(rows, dim, hidden, dt, grad=False):
 
 
 REPLAY = {"dropout": _dropout, "delta_token": _delta(1, np.float16), "delta_8": _delta(8, np.float32),
-          "ffn": _ffn(70, 96, 64, np.float16), "ffn_few": _ffn(3, 512, 264, np.float16)}
-REFUSED = {"delta": _delta(9, np.float16), "delta_long": _delta(700, np.float32), "ffn32": _ffn(5, 8, 8, np.float32),
+          "ffn": _ffn(70, 96, 64, np.float16), "ffn_few": _ffn(3, 512, 264, np.float16),
+          "ffn32": _ffn(5, 8, 8, np.float32), "ffn32_few": _ffn(3, 512, 264, np.float32)}
+REFUSED = {"delta": _delta(9, np.float16), "delta_long": _delta(700, np.float32),
            "ffn_odd": _ffn(5, 9, 8, np.float16), "ffn_grad": _ffn(5, 8, 8, np.float16, True),
            "ffn_grad32": _ffn(5, 8, 8, np.float32, True)}
 
@@ -97,7 +98,7 @@ def test_replays_follow_the_inputs(name):
             call()
             for k, a in zip(outs, got):
                 b = d.get(k)
-                if name == "ffn_few":
+                if name.endswith("_few"):
                     assert np.allclose(a.astype(float), b.astype(float), rtol=2.0 ** -9, atol=512 * 2.0 ** -24 * 512)
                 else:
                     assert np.array_equal(a, b)
