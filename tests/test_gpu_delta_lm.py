@@ -1,8 +1,7 @@
-"""The matrix state language model: its gradients against the whole model's in 64
-bits on the CPU, and answers a token at a time against the whole text's."""
+"""The matrix state language model: its loss and gradients against the whole model in plain
+NumPy in 64 bits, and answers a token at a time against the whole text's."""
 import numpy as np
 import pytest
-import torch
 
 import macmetalpy_amd as cp
 from macmetalpy_amd import nn
@@ -12,33 +11,32 @@ pytestmark = pytest.mark.gpu
 
 
 def plain_loss(model, weights, tokens, targets, keep):
-    """The model in elementary torch operations; ``keep``: the dropouts' factors in order."""
+    """The model step by step; ``keep``: the dropouts' factors in order."""
     batch, steps = tokens.shape
     h, dk, dv = model.heads, model.dk, model.dv
+    sigmoid = lambda x: 1.0 / (1.0 + np.exp(-x))  # noqa: E731
     y = weights[0][tokens] * model.scale
     for i in range(model.layers):
         into, back, ffn, down = weights[1 + 4 * i:5 + 4 * i]
-        parts = y @ into
-        q, k, v, a, b = parts.split([h * dk, h * dk, h * dv, h, h], -1)
+        q, k, v, a, b = np.split(y @ into, np.cumsum([h * dk, h * dk, h * dv, h]), -1)
         q, k, v = (x.reshape(batch, steps, h, -1) for x in (q, k, v))
-        q, k = (x / (x.square().sum(-1, keepdim=True) + 1e-12).sqrt() for x in (q, k))
-        decay, beta = torch.sigmoid(a + 3.0), torch.sigmoid(b)
-        state, out = torch.zeros(batch, h, dk, dv, dtype=y.dtype), []
+        q, k = (x / np.sqrt((x * x).sum(-1, keepdims=True) + 1e-12) for x in (q, k))
+        decay, beta = sigmoid(a + 3.0), sigmoid(b)
+        state, out = np.zeros((batch, h, dk, dv)), []
         for t in range(steps):
             state = decay[:, t, :, None, None] * state
             u = beta[:, t, :, None] * (v[:, t] - (state * k[:, t, :, :, None]).sum(2))
             state = state + k[:, t, :, :, None] * u[:, :, None]
             out.append((state * q[:, t, :, :, None]).sum(2))
-        o = torch.stack(out, 1).reshape(batch, steps, h * dv)
+        o = np.stack(out, 1).reshape(batch, steps, h * dv)
         y = y + keep[2 * i] * (o @ back)
-        both = y @ ffn
-        half = both.shape[-1] // 2
-        g = both[..., :half]
-        y = y + keep[2 * i + 1] * ((g * torch.sigmoid(g) * both[..., half:]) @ down)
+        g, up = np.split(y @ ffn, 2, -1)
+        y = y + keep[2 * i + 1] * ((g * sigmoid(g) * up) @ down)
     logits = y @ weights[-1]
-    at = targets >= 0
-    loss = torch.logsumexp(logits, -1) - logits.gather(-1, targets.clamp(min=0)[..., None])[..., 0]
-    return (loss * at).sum() / at.sum()
+    top = logits.max(-1, keepdims=True)
+    lse = np.log(np.exp(logits - top).sum(-1)) + top[..., 0]
+    loss = lse - np.take_along_axis(logits, np.maximum(targets, 0)[..., None], -1)[..., 0]
+    return (loss * (targets >= 0)).sum() / (targets >= 0).sum()
 
 
 def test_gradients():
@@ -51,17 +49,22 @@ def test_gradients():
     first = model.drawn
     loss, grads = model.gradients(cp.array(tokens), targets)
     size = tokens.size * model.dim
-    keep = [torch.from_numpy(nn.dropout(cp.ones(tokens.shape + (24,), dtype=np.float64), 0.2, 9,
-                                        first + j * size).get()) for j in range(4)]
+    keep = [nn.dropout(cp.ones(tokens.shape + (24,), dtype=np.float64), 0.2, 9, first + j * size).get()
+            for j in range(4)]
     assert model.drawn == first + 4 * size
-    weights = [torch.from_numpy(w.get()).requires_grad_() for w in model.weights]
-    want = plain_loss(model, weights, torch.from_numpy(tokens.astype(np.int64)),
-                      torch.from_numpy(targets), keep)
-    want.backward()
+    weights = [w.get() for w in model.weights]
     # sums of some thousand terms of order 1 in 64 bits, through a few products
-    assert abs(float(loss) - want.item()) < 1e-11
-    for g, w in zip(grads, weights):
-        assert np.abs(g.get() - w.grad.numpy()).max() < 1e-11
+    assert abs(float(loss) - plain_loss(model, weights, tokens, targets, keep)) < 1e-11
+    # each weight's gradient along a few directions of length 1, against differences of the plain
+    # model: third derivatives of order 1e2 times step^2 / 6, and 2^-53 of some units over step
+    step = 1e-5
+    for i, g in enumerate(grads):
+        for _ in range(3):
+            d = rng.standard_normal(g.shape)
+            d /= np.linalg.norm(d)
+            at = lambda by: plain_loss(model, weights[:i] + [weights[i] + by * d] + weights[i + 1:], tokens, targets, keep)  # noqa: E731
+            slope = (at(step) - at(-step)) / (2 * step)
+            assert abs(slope - float((g.get() * d).sum())) < 1e2 * step ** 2 + 16 * 2.0 ** -53 / step, i
 
 
 def test_answers_token_by_token():
