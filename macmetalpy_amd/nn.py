@@ -338,9 +338,10 @@ def gated_delta_rule(q, k, v, gate, beta, initial=None, *, scale=None):
     ``gate`` holds logarithms of the decay, at most 0; ``-inf`` starts a head
     anew from any finite state, and a step with a gate and a beta of 0 leaves the
     state as it is (with finite keys and values), so packed and filled up sequences
-    need no mask.  Use keys
-    with ``beta * sum(k * k)`` of at most 2: beyond that the recurrence itself
-    grows.  float16 holds a chunk's states, corrections and values in its range:
+    need no mask.  A NaN or an infinity stays in its head (in a key or a query, in the
+    heads that share it), but reaches up to 63 steps back in it, as those are
+    worked out together.  Use keys with ``beta * sum(k * k)`` of at most 2: beyond
+    that the recurrence itself grows.  float16 holds a chunk's states, corrections and values in its range:
     65504 is the most they may reach."""
     arrays, initial, scale, (batch, steps, key_heads, heads, dk, dv), dtype = _delta(
         q, k, v, gate, beta, initial, scale)
